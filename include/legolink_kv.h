@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define LL_ABI_VERSION 17
+#define LL_ABI_VERSION 18
 
 /* hipStream_t, declared without pulling in the HIP headers. */
 struct ihipStream_t;
@@ -603,6 +603,84 @@ int ll_repair_attention(const ll_repair_attention_args *args, ll_stream_t stream
 int ll_repair_attention_noalloc(const ll_repair_attention_args *args, ll_stream_t stream);
 /* LL_REPAIR_SCRATCH_BYTES, as built into the library. */
 int64_t ll_repair_scratch_bytes(void);
+
+/*
+ * Norms of queries and keys for each head with their position rotation in the
+ * same pass, and, with a pool, the write of a step's new keys and values to
+ * their slots on the way (ABI 18).  No counterpart on the reference's link
+ * path: its model calls a norm, the rotary module and the pool's write one
+ * after another.
+ *
+ * For every token t, query or key head h, row x of head_dim values, in fp32
+ * and rounded once at the end:
+ *     y = x * rsqrt(mean(x^2) + norm_eps) * weight       (with a norm weight)
+ *     (y_i, y_j) = (y_i c - y_j s, y_j c + y_i s)         (rotary pairs)
+ * with c, s from row positions[t] of the cos/sin table (cos in columns [0,
+ * rotary_dim / 2), sin behind them) and the pairs (i, i + rotary_dim / 2) of a
+ * neox rotation or else (2 i, 2 i + 1); values from rotary_dim on are not
+ * rotated.  Keys go to key_output or, with destination_slots, to row
+ * destination_slots[t] of the pool's key_buffer, and the values unchanged to that
+ * row of value_buffer.
+ *
+ * A token whose position lies outside the table is left out: nothing of it is
+ * written.  A token whose slot is negative is padding: its queries are rotated
+ * and its keys and values not written; so is one whose slot is num_slots or
+ * more.  skipped_rows counts the tokens of a position outside the table or a
+ * slot past the pool, once each.
+ *
+ * Strides are in elements, and a row's values are neighbours.  An output may be
+ * its own input (the same address and strides); otherwise outputs, inputs and
+ * pool do not overlap, and the slots that are written are pairwise distinct.
+ * One launch; head dims and rotary dims of whole 16-value chunks with 16-byte
+ * aligned rows run a vector kernel, everything else an element-wise one with
+ * the same result up to the order of the norm's sum.
+ */
+typedef struct ll_head_rotary_args {
+  int64_t struct_size;             /* sizeof(ll_head_rotary_args) */
+  int64_t num_tokens;              /* 0: nothing is launched */
+  int64_t num_q_heads;             /* 1 .. 65535 */
+  int64_t num_kv_heads;            /* 1 .. 65535 (any ratio) */
+  int64_t head_dim;                /* 1 .. 256 */
+  int64_t value_head_dim;          /* 1 .. 256 (with a pool) */
+  int64_t dtype;                   /* LL_DTYPE_FLOAT16 or LL_DTYPE_BFLOAT16: rows, outputs and pool */
+  const void *query;               /* device [num_tokens, num_q_heads, head_dim], strided */
+  int64_t query_token_stride;
+  int64_t query_head_stride;
+  void *query_output;
+  int64_t query_output_token_stride;
+  int64_t query_output_head_stride;
+  const void *key;                 /* device [num_tokens, num_kv_heads, head_dim], strided */
+  int64_t key_token_stride;
+  int64_t key_head_stride;
+  void *key_output;                /* NULL with a pool */
+  int64_t key_output_token_stride;
+  int64_t key_output_head_stride;
+  const void *value;               /* device [num_tokens, num_kv_heads, value_head_dim], strided (with a pool) */
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  const void *positions;           /* device int32/int64 [num_tokens] */
+  int64_t positions_dtype;
+  const void *cos_sin_cache;       /* device [cos_sin_rows, cos_sin_cols], columns dense */
+  int64_t cos_sin_dtype;           /* fp16, bf16 or fp32 */
+  int64_t cos_sin_rows;
+  int64_t cos_sin_cols;            /* >= rotary_dim */
+  int64_t cos_sin_stride_row;
+  int64_t rotary_dim;              /* positive, even, at most head_dim */
+  int64_t is_neox_style;
+  const void *query_norm_weight;   /* device [head_dim], or NULL: no norm */
+  const void *key_norm_weight;
+  int64_t norm_weight_dtype;       /* fp16, bf16 or fp32, of both weights */
+  double norm_eps;
+  void *key_buffer;                /* device [num_slots, num_kv_heads, head_dim], dense: one layer (with a pool) */
+  void *value_buffer;              /* device [num_slots, num_kv_heads, value_head_dim], dense (with a pool) */
+  int64_t num_slots;
+  const void *destination_slots;   /* device int32/int64 [num_tokens]: the keys go to a pool; or NULL */
+  int64_t destination_slots_dtype;
+  int64_t *skipped_rows;           /* device counter, added to; or NULL */
+} ll_head_rotary_args;
+
+int ll_head_rotary(const ll_head_rotary_args *args, ll_stream_t stream);
+int64_t ll_head_rotary_args_size(void);
 
 /* Which kernel and launch shape ll_kv_link would use (no GPU work). */
 typedef struct ll_launch_info {

@@ -12,6 +12,7 @@ There is no fallback: when the library is missing every entry raises
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -23,7 +24,7 @@ LIB_DIR = Path(__file__).resolve().parent / "lib"
 # LEGOLINK_KV_LIBRARY names another build of the library (the host-sanitized
 # one of the CPU sanitizer test).
 LIB_PATH = Path(os.environ.get("LEGOLINK_KV_LIBRARY") or LIB_DIR / "liblegolink_kv.so")
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 # Element type codes (include/legolink_kv.h).
 DTYPE_FLOAT16 = 1
@@ -75,6 +76,8 @@ EXPORTED_SYMBOLS = (
     "ll_repair_attention_noalloc",
     "ll_repair_scratch_bytes",
     "ll_plan_link_runs",
+    "ll_head_rotary",
+    "ll_head_rotary_args_size",
 )
 
 _i64 = ctypes.c_int64
@@ -304,6 +307,54 @@ class RepairAttentionArgs(ctypes.Structure):
     ]
 
 
+class HeadRotaryArgs(ctypes.Structure):
+    """Mirror of ``ll_head_rotary_args``."""
+
+    _fields_ = [
+        ("struct_size", _i64),
+        ("num_tokens", _i64),
+        ("num_q_heads", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("value_head_dim", _i64),
+        ("dtype", _i64),
+        ("query", _ptr),
+        ("query_token_stride", _i64),
+        ("query_head_stride", _i64),
+        ("query_output", _ptr),
+        ("query_output_token_stride", _i64),
+        ("query_output_head_stride", _i64),
+        ("key", _ptr),
+        ("key_token_stride", _i64),
+        ("key_head_stride", _i64),
+        ("key_output", _ptr),
+        ("key_output_token_stride", _i64),
+        ("key_output_head_stride", _i64),
+        ("value", _ptr),
+        ("value_token_stride", _i64),
+        ("value_head_stride", _i64),
+        ("positions", _ptr),
+        ("positions_dtype", _i64),
+        ("cos_sin_cache", _ptr),
+        ("cos_sin_dtype", _i64),
+        ("cos_sin_rows", _i64),
+        ("cos_sin_cols", _i64),
+        ("cos_sin_stride_row", _i64),
+        ("rotary_dim", _i64),
+        ("is_neox_style", _i64),
+        ("query_norm_weight", _ptr),
+        ("key_norm_weight", _ptr),
+        ("norm_weight_dtype", _i64),
+        ("norm_eps", ctypes.c_double),
+        ("key_buffer", _ptr),
+        ("value_buffer", _ptr),
+        ("num_slots", _i64),
+        ("destination_slots", _ptr),
+        ("destination_slots_dtype", _i64),
+        ("skipped_rows", _ptr),
+    ]
+
+
 REPAIR_ITEM_INTS = 86
 REPAIR_ITEM_HEADER = 6  # kv_offset, kv_begin, kv_end, tiles, first pair's head, pair count
 REPAIR_TILE_INTS = 5   # per tile of an item: first query, lowest position, count, partial, key end
@@ -408,6 +459,10 @@ def load_library() -> ctypes.CDLL:
         lib.ll_repair_attention_noalloc.restype = ctypes.c_int
         lib.ll_repair_scratch_bytes.argtypes = []
         lib.ll_repair_scratch_bytes.restype = _i64
+        lib.ll_head_rotary.argtypes = [ctypes.POINTER(HeadRotaryArgs), _ptr]
+        lib.ll_head_rotary.restype = ctypes.c_int
+        lib.ll_head_rotary_args_size.argtypes = []
+        lib.ll_head_rotary_args_size.restype = _i64
         if lib.ll_abi_version() != ABI_VERSION:
             raise NativeLibraryUnavailable(
                 f"{LIB_PATH} has ABI {lib.ll_abi_version()}, expected {ABI_VERSION}; rebuild it"
@@ -416,7 +471,8 @@ def load_library() -> ctypes.CDLL:
                 or lib.ll_kv_scatter_args_size() != ctypes.sizeof(ScatterArgs)
                 or lib.ll_link_maps_args_size() != ctypes.sizeof(LinkMapsArgs)
                 or lib.ll_order_maps_args_size() != ctypes.sizeof(OrderMapsArgs)
-                or lib.ll_repair_attention_args_size() != ctypes.sizeof(RepairAttentionArgs)):
+                or lib.ll_repair_attention_args_size() != ctypes.sizeof(RepairAttentionArgs)
+                or lib.ll_head_rotary_args_size() != ctypes.sizeof(HeadRotaryArgs)):
             raise NativeLibraryUnavailable(f"{LIB_PATH} struct layout differs; rebuild it")
         _lib = lib
         return lib
@@ -456,6 +512,16 @@ def stream_handle(stream, device) -> int:
     tensor's device, so it has an index)."""
 
     return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context with ``device`` current: a launch on its stream needs it, also
+    where the caller's current device is another."""
+
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def kv_link(args: LinkArgs, stream: int) -> None:
@@ -565,3 +631,8 @@ def repair_attention_noalloc(args: RepairAttentionArgs, stream: int) -> None:
 
 def repair_scratch_bytes() -> int:
     return int(load_library().ll_repair_scratch_bytes())
+
+
+def head_rotary(args: HeadRotaryArgs, stream: int) -> None:
+    args.struct_size = ctypes.sizeof(HeadRotaryArgs)
+    _check(load_library().ll_head_rotary(ctypes.byref(args), _ptr(int(stream))))
