@@ -682,6 +682,68 @@ typedef struct ll_head_rotary_args {
 int ll_head_rotary(const ll_head_rotary_args *args, ll_stream_t stream);
 int64_t ll_head_rotary_args_size(void);
 
+/*
+ * Attention of each request's new tokens over its pages of one layer of the
+ * pool (ABI 18): a chunk of a prompt behind what is cached, or the single tokens
+ * of a decode batch.  The reference leaves this to its runtime's attention
+ * backend; it is the link's continuation over the same pool.
+ *
+ * Request r holds the queries [query_starts[r], query_starts[r + 1]) (without
+ * query_starts: query r alone) and kv_lengths[r] keys, those of its own queries
+ * among them and last.  Key j is row page_table[r][j / page_size] * page_size +
+ * j % page_size of the pool (page_size 1: the slots themselves, as in the
+ * reference's req_to_token).  The request's query i of n stands at position p =
+ * kv_lengths[r] - n + i and sees the keys j <= p; query head h reads KV head
+ * h / (num_q_heads / num_kv_heads):
+ *     output[i][h] = sum_j softmax_j(softmax_scale * q . K_j) V_j
+ * with the softmax in fp32, its weights rounded to the KV type for the value
+ * product and the output rounded once.  A query that sees no key gets zeros.
+ *
+ * The lengths, starts and pages are read on the device, so that one captured
+ * call serves any lengths that its shapes hold: lengths are held to [0,
+ * page_table_columns * page_size], starts to [0, num_queries] and to growing
+ * order.  Keys of a page outside the pool are invisible (never read), as is
+ * everything behind a request's length, whatever it holds.  Queries of no
+ * request keep their output rows.
+ *
+ * Workspace: ll_paged_attention_workspace_bytes(args), a bound that follows from
+ * the shapes alone.  Calls that share one must not overlap; nothing in it
+ * outlives the call.  One launch, and a second where a table row holds more than
+ * 128 keys (it joins the parts of requests whose keys were split).
+ */
+typedef struct ll_paged_attention_args {
+  int64_t struct_size;             /* sizeof(ll_paged_attention_args) */
+  const void *query;               /* device kv_dtype [num_queries, num_q_heads, head_dim], 16-byte aligned */
+  int64_t query_token_stride;      /* in elements, multiples of 8; a row's values are dense */
+  int64_t query_head_stride;
+  void *output;                    /* device kv_dtype [num_queries, num_q_heads, head_dim], dense, 16-byte aligned */
+  int64_t num_queries;             /* times query heads per KV head: below 2^30 */
+  const void *key_buffer;          /* device kv_dtype [num_slots, num_kv_heads, head_dim]: one layer */
+  const void *value_buffer;        /* device kv_dtype [num_slots, num_kv_heads, head_dim] */
+  int64_t num_slots;               /* below 2^31; its whole pages are the pool's */
+  int64_t num_q_heads;             /* a multiple of num_kv_heads, at most 65535 */
+  int64_t num_kv_heads;
+  int64_t head_dim;                /* 64, 128 or 256 */
+  int64_t kv_dtype;                /* LL_DTYPE_BFLOAT16 or LL_DTYPE_FLOAT16 */
+  double softmax_scale;            /* positive */
+  const int32_t *page_table;       /* device int32 [num_requests, page_table_columns] */
+  int64_t page_table_stride;       /* of a request's row, in entries */
+  int64_t page_table_columns;      /* times page_size: below 2^30 */
+  int64_t page_size;
+  const void *kv_lengths;          /* device int32/int64 [num_requests] */
+  int64_t kv_lengths_dtype;
+  const void *query_starts;        /* device int32/int64 [num_requests + 1], or NULL: one query a request */
+  int64_t query_starts_dtype;
+  int64_t num_requests;
+  void *workspace;                 /* device, 16-byte aligned (NULL where none is needed) */
+  int64_t workspace_bytes;
+} ll_paged_attention_args;
+
+/* Bytes of workspace that the call needs (negative: an LL_ERR_* code). */
+int64_t ll_paged_attention_workspace_bytes(const ll_paged_attention_args *args);
+int ll_paged_attention(const ll_paged_attention_args *args, ll_stream_t stream);
+int64_t ll_paged_attention_args_size(void);
+
 /* Which kernel and launch shape ll_kv_link would use (no GPU work). */
 typedef struct ll_launch_info {
   int64_t kernel;                  /* LL_KERNEL_VECTOR or LL_KERNEL_GENERIC (ll_kv_link_kernel_name tells

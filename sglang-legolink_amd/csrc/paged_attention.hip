@@ -1,0 +1,832 @@
+// Attention of each request's new tokens over its pages of the KV pool, on
+// gfx950 (MI355X).
+//
+// Request r has n query rows (its last n tokens) and L keys in the pool; query
+// i stands at position p = L - n + i and sees the keys j <= p.  G query heads
+// share a KV head.  For one KV head the (query, head) pairs of a request are
+// the columns of one matrix, token-major: column c is query c / G, head c % G.
+// So single tokens fill G columns of an MFMA and chunks fill every one.
+//
+//   tile   = `columns` neighbouring columns of one request
+//   chunk  = `chunk_keys` neighbouring keys
+//   unit   = (request, tile, chunk); workgroup = (unit, KV head)
+//
+// The lengths are on the device, and no host plan or synchronisation comes
+// before a call: every workgroup reads the requests' lengths, derives the chunk
+// length that cuts the whole call's work into about `target` units, and finds
+// its own unit by a prefix sum.  A tile of one chunk writes its output; the
+// others leave partial results (fp32) that a second launch joins.
+//
+// Per 32 or 64 keys, with S^T = K Q^T and O^T += V^T P^T on MFMAs: K and V rows
+// are gathered by slot straight into LDS; the softmax runs in fp32 with exp2
+// and a maximum that is only raised where a score passes it by 8 (in log2);
+// the probabilities go from the S^T accumulators to the value product rounded
+// to the KV type, V^T through transposed LDS reads.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "attention_device.h"
+#include "legolink_kv.h"
+#include "ll_internal.h"
+
+namespace {
+
+constexpr int kWave = 64;
+constexpr int kPageTile = 64;  // chunk lengths are multiples of this many keys
+constexpr float kSlack = 8.f;  // log2 headroom of the lazily updated softmax maximum
+
+int fail(int code, const char *fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  const int rc = ll_record_error(code, fmt, ap);
+  va_end(ap);
+  return rc;
+}
+
+struct PagedParams {
+  const uint16_t *q;
+  uint16_t *out;
+  const uint16_t *k, *v;
+  const int *pages;
+  const void *kv_lengths, *query_starts;  // query_starts NULL: one query each
+  float *ws;
+  long long q_token, q_head, pages_stride, row_values;  // row_values: of one slot, hkv * D
+  unsigned long long page_magic;
+  double inv_target;
+  int page_shift, page_size, num_pages, max_keys;
+  int num_queries, num_requests, hq, hkv, group;
+  int lengths64, starts64;
+  int min_chunk;  // key tiles
+  int max_units, max_tiles;
+  float scale_log2;
+};
+
+struct Request {
+  int q_start, q_len, kv_len;
+};
+
+__device__ inline long long index_at(const void *values, int is64, int i) {
+  return is64 ? static_cast<const int64_t *>(values)[i] : static_cast<const int32_t *>(values)[i];
+}
+
+// Request r's sizes, held within the call's queries and page table.
+__device__ inline Request request_at(const PagedParams &p, int r) {
+  Request x;
+  if (p.query_starts == nullptr) {
+    x.q_start = r;
+    x.q_len = 1;
+  } else {
+    const long long all = p.num_queries;
+    const long long begin = min(max(index_at(p.query_starts, p.starts64, r), 0ll), all);
+    const long long end = min(max(index_at(p.query_starts, p.starts64, r + 1), begin), all);
+    x.q_start = static_cast<int>(begin);
+    x.q_len = static_cast<int>(end - begin);
+  }
+  x.kv_len = static_cast<int>(min(max(index_at(p.kv_lengths, p.lengths64, r), 0ll), static_cast<long long>(p.max_keys)));
+  return x;
+}
+
+__device__ inline int inclusive_scan(int value, int lane) {
+#pragma unroll
+  for (int step = 1; step < kWave; step *= 2) {
+    const int other = __shfl_up(value, step);
+    if (lane >= step) value += other;
+  }
+  return value;
+}
+
+// What a workgroup has to do: the tile and its request, the chunk of a unit,
+// the tile's first unit and its count of chunks.
+struct Work {
+  Request request;
+  int index;  // of the request; -1: none
+  int tile, chunk, chunk_keys;
+  int first_unit, chunks;  // of the tile
+  int key_end;             // keys that some column of the tile sees
+};
+
+// The request's columns (num_queries * G stays below 2^31).
+__device__ inline int tiles_of(const PagedParams &p, int q_len, int columns) {
+  return (q_len * p.group + columns - 1) / columns;
+}
+
+// Unit `index` of the call (kOfTiles: tile `index`).  Every wave finds it for
+// itself: two passes over the requests, 64 at a time, the first for the call's
+// work in key tiles times column tiles.  With L = max(min_chunk, work / target)
+// key tiles a chunk, the units number at most work / L + tiles <= target +
+// tiles, which the launch holds.
+template <bool kOfTiles>
+__device__ inline Work find_work(const PagedParams &p, int columns, int index) {
+  const int lane = threadIdx.x % kWave;
+  Request mine = Request{0, 0, 0};
+  long long work = 0;
+  for (int r0 = 0; r0 < p.num_requests; r0 += kWave) {
+    Request x = Request{0, 0, 0};
+    if (r0 + lane < p.num_requests) x = request_at(p, r0 + lane);
+    if (r0 == 0) mine = x;
+    work += static_cast<long long>(tiles_of(p, x.q_len, columns)) * ((x.kv_len + kPageTile - 1) / kPageTile);
+  }
+  if (p.num_requests > 1) {
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2) work += __shfl_xor(work, step);
+  } else {
+    work = __shfl(work, 0);
+  }
+  const double share = static_cast<double>(work) * p.inv_target;
+  const int chunk = max(p.min_chunk, static_cast<int>(min(ceil(share - 1e-6), 33554432.0)));  // 2^25 tiles: any length
+
+  Work w;
+  w.index = -1;
+  w.chunk_keys = min(chunk, 33554431) * kPageTile;
+  int units_before = 0, tiles_before = 0;
+  for (int r0 = 0; r0 < p.num_requests; r0 += kWave) {
+    Request x = mine;
+    if (r0 > 0) {
+      x = Request{0, 0, 0};
+      if (r0 + lane < p.num_requests) x = request_at(p, r0 + lane);
+    }
+    const int tiles = tiles_of(p, x.q_len, columns);
+    const int key_tiles = (x.kv_len + kPageTile - 1) / kPageTile;
+    const int chunks = max(1, (key_tiles + chunk - 1) / chunk);
+    int units_to = tiles * chunks, tiles_to = tiles;
+    if (p.num_requests > 1) {
+      units_to = inclusive_scan(units_to, lane);
+      if constexpr (kOfTiles) tiles_to = inclusive_scan(tiles_to, lane);
+    }
+    const int reached = kOfTiles ? tiles_before + tiles_to : units_before + units_to;
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(reached > index && r0 + lane < p.num_requests);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      w.index = r0 + at;
+      w.request.q_start = __builtin_amdgcn_readlane(x.q_start, at);
+      w.request.q_len = __builtin_amdgcn_readlane(x.q_len, at);
+      w.request.kv_len = __builtin_amdgcn_readlane(x.kv_len, at);
+      const int own_tiles = __builtin_amdgcn_readlane(tiles, at);
+      const int own_chunks = __builtin_amdgcn_readlane(chunks, at);
+      const int first_unit = units_before + __builtin_amdgcn_readlane(units_to, at) - own_tiles * own_chunks;
+      if constexpr (kOfTiles) {
+        w.tile = index - (tiles_before + __builtin_amdgcn_readlane(tiles_to, at) - own_tiles);
+        w.chunk = 0;
+      } else {
+        w.tile = (index - first_unit) / own_chunks;
+        w.chunk = (index - first_unit) - w.tile * own_chunks;
+      }
+      w.first_unit = first_unit + w.tile * own_chunks;
+      // The tile's last query and its position bound the keys.
+      const int last_query = min(w.request.q_len - 1, ((w.tile + 1) * columns - 1) / p.group);
+      w.key_end = max(0, w.request.kv_len - w.request.q_len + last_query + 1);
+      w.chunks = max(1, (w.key_end + w.chunk_keys - 1) / w.chunk_keys);
+      break;
+    }
+    units_before += __builtin_amdgcn_readlane(units_to, kWave - 1);
+    if constexpr (kOfTiles) tiles_before += __builtin_amdgcn_readlane(tiles_to, kWave - 1);
+  }
+  return w;
+}
+
+// Partial result of a unit's KV head: `columns` rows of D floats (the sum of
+// the weighted values, unnormalised), then (maximum, sum) pairs.
+template <int D>
+__device__ inline float *partial_of(const PagedParams &p, int columns, int unit, int head) {
+  return p.ws + (static_cast<long long>(unit) * p.hkv + head) * columns * (D + 2);
+}
+
+__device__ inline uint16_t *output_row(const PagedParams &p, const Work &w, int head, int column, int dim) {
+  const int token = column / p.group;
+  const int h = head * p.group + (column - token * p.group);
+  return p.out + ((static_cast<long long>(w.request.q_start) + token) * p.hq + h) * dim;
+}
+
+// A value product in which a column must not meet the infinities and NaN of
+// rows that it does not see (their probability is 0, and 0 * inf is NaN): the
+// rows' finite values, and each kind of the others as ones whose weight says
+// whether the column sees any.
+template <typename E>
+__device__ inline bool any_nonfinite(u32x4 bits) {
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    any = any || (bits[i] & E::kExponent) == E::kExponent || ((bits[i] >> 16) & E::kExponent) == E::kExponent;
+  return any;
+}
+
+enum { kFinite, kPlusInfinity, kMinusInfinity, kNan };
+template <typename E>
+__device__ inline uint32_t only(uint32_t pair, int kind) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t x = (pair >> (16 * half)) & 0xffffu;
+    const bool special = (x & E::kExponent) == E::kExponent;
+    const bool nan = special && (x & E::kFraction) != 0;
+    const int is = !special ? kFinite : nan ? kNan : (x >> 15) != 0 ? kMinusInfinity : kPlusInfinity;
+    const uint32_t y = is != kind ? 0u : kind == kFinite ? x : E::kOne;
+    out |= y << (16 * half);
+  }
+  return out;
+}
+
+template <typename E, typename Acc, typename Product>
+__device__ inline Acc guarded_product(u32x4 rows, Acc acc, Product product) {
+  auto part = [&](int kind) {
+    u32x4 bits;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits[i] = only<E>(rows[i], kind);
+    return __builtin_bit_cast(typename E::frag, bits);
+  };
+  acc = product(part(kFinite), acc);
+  Acc zero;
+  constexpr int kValues = sizeof(Acc) / sizeof(float);
+#pragma unroll
+  for (int i = 0; i < kValues; ++i) zero[i] = 0.f;
+  const Acc plus = product(part(kPlusInfinity), zero);
+  const Acc minus = product(part(kMinusInfinity), zero);
+  const Acc nan = product(part(kNan), zero);
+#pragma unroll
+  for (int i = 0; i < kValues; ++i) {
+    if (plus[i] > 0.f) acc[i] += INFINITY;
+    if (minus[i] > 0.f) acc[i] -= INFINITY;
+    if (nan[i] > 0.f) acc[i] = NAN;
+  }
+  return acc;
+}
+
+// Column statistics across the four lane groups of a 16-column MFMA.
+__device__ inline float max_of_groups(float x) {
+  unsigned a = __builtin_bit_cast(unsigned, x), b = a;
+  permlane16_swap(a, b);
+  x = max_f32(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+  a = b = __builtin_bit_cast(unsigned, x);
+  permlane32_swap(a, b);
+  return max_f32(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ inline float sum_of_groups(float x) {
+  unsigned a = __builtin_bit_cast(unsigned, x), b = a;
+  permlane16_swap(a, b);
+  x = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  a = b = __builtin_bit_cast(unsigned, x);
+  permlane32_swap(a, b);
+  return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+template <int n>
+__device__ inline void wait_vm() {
+  __builtin_amdgcn_s_waitcnt(0xF70 | (n & 15) | ((n >> 4) << 14));
+}
+
+// Few columns (16 kTiles): single tokens and short chunks, bound by reading
+// the keys and values once.  The waves of a workgroup take turns at its 32-key
+// subtiles, each through an LDS ring of its own (no barriers: a wave waits for
+// its own gathers alone), and join their results at the end.  v_mfma_f32_16x16x32,
+// lane layouts: A and B lane l element e -> row / column l % 16, k = 8 (l / 16)
+// + e; accumulator register r -> row 4 (l / 16) + r, column l % 16.  The value
+// product's k order is the scores' register order: k = 8 g + e is token 4 g + e
+// (e < 4) or 16 + 4 g + e - 4.
+// LDS rows are token-major with their 16-byte chunks swizzled by token, so that
+// the 16 lanes of a K read (16 tokens, one chunk) and the 32 lanes of a
+// transposed V read (8 tokens x 32 bytes) each cover the 64 banks once.
+template <int D>
+struct Narrow {
+  static constexpr int kKeys = 32;
+  static constexpr int kWaves = D == 256 ? 2 : 4;
+  static constexpr int kStages = D == 64 ? 4 : 2;  // 128 KB of rings
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kHalf = kKeys * kRowBytes;  // a subtile's K or V rows
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kChunksPerRow = D / 8;
+  static constexpr int kGathers = kHalf / (16 * kWave);  // of K and of V, per subtile
+  static constexpr int kList = 4096;                     // slots held at a time
+  __device__ static int k_swizzle(int t) { return D >= 128 ? t % 16 : (t / 2) % 8; }
+  __device__ static int v_swizzle(int t) { return D >= 128 ? 2 * (t % 8) : 2 * ((t / 2) % 4); }
+};
+
+template <int D, typename E, int kTiles>
+__global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const PagedParams p) {
+  typedef Narrow<D> N;
+  typedef typename E::frag frag;
+  constexpr int kColumns = 16 * kTiles;
+  constexpr int kKSteps = D / 32;
+  constexpr int kBlocks = D / 16;
+  constexpr int kPitch = D + 4;  // floats of a joined row: 16 lanes' 16-byte writes meet 64 banks
+  static_assert(N::kWaves * 16 * kPitch * 4 <= N::kWaves * N::kRing, "a tile's results fit the rings");
+  __shared__ __attribute__((aligned(16))) unsigned char rings[N::kWaves * N::kRing];
+  __shared__ int slot_list[N::kList];
+  __shared__ float stats[N::kWaves][kColumns][2];
+
+  const int head = blockIdx.x % p.hkv;
+  const int unit = blockIdx.x / p.hkv;
+  const Work w = find_work<false>(p, kColumns, unit);
+  if (w.index < 0 || w.chunk >= w.chunks) return;
+  const int key_begin = w.chunk * w.chunk_keys;  // below the tile's key_end, or 0
+  int key_end = key_begin + min(w.chunk_keys, w.key_end - key_begin);
+  if (p.num_pages == 0) key_end = key_begin;  // no row that may be read
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid % kWave;
+  const int g = lane / 16;
+  const int col = lane % 16;
+  unsigned char *ring = rings + wave * N::kRing;
+
+  // The lane's queries: one column of each 16-column tile.
+  frag qf[kTiles][kKSteps];
+  int pos[kTiles];
+  int seen_by_all = 0x7fffffff;  // keys below it are visible to every column
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    const int column = w.tile * kColumns + 16 * n + col;
+    const int token = column / p.group;
+    const bool exists = token < w.request.q_len;
+    const int h = head * p.group + (column - token * p.group);
+    pos[n] = exists ? w.request.kv_len - w.request.q_len + token : -1;
+    const uint16_t *row = p.q + (static_cast<long long>(w.request.q_start) + token) * p.q_token + h * p.q_head + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < kKSteps; ++ks) {
+      u32x4 bits = u32x4{0u, 0u, 0u, 0u};
+      if (exists) bits = *reinterpret_cast<const u32x4 *>(row + 32 * ks);
+      qf[n][ks] = __builtin_bit_cast(frag, bits);
+    }
+  }
+  seen_by_all = w.request.kv_len - w.request.q_len + (w.tile * kColumns) / p.group + 1;  // the first column's
+
+  float m[kTiles], l[kTiles];
+  f32x4 o[kTiles][kBlocks];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) o[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale_log2 = p.scale_log2;
+  const float slack = kSlack / scale_log2;
+
+  // The lane's share of a gather: its 16 bytes of instruction j hold chunk
+  // (64 j + lane) of the subtile's rows in LDS order.
+  const uint16_t *k_base = p.k + static_cast<long long>(head) * D;
+  const uint16_t *v_base = p.v + static_cast<long long>(head) * D;
+  auto gather = [&](int sub, int stage) {
+    unsigned char *dst = ring + stage * N::kStage;
+#pragma unroll
+    for (int j = 0; j < N::kGathers; ++j) {
+      const int at = j * kWave + lane;
+      const int token = at / N::kChunksPerRow;
+      const int place = at % N::kChunksPerRow;
+      const int slot = max(slot_list[sub * N::kKeys + token], 0);
+      const long long row = slot * p.row_values;
+      dma_pair(k_base + row + 8 * (place ^ N::k_swizzle(token)), dst + j * 16 * kWave,
+               v_base + row + 8 * (place ^ N::v_swizzle(token)), dst + N::kHalf + j * 16 * kWave);
+    }
+  };
+  // Offsets of the lane's fragments within a stage.
+  int k_off[kKSteps];
+#pragma unroll
+  for (int ks = 0; ks < kKSteps; ++ks) k_off[ks] = col * N::kRowBytes + (((4 * ks + g) ^ N::k_swizzle(col)) * 16);
+  const int v_token = 4 * g + col / 4;
+  int v_off[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b)
+    v_off[b] = N::kHalf + v_token * N::kRowBytes + (((2 * b + (col % 4) / 2) ^ N::v_swizzle(v_token)) * 16) + 8 * (col % 2);
+  const unsigned ring_lds =
+      static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char *)ring));
+
+  const int *pages = p.pages + static_cast<long long>(w.index) * p.pages_stride;
+  for (int list_begin = key_begin; list_begin < key_end; list_begin += N::kList) {
+    const int listed = min(key_end - list_begin, N::kList);
+    const int subs = (listed + N::kKeys - 1) / N::kKeys;
+    __syncthreads();  // every wave is past the former list
+    for (int i = tid; i < subs * N::kKeys; i += N::kThreads) {
+      const unsigned key = static_cast<unsigned>(list_begin + min(i, listed - 1));
+      const unsigned page = static_cast<unsigned>((key * p.page_magic) >> p.page_shift);
+      const int entry = pages[page];
+      const bool valid = i < listed && static_cast<unsigned>(entry) < static_cast<unsigned>(p.num_pages);
+      slot_list[i] = valid ? entry * p.page_size + static_cast<int>(key - page * p.page_size) : -1;
+    }
+    // The compiler does not count the gathers: nothing that it waits for in the
+    // loop below may be left in flight.
+    wait_vm<0>();
+    __syncthreads();
+
+#pragma unroll
+    for (int s = 0; s < N::kStages; ++s)
+      if (wave + s * N::kWaves < subs) gather(wave + s * N::kWaves, s);
+    int stage = 0;
+    for (int sub = wave; sub < subs; sub += N::kWaves) {
+      const int key0 = list_begin + sub * N::kKeys;
+      const int own_slot = slot_list[sub * N::kKeys + lane % N::kKeys];
+      const unsigned valid =
+          static_cast<unsigned>(__builtin_amdgcn_ballot_w64(own_slot >= 0));  // both halves hold the same keys
+      // This stage's gathers are complete when at most the later stages' are outstanding.
+      const int later = min(N::kStages - 1, (subs - 1 - sub) / N::kWaves);
+      if (N::kStages == 4 && later == 3) wait_vm<3 * 2 * N::kGathers % 64>();
+      else if (N::kStages == 4 && later == 2) wait_vm<2 * 2 * N::kGathers % 64>();
+      else if (later >= 1) wait_vm<2 * N::kGathers>();
+      else wait_vm<0>();
+      asm volatile("" ::: "memory");
+      unsigned char *rows = ring + stage * N::kStage;
+      const bool whole = valid == 0xffffffffu && key0 + N::kKeys <= seen_by_all;
+      if (valid != 0xffffffffu) {
+        // Rows that no column sees may hold anything: zeros in their place.
+        for (int c = lane; c < N::kKeys * N::kChunksPerRow; c += kWave)
+          if (((valid >> (c / N::kChunksPerRow)) & 1u) == 0)
+            *reinterpret_cast<u32x4 *>(rows + N::kHalf + c * 16) = u32x4{0u, 0u, 0u, 0u};
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+      }
+
+      f32x4 s[kTiles][2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) s[n][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < kKSteps; ++ks) {
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          const frag kf = *reinterpret_cast<const frag *>(rows + k_off[ks] + rb * 16 * N::kRowBytes);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) s[n][rb] = E::mfma16(kf, qf[n][ks], s[n][rb]);
+        }
+      }
+      frag pb[kTiles];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        if (!whole) {
+#pragma unroll
+          for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int rel = 16 * rb + 4 * g + r;
+              const bool visible = ((valid >> rel) & 1u) != 0 && key0 + rel <= pos[n];
+              s[n][rb][r] = visible ? s[n][rb][r] : -INFINITY;
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[n][rb][r]);
+        top = max_of_groups(top);
+        const bool raise = top > m[n] + slack;
+        const float m_new = raise ? top : m[n];
+        const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[n][rb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][rb][r], scale_log2, bias));
+        if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+          const float alpha = raise ? __builtin_amdgcn_exp2f((m[n] - m_new) * scale_log2) : 1.f;
+          l[n] *= alpha;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) o[n][b] *= alpha;
+        }
+        m[n] = m_new;
+        u32x4 bits;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bits[j] = E::pack(s[n][j / 2][2 * (j % 2)], s[n][j / 2][2 * (j % 2) + 1]);
+          l[n] = E::dot2_ones(bits[j], l[n]);  // the weights that the value product sees
+        }
+        pb[n] = __builtin_bit_cast(frag, bits);
+      }
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const unsigned at = ring_lds + stage * N::kStage + v_off[b];
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at)));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at + 16 * N::kRowBytes)));
+        u32x4 va;
+        va[0] = __builtin_bit_cast(u32x2, lo)[0];
+        va[1] = __builtin_bit_cast(u32x2, lo)[1];
+        va[2] = __builtin_bit_cast(u32x2, hi)[0];
+        va[3] = __builtin_bit_cast(u32x2, hi)[1];
+        if (!whole && __builtin_amdgcn_ballot_w64(any_nonfinite<E>(va)) != 0) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+            o[n][b] = guarded_product<E>(va, o[n][b], [&](frag a, f32x4 acc) { return E::mfma16(a, pb[n], acc); });
+        } else {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) o[n][b] = E::mfma16(__builtin_bit_cast(frag, va), pb[n], o[n][b]);
+        }
+      }
+      // The stage's reads are done: the gather kStages turns ahead takes it.
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (sub + N::kStages * N::kWaves < subs) gather(sub + N::kStages * N::kWaves, stage);
+      stage = stage + 1 == N::kStages ? 0 : stage + 1;
+    }
+  }
+
+  // The waves' results joined, 16 columns at a time.
+  const bool direct = w.chunks == 1;
+  float *partial = direct ? nullptr : partial_of<D>(p, kColumns, unit, head);
+  float *joined = reinterpret_cast<float *>(rings);
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    __syncthreads();  // the rings (or the tile before) are read
+    const float total = sum_of_groups(l[n]);
+    if (g == 0) {
+      stats[wave][16 * n + col][0] = m[n] == -INFINITY ? -INFINITY : m[n] * scale_log2;
+      stats[wave][16 * n + col][1] = total;
+    }
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+      *reinterpret_cast<f32x4 *>(joined + (wave * 16 + col) * kPitch + 16 * b + 4 * g) = o[n][b];
+    __syncthreads();
+    for (int i = tid; i < 16 * (D / 4); i += N::kThreads) {
+      const int c = i / (D / 4);
+      const int quad = i % (D / 4);
+      const int column = w.tile * kColumns + 16 * n + c;
+      if (column / p.group >= w.request.q_len) continue;
+      float top = stats[0][16 * n + c][0];
+#pragma unroll
+      for (int v = 1; v < N::kWaves; ++v) top = fmaxf(top, stats[v][16 * n + c][0]);
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < N::kWaves; ++v) {
+        const float own = stats[v][16 * n + c][0];
+        const float weight = own == -INFINITY && top == -INFINITY ? 1.f : exp2f(own - top);
+        sum += weight * stats[v][16 * n + c][1];
+        acc += weight * *reinterpret_cast<const f32x4 *>(joined + (v * 16 + c) * kPitch + 4 * quad);
+      }
+      if (direct) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+        u32x2 packed;
+        packed[0] = E::pack(acc[0] * inv, acc[1] * inv);
+        packed[1] = E::pack(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<u32x2 *>(output_row(p, w, head, column, D) + 4 * quad) = packed;
+      } else {
+        *reinterpret_cast<f32x4 *>(partial + (16 * n + c) * D + 4 * quad) = acc;
+        if (quad == 0) {
+          partial[kColumns * D + 2 * (16 * n + c)] = top;
+          partial[kColumns * D + 2 * (16 * n + c) + 1] = sum;
+        }
+      }
+    }
+  }
+}
+
+// Joins the partial results of tiles of more than one chunk.  kSplit waves a
+// column take turns at its chunks: 4 where few tiles leave many partials each
+// (their latency adds up), else 1.
+template <int D, typename E, int kSplit>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p, int columns) {
+  constexpr int kPer = D / kWave;  // values of a lane
+  constexpr int kBatch = 4;        // partials whose loads are in flight together
+  constexpr int kColumnsPerGroup = 4 / kSplit;
+  const int groups = columns / kColumnsPerGroup;
+  const int tile_head = blockIdx.x / groups;
+  const int head = tile_head % p.hkv;
+  const Work w = find_work<true>(p, columns, tile_head / p.hkv);
+  if (w.index < 0 || w.chunks <= 1 || w.first_unit < 0 || w.first_unit + w.chunks > p.max_units) return;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int c = (blockIdx.x % groups) * kColumnsPerGroup + wave / kSplit;
+  const int column = w.tile * columns + c;
+  const bool exists = column / p.group < w.request.q_len;
+  if (kSplit == 1 && !exists) return;
+
+  float top = -INFINITY, sum = 0.f;
+  float acc[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+  for (int s0 = (wave % kSplit) * kBatch; s0 < w.chunks; s0 += kSplit * kBatch) {
+    float tops[kBatch], sums[kBatch], rows[kBatch][kPer];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float *part = partial_of<D>(p, columns, w.first_unit + min(s0 + i, w.chunks - 1), head);
+      tops[i] = exists ? part[columns * D + 2 * c] : -INFINITY;
+      sums[i] = exists ? part[columns * D + 2 * c + 1] : 0.f;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) rows[i][d] = exists ? part[c * D + lane * kPer + d] : 0.f;
+    }
+    float high = top;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (s0 + i < w.chunks) high = fmaxf(high, tops[i]);
+    const float old = top == -INFINITY ? 0.f : exp2f(top - high);
+    sum *= top == -INFINITY && high == -INFINITY ? 1.f : old;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) acc[d] *= top == -INFINITY && high == -INFINITY ? 1.f : old;
+    top = high;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (s0 + i >= w.chunks) continue;
+      const float weight = tops[i] == -INFINITY && top == -INFINITY ? 1.f : exp2f(tops[i] - top);
+      sum += weight * sums[i];
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) acc[d] += weight * rows[i][d];
+    }
+  }
+  if constexpr (kSplit > 1) {
+    __shared__ float tops[kSplit], sums[kSplit], parts[kSplit][D];
+    if (lane == 0) {
+      tops[wave] = top;
+      sums[wave] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) parts[wave][lane * kPer + d] = acc[d];
+    __syncthreads();
+    if (wave > 0 || !exists) return;
+    float high = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < kSplit; ++v) high = fmaxf(high, tops[v]);
+    sum = 0.f;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) acc[d] = 0.f;
+#pragma unroll
+    for (int v = 0; v < kSplit; ++v) {
+      const float weight = tops[v] == -INFINITY && high == -INFINITY ? 1.f : exp2f(tops[v] - high);
+      sum += weight * sums[v];
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) acc[d] += weight * parts[v][lane * kPer + d];
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t *dst = output_row(p, w, head, column, D) + lane * kPer;
+  if constexpr (kPer == 1) {
+    dst[0] = static_cast<uint16_t>(E::pack(acc[0] * inv, 0.f));
+  } else {
+#pragma unroll
+    for (int d = 0; d < kPer; d += 2)
+      *reinterpret_cast<uint32_t *>(dst + d) = E::pack(acc[d] * inv, acc[d + 1] * inv);
+  }
+}
+
+// How a call is launched: known from sizes that the host has.
+struct Launch {
+  int columns;
+  int max_tiles, max_units, target, min_chunk;
+  bool splits;
+  long long ws_floats;
+};
+
+constexpr int kComputeUnits = 256;  // MI355X
+
+Launch plan_launch(const ll_paged_attention_args *a) {
+  Launch x;
+  const long long group = a->num_q_heads / a->num_kv_heads;
+  const long long queries = a->num_queries, requests = a->num_requests;
+  // Columns by the average request: whole chunks in as few tiles as they fill.
+  const long long average = queries == 0 ? 1 : (queries + requests - 1) / requests;
+  const long long wanted = average * group;
+  x.columns = wanted <= 16 ? 16 : wanted <= 32 || a->head_dim == 256 ? 32 : 64;
+  const long long tiles = a->query_starts == nullptr
+                              ? requests * ((group + x.columns - 1) / x.columns)
+                              : queries * group / x.columns + requests;
+  x.max_tiles = static_cast<int>(std::min(tiles, 0x7fffffffll));
+  x.min_chunk = 2;
+  x.target = std::max(1, 2 * kComputeUnits / static_cast<int>(a->num_kv_heads));
+  const long long max_keys = a->page_table_columns * a->page_size;
+  x.splits = max_keys > x.min_chunk * kPageTile;
+  const long long units = tiles + (x.splits ? x.target + 1 : 0);
+  x.max_units = static_cast<int>(std::min(units, 0x7fffffffll));
+  x.ws_floats = x.splits ? units * a->num_kv_heads * x.columns * (a->head_dim + 2) : 0;
+  return x;
+}
+
+bool aligned(const void *p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+bool index_code(int64_t dtype) { return dtype == LL_DTYPE_INT32 || dtype == LL_DTYPE_INT64; }
+
+int check_args(const ll_paged_attention_args *a) {
+  if (a == nullptr) return fail(LL_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->struct_size != static_cast<int64_t>(sizeof(ll_paged_attention_args)))
+    return fail(LL_ERR_INVALID_ARGUMENT, "struct_size %lld, expected %lld", static_cast<long long>(a->struct_size),
+                static_cast<long long>(sizeof(ll_paged_attention_args)));
+  if (a->num_q_heads < 1 || a->num_kv_heads < 1 || a->num_q_heads > 65535 || a->num_q_heads % a->num_kv_heads != 0)
+    return fail(LL_ERR_KV_HEAD_LAYOUT_MISMATCH, "num_q_heads must be a multiple of num_kv_heads, at most 65535");
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+    return fail(LL_ERR_HEAD_DIMENSION_OUT_OF_RANGE, "head_dim must be 64, 128 or 256");
+  if (a->kv_dtype != LL_DTYPE_FLOAT16 && a->kv_dtype != LL_DTYPE_BFLOAT16)
+    return fail(LL_ERR_FP16_OR_BF16_REQUIRED, "kv_dtype must be fp16 or bf16");
+  if (!(a->softmax_scale > 0.0) || !(a->softmax_scale < 1e30))
+    return fail(LL_ERR_INVALID_ARGUMENT, "softmax_scale must be positive and finite");
+  const long long group = a->num_q_heads / a->num_kv_heads;
+  if (a->num_queries < 0 || a->num_requests < 0 || a->num_requests > 0x3fffffff ||
+      a->num_queries > 0x3fffffff / group)
+    return fail(LL_ERR_INVALID_ARGUMENT, "num_queries and num_requests must not be negative and stay below 2^30 "
+                "(queries times query heads per KV head)");
+  if (a->query_starts == nullptr && a->num_queries != a->num_requests)
+    return fail(LL_ERR_INVALID_ARGUMENT, "without query_starts every request has one query");
+  if (a->query_starts != nullptr && !index_code(a->query_starts_dtype))
+    return fail(LL_ERR_INTEGER_TOKEN_MAPS_REQUIRED, "query_starts dtype");
+  if (!index_code(a->kv_lengths_dtype)) return fail(LL_ERR_INTEGER_TOKEN_MAPS_REQUIRED, "kv_lengths dtype");
+  if (a->page_size < 1 || a->page_size > 0x3fffffff || a->page_table_columns < 0 ||
+      a->page_table_columns > 0x3fffffff / a->page_size)
+    return fail(LL_ERR_INVALID_ARGUMENT, "page_size must be positive and a table row hold fewer than 2^30 keys");
+  if (a->page_table_stride < 0) return fail(LL_ERR_INVALID_ARGUMENT, "page_table_stride is negative");
+  if (a->num_slots < 0 || a->num_slots > 0x7fffffff)
+    return fail(LL_ERR_INVALID_ARGUMENT, "num_slots must be in [0, 2^31)");
+  if (a->query_token_stride % 8 != 0 || a->query_head_stride % 8 != 0)
+    return fail(LL_ERR_INVALID_ARGUMENT, "query strides must be multiples of 8 values");
+  if (a->num_queries == 0 || a->num_requests == 0) return LL_OK;
+  if (a->query == nullptr || a->output == nullptr || a->kv_lengths == nullptr)
+    return fail(LL_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
+  if (a->num_slots > 0 && (a->key_buffer == nullptr || a->value_buffer == nullptr))
+    return fail(LL_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
+  if (a->page_table_columns > 0 && a->page_table == nullptr)
+    return fail(LL_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
+  if (!aligned(a->query, 16) || !aligned(a->output, 16) || !aligned(a->key_buffer, 16) ||
+      !aligned(a->value_buffer, 16))
+    return fail(LL_ERR_INVALID_ARGUMENT, "query, output and KV buffers must be 16-byte aligned");
+  const Launch x = plan_launch(a);
+  // A launch holds fewer than 2^32 threads.
+  if (static_cast<long long>(x.max_units) * a->num_kv_heads > 0xffffffll ||
+      static_cast<long long>(x.max_tiles) * a->num_kv_heads * x.columns > 0xffffffll)
+    return fail(LL_ERR_INVALID_ARGUMENT, "too many queries for one launch");
+  return LL_OK;
+}
+
+template <int D, typename E>
+void launch_narrow(const PagedParams &p, const Launch &x, unsigned grid, hipStream_t s) {
+  constexpr int kThreads = Narrow<D>::kThreads;
+  if (x.columns == 16) paged_narrow_kernel<D, E, 1><<<grid, kThreads, 0, s>>>(p);
+  else if (x.columns == 32) paged_narrow_kernel<D, E, 2><<<grid, kThreads, 0, s>>>(p);
+  else if constexpr (D != 256) paged_narrow_kernel<D, E, 4><<<grid, kThreads, 0, s>>>(p);
+}
+
+template <int D, typename E>
+int launch_all(const PagedParams &p, const Launch &x, hipStream_t s) {
+  launch_narrow<D, E>(p, x, static_cast<unsigned>(x.max_units) * static_cast<unsigned>(p.hkv), s);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  if (!x.splits) return LL_OK;
+  const unsigned tile_heads = static_cast<unsigned>(x.max_tiles) * static_cast<unsigned>(p.hkv);
+  const unsigned columns = static_cast<unsigned>(x.columns);
+  if (x.target >= 8 * x.max_tiles) paged_combine_kernel<D, E, 4><<<tile_heads * columns, 256, 0, s>>>(p, x.columns);
+  else paged_combine_kernel<D, E, 1><<<tile_heads * (columns / 4), 256, 0, s>>>(p, x.columns);
+  err = hipGetLastError();
+  if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return LL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ll_paged_attention_args_size(void) { return static_cast<int64_t>(sizeof(ll_paged_attention_args)); }
+
+int64_t ll_paged_attention_workspace_bytes(const ll_paged_attention_args *a) {
+  const int rc = check_args(a);
+  if (rc != LL_OK) return rc;
+  if (a->num_queries == 0 || a->num_requests == 0) return 0;
+  return plan_launch(a).ws_floats * 4;
+}
+
+int ll_paged_attention(const ll_paged_attention_args *a, ll_stream_t stream) {
+  const int rc = check_args(a);
+  if (rc != LL_OK || a->num_queries == 0 || a->num_requests == 0) return rc;
+  const Launch x = plan_launch(a);
+  if (x.splits && (a->workspace == nullptr || a->workspace_bytes < x.ws_floats * 4 || !aligned(a->workspace, 16)))
+    return fail(LL_ERR_INVALID_ARGUMENT, "the call needs a 16-byte aligned workspace of %lld bytes",
+                static_cast<long long>(x.ws_floats * 4));
+  PagedParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = static_cast<const uint16_t *>(a->query);
+  p.out = static_cast<uint16_t *>(a->output);
+  p.k = static_cast<const uint16_t *>(a->key_buffer);
+  p.v = static_cast<const uint16_t *>(a->value_buffer);
+  p.pages = static_cast<const int *>(a->page_table);
+  p.kv_lengths = a->kv_lengths;
+  p.query_starts = a->query_starts;
+  p.ws = static_cast<float *>(a->workspace);
+  p.q_token = a->query_token_stride;
+  p.q_head = a->query_head_stride;
+  p.pages_stride = a->page_table_stride;
+  p.row_values = a->num_kv_heads * a->head_dim;
+  // key / page_size = key * magic >> shift for every key below 2^31: magic
+  // exceeds 2^shift / page_size by at most 1, and 2^(shift - 31) >= page_size.
+  int bits = 0;
+  while ((1ll << bits) < a->page_size) ++bits;
+  p.page_shift = 31 + bits;
+  p.page_magic = (1ull << p.page_shift) / static_cast<unsigned long long>(a->page_size) + 1;
+  p.page_size = static_cast<int>(a->page_size);
+  p.num_pages = static_cast<int>(a->num_slots / a->page_size);
+  p.max_keys = static_cast<int>(a->page_table_columns * a->page_size);
+  p.num_queries = static_cast<int>(a->num_queries);
+  p.num_requests = static_cast<int>(a->num_requests);
+  p.hq = static_cast<int>(a->num_q_heads);
+  p.hkv = static_cast<int>(a->num_kv_heads);
+  p.group = p.hq / p.hkv;
+  p.lengths64 = a->kv_lengths_dtype == LL_DTYPE_INT64 ? 1 : 0;
+  p.starts64 = a->query_starts_dtype == LL_DTYPE_INT64 ? 1 : 0;
+  p.min_chunk = x.splits ? x.min_chunk : 33554431;  // one chunk of any length
+  p.inv_target = 1.0 / x.target;
+  p.max_units = x.max_units;
+  p.max_tiles = x.max_tiles;
+  p.scale_log2 = static_cast<float>(a->softmax_scale * 1.4426950408889634);  // log2(e)
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool f16 = a->kv_dtype == LL_DTYPE_FLOAT16;
+  if (a->head_dim == 64) return f16 ? launch_all<64, F16>(p, x, s) : launch_all<64, Bf16>(p, x, s);
+  if (a->head_dim == 128) return f16 ? launch_all<128, F16>(p, x, s) : launch_all<128, Bf16>(p, x, s);
+  return f16 ? launch_all<256, F16>(p, x, s) : launch_all<256, Bf16>(p, x, s);
+}
+
+}  // extern "C"

@@ -78,6 +78,9 @@ EXPORTED_SYMBOLS = (
     "ll_plan_link_runs",
     "ll_head_rotary",
     "ll_head_rotary_args_size",
+    "ll_paged_attention",
+    "ll_paged_attention_workspace_bytes",
+    "ll_paged_attention_args_size",
 )
 
 _i64 = ctypes.c_int64
@@ -355,6 +358,38 @@ class HeadRotaryArgs(ctypes.Structure):
     ]
 
 
+class PagedAttentionArgs(ctypes.Structure):
+    """Mirror of ``ll_paged_attention_args``."""
+
+    _fields_ = [
+        ("struct_size", _i64),
+        ("query", _ptr),
+        ("query_token_stride", _i64),
+        ("query_head_stride", _i64),
+        ("output", _ptr),
+        ("num_queries", _i64),
+        ("key_buffer", _ptr),
+        ("value_buffer", _ptr),
+        ("num_slots", _i64),
+        ("num_q_heads", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+        ("kv_dtype", _i64),
+        ("softmax_scale", ctypes.c_double),
+        ("page_table", _ptr),
+        ("page_table_stride", _i64),
+        ("page_table_columns", _i64),
+        ("page_size", _i64),
+        ("kv_lengths", _ptr),
+        ("kv_lengths_dtype", _i64),
+        ("query_starts", _ptr),
+        ("query_starts_dtype", _i64),
+        ("num_requests", _i64),
+        ("workspace", _ptr),
+        ("workspace_bytes", _i64),
+    ]
+
+
 REPAIR_ITEM_INTS = 86
 REPAIR_ITEM_HEADER = 6  # kv_offset, kv_begin, kv_end, tiles, first pair's head, pair count
 REPAIR_TILE_INTS = 5   # per tile of an item: first query, lowest position, count, partial, key end
@@ -463,6 +498,12 @@ def load_library() -> ctypes.CDLL:
         lib.ll_head_rotary.restype = ctypes.c_int
         lib.ll_head_rotary_args_size.argtypes = []
         lib.ll_head_rotary_args_size.restype = _i64
+        lib.ll_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), _ptr]
+        lib.ll_paged_attention.restype = ctypes.c_int
+        lib.ll_paged_attention_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttentionArgs)]
+        lib.ll_paged_attention_workspace_bytes.restype = _i64
+        lib.ll_paged_attention_args_size.argtypes = []
+        lib.ll_paged_attention_args_size.restype = _i64
         if lib.ll_abi_version() != ABI_VERSION:
             raise NativeLibraryUnavailable(
                 f"{LIB_PATH} has ABI {lib.ll_abi_version()}, expected {ABI_VERSION}; rebuild it"
@@ -472,7 +513,8 @@ def load_library() -> ctypes.CDLL:
                 or lib.ll_link_maps_args_size() != ctypes.sizeof(LinkMapsArgs)
                 or lib.ll_order_maps_args_size() != ctypes.sizeof(OrderMapsArgs)
                 or lib.ll_repair_attention_args_size() != ctypes.sizeof(RepairAttentionArgs)
-                or lib.ll_head_rotary_args_size() != ctypes.sizeof(HeadRotaryArgs)):
+                or lib.ll_head_rotary_args_size() != ctypes.sizeof(HeadRotaryArgs)
+                or lib.ll_paged_attention_args_size() != ctypes.sizeof(PagedAttentionArgs)):
             raise NativeLibraryUnavailable(f"{LIB_PATH} struct layout differs; rebuild it")
         _lib = lib
         return lib
@@ -636,3 +678,15 @@ def repair_scratch_bytes() -> int:
 def head_rotary(args: HeadRotaryArgs, stream: int) -> None:
     args.struct_size = ctypes.sizeof(HeadRotaryArgs)
     _check(load_library().ll_head_rotary(ctypes.byref(args), _ptr(int(stream))))
+
+
+def paged_attention_workspace_bytes(args: PagedAttentionArgs) -> int:
+    args.struct_size = ctypes.sizeof(PagedAttentionArgs)
+    needed = load_library().ll_paged_attention_workspace_bytes(ctypes.byref(args))
+    _check(min(needed, LL_OK))
+    return needed
+
+
+def paged_attention(args: PagedAttentionArgs, stream: int) -> None:
+    args.struct_size = ctypes.sizeof(PagedAttentionArgs)
+    _check(load_library().ll_paged_attention(ctypes.byref(args), _ptr(int(stream))))

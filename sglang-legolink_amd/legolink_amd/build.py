@@ -21,8 +21,9 @@ from pathlib import Path
 PACKAGE_DIR = Path(__file__).resolve().parent
 SOURCE = PACKAGE_DIR.parent / "csrc" / "legolink_kv.hip"
 # Translation units of liblegolink_kv.so: the link kernels, the repair
-# attention, and the norms and rotation of a step's heads.
-SOURCES = (SOURCE, *(PACKAGE_DIR.parent / "csrc" / name for name in ("repair_attention.hip", "head_rotary.hip")))
+# attention, the norms and rotation of a step's heads, and its attention.
+SOURCES = (SOURCE, *(PACKAGE_DIR.parent / "csrc" / name
+                     for name in ("repair_attention.hip", "head_rotary.hip", "paged_attention.hip")))
 INCLUDE_DIR = PACKAGE_DIR.parents[1] / "include"
 OUTPUT = PACKAGE_DIR / "lib" / "liblegolink_kv.so"
 # The row-access calibration kernels of bench.py's sweep (measurement only,
