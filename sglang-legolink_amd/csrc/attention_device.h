@@ -119,7 +119,24 @@ __device__ inline void dma_pair(const void *src0, void *lds0, const void *src1, 
       : "memory");
 }
 
-// The same with 32-bit byte offsets into the K and V buffers (buffer loads:
+// One of them.
+__device__ inline void dma_row(const void *src, void *lds) {
+  const unsigned base = __builtin_amdgcn_readfirstlane(
+      static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds)));
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off\n\t"
+      "s_nop 0\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(src), "s"(base)
+      : "memory");
+}
+
+// dma_pair with 32-bit byte offsets into the K and V buffers (buffer loads:
 // one multiply-add per address instead of 64-bit address arithmetic), for
 // pools whose K and V buffers each fit in 4 GiB.  The resources hold the
 // buffer's base and size (loads past it would read zeros; the offsets used

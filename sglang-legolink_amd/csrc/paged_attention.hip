@@ -29,6 +29,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_device.h"
 #include "legolink_kv.h"
@@ -202,58 +203,38 @@ __device__ inline uint16_t *output_row(const PagedParams &p, const Work &w, int 
   return p.out + ((static_cast<long long>(w.request.q_start) + token) * p.hq + h) * dim;
 }
 
-// A value product in which a column must not meet the infinities and NaN of
-// rows that it does not see (their probability is 0, and 0 * inf is NaN): the
-// rows' finite values, and each kind of the others as ones whose weight says
-// whether the column sees any.
+// Infinities and NaN among a tile's values.  A column that does not see a row
+// weighs it 0, and 0 * inf is NaN; so in the tiles that some columns see in part,
+// the values that are not finite are taken out of LDS before the product, and
+// added to the columns that do see their rows afterwards (inf or NaN, whatever the
+// weight).
+template <typename E>
+__device__ inline bool nonfinite(uint32_t value) { return (value & E::kExponent) == E::kExponent; }
 template <typename E>
 __device__ inline bool any_nonfinite(u32x4 bits) {
   bool any = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    any = any || (bits[i] & E::kExponent) == E::kExponent || ((bits[i] >> 16) & E::kExponent) == E::kExponent;
+  for (int i = 0; i < 4; ++i) any = any || nonfinite<E>(bits[i]) || nonfinite<E>(bits[i] >> 16);
   return any;
 }
-
-enum { kFinite, kPlusInfinity, kMinusInfinity, kNan };
 template <typename E>
-__device__ inline uint32_t only(uint32_t pair, int kind) {
-  uint32_t out = 0;
+__device__ inline u32x4 finite_only(u32x4 bits) {
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const uint32_t x = (pair >> (16 * half)) & 0xffffu;
-    const bool special = (x & E::kExponent) == E::kExponent;
-    const bool nan = special && (x & E::kFraction) != 0;
-    const int is = !special ? kFinite : nan ? kNan : (x >> 15) != 0 ? kMinusInfinity : kPlusInfinity;
-    const uint32_t y = is != kind ? 0u : kind == kFinite ? x : E::kOne;
-    out |= y << (16 * half);
+  for (int i = 0; i < 4; ++i) {
+    if (nonfinite<E>(bits[i])) bits[i] &= 0xffff0000u;
+    if (nonfinite<E>(bits[i] >> 16)) bits[i] &= 0xffffu;
+  }
+  return bits;
+}
+template <typename E>
+__device__ inline f32x4 nonfinite_only(u32x2 bits) {  // four values, the finite ones 0
+  f32x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t value = bits[i / 2] >> (16 * (i % 2));
+    out[i] = nonfinite<E>(value) ? E::unpack(bits[i / 2])[i % 2] : 0.f;
   }
   return out;
-}
-
-template <typename E, typename Acc, typename Product>
-__device__ inline Acc guarded_product(u32x4 rows, Acc acc, Product product) {
-  auto part = [&](int kind) {
-    u32x4 bits;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bits[i] = only<E>(rows[i], kind);
-    return __builtin_bit_cast(typename E::frag, bits);
-  };
-  acc = product(part(kFinite), acc);
-  Acc zero;
-  constexpr int kValues = sizeof(Acc) / sizeof(float);
-#pragma unroll
-  for (int i = 0; i < kValues; ++i) zero[i] = 0.f;
-  const Acc plus = product(part(kPlusInfinity), zero);
-  const Acc minus = product(part(kMinusInfinity), zero);
-  const Acc nan = product(part(kNan), zero);
-#pragma unroll
-  for (int i = 0; i < kValues; ++i) {
-    if (plus[i] > 0.f) acc[i] += INFINITY;
-    if (minus[i] > 0.f) acc[i] -= INFINITY;
-    if (nan[i] > 0.f) acc[i] = NAN;
-  }
-  return acc;
 }
 
 // Column statistics across the four lane groups of a 16-column MFMA.
@@ -440,6 +421,23 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
         asm volatile("" ::: "memory");
       }
+      unsigned odd = 0;  // rows whose values are not all finite, where some columns do not see the subtile whole
+      if (key0 + N::kKeys > seen_by_all && seen_by_all < w.key_end) {
+        for (int c = lane; c < N::kKeys * N::kChunksPerRow; c += kWave) {
+          u32x4 *chunk = reinterpret_cast<u32x4 *>(rows + N::kHalf + c * 16);
+          if (any_nonfinite<E>(*chunk)) {
+            odd |= 1u << (c / N::kChunksPerRow);
+            *chunk = finite_only<E>(*chunk);
+          }
+        }
+        if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
+#pragma unroll
+          for (int step = 1; step < kWave; step *= 2) odd |= __shfl_xor(odd, step);
+        }
+        odd = __builtin_amdgcn_readfirstlane(odd);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+      }
 
       f32x4 s[kTiles][2];
 #pragma unroll
@@ -508,13 +506,20 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
         va[1] = __builtin_bit_cast(u32x2, lo)[1];
         va[2] = __builtin_bit_cast(u32x2, hi)[0];
         va[3] = __builtin_bit_cast(u32x2, hi)[1];
-        if (!whole && __builtin_amdgcn_ballot_w64(any_nonfinite<E>(va)) != 0) {
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) o[n][b] = E::mfma16(__builtin_bit_cast(frag, va), pb[n], o[n][b]);
+      }
+      while (odd != 0) {
+        const int rel = __builtin_ctz(odd);
+        odd &= odd - 1;
+        const uint16_t *row = v_base + slot_list[sub * N::kKeys + rel] * p.row_values + 4 * g;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+          const f32x4 x = nonfinite_only<E>(*reinterpret_cast<const u32x2 *>(row + 16 * b));
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
-            o[n][b] = guarded_product<E>(va, o[n][b], [&](frag a, f32x4 acc) { return E::mfma16(a, pb[n], acc); });
-        } else {
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) o[n][b] = E::mfma16(__builtin_bit_cast(frag, va), pb[n], o[n][b]);
+            if (key0 + rel <= pos[n]) o[n][b] += x;
+          __builtin_amdgcn_sched_barrier(0);  // (rare: few registers rather than loads in flight)
         }
       }
       // The stage's reads are done: the gather kStages turns ahead takes it.
@@ -572,6 +577,416 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
       }
     }
   }
+}
+
+// Many columns: chunks, bound by the matrix products.  Eight waves of 32 columns
+// each (four at head dim 256, whose registers do not leave room for a second wave
+// per SIMD) share every gathered tile of 64 keys.  v_mfma_f32_32x32x16, lane
+// layouts: A and B lane l element e -> row / column l % 32, k = 8 (l / 32) + e;
+// accumulator register r -> row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.
+// The value product's k order is the scores' register order.
+//
+// A tile is two phases, the products (the values of tile t - 1, the scores of
+// tile t) and the softmax, about as long as each other: the products keep the
+// matrix unit busy for 1,024 cycles at head dim 128, the softmax the vector unit
+// for about 900.  With two waves per SIMD in step, both would want the same
+// unit; so the second half of the waves runs one phase behind the first (one
+// barrier more in front), and a SIMD's waves alternate.
+//
+// LDS: K and V rings of kStages tiles, rows token-major with their 16-byte chunks
+// swizzled by token as in the narrow kernel (for 32 lanes of 4 tokens x 64 bytes
+// a transposed read).  In iteration t every wave issues its share of K tile t +
+// kLead and V tile t + kLead - 1, into the stages of K tile t - 1 and V tile t - 2,
+// which every wave has left; before the iteration's second barrier it waits for
+// its share of K tile t + 1 and V tile t.
+template <int D>
+struct Wide {
+  static constexpr int kKeys = 64;
+  static constexpr int kWaves = D == 256 ? 4 : 8;
+  static constexpr int kStages = D == 256 ? 2 : 4;
+  static constexpr int kLead = kStages - 1;
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kColumns = 32 * kWaves;
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kStage = kKeys * kRowBytes;
+  static constexpr int kChunksPerRow = D / 8;
+  static constexpr int kGathers = kStage / (16 * kWave) / kWaves;  // a wave's, of K and of V, per tile
+  static constexpr int kList = 7168;                               // slots held at a time
+  __device__ static int k_swizzle(int t) { return D >= 128 ? t % 16 : (t / 2) % 8; }
+  __device__ static int v_swizzle(int t) { return D >= 128 ? 4 * (t % 4) : 4 * ((t / 2) % 2); }
+};
+
+template <int D, typename E>
+__global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const PagedParams p) {
+  typedef Wide<D> W;
+  typedef typename E::frag frag;
+  constexpr int kKSteps = D / 16;
+  constexpr int kBlocks = D / 32;
+  constexpr int kLead = W::kLead;
+  __shared__ __attribute__((aligned(16))) unsigned char k_ring[W::kStages * W::kStage];
+  __shared__ __attribute__((aligned(16))) unsigned char v_ring[W::kStages * W::kStage];
+  __shared__ int slot_list[W::kList];
+  __shared__ unsigned long long tile_valid[W::kList / W::kKeys];
+  __shared__ unsigned odd_rows[W::kList / 32];  // a bit per key: values that are not all finite
+
+  const int head = blockIdx.x % p.hkv;
+  const int unit = blockIdx.x / p.hkv;
+  const Work w = find_work<false>(p, W::kColumns, unit);
+  if (w.index < 0 || w.chunk >= w.chunks) return;
+  const int key_begin = w.chunk * w.chunk_keys;  // below the tile's key_end, or 0
+  int key_end = key_begin + min(w.chunk_keys, w.key_end - key_begin);
+  if (p.num_pages == 0) key_end = key_begin;  // no row that may be read
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int lane = tid % kWave;
+  const int h = lane / 32;
+  const int col = lane % 32;
+
+  // The lane's column.
+  const int column = w.tile * W::kColumns + 32 * wave + col;
+  const int token = column / p.group;
+  const bool exists = token < w.request.q_len;
+  const int first_pos = w.request.kv_len - w.request.q_len;  // of the request's query 0
+  const int pos = exists ? first_pos + token : -1;
+  // Of the wave's columns: keys that all of them see, keys that any of them sees.
+  const int wave_first = (w.tile * W::kColumns + 32 * wave) / p.group;
+  const int wave_last = min(w.request.q_len - 1, (w.tile * W::kColumns + 32 * wave + 31) / p.group);
+  const bool wave_computes = wave_first < w.request.q_len;
+  // Keys from here on are not seen by every column of the workgroup (none, where all stand at one position).
+  const int tile_first_seen = first_pos + (w.tile * W::kColumns) / p.group + 1;
+  const int seen_in_part = tile_first_seen < w.key_end ? tile_first_seen : 0x7fffffff;
+  const int seen_by_all = first_pos + wave_first + 1;
+  const int wave_stop = wave_computes ? min(key_end, first_pos + wave_last + 1) : key_begin;
+
+  frag qf[kKSteps];
+  {
+    const int q_head = head * p.group + (column - token * p.group);
+    const uint16_t *row =
+        p.q + (static_cast<long long>(w.request.q_start) + token) * p.q_token + q_head * p.q_head + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < kKSteps; ++ks) {
+      u32x4 bits = u32x4{0u, 0u, 0u, 0u};
+      if (exists) bits = *reinterpret_cast<const u32x4 *>(row + 16 * ks);
+      qf[ks] = __builtin_bit_cast(frag, bits);
+    }
+  }
+
+  float m = -INFINITY, l = 0.f;
+  f32x16 o[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[b][r] = 0.f;
+  const float scale_log2 = p.scale_log2;
+  const float slack = kSlack / scale_log2;
+
+  // The wave's share of a tile's gathers: instruction j fills the 64 16-byte
+  // chunks from 64 (kGathers wave + j) on; a lane's chunk is of row `token`.
+  const uint16_t *k_base = p.k + static_cast<long long>(head) * D;
+  const uint16_t *v_base = p.v + static_cast<long long>(head) * D;
+  int g_token[W::kGathers];
+  int g_kchunk[W::kGathers], g_vchunk[W::kGathers];
+#pragma unroll
+  for (int j = 0; j < W::kGathers; ++j) {
+    const int at = (W::kGathers * wave + j) * kWave + lane;
+    g_token[j] = at / W::kChunksPerRow;
+    g_kchunk[j] = 8 * ((at % W::kChunksPerRow) ^ W::k_swizzle(g_token[j]));
+    g_vchunk[j] = 8 * ((at % W::kChunksPerRow) ^ W::v_swizzle(g_token[j]));
+  }
+  const int share = W::kGathers * wave * kWave * 16;  // its first byte of a stage
+  auto gather = [&](int k_tile, int k_stage, bool k_due, int v_tile, int v_stage, bool v_due) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < W::kGathers; ++j) {
+      if (k_due) {
+        const int slot = max(slot_list[k_tile * W::kKeys + g_token[j]], 0);
+        dma_row(k_base + slot * p.row_values + g_kchunk[j], k_ring + k_stage * W::kStage + share + j * kWave * 16);
+      }
+      if (v_due) {
+        const int slot = max(slot_list[v_tile * W::kKeys + g_token[j]], 0);
+        dma_row(v_base + slot * p.row_values + g_vchunk[j], v_ring + v_stage * W::kStage + share + j * kWave * 16);
+      }
+    }
+  };
+
+  // Offsets of the lane's fragments within a stage.
+  int k_off[kKSteps];
+#pragma unroll
+  for (int ks = 0; ks < kKSteps; ++ks) {
+    k_off[ks] = col * W::kRowBytes + ((2 * ks + h) ^ W::k_swizzle(col)) * 16;
+    asm volatile("" : "+v"(k_off[ks]));  // kept, not recomputed per tile
+  }
+  const int li = lane % 16;
+  const int v_token = 4 * h + li / 4;
+  const unsigned v_lds =
+      static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char *)v_ring));
+  unsigned v_off[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const int chunk = 4 * b + 2 * ((lane / 16) % 2) + (li % 4) / 2;
+    v_off[b] = v_lds + v_token * W::kRowBytes + (chunk ^ W::v_swizzle(v_token)) * 16 + 8 * (li % 2);
+    asm volatile("" : "+v"(v_off[b]));
+  }
+
+  f32x16 s[2];
+  frag pb[4];
+  bool scored = false, weighed = false;  // s holds scores; pb weights
+
+  // The scores of tile t (its first key key0) into s.
+  auto score_tile = [&](int stage) __attribute__((always_inline)) {
+    const unsigned char *rows = k_ring + stage * W::kStage;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+    frag kf[2][4];
+    auto load = [&](int batch, frag *dst) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          dst[2 * j + kb] = *reinterpret_cast<const frag *>(rows + k_off[2 * batch + j] + kb * 32 * W::kRowBytes);
+    };
+    load(0, kf[0]);
+#pragma unroll
+    for (int batch = 0; batch < kKSteps / 2; ++batch) {
+      if (batch + 1 < kKSteps / 2) load(batch + 1, kf[(batch + 1) % 2]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma32(kf[batch % 2][2 * j + kb], qf[2 * batch + j], s[kb]);
+    }
+  };
+  // The weights of the scores in s, into pb; the sums so far rescaled where the maximum rises.
+  auto weigh_tile = [&](int key0, unsigned long long valid) __attribute__((always_inline)) {
+    const bool whole = valid == ~0ull && key0 + W::kKeys <= seen_by_all;
+    if (!whole) {
+      // Register r of block kb: key 32 kb + 8 (r / 4) + 4 h + r % 4.
+      const int limit = pos - key0 - 4 * h;
+      const unsigned long long lane_valid = valid >> (4 * h);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int rel = 32 * kb + 8 * (r / 4) + r % 4;
+          const bool visible = rel <= limit && ((lane_valid >> rel) & 1ull) != 0;
+          s[kb][r] = visible ? s[kb][r] : -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+    {
+      unsigned a = __builtin_bit_cast(unsigned, top), b = a;
+      permlane32_swap(a, b);
+      top = max_f32(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    }
+    const bool raise = top > m + slack;
+    const float m_new = raise ? top : m;
+    const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], scale_log2, bias));
+    if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+      const float alpha = raise ? __builtin_amdgcn_exp2f((m - m_new) * scale_log2) : 1.f;
+      l *= alpha;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) o[b] *= alpha;
+    }
+    m = m_new;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        u32x4 bits;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bits[j] = E::pack(s[kb][8 * st + 2 * j], s[kb][8 * st + 2 * j + 1]);
+          l = E::dot2_ones(bits[j], l);  // the weights that the value product sees
+        }
+        pb[2 * kb + st] = __builtin_bit_cast(frag, bits);
+      }
+  };
+  // O^T += V^T P^T of the tile that pb weighs.  Step st covers its keys 16 st + 4 h
+  // .. + 3 and, 8 further, the second read.
+  auto add_values = [&](int stage) __attribute__((always_inline)) {
+    auto load = [&](int step, u32x4 *dst) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const unsigned at = v_off[b] + stage * W::kStage + 16 * step * W::kRowBytes;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at)));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at + 8 * W::kRowBytes)));
+        dst[b][0] = __builtin_bit_cast(u32x2, lo)[0];
+        dst[b][1] = __builtin_bit_cast(u32x2, lo)[1];
+        dst[b][2] = __builtin_bit_cast(u32x2, hi)[0];
+        dst[b][3] = __builtin_bit_cast(u32x2, hi)[1];
+      }
+    };
+    u32x4 vf[2][kBlocks];
+    load(0, vf[0]);
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      if (step + 1 < 4) load(step + 1, vf[(step + 1) % 2]);
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) o[b] = E::mfma32(__builtin_bit_cast(frag, vf[step % 2][b]), pb[step], o[b]);
+    }
+  };
+
+  const int *pages = p.pages + static_cast<long long>(w.index) * p.pages_stride;
+  const bool behind = W::kWaves == 8 && wave >= W::kWaves / 2;  // one phase behind the others
+  for (int list_begin = key_begin; list_begin < key_end; list_begin += W::kList) {
+    const int listed = min(key_end - list_begin, W::kList);
+    const int tiles = (listed + W::kKeys - 1) / W::kKeys;
+    __syncthreads();  // every wave is past the former list and its tiles
+    for (int i = tid; i < tiles * W::kKeys; i += W::kThreads) {
+      const unsigned key = static_cast<unsigned>(list_begin + min(i, listed - 1));
+      const unsigned page = static_cast<unsigned>((key * p.page_magic) >> p.page_shift);
+      const int entry = pages[page];
+      const bool valid = i < listed && static_cast<unsigned>(entry) < static_cast<unsigned>(p.num_pages);
+      slot_list[i] = valid ? entry * p.page_size + static_cast<int>(key - page * p.page_size) : -1;
+      const unsigned long long bits = __builtin_amdgcn_ballot_w64(valid);  // whole tiles: the loop strides by waves
+      if (lane == 0) tile_valid[i / W::kKeys] = bits;
+    }
+    for (int i = tid; i < 2 * tiles; i += W::kThreads) odd_rows[i] = 0;
+    // The compiler does not count the gathers: nothing that it waits for in the
+    // loop below may be left in flight.
+    wait_vm<0>();
+    __syncthreads();
+
+    // K tiles 0 .. kLead - 1 and V tiles 0 .. kLead - 2.
+#pragma unroll
+    for (int t = 0; t < kLead; ++t)
+      gather(t, t, t < tiles, t - 1, t - 1 < 0 ? 0 : t - 1, t >= 1 && t - 1 < tiles);
+    wait_vm<0>();
+    workgroup_barrier();
+    if (behind) workgroup_barrier();
+    auto iteration = [&](const int t, auto stage_tag) __attribute__((always_inline)) {
+      constexpr int stage = decltype(stage_tag)::value;                    // t % kStages
+      constexpr int last_stage = (stage + W::kStages - 1) % W::kStages;    // of tile t - 1
+      constexpr int v_stage = (stage + kLead - 1) % W::kStages;            // of tile t + kLead - 1
+      const int key0 = list_begin + t * W::kKeys;
+      gather(t + kLead, last_stage, t + kLead < tiles, t + kLead - 1, v_stage, t + kLead - 1 < tiles);
+      __builtin_amdgcn_s_setprio(1);
+      if (weighed) add_values(last_stage);
+      scored = t < tiles && key0 < wave_stop;
+      if (scored) score_tile(stage);
+      __builtin_amdgcn_s_setprio(0);
+      // The share of K tile t + 1 and V tile t: all but what the last kLead - 1
+      // iterations issued.
+      if (t + kLead < tiles) wait_vm<2 * W::kGathers * (kLead - 1)>();
+      else wait_vm<0>();
+      unsigned long long valid = 0;
+      if (t < tiles) {
+        const unsigned long long bits = tile_valid[t];
+        // readfirstlane returns int: each half goes through unsigned.
+        const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits))));
+        const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits >> 32))));
+        valid = (static_cast<unsigned long long>(hi) << 32) | lo;
+        if (valid != ~0ull) {
+          // Rows that no column sees may hold anything: zeros in their place, by
+          // the wave that gathered them.
+#pragma unroll
+          for (int j = 0; j < W::kGathers; ++j)
+            if (((valid >> g_token[j]) & 1ull) == 0)
+              *reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16) =
+                  u32x4{0u, 0u, 0u, 0u};
+        }
+        if (key0 + W::kKeys > seen_in_part) {
+#pragma unroll
+          for (int j = 0; j < W::kGathers; ++j) {
+            u32x4 *chunk = reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16);
+            if (any_nonfinite<E>(*chunk)) {
+              *chunk = finite_only<E>(*chunk);
+              atomicOr(&odd_rows[2 * t + g_token[j] / 32], 1u << (g_token[j] % 32));
+            }
+          }
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's reads and writes of the stages are done
+      __builtin_amdgcn_sched_barrier(0);
+      workgroup_barrier();
+      if (scored) weigh_tile(key0, valid);
+      weighed = scored;
+      __builtin_amdgcn_sched_barrier(0);
+      workgroup_barrier();
+    };
+    // Iteration `tiles` adds the last tile's values.
+    for (int t = 0; t <= tiles; t += W::kStages) {
+      iteration(t, std::integral_constant<int, 0>{});
+      if (t + 1 <= tiles) iteration(t + 1, std::integral_constant<int, 1>{});
+      if constexpr (W::kStages == 4) {
+        if (t + 2 <= tiles) iteration(t + 2, std::integral_constant<int, 2>{});
+        if (t + 3 <= tiles) iteration(t + 3, std::integral_constant<int, 3>{});
+      }
+    }
+    if (W::kWaves == 8 && !behind) workgroup_barrier();
+    if (list_begin + listed > seen_in_part) {
+      for (int base = 0; base < 2 * tiles; base += kWave) {
+        const unsigned word = base + lane < 2 * tiles ? odd_rows[base + lane] : 0u;
+        unsigned long long words = __builtin_amdgcn_ballot_w64(word != 0);
+        while (words != 0) {
+          const int at = __builtin_ctzll(words);
+          words &= words - 1;
+          for (unsigned bits = __builtin_amdgcn_readlane(word, at); bits != 0; bits &= bits - 1) {
+            const int key = (base + at) * 32 + __builtin_ctz(bits);  // of the list
+            const uint16_t *row = v_base + slot_list[key] * p.row_values + 4 * h;
+            if (list_begin + key > pos) continue;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+              for (int rr = 0; rr < 4; ++rr) {
+                const f32x4 x = nonfinite_only<E>(*reinterpret_cast<const u32x2 *>(row + 32 * b + 8 * rr));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[b][4 * rr + e] += x[e];
+                __builtin_amdgcn_sched_barrier(0);  // (rare: few registers rather than loads in flight)
+              }
+          }
+        }
+      }
+    }
+  }
+
+  {  // the column's other half (lane l ^ 32) summed the other keys
+    unsigned a = __builtin_bit_cast(unsigned, l), b = a;
+    permlane32_swap(a, b);
+    l = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  if (!exists) return;
+  // Register r of block b: dim 32 b + 8 (r / 4) + 4 h + r % 4.
+  if (w.chunks == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is zero
+    uint16_t *dst = output_row(p, w, head, column, D) + 4 * h;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) {
+        u32x2 packed;
+        packed[0] = E::pack(o[b][4 * rr] * inv, o[b][4 * rr + 1] * inv);
+        packed[1] = E::pack(o[b][4 * rr + 2] * inv, o[b][4 * rr + 3] * inv);
+        *reinterpret_cast<u32x2 *>(dst + 32 * b + 8 * rr) = packed;
+      }
+    return;
+  }
+  float *partial = partial_of<D>(p, W::kColumns, unit, head);
+  const int c = 32 * wave + col;
+  if (h == 0) {
+    partial[W::kColumns * D + 2 * c] = m == -INFINITY ? -INFINITY : m * scale_log2;
+    partial[W::kColumns * D + 2 * c + 1] = l;
+  }
+  float *dst = partial + c * D + 4 * h;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      f32x4 row;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) row[e] = o[b][4 * rr + e];
+      *reinterpret_cast<f32x4 *>(dst + 32 * b + 8 * rr) = row;
+    }
 }
 
 // Joins the partial results of tiles of more than one chunk.  kSplit waves a
@@ -664,7 +1079,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p,
 struct Launch {
   int columns;
   int max_tiles, max_units, target, min_chunk;
-  bool splits;
+  bool wide, splits;
   long long ws_floats;
 };
 
@@ -677,7 +1092,8 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   // Columns by the average request: whole chunks in as few tiles as they fill.
   const long long average = queries == 0 ? 1 : (queries + requests - 1) / requests;
   const long long wanted = average * group;
-  x.columns = wanted <= 16 ? 16 : wanted <= 32 || a->head_dim == 256 ? 32 : 64;
+  x.wide = wanted > (a->head_dim == 256 ? 32 : 64);
+  x.columns = x.wide ? (a->head_dim == 256 ? 128 : 256) : wanted <= 16 ? 16 : wanted <= 32 ? 32 : 64;
   const long long tiles = a->query_starts == nullptr
                               ? requests * ((group + x.columns - 1) / x.columns)
                               : queries * group / x.columns + requests;
@@ -754,13 +1170,15 @@ void launch_narrow(const PagedParams &p, const Launch &x, unsigned grid, hipStre
 
 template <int D, typename E>
 int launch_all(const PagedParams &p, const Launch &x, hipStream_t s) {
-  launch_narrow<D, E>(p, x, static_cast<unsigned>(x.max_units) * static_cast<unsigned>(p.hkv), s);
+  const unsigned grid = static_cast<unsigned>(x.max_units) * static_cast<unsigned>(p.hkv);
+  if (x.wide) paged_wide_kernel<D, E><<<grid, Wide<D>::kThreads, 0, s>>>(p);
+  else launch_narrow<D, E>(p, x, grid, s);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   if (!x.splits) return LL_OK;
   const unsigned tile_heads = static_cast<unsigned>(x.max_tiles) * static_cast<unsigned>(p.hkv);
   const unsigned columns = static_cast<unsigned>(x.columns);
-  if (x.target >= 8 * x.max_tiles) paged_combine_kernel<D, E, 4><<<tile_heads * columns, 256, 0, s>>>(p, x.columns);
+  if (x.target >= 8 * x.max_tiles && !x.wide) paged_combine_kernel<D, E, 4><<<tile_heads * columns, 256, 0, s>>>(p, x.columns);
   else paged_combine_kernel<D, E, 1><<<tile_heads * (columns / 4), 256, 0, s>>>(p, x.columns);
   err = hipGetLastError();
   if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
