@@ -56,9 +56,10 @@ struct PagedParams {
   const int *pages;
   const void *kv_lengths, *query_starts;  // query_starts NULL: one query each
   float *ws;
-  long long q_token, q_head, pages_stride, row_values;  // row_values: of one slot, hkv * D
+  long long q_token, q_head, pages_stride;
   unsigned long long page_magic;
   double inv_target;
+  unsigned row_bytes;  // of one slot's K (or V) row: hkv * D values
   int page_shift, page_size, num_pages, max_keys;
   int num_queries, num_requests, hq, hkv, group;
   int lengths64, starts64;
@@ -92,6 +93,11 @@ __device__ inline Request request_at(const PagedParams &p, int r) {
   return x;
 }
 
+// The bytes of slot's row from `base` on (one 32 x 32 + 64-bit multiply-add).
+__device__ inline const unsigned char *row_at(const PagedParams &p, const unsigned char *base, int slot) {
+  return base + static_cast<unsigned long long>(static_cast<unsigned>(slot)) * p.row_bytes;
+}
+
 __device__ inline int inclusive_scan(int value, int lane) {
 #pragma unroll
   for (int step = 1; step < kWave; step *= 2) {
@@ -107,7 +113,7 @@ struct Work {
   Request request;
   int index;  // of the request; -1: none
   int tile, chunk, chunk_keys;
-  int first_unit, chunks;  // of the tile
+  int first_unit, unit_step, chunks;  // the tile's chunk c is unit first_unit + c unit_step
   int key_end;             // keys that some column of the tile sees
 };
 
@@ -139,7 +145,9 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
     work = __shfl(work, 0);
   }
   const double share = static_cast<double>(work) * p.inv_target;
-  const int chunk = max(p.min_chunk, static_cast<int>(min(ceil(share - 1e-6), 33554432.0)));  // 2^25 tiles: any length
+  // (2^25 key tiles are more than any length; readfirstlane: uniform to the compiler too)
+  const int chunk = __builtin_amdgcn_readfirstlane(
+      max(p.min_chunk, static_cast<int>(min(ceil(share - 1e-6), 33554432.0))));
 
   Work w;
   w.index = -1;
@@ -167,17 +175,23 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
       w.request.q_start = __builtin_amdgcn_readlane(x.q_start, at);
       w.request.q_len = __builtin_amdgcn_readlane(x.q_len, at);
       w.request.kv_len = __builtin_amdgcn_readlane(x.kv_len, at);
-      const int own_tiles = __builtin_amdgcn_readlane(tiles, at);
+      const int own_tiles = __builtin_amdgcn_readlane(tiles, at);  // at least 1
       const int own_chunks = __builtin_amdgcn_readlane(chunks, at);
       const int first_unit = units_before + __builtin_amdgcn_readlane(units_to, at) - own_tiles * own_chunks;
+      // A request's units in order of falling length: chunk 0 of every tile, the
+      // last tile (which sees the most keys) first, and so on.  The units that run
+      // together then read the same keys, and the short ones fill the last round.
+      int nth;
       if constexpr (kOfTiles) {
-        w.tile = index - (tiles_before + __builtin_amdgcn_readlane(tiles_to, at) - own_tiles);
+        nth = index - (tiles_before + __builtin_amdgcn_readlane(tiles_to, at) - own_tiles);
         w.chunk = 0;
       } else {
-        w.tile = (index - first_unit) / own_chunks;
-        w.chunk = (index - first_unit) - w.tile * own_chunks;
+        w.chunk = (index - first_unit) / own_tiles;
+        nth = (index - first_unit) - w.chunk * own_tiles;
       }
-      w.first_unit = first_unit + w.tile * own_chunks;
+      w.tile = own_tiles - 1 - nth;
+      w.first_unit = first_unit + nth;
+      w.unit_step = own_tiles;
       // The tile's last query and its position bound the keys.
       const int last_query = min(w.request.q_len - 1, ((w.tile + 1) * columns - 1) / p.group);
       w.key_end = max(0, w.request.kv_len - w.request.q_len + last_query + 1);
@@ -235,6 +249,11 @@ __device__ inline f32x4 nonfinite_only(u32x2 bits) {  // four values, the finite
     out[i] = nonfinite<E>(value) ? E::unpack(bits[i / 2])[i % 2] : 0.f;
   }
   return out;
+}
+
+// The weight, under the maximum `top` of several, of a result with the maximum `own`.
+__device__ inline float joined_weight(float own, float top) {
+  return own == -INFINITY && top == -INFINITY ? 1.f : exp2f(own - top);  // (sums of nothing seen are 0)
 }
 
 // Column statistics across the four lane groups of a 16-column MFMA.
@@ -351,8 +370,8 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 
   // The lane's share of a gather: its 16 bytes of instruction j hold chunk
   // (64 j + lane) of the subtile's rows in LDS order.
-  const uint16_t *k_base = p.k + static_cast<long long>(head) * D;
-  const uint16_t *v_base = p.v + static_cast<long long>(head) * D;
+  const unsigned char *k_base = reinterpret_cast<const unsigned char *>(p.k + static_cast<long long>(head) * D);
+  const unsigned char *v_base = reinterpret_cast<const unsigned char *>(p.v + static_cast<long long>(head) * D);
   auto gather = [&](int sub, int stage) {
     unsigned char *dst = ring + stage * N::kStage;
 #pragma unroll
@@ -361,9 +380,8 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
       const int token = at / N::kChunksPerRow;
       const int place = at % N::kChunksPerRow;
       const int slot = max(slot_list[sub * N::kKeys + token], 0);
-      const long long row = slot * p.row_values;
-      dma_pair(k_base + row + 8 * (place ^ N::k_swizzle(token)), dst + j * 16 * kWave,
-               v_base + row + 8 * (place ^ N::v_swizzle(token)), dst + N::kHalf + j * 16 * kWave);
+      dma_pair(row_at(p, k_base + 16 * (place ^ N::k_swizzle(token)), slot), dst + j * 16 * kWave,
+               row_at(p, v_base + 16 * (place ^ N::v_swizzle(token)), slot), dst + N::kHalf + j * 16 * kWave);
     }
   };
   // Offsets of the lane's fragments within a stage.
@@ -512,10 +530,10 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
       while (odd != 0) {
         const int rel = __builtin_ctz(odd);
         odd &= odd - 1;
-        const uint16_t *row = v_base + slot_list[sub * N::kKeys + rel] * p.row_values + 4 * g;
+        const unsigned char *row = row_at(p, v_base, slot_list[sub * N::kKeys + rel]) + 8 * g;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-          const f32x4 x = nonfinite_only<E>(*reinterpret_cast<const u32x2 *>(row + 16 * b));
+          const f32x4 x = nonfinite_only<E>(*reinterpret_cast<const u32x2 *>(row + 32 * b));
 #pragma unroll
           for (int n = 0; n < kTiles; ++n)
             if (key0 + rel <= pos[n]) o[n][b] += x;
@@ -558,7 +576,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 #pragma unroll
       for (int v = 0; v < N::kWaves; ++v) {
         const float own = stats[v][16 * n + c][0];
-        const float weight = own == -INFINITY && top == -INFINITY ? 1.f : exp2f(own - top);
+        const float weight = joined_weight(own, top);
         sum += weight * stats[v][16 * n + c][1];
         acc += weight * *reinterpret_cast<const f32x4 *>(joined + (v * 16 + c) * kPitch + 4 * quad);
       }
@@ -595,16 +613,18 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 //
 // LDS: K and V rings of kStages tiles, rows token-major with their 16-byte chunks
 // swizzled by token as in the narrow kernel (for 32 lanes of 4 tokens x 64 bytes
-// a transposed read).  In iteration t every wave issues its share of K tile t +
-// kLead and V tile t + kLead - 1, into the stages of K tile t - 1 and V tile t - 2,
-// which every wave has left; before the iteration's second barrier it waits for
-// its share of K tile t + 1 and V tile t.
+// a transposed read).  Iteration t is the softmax of tile t, then the products:
+// the values of tile t, the scores of tile t + 1.  Before its first barrier a
+// wave waits for its share of V tile t and K tile t + 1; behind it, it issues its
+// share of K tile t + kLead and V tile t + kLead - 1.  Their stages held K tile t -
+// 1 and V tile t - 2 (four stages; the waves one phase behind have left them too),
+// or K tile t and V tile t - 1 (two stages, all waves in step).
 template <int D>
 struct Wide {
   static constexpr int kKeys = 64;
   static constexpr int kWaves = D == 256 ? 4 : 8;
   static constexpr int kStages = D == 256 ? 2 : 4;
-  static constexpr int kLead = kStages - 1;
+  static constexpr int kLead = D == 256 ? 2 : 3;  // tiles that K gathers run ahead
   static constexpr int kThreads = kWaves * kWave;
   static constexpr int kColumns = 32 * kWaves;
   static constexpr int kRowBytes = 2 * D;
@@ -683,39 +703,38 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
 
   // The wave's share of a tile's gathers: instruction j fills the 64 16-byte
   // chunks from 64 (kGathers wave + j) on; a lane's chunk is of row `token`.
-  const uint16_t *k_base = p.k + static_cast<long long>(head) * D;
-  const uint16_t *v_base = p.v + static_cast<long long>(head) * D;
+  const unsigned char *k_base = reinterpret_cast<const unsigned char *>(p.k + static_cast<long long>(head) * D);
+  const unsigned char *v_base = reinterpret_cast<const unsigned char *>(p.v + static_cast<long long>(head) * D);
   int g_token[W::kGathers];
-  int g_kchunk[W::kGathers], g_vchunk[W::kGathers];
+  unsigned g_k[W::kGathers], g_v[W::kGathers];  // the bytes of the lane's chunk within a row
 #pragma unroll
   for (int j = 0; j < W::kGathers; ++j) {
     const int at = (W::kGathers * wave + j) * kWave + lane;
     g_token[j] = at / W::kChunksPerRow;
-    g_kchunk[j] = 8 * ((at % W::kChunksPerRow) ^ W::k_swizzle(g_token[j]));
-    g_vchunk[j] = 8 * ((at % W::kChunksPerRow) ^ W::v_swizzle(g_token[j]));
+    g_k[j] = 16 * ((at % W::kChunksPerRow) ^ W::k_swizzle(g_token[j]));
+    g_v[j] = 16 * ((at % W::kChunksPerRow) ^ W::v_swizzle(g_token[j]));
   }
   const int share = W::kGathers * wave * kWave * 16;  // its first byte of a stage
-  auto gather = [&](int k_tile, int k_stage, bool k_due, int v_tile, int v_stage, bool v_due) __attribute__((always_inline)) {
+  auto slots_of = [&](int tile, int *slots) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < W::kGathers; ++j) {
-      if (k_due) {
-        const int slot = max(slot_list[k_tile * W::kKeys + g_token[j]], 0);
-        dma_row(k_base + slot * p.row_values + g_kchunk[j], k_ring + k_stage * W::kStage + share + j * kWave * 16);
-      }
-      if (v_due) {
-        const int slot = max(slot_list[v_tile * W::kKeys + g_token[j]], 0);
-        dma_row(v_base + slot * p.row_values + g_vchunk[j], v_ring + v_stage * W::kStage + share + j * kWave * 16);
-      }
-    }
+    for (int j = 0; j < W::kGathers; ++j) slots[j] = max(slot_list[tile * W::kKeys + g_token[j]], 0);
+  };
+  auto gather_k = [&](const int *slots, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < W::kGathers; ++j)
+      dma_row(row_at(p, k_base, slots[j]) + g_k[j], k_ring + stage * W::kStage + share + j * kWave * 16);
+  };
+  auto gather_v = [&](const int *slots, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < W::kGathers; ++j)
+      dma_row(row_at(p, v_base, slots[j]) + g_v[j], v_ring + stage * W::kStage + share + j * kWave * 16);
   };
 
   // Offsets of the lane's fragments within a stage.
-  int k_off[kKSteps];
-#pragma unroll
-  for (int ks = 0; ks < kKSteps; ++ks) {
-    k_off[ks] = col * W::kRowBytes + ((2 * ks + h) ^ W::k_swizzle(col)) * 16;
-    asm volatile("" : "+v"(k_off[ks]));  // kept, not recomputed per tile
-  }
+  // Step ks of the scores reads chunk 2 ks + h, at (2 ks + h) ^ swizzle = (h ^
+  // swizzle) ^ 2 ks: an xor of the offset's bits 5 on with ks.
+  static_assert(W::kRowBytes >= 2 * 16 * kKSteps, "ks stays within the row's bits");
+  const int k_off = col * W::kRowBytes + ((h ^ W::k_swizzle(col)) * 16);
   const int li = lane % 16;
   const int v_token = 4 * h + li / 4;
   const unsigned v_lds =
@@ -730,31 +749,81 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
 
   f32x16 s[2];
   frag pb[4];
-  bool scored = false, weighed = false;  // s holds scores; pb weights
 
-  // The scores of tile t (its first key key0) into s.
-  auto score_tile = [&](int stage) __attribute__((always_inline)) {
-    const unsigned char *rows = k_ring + stage * W::kStage;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+  // The products: the values of the tile that pb weighs (stage v_stage) onto O^T,
+  // the scores of the next (stage k_stage) into s.  Fragments are read one batch
+  // ahead of the MFMAs that take them: eight transposed reads (every dim block of a
+  // 16-key step; keys 16 step + 4 h .. + 3 and, 8 further, the second read), or
+  // four rows' chunks (two 16-dim steps of both 32-key blocks).
+  auto products = [&](int v_stage, int k_stage, auto values_tag) __attribute__((always_inline)) {
+    constexpr bool values = decltype(values_tag)::value;  // else scores alone
+    constexpr int kBatches = kKSteps / 2;
+    const unsigned char *rows = k_ring + k_stage * W::kStage;
+    int k_at = k_off;
+    asm volatile("" : "+v"(k_at));  // the steps' offsets made per tile: eight registers fewer over the loop
+    u32x4 vf[2][kBlocks];
     frag kf[2][4];
-    auto load = [&](int batch, frag *dst) {
+    auto load_v = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const unsigned at = v_off[b] + v_stage * W::kStage + 16 * step * W::kRowBytes;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at)));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at + 8 * W::kRowBytes)));
+        vf[step % 2][b][0] = __builtin_bit_cast(u32x2, lo)[0];
+        vf[step % 2][b][1] = __builtin_bit_cast(u32x2, lo)[1];
+        vf[step % 2][b][2] = __builtin_bit_cast(u32x2, hi)[0];
+        vf[step % 2][b][3] = __builtin_bit_cast(u32x2, hi)[1];
+      }
+    };
+    auto load_k = [&](int batch) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
-          dst[2 * j + kb] = *reinterpret_cast<const frag *>(rows + k_off[2 * batch + j] + kb * 32 * W::kRowBytes);
+          kf[batch % 2][2 * j + kb] =
+              *reinterpret_cast<const frag *>(rows + (k_at ^ (32 * (2 * batch + j))) + kb * 32 * W::kRowBytes);
     };
-    load(0, kf[0]);
+    if constexpr (values) {
+      load_v(0);
 #pragma unroll
-    for (int batch = 0; batch < kKSteps / 2; ++batch) {
-      if (batch + 1 < kKSteps / 2) load(batch + 1, kf[(batch + 1) % 2]);
+      for (int step = 0; step < 4; ++step) {
+        if (step + 1 < 4) load_v(step + 1);
+        else load_k(0);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) o[b] = E::mfma32(__builtin_bit_cast(frag, vf[step % 2][b]), pb[step], o[b]);
+      }
+    } else {
+      load_k(0);
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+    for (int batch = 0; batch < kBatches; ++batch) {
+      if (batch + 1 < kBatches) load_k(batch + 1);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma32(kf[batch % 2][2 * j + kb], qf[2 * batch + j], s[kb]);
+    }
+    // The order above, kept: reads (0x100) and MFMAs (0x008) in turn.
+    if constexpr (values) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * kBlocks, 0);
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        if (step + 1 < 4) __builtin_amdgcn_sched_group_barrier(0x100, 2 * kBlocks, 0);
+        else __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, kBlocks, 0);
+      }
+    } else {
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    }
+#pragma unroll
+    for (int batch = 0; batch < kBatches; ++batch) {
+      if (batch + 1 < kBatches) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
   };
   // The weights of the scores in s, into pb; the sums so far rescaled where the maximum rises.
@@ -810,31 +879,6 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
         pb[2 * kb + st] = __builtin_bit_cast(frag, bits);
       }
   };
-  // O^T += V^T P^T of the tile that pb weighs.  Step st covers its keys 16 st + 4 h
-  // .. + 3 and, 8 further, the second read.
-  auto add_values = [&](int stage) __attribute__((always_inline)) {
-    auto load = [&](int step, u32x4 *dst) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const unsigned at = v_off[b] + stage * W::kStage + 16 * step * W::kRowBytes;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at)));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at + 8 * W::kRowBytes)));
-        dst[b][0] = __builtin_bit_cast(u32x2, lo)[0];
-        dst[b][1] = __builtin_bit_cast(u32x2, lo)[1];
-        dst[b][2] = __builtin_bit_cast(u32x2, hi)[0];
-        dst[b][3] = __builtin_bit_cast(u32x2, hi)[1];
-      }
-    };
-    u32x4 vf[2][kBlocks];
-    load(0, vf[0]);
-#pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      if (step + 1 < 4) load(step + 1, vf[(step + 1) % 2]);
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) o[b] = E::mfma32(__builtin_bit_cast(frag, vf[step % 2][b]), pb[step], o[b]);
-    }
-  };
 
   const int *pages = p.pages + static_cast<long long>(w.index) * p.pages_stride;
   const bool behind = W::kWaves == 8 && wave >= W::kWaves / 2;  // one phase behind the others
@@ -859,68 +903,72 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
 
     // K tiles 0 .. kLead - 1 and V tiles 0 .. kLead - 2.
 #pragma unroll
-    for (int t = 0; t < kLead; ++t)
-      gather(t, t, t < tiles, t - 1, t - 1 < 0 ? 0 : t - 1, t >= 1 && t - 1 < tiles);
+    for (int t = 0; t < kLead; ++t) {
+      if (t >= tiles) break;
+      int slots[W::kGathers];
+      slots_of(t, slots);
+      gather_k(slots, t % W::kStages);
+      if (t + 1 < kLead) gather_v(slots, t);
+    }
     wait_vm<0>();
     workgroup_barrier();
     if (behind) workgroup_barrier();
+    if (list_begin < wave_stop) products(0, 0, std::false_type{});
     auto iteration = [&](const int t, auto stage_tag) __attribute__((always_inline)) {
-      constexpr int stage = decltype(stage_tag)::value;                    // t % kStages
-      constexpr int last_stage = (stage + W::kStages - 1) % W::kStages;    // of tile t - 1
-      constexpr int v_stage = (stage + kLead - 1) % W::kStages;            // of tile t + kLead - 1
+      constexpr int stage = decltype(stage_tag)::value;  // t % kStages
       const int key0 = list_begin + t * W::kKeys;
-      gather(t + kLead, last_stage, t + kLead < tiles, t + kLead - 1, v_stage, t + kLead - 1 < tiles);
-      __builtin_amdgcn_s_setprio(1);
-      if (weighed) add_values(last_stage);
-      scored = t < tiles && key0 < wave_stop;
-      if (scored) score_tile(stage);
-      __builtin_amdgcn_s_setprio(0);
-      // The share of K tile t + 1 and V tile t: all but what the last kLead - 1
+      const bool computes = key0 < wave_stop;
+      // The next gathers' slots are read ahead of the barrier that they wait for.
+      int k_slots[W::kGathers], v_slots[W::kGathers];
+      if (t + kLead < tiles) slots_of(t + kLead, k_slots);
+      if (t + kLead - 1 < tiles) slots_of(t + kLead - 1, v_slots);
+      // The share of K tile t + 1 and V tile t: all but what the last kLead - 2
       // iterations issued.
-      if (t + kLead < tiles) wait_vm<2 * W::kGathers * (kLead - 1)>();
+      if (t + kLead - 1 < tiles) wait_vm<2 * W::kGathers * (kLead - 2)>();
       else wait_vm<0>();
-      unsigned long long valid = 0;
-      if (t < tiles) {
-        const unsigned long long bits = tile_valid[t];
-        // readfirstlane returns int: each half goes through unsigned.
-        const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits))));
-        const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits >> 32))));
-        valid = (static_cast<unsigned long long>(hi) << 32) | lo;
-        if (valid != ~0ull) {
-          // Rows that no column sees may hold anything: zeros in their place, by
-          // the wave that gathered them.
+      const unsigned long long bits = tile_valid[t];
+      // readfirstlane returns int: each half goes through unsigned.
+      const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits))));
+      const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits >> 32))));
+      const unsigned long long valid = (static_cast<unsigned long long>(hi) << 32) | lo;
+      if (valid != ~0ull) {
+        // Rows that no column sees may hold anything: zeros in their place, by
+        // the wave that gathered them.
 #pragma unroll
-          for (int j = 0; j < W::kGathers; ++j)
-            if (((valid >> g_token[j]) & 1ull) == 0)
-              *reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16) =
-                  u32x4{0u, 0u, 0u, 0u};
-        }
-        if (key0 + W::kKeys > seen_in_part) {
+        for (int j = 0; j < W::kGathers; ++j)
+          if (((valid >> g_token[j]) & 1ull) == 0)
+            *reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16) =
+                u32x4{0u, 0u, 0u, 0u};
+      }
+      if (key0 + W::kKeys > seen_in_part) {
 #pragma unroll
-          for (int j = 0; j < W::kGathers; ++j) {
-            u32x4 *chunk = reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16);
-            if (any_nonfinite<E>(*chunk)) {
-              *chunk = finite_only<E>(*chunk);
-              atomicOr(&odd_rows[2 * t + g_token[j] / 32], 1u << (g_token[j] % 32));
-            }
+        for (int j = 0; j < W::kGathers; ++j) {
+          u32x4 *chunk = reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16);
+          if (any_nonfinite<E>(*chunk)) {
+            *chunk = finite_only<E>(*chunk);
+            atomicOr(&odd_rows[2 * t + g_token[j] / 32], 1u << (g_token[j] % 32));
           }
         }
       }
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's reads and writes of the stages are done
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
-      if (scored) weigh_tile(key0, valid);
-      weighed = scored;
+      if (t + kLead < tiles) gather_k(k_slots, (stage + kLead) % W::kStages);
+      if (t + kLead - 1 < tiles) gather_v(v_slots, (stage + kLead - 1) % W::kStages);
+      if (computes) weigh_tile(key0, valid);
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
+      __builtin_amdgcn_s_setprio(1);
+      // (Behind the wave's last tile the scores are of an old stage, and not used.)
+      if (computes) products(stage, (stage + 1) % W::kStages, std::true_type{});
+      __builtin_amdgcn_s_setprio(0);
     };
-    // Iteration `tiles` adds the last tile's values.
-    for (int t = 0; t <= tiles; t += W::kStages) {
+    for (int t = 0; t < tiles; t += W::kStages) {
       iteration(t, std::integral_constant<int, 0>{});
-      if (t + 1 <= tiles) iteration(t + 1, std::integral_constant<int, 1>{});
+      if (t + 1 < tiles) iteration(t + 1, std::integral_constant<int, 1>{});
       if constexpr (W::kStages == 4) {
-        if (t + 2 <= tiles) iteration(t + 2, std::integral_constant<int, 2>{});
-        if (t + 3 <= tiles) iteration(t + 3, std::integral_constant<int, 3>{});
+        if (t + 2 < tiles) iteration(t + 2, std::integral_constant<int, 2>{});
+        if (t + 3 < tiles) iteration(t + 3, std::integral_constant<int, 3>{});
       }
     }
     if (W::kWaves == 8 && !behind) workgroup_barrier();
@@ -933,13 +981,13 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
           words &= words - 1;
           for (unsigned bits = __builtin_amdgcn_readlane(word, at); bits != 0; bits &= bits - 1) {
             const int key = (base + at) * 32 + __builtin_ctz(bits);  // of the list
-            const uint16_t *row = v_base + slot_list[key] * p.row_values + 4 * h;
+            const unsigned char *row = row_at(p, v_base, slot_list[key]) + 8 * h;
             if (list_begin + key > pos) continue;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
               for (int rr = 0; rr < 4; ++rr) {
-                const f32x4 x = nonfinite_only<E>(*reinterpret_cast<const u32x2 *>(row + 32 * b + 8 * rr));
+                const f32x4 x = nonfinite_only<E>(*reinterpret_cast<const u32x2 *>(row + 64 * b + 16 * rr));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[b][4 * rr + e] += x[e];
                 __builtin_amdgcn_sched_barrier(0);  // (rare: few registers rather than loads in flight)
@@ -989,89 +1037,94 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     }
 }
 
-// Joins the partial results of tiles of more than one chunk.  kSplit waves a
-// column take turns at its chunks: 4 where few tiles leave many partials each
-// (their latency adds up), else 1.
+// Joins the partial results of tiles of more than one chunk.  A lane holds four
+// values of a column, so a wave 256 / D columns; a workgroup 16 columns or, with
+// kSplit 4 (few tiles of many chunks each, whose latency adds up), the columns of
+// one wave, the four waves taking turns at their chunks.  A batch's loads are in
+// flight together.
+template <int D, int kSplit>
+struct Combine {
+  static constexpr int kPerWave = 256 / D;
+  static constexpr int kColumns = kSplit == 1 ? 16 : kPerWave;  // of a workgroup
+  static constexpr int kTurns = kSplit == 1 ? kColumns / (4 * kPerWave) : 1;
+  static constexpr int kBatch = kSplit == 1 ? 4 : 8;
+};
+
 template <int D, typename E, int kSplit>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p, int columns) {
-  constexpr int kPer = D / kWave;  // values of a lane
-  constexpr int kBatch = 4;        // partials whose loads are in flight together
-  constexpr int kColumnsPerGroup = 4 / kSplit;
-  const int groups = columns / kColumnsPerGroup;
+  typedef Combine<D, kSplit> C;
+  const int groups = columns / C::kColumns;
   const int tile_head = blockIdx.x / groups;
   const int head = tile_head % p.hkv;
   const Work w = find_work<true>(p, columns, tile_head / p.hkv);
-  if (w.index < 0 || w.chunks <= 1 || w.first_unit < 0 || w.first_unit + w.chunks > p.max_units) return;
+  if (w.index < 0 || w.chunks <= 1 || w.first_unit < 0 ||
+      w.first_unit + static_cast<long long>(w.chunks - 1) * w.unit_step >= p.max_units)
+    return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int c = (blockIdx.x % groups) * kColumnsPerGroup + wave / kSplit;
-  const int column = w.tile * columns + c;
-  const bool exists = column / p.group < w.request.q_len;
-  if (kSplit == 1 && !exists) return;
-
-  float top = -INFINITY, sum = 0.f;
-  float acc[kPer];
+  const int quad = lane % (D / 4);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int s0 = (wave % kSplit) * kBatch; s0 < w.chunks; s0 += kSplit * kBatch) {
-    float tops[kBatch], sums[kBatch], rows[kBatch][kPer];
+  for (int turn = 0; turn < C::kTurns; ++turn) {
+    const int c = (blockIdx.x % groups) * C::kColumns + (kSplit == 1 ? (turn * 4 + wave) * C::kPerWave : 0) +
+                  lane / (D / 4);
+    const int column = w.tile * columns + c;
+    const bool exists = column / p.group < w.request.q_len;
+    if (kSplit == 1 && __builtin_amdgcn_ballot_w64(exists) == 0) return;  // (columns behind are none either)
+    float top = -INFINITY, sum = 0.f;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = kSplit == 1 ? 0 : wave; s0 < w.chunks; s0 += kSplit * C::kBatch) {
+      float tops[C::kBatch], sums[C::kBatch];
+      f32x4 rows[C::kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const float *part = partial_of<D>(p, columns, w.first_unit + min(s0 + i, w.chunks - 1), head);
-      tops[i] = exists ? part[columns * D + 2 * c] : -INFINITY;
-      sums[i] = exists ? part[columns * D + 2 * c + 1] : 0.f;
+      for (int i = 0; i < C::kBatch; ++i) {
+        // Past the last chunk: the last again, dropped.  (Columns that do not exist
+        // are within the partial, and dropped too.)
+        const int chunk = min(s0 + i * kSplit, w.chunks - 1);
+        const float *part = partial_of<D>(p, columns, w.first_unit + chunk * w.unit_step, head);
+        tops[i] = part[columns * D + 2 * c];
+        sums[i] = part[columns * D + 2 * c + 1];
+        rows[i] = *reinterpret_cast<const f32x4 *>(part + c * D + 4 * quad);
+      }
+      float high = top;
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) rows[i][d] = exists ? part[c * D + lane * kPer + d] : 0.f;
+      for (int i = 0; i < C::kBatch; ++i)
+        if (s0 + i * kSplit < w.chunks) high = fmaxf(high, tops[i]);
+      const float old = joined_weight(top, high);
+      sum *= old;
+      acc *= old;
+      top = high;
+#pragma unroll
+      for (int i = 0; i < C::kBatch; ++i)
+        if (s0 + i * kSplit < w.chunks) {
+          const float weight = joined_weight(tops[i], top);
+          sum += weight * sums[i];
+          acc += weight * rows[i];
+        }
     }
-    float high = top;
+    if constexpr (kSplit > 1) {
+      __shared__ float tops[kSplit][kWave], sums[kSplit][kWave];
+      __shared__ f32x4 parts[kSplit][kWave];
+      tops[wave][lane] = top;
+      sums[wave][lane] = sum;
+      parts[wave][lane] = acc;
+      __syncthreads();
+      if (wave > 0) return;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (s0 + i < w.chunks) high = fmaxf(high, tops[i]);
-    const float old = top == -INFINITY ? 0.f : exp2f(top - high);
-    sum *= top == -INFINITY && high == -INFINITY ? 1.f : old;
+      for (int v = 1; v < kSplit; ++v) top = fmaxf(top, tops[v][lane]);
+      sum = 0.f;
+      acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int d = 0; d < kPer; ++d) acc[d] *= top == -INFINITY && high == -INFINITY ? 1.f : old;
-    top = high;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (s0 + i >= w.chunks) continue;
-      const float weight = tops[i] == -INFINITY && top == -INFINITY ? 1.f : exp2f(tops[i] - top);
-      sum += weight * sums[i];
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) acc[d] += weight * rows[i][d];
+      for (int v = 0; v < kSplit; ++v) {
+        const float weight = joined_weight(tops[v][lane], top);
+        sum += weight * sums[v][lane];
+        acc += weight * parts[v][lane];
+      }
     }
-  }
-  if constexpr (kSplit > 1) {
-    __shared__ float tops[kSplit], sums[kSplit], parts[kSplit][D];
-    if (lane == 0) {
-      tops[wave] = top;
-      sums[wave] = sum;
-    }
-#pragma unroll
-    for (int d = 0; d < kPer; ++d) parts[wave][lane * kPer + d] = acc[d];
-    __syncthreads();
-    if (wave > 0 || !exists) return;
-    float high = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < kSplit; ++v) high = fmaxf(high, tops[v]);
-    sum = 0.f;
-#pragma unroll
-    for (int d = 0; d < kPer; ++d) acc[d] = 0.f;
-#pragma unroll
-    for (int v = 0; v < kSplit; ++v) {
-      const float weight = tops[v] == -INFINITY && high == -INFINITY ? 1.f : exp2f(tops[v] - high);
-      sum += weight * sums[v];
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) acc[d] += weight * parts[v][lane * kPer + d];
-    }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t *dst = output_row(p, w, head, column, D) + lane * kPer;
-  if constexpr (kPer == 1) {
-    dst[0] = static_cast<uint16_t>(E::pack(acc[0] * inv, 0.f));
-  } else {
-#pragma unroll
-    for (int d = 0; d < kPer; d += 2)
-      *reinterpret_cast<uint32_t *>(dst + d) = E::pack(acc[d] * inv, acc[d + 1] * inv);
+    if (!exists) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    u32x2 packed;
+    packed[0] = E::pack(acc[0] * inv, acc[1] * inv);
+    packed[1] = E::pack(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<u32x2 *>(output_row(p, w, head, column, D) + 4 * quad) = packed;
   }
 }
 
@@ -1099,7 +1152,12 @@ Launch plan_launch(const ll_paged_attention_args *a) {
                               : queries * group / x.columns + requests;
   x.max_tiles = static_cast<int>(std::min(tiles, 0x7fffffffll));
   x.min_chunk = 2;
-  x.target = std::max(1, 2 * kComputeUnits / static_cast<int>(a->num_kv_heads));
+  // A workgroup fills a compute unit (its LDS rings), so `places` units of every
+  // KV head run at once.  Chunks: as many units as places, the longest first, leave
+  // the least over.  Single tokens: where the tiles are few, as many units as run
+  // at once; where they are many, their lengths average out over four rounds.
+  const int places = std::max(1, kComputeUnits / static_cast<int>(a->num_kv_heads));
+  x.target = x.wide ? places : 2 * x.max_tiles <= places ? places - x.max_tiles + 1 : 4 * places;
   const long long max_keys = a->page_table_columns * a->page_size;
   x.splits = max_keys > x.min_chunk * kPageTile;
   const long long units = tiles + (x.splits ? x.target + 1 : 0);
@@ -1178,8 +1236,10 @@ int launch_all(const PagedParams &p, const Launch &x, hipStream_t s) {
   if (!x.splits) return LL_OK;
   const unsigned tile_heads = static_cast<unsigned>(x.max_tiles) * static_cast<unsigned>(p.hkv);
   const unsigned columns = static_cast<unsigned>(x.columns);
-  if (x.target >= 8 * x.max_tiles && !x.wide) paged_combine_kernel<D, E, 4><<<tile_heads * columns, 256, 0, s>>>(p, x.columns);
-  else paged_combine_kernel<D, E, 1><<<tile_heads * (columns / 4), 256, 0, s>>>(p, x.columns);
+  if (x.target >= 8 * x.max_tiles && !x.wide)
+    paged_combine_kernel<D, E, 4><<<tile_heads * (columns / Combine<D, 4>::kColumns), 256, 0, s>>>(p, x.columns);
+  else
+    paged_combine_kernel<D, E, 1><<<tile_heads * (columns / Combine<D, 1>::kColumns), 256, 0, s>>>(p, x.columns);
   err = hipGetLastError();
   if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   return LL_OK;
@@ -1218,7 +1278,7 @@ int ll_paged_attention(const ll_paged_attention_args *a, ll_stream_t stream) {
   p.q_token = a->query_token_stride;
   p.q_head = a->query_head_stride;
   p.pages_stride = a->page_table_stride;
-  p.row_values = a->num_kv_heads * a->head_dim;
+  p.row_bytes = static_cast<unsigned>(a->num_kv_heads * a->head_dim * 2);
   // key / page_size = key * magic >> shift for every key below 2^31: magic
   // exceeds 2^shift / page_size by at most 1, and 2^(shift - 31) >= page_size.
   int bits = 0;
