@@ -690,3 +690,37 @@ def paged_attention_workspace_bytes(args: PagedAttentionArgs) -> int:
 def paged_attention(args: PagedAttentionArgs, stream: int) -> None:
     args.struct_size = ctypes.sizeof(PagedAttentionArgs)
     _check(load_library().ll_paged_attention(ctypes.byref(args), _ptr(int(stream))))
+
+
+def step_calls():
+    """The native module that makes a step's calls from their tensors, or None
+    where it is not built or was built for another torch or other argument
+    blocks: the Python checks then take every call, with the same result."""
+
+    try:
+        from . import _step_calls as module
+    except ImportError:
+        return None
+    built_for = tuple(getattr(module, name, None)
+                      for name in ("TORCH_VERSION", "HEAD_ROTARY_ARGS_SIZE", "PAGED_ATTENTION_ARGS_SIZE"))
+    here = (torch.__version__.split("+")[0], ctypes.sizeof(HeadRotaryArgs), ctypes.sizeof(PagedAttentionArgs))
+    return module if built_for == here else None
+
+
+_entry_addresses: dict[str, int] = {}
+
+
+def entry_address(name: str) -> int:
+    """Address of a library entry, for the native step calls."""
+
+    address = _entry_addresses.get(name)
+    if address is None:
+        address = ctypes.cast(getattr(load_library(), name), _ptr).value
+        _entry_addresses[name] = address
+    return address
+
+
+def check_status(status: int) -> None:
+    """Raises for a status that a native step call brought back."""
+
+    _check(status)

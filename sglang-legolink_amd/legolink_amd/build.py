@@ -38,6 +38,10 @@ HOST_SEQUENCES_OUTPUT = PACKAGE_DIR / f"_host_sequences{sysconfig.get_config_var
 # built with the C++ compiler against this interpreter and its torch).
 LINK_ARGUMENTS_SOURCE = PACKAGE_DIR.parent / "csrc" / "link_arguments.cpp"
 LINK_ARGUMENTS_OUTPUT = PACKAGE_DIR / f"_link_arguments{sysconfig.get_config_var('EXT_SUFFIX')}"
+# The Python module that makes a step's calls from their tensors (host code only,
+# built likewise).
+STEP_CALLS_SOURCE = PACKAGE_DIR.parent / "csrc" / "step_calls.cpp"
+STEP_CALLS_OUTPUT = PACKAGE_DIR / f"_step_calls{sysconfig.get_config_var('EXT_SUFFIX')}"
 # The same library with its host code under AddressSanitizer and
 # UndefinedBehaviorSanitizer (device code unchanged), for the CPU tests of the
 # host entries; never loaded on a GPU.
@@ -76,7 +80,7 @@ def build_library(verbose: bool = False, *, sanitize_host: bool = False) -> Path
     output is replaced atomically.  ``sanitize_host`` builds the host-sanitized
     copy (SANITIZED_OUTPUT) instead.  The unsanitized build also builds the
     calibration library (CALIBRATION_OUTPUT) and the host modules
-    (HOST_SEQUENCES_OUTPUT, LINK_ARGUMENTS_OUTPUT)."""
+    (HOST_SEQUENCES_OUTPUT, LINK_ARGUMENTS_OUTPUT, STEP_CALLS_OUTPUT)."""
 
     output = SANITIZED_OUTPUT if sanitize_host else OUTPUT
     extra = SANITIZE_FLAGS if sanitize_host else []
@@ -103,17 +107,19 @@ def build_library(verbose: bool = False, *, sanitize_host: bool = False) -> Path
                                            str(HOST_SEQUENCES_SOURCE)],
                                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True),
                          HOST_SEQUENCES_SOURCE))
-            link_arguments_tmp = Path(scratch) / LINK_ARGUMENTS_OUTPUT.name
             torch_dir = Path(importlib.util.find_spec("torch").origin).parent
-            jobs.append((subprocess.Popen([os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17",
-                                           "-shared", "-fPIC", "-Wall", f"-I{INCLUDE_DIR}",
-                                           f"-I{torch_dir / 'include'}",
-                                           f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-                                           f"-I{sysconfig.get_paths()['include']}", "-o", str(link_arguments_tmp),
-                                           str(LINK_ARGUMENTS_SOURCE), f"-L{torch_dir / 'lib'}", "-ltorch_python",
-                                           "-ltorch", "-ltorch_cpu", "-lc10"],
-                                          stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True),
-                         LINK_ARGUMENTS_SOURCE))
+            torch_modules = []
+            for source, target in ((LINK_ARGUMENTS_SOURCE, LINK_ARGUMENTS_OUTPUT), (STEP_CALLS_SOURCE, STEP_CALLS_OUTPUT)):
+                temporary = Path(scratch) / target.name
+                torch_modules.append((temporary, target))
+                jobs.append((subprocess.Popen([os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2",
+                                               "-std=c++17", "-shared", "-fPIC", "-Wall", f"-I{INCLUDE_DIR}",
+                                               f"-I{torch_dir / 'include'}",
+                                               f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+                                               f"-I{sysconfig.get_paths()['include']}", "-o", str(temporary),
+                                               str(source), f"-L{torch_dir / 'lib'}", "-ltorch_python",
+                                               "-ltorch", "-ltorch_cpu", "-lc10"],
+                                              stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True), source))
         failures = []
         for job, source in jobs:
             printed, _ = job.communicate()
@@ -134,7 +140,8 @@ def build_library(verbose: bool = False, *, sanitize_host: bool = False) -> Path
         if calibration is not None:
             os.replace(calibration_tmp, CALIBRATION_OUTPUT)
             os.replace(host_sequences_tmp, HOST_SEQUENCES_OUTPUT)
-            os.replace(link_arguments_tmp, LINK_ARGUMENTS_OUTPUT)
+            for temporary, target in torch_modules:
+                os.replace(temporary, target)
     return output
 
 

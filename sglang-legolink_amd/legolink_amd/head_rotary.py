@@ -32,6 +32,11 @@ _TABLE_DTYPES = {**_DTYPES, torch.float32: _native.DTYPE_FLOAT32}
 _INDEX_DTYPES = {torch.int32: _native.DTYPE_INT32, torch.int64: _native.DTYPE_INT64}
 
 
+# Both calls in one native call where it takes them; the Python checks take the
+# others, and name the reason where a call must not run.
+_calls = _native.step_calls()
+
+
 class HeadRotaryError(RuntimeError):
     """A norm-and-rotate or append call that must not run."""
 
@@ -194,6 +199,16 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, *, positions: torch.Ten
     ``skipped_rows`` counts it.
     """
 
+    if _calls is not None and query.is_cuda:
+        device = torch._C._cuda_getDevice()
+        done = _calls.rotate_heads(
+            _native.entry_address("ll_head_rotary"), torch._C._cuda_getCurrentRawStream(device), device, query, key,
+            positions, cos_sin_cache, rotary_dim, is_neox_style, query_norm_weight, key_norm_weight, norm_eps,
+            skipped_rows, query_output, key_output)
+        if type(done) is tuple:
+            return done
+        if done is not None:
+            _native.check_status(done)
     _refuse_gradients(query, key, query_norm_weight, key_norm_weight, cos_sin_cache, query_output, key_output)
     args = _rotary_args(query, key, positions, cos_sin_cache, rotary_dim, is_neox_style, query_norm_weight,
                         key_norm_weight, norm_eps, skipped_rows)
@@ -235,6 +250,16 @@ def append_rotated_kv_inplace(*, key_buffer: torch.Tensor, value_buffer: torch.T
     are written must be pairwise distinct.
     """
 
+    if _calls is not None and query.is_cuda:
+        device = torch._C._cuda_getDevice()
+        done = _calls.append(
+            _native.entry_address("ll_head_rotary"), torch._C._cuda_getCurrentRawStream(device), device, query, key,
+            positions, cos_sin_cache, rotary_dim, is_neox_style, query_norm_weight, key_norm_weight, norm_eps,
+            skipped_rows, query_output, value, key_buffer, value_buffer, destination_slots)
+        if type(done) is int:
+            _native.check_status(done)
+        elif done is not None:
+            return done
     _refuse_gradients(query, key, value, query_norm_weight, key_norm_weight, cos_sin_cache, query_output,
                       key_buffer, value_buffer)
     args = _rotary_args(query, key, positions, cos_sin_cache, rotary_dim, is_neox_style, query_norm_weight,

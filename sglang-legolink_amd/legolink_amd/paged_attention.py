@@ -25,6 +25,12 @@ _DTYPES = {torch.float16: _native.DTYPE_FLOAT16, torch.bfloat16: _native.DTYPE_B
 _INDEX_DTYPES = {torch.int32: _native.DTYPE_INT32, torch.int64: _native.DTYPE_INT64}
 
 
+# The call in one native call where it takes it (an output of its own among
+# others is left to the Python checks, which also name the reason where a call
+# must not run).
+_calls = _native.step_calls()
+
+
 class PagedAttentionError(RuntimeError):
     """A paged attention call that must not run."""
 
@@ -59,6 +65,16 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
     to that stream (or to the graph that captures the call).
     """
 
+    if _calls is not None and output is None and query.is_cuda:
+        current = torch._C._cuda_getDevice()
+        done = _calls.paged_attention(
+            _native.entry_address("ll_paged_attention"), torch._C._cuda_getCurrentRawStream(current), current,
+            _native.entry_address("ll_paged_attention_workspace_bytes"), query, key_buffer, value_buffer, page_table,
+            kv_lengths, page_size, query_starts, scale)
+        if type(done) is int:
+            _native.check_status(done)
+        elif done is not None:
+            return done
     if torch.is_grad_enabled() and any(t.requires_grad for t in (query, key_buffer, value_buffer)):
         raise PagedAttentionError("paged attention has no gradient: call it under torch.no_grad()")
     device, dtype = query.device, query.dtype
