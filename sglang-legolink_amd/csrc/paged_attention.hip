@@ -632,8 +632,8 @@ struct Wide {
   static constexpr int kChunksPerRow = D / 8;
   static constexpr int kGathers = kStage / (16 * kWave) / kWaves;  // a wave's, of K and of V, per tile
   static constexpr int kList = 7168;                               // slots held at a time
-  __device__ static int k_swizzle(int t) { return D >= 128 ? t % 16 : (t / 2) % 8; }
-  __device__ static int v_swizzle(int t) { return D >= 128 ? 4 * (t % 4) : 4 * ((t / 2) % 2); }
+  __host__ __device__ static constexpr int k_swizzle(int t) { return D >= 128 ? t % 16 : (t / 2) % 8; }
+  __host__ __device__ static constexpr int v_swizzle(int t) { return D >= 128 ? 4 * (t % 4) : 4 * ((t / 2) % 2); }
 };
 
 template <int D, typename E>
@@ -702,32 +702,28 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   const float slack = kSlack / scale_log2;
 
   // The wave's share of a tile's gathers: instruction j fills the 64 16-byte
-  // chunks from 64 (kGathers wave + j) on; a lane's chunk is of row `token`.
+  // chunks from 64 (kGathers wave + j) on.  Its rows are kRows j further than
+  // instruction 0's, which changes their swizzles by an xor (tokens of a wave begin
+  // at a multiple of kGathers kRows).
   const unsigned char *k_base = reinterpret_cast<const unsigned char *>(p.k + static_cast<long long>(head) * D);
   const unsigned char *v_base = reinterpret_cast<const unsigned char *>(p.v + static_cast<long long>(head) * D);
-  int g_token[W::kGathers];
-  unsigned g_k[W::kGathers], g_v[W::kGathers];  // the bytes of the lane's chunk within a row
-#pragma unroll
-  for (int j = 0; j < W::kGathers; ++j) {
-    const int at = (W::kGathers * wave + j) * kWave + lane;
-    g_token[j] = at / W::kChunksPerRow;
-    g_k[j] = 16 * ((at % W::kChunksPerRow) ^ W::k_swizzle(g_token[j]));
-    g_v[j] = 16 * ((at % W::kChunksPerRow) ^ W::v_swizzle(g_token[j]));
-  }
-  const int share = W::kGathers * wave * kWave * 16;  // its first byte of a stage
-  auto slots_of = [&](int tile, int *slots) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < W::kGathers; ++j) slots[j] = max(slot_list[tile * W::kKeys + g_token[j]], 0);
+  constexpr int kRows = kWave / W::kChunksPerRow;
+  const int g_token = W::kGathers * wave * kRows + lane / W::kChunksPerRow;
+  unsigned g_k = 16 * ((lane % W::kChunksPerRow) ^ W::k_swizzle(g_token));  // the lane's bytes of a row
+  unsigned g_v = 16 * ((lane % W::kChunksPerRow) ^ W::v_swizzle(g_token));
+  const int share = W::kGathers * wave * kWave * 16;  // the wave's first byte of a stage
+  auto slot_of = [&](int tile, int j) __attribute__((always_inline)) {
+    return max(slot_list[tile * W::kKeys + g_token + j * kRows], 0);
   };
-  auto gather_k = [&](const int *slots, int stage) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < W::kGathers; ++j)
-      dma_row(row_at(p, k_base, slots[j]) + g_k[j], k_ring + stage * W::kStage + share + j * kWave * 16);
+  auto gather_k = [&](int slot, int stage, int j) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(g_k));  // (made per use: fewer registers over the loop)
+    dma_row(row_at(p, k_base, slot) + (g_k ^ (16u * W::k_swizzle(j * kRows))),
+            k_ring + stage * W::kStage + share + j * kWave * 16);
   };
-  auto gather_v = [&](const int *slots, int stage) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < W::kGathers; ++j)
-      dma_row(row_at(p, v_base, slots[j]) + g_v[j], v_ring + stage * W::kStage + share + j * kWave * 16);
+  auto gather_v = [&](int slot, int stage, int j) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(g_v));
+    dma_row(row_at(p, v_base, slot) + (g_v ^ (16u * W::v_swizzle(j * kRows))),
+            v_ring + stage * W::kStage + share + j * kWave * 16);
   };
 
   // Offsets of the lane's fragments within a stage.
@@ -755,7 +751,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   // ahead of the MFMAs that take them: eight transposed reads (every dim block of a
   // 16-key step; keys 16 step + 4 h .. + 3 and, 8 further, the second read), or
   // four rows' chunks (two 16-dim steps of both 32-key blocks).
-  auto products = [&](int v_stage, int k_stage, auto values_tag) __attribute__((always_inline)) {
+  // Four waves: before(i) is called ahead of the reads of batch i, after(i) behind
+  // its MFMAs.
+  auto products = [&](int v_stage, int k_stage, auto values_tag, auto before, auto after) __attribute__((always_inline)) {
+    auto fence = [] { if constexpr (W::kWaves == 4) __builtin_amdgcn_sched_barrier(0); };
     constexpr bool values = decltype(values_tag)::value;  // else scores alone
     constexpr int kBatches = kKSteps / 2;
     const unsigned char *rows = k_ring + k_stage * W::kStage;
@@ -788,10 +787,14 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       load_v(0);
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
+        before(step);
         if (step + 1 < 4) load_v(step + 1);
         else load_k(0);
+        fence();
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) o[b] = E::mfma32(__builtin_bit_cast(frag, vf[step % 2][b]), pb[step], o[b]);
+        after(step);
+        fence();
       }
     } else {
       load_k(0);
@@ -802,12 +805,17 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
     for (int batch = 0; batch < kBatches; ++batch) {
+      before(4 + batch);
       if (batch + 1 < kBatches) load_k(batch + 1);
+      fence();
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma32(kf[batch % 2][2 * j + kb], qf[2 * batch + j], s[kb]);
+      after(4 + batch);
+      fence();
     }
+    if constexpr (W::kWaves == 4) return;
     // The order above, kept: reads (0x100) and MFMAs (0x008) in turn.
     if constexpr (values) {
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * kBlocks, 0);
@@ -901,77 +909,141 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     wait_vm<0>();
     __syncthreads();
 
-    // K tiles 0 .. kLead - 1 and V tiles 0 .. kLead - 2.
+    // K tiles 0 .. kLead - 1 and V tiles 0 .. kLead - 2.  (Past the last tile the
+    // last is gathered again, into stages that no products take: every iteration
+    // issues the same count, without branches.)
+    const int last = tiles - 1;
 #pragma unroll
     for (int t = 0; t < kLead; ++t) {
-      if (t >= tiles) break;
-      int slots[W::kGathers];
-      slots_of(t, slots);
-      gather_k(slots, t % W::kStages);
-      if (t + 1 < kLead) gather_v(slots, t);
+#pragma unroll
+      for (int j = 0; j < W::kGathers; ++j) {
+        const int slot = slot_of(min(t, last), j);
+        gather_k(slot, t % W::kStages, j);
+        if (t + 1 < kLead) gather_v(slot, t, j);
+      }
     }
     wait_vm<0>();
     workgroup_barrier();
     if (behind) workgroup_barrier();
-    if (list_begin < wave_stop) products(0, 0, std::false_type{});
+    const auto nothing = [](int) {};
+    if (list_begin < wave_stop) products(0, 0, std::false_type{}, nothing, nothing);
+    // Tile t's bits of keys with a row.
+    auto valid_keys = [&](int t) __attribute__((always_inline)) {
+      const unsigned long long bits = tile_valid[t];
+      // readfirstlane returns int: each half goes through unsigned.
+      const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits))));
+      const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits >> 32))));
+      return (static_cast<unsigned long long>(hi) << 32) | lo;
+    };
+    // The wave's share of V tile t, gathered, as the products may take it.
+    auto settle_values = [&](int t, int stage, unsigned long long valid) __attribute__((always_inline)) {
+      unsigned char *own = v_ring + stage * W::kStage + share + lane * 16;
+      if (valid != ~0ull) {
+        // Rows that no column sees may hold anything: zeros in their place.
+#pragma unroll
+        for (int j = 0; j < W::kGathers; ++j)
+          if (((valid >> (g_token + j * kRows)) & 1ull) == 0)
+            *reinterpret_cast<u32x4 *>(own + j * kWave * 16) = u32x4{0u, 0u, 0u, 0u};
+      }
+      if (list_begin + (t + 1) * W::kKeys > seen_in_part) {
+#pragma unroll 1
+        for (int j = 0; j < W::kGathers; ++j) {
+          u32x4 *chunk = reinterpret_cast<u32x4 *>(own + j * kWave * 16);
+          if (any_nonfinite<E>(*chunk)) {
+            *chunk = finite_only<E>(*chunk);
+            const int row = g_token + j * kRows;
+            atomicOr(&odd_rows[2 * t + row / 32], 1u << (row % 32));
+          }
+        }
+      }
+    };
+    // Eight waves, one half a phase behind the other.
     auto iteration = [&](const int t, auto stage_tag) __attribute__((always_inline)) {
       constexpr int stage = decltype(stage_tag)::value;  // t % kStages
       const int key0 = list_begin + t * W::kKeys;
       const bool computes = key0 < wave_stop;
       // The next gathers' slots are read ahead of the barrier that they wait for.
       int k_slots[W::kGathers], v_slots[W::kGathers];
-      if (t + kLead < tiles) slots_of(t + kLead, k_slots);
-      if (t + kLead - 1 < tiles) slots_of(t + kLead - 1, v_slots);
+#pragma unroll
+      for (int j = 0; j < W::kGathers; ++j) {
+        k_slots[j] = slot_of(min(t + kLead, last), j);
+        v_slots[j] = slot_of(min(t + kLead - 1, last), j);
+      }
       // The share of K tile t + 1 and V tile t: all but what the last kLead - 2
       // iterations issued.
-      if (t + kLead - 1 < tiles) wait_vm<2 * W::kGathers * (kLead - 2)>();
-      else wait_vm<0>();
-      const unsigned long long bits = tile_valid[t];
-      // readfirstlane returns int: each half goes through unsigned.
-      const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits))));
-      const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits >> 32))));
-      const unsigned long long valid = (static_cast<unsigned long long>(hi) << 32) | lo;
-      if (valid != ~0ull) {
-        // Rows that no column sees may hold anything: zeros in their place, by
-        // the wave that gathered them.
-#pragma unroll
-        for (int j = 0; j < W::kGathers; ++j)
-          if (((valid >> g_token[j]) & 1ull) == 0)
-            *reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16) =
-                u32x4{0u, 0u, 0u, 0u};
-      }
-      if (key0 + W::kKeys > seen_in_part) {
-#pragma unroll
-        for (int j = 0; j < W::kGathers; ++j) {
-          u32x4 *chunk = reinterpret_cast<u32x4 *>(v_ring + stage * W::kStage + share + (j * kWave + lane) * 16);
-          if (any_nonfinite<E>(*chunk)) {
-            *chunk = finite_only<E>(*chunk);
-            atomicOr(&odd_rows[2 * t + g_token[j] / 32], 1u << (g_token[j] % 32));
-          }
-        }
-      }
+      wait_vm<2 * W::kGathers * (kLead - 2)>();
+      const unsigned long long valid = valid_keys(t);
+      settle_values(t, stage, valid);
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's reads and writes of the stages are done
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
-      if (t + kLead < tiles) gather_k(k_slots, (stage + kLead) % W::kStages);
-      if (t + kLead - 1 < tiles) gather_v(v_slots, (stage + kLead - 1) % W::kStages);
+#pragma unroll
+      for (int j = 0; j < W::kGathers; ++j) {
+        gather_k(k_slots[j], (stage + kLead) % W::kStages, j);
+        gather_v(v_slots[j], (stage + kLead - 1) % W::kStages, j);
+      }
       if (computes) weigh_tile(key0, valid);
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
       __builtin_amdgcn_s_setprio(1);
       // (Behind the wave's last tile the scores are of an old stage, and not used.)
-      if (computes) products(stage, (stage + 1) % W::kStages, std::true_type{});
+      if (computes) products(stage, (stage + 1) % W::kStages, std::true_type{}, nothing, nothing);
       __builtin_amdgcn_s_setprio(0);
     };
-    for (int t = 0; t < tiles; t += W::kStages) {
-      iteration(t, std::integral_constant<int, 0>{});
-      if (t + 1 < tiles) iteration(t + 1, std::integral_constant<int, 1>{});
-      if constexpr (W::kStages == 4) {
+    // Four waves, alone on their SIMDs: one barrier a tile, and the gathers of K
+    // tile t + 2 and V tile t + 1 between the batches of its products, so that none
+    // waits behind the others' requests.
+    auto iteration_alone = [&](const int t, auto stage_tag) __attribute__((always_inline)) {
+      constexpr int stage = decltype(stage_tag)::value;  // t % kStages
+      const int key0 = list_begin + t * W::kKeys;
+      const bool computes = key0 < wave_stop;
+      const unsigned long long valid = valid_keys(t);
+      if (computes) weigh_tile(key0, valid);
+      wait_vm<0>();  // the share of K tile t + 1 and V tile t
+      settle_values(t, stage, valid);
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+      __builtin_amdgcn_sched_barrier(0);
+      workgroup_barrier();
+      // Turn i of 12: the gathers 4 i / 3 .. 4 (i + 1) / 3 - 1 of the 16; their
+      // slots first.
+      int slots[2];
+      auto slots_turn = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 4 * i / 3; g < 4 * (i + 1) / 3; ++g)
+          slots[g - 4 * i / 3] = slot_of(min(t + (g % 2 == 0 ? 1 : 2), last), g / 2);
+      };
+      auto gather_turn = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 4 * i / 3; g < 4 * (i + 1) / 3; ++g) {
+          if (g % 2 == 0) gather_v(slots[g - 4 * i / 3], (stage + 1) % W::kStages, g / 2);
+          else gather_k(slots[g - 4 * i / 3], stage, g / 2);
+        }
+      };
+      if (computes) {
+        products(stage, (stage + 1) % W::kStages, std::true_type{}, slots_turn, gather_turn);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 12; ++i) {
+          slots_turn(i);
+          gather_turn(i);
+        }
+      }
+    };
+    if constexpr (W::kWaves == 8) {
+      for (int t = 0; t < tiles; t += 4) {
+        iteration(t, std::integral_constant<int, 0>{});
+        if (t + 1 < tiles) iteration(t + 1, std::integral_constant<int, 1>{});
         if (t + 2 < tiles) iteration(t + 2, std::integral_constant<int, 2>{});
         if (t + 3 < tiles) iteration(t + 3, std::integral_constant<int, 3>{});
       }
+      if (!behind) workgroup_barrier();
+    } else {
+      for (int t = 0; t < tiles; t += 2) {
+        iteration_alone(t, std::integral_constant<int, 0>{});
+        if (t + 1 < tiles) iteration_alone(t + 1, std::integral_constant<int, 1>{});
+      }
     }
-    if (W::kWaves == 8 && !behind) workgroup_barrier();
+    wait_vm<0>();  // the last gathers, before their stages are taken again (or the workgroup ends)
     if (list_begin + listed > seen_in_part) {
       for (int base = 0; base < 2 * tiles; base += kWave) {
         const unsigned word = base + lane < 2 * tiles ? odd_rows[base + lane] : 0u;
