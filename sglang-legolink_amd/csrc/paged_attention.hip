@@ -98,13 +98,34 @@ __device__ inline const unsigned char *row_at(const PagedParams &p, const unsign
   return base + static_cast<unsigned long long>(static_cast<unsigned>(slot)) * p.row_bytes;
 }
 
-__device__ inline int inclusive_scan(int value, int lane) {
-#pragma unroll
-  for (int step = 1; step < kWave; step *= 2) {
-    const int other = __shfl_up(value, step);
-    if (lane >= step) value += other;
-  }
+// Lanes below, added within rows of 16 and then across them by DPP moves (a lane
+// without a source adds 0).
+template <int kControl, int kRows>
+__device__ inline int moved(int value) {
+  return __builtin_amdgcn_update_dpp(0, value, kControl, kRows, 0xf, false);
+}
+__device__ inline int inclusive_scan(int value) {
+  value += moved<0x111, 0xf>(value);  // row_shr 1, 2, 4, 8
+  value += moved<0x112, 0xf>(value);
+  value += moved<0x114, 0xf>(value);
+  value += moved<0x118, 0xf>(value);
+  value += moved<0x142, 0xa>(value);  // row_bcast 15: rows 1 and 3
+  value += moved<0x143, 0xc>(value);  // row_bcast 31: rows 2 and 3
   return value;
+}
+template <int kControl, int kRows>
+__device__ inline double moved(double value) {
+  return __hiloint2double(moved<kControl, kRows>(__double2hiint(value)), moved<kControl, kRows>(__double2loint(value)));
+}
+__device__ inline double sum_of_wave(double value) {
+  value += moved<0x111, 0xf>(value);
+  value += moved<0x112, 0xf>(value);
+  value += moved<0x114, 0xf>(value);
+  value += moved<0x118, 0xf>(value);
+  value += moved<0x142, 0xa>(value);
+  value += moved<0x143, 0xc>(value);
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(value), kWave - 1),
+                          __builtin_amdgcn_readlane(__double2loint(value), kWave - 1));
 }
 
 // What a workgroup has to do: the tile and its request, the chunk of a unit,
@@ -119,7 +140,7 @@ struct Work {
 
 // The request's columns (num_queries * G stays below 2^31).
 __device__ inline int tiles_of(const PagedParams &p, int q_len, int columns) {
-  return (q_len * p.group + columns - 1) / columns;
+  return (q_len * p.group + columns - 1) >> (31 - __builtin_clz(columns));  // (a power of two)
 }
 
 // Unit `index` of the call (kOfTiles: tile `index`).  Every wave finds it for
@@ -131,20 +152,14 @@ template <bool kOfTiles>
 __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
   const int lane = threadIdx.x % kWave;
   Request mine = Request{0, 0, 0};
-  long long work = 0;
+  double work = 0.0;  // (exact below 2^53)
   for (int r0 = 0; r0 < p.num_requests; r0 += kWave) {
     Request x = Request{0, 0, 0};
     if (r0 + lane < p.num_requests) x = request_at(p, r0 + lane);
     if (r0 == 0) mine = x;
-    work += static_cast<long long>(tiles_of(p, x.q_len, columns)) * ((x.kv_len + kPageTile - 1) / kPageTile);
+    work += static_cast<double>(tiles_of(p, x.q_len, columns)) * ((x.kv_len + kPageTile - 1) / kPageTile);
   }
-  if (p.num_requests > 1) {
-#pragma unroll
-    for (int step = 1; step < kWave; step *= 2) work += __shfl_xor(work, step);
-  } else {
-    work = __shfl(work, 0);
-  }
-  const double share = static_cast<double>(work) * p.inv_target;
+  const double share = sum_of_wave(work) * p.inv_target;
   // (2^25 key tiles are more than any length; readfirstlane: uniform to the compiler too)
   const int chunk = __builtin_amdgcn_readfirstlane(
       max(p.min_chunk, static_cast<int>(min(ceil(share - 1e-6), 33554432.0))));
@@ -163,10 +178,8 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
     const int key_tiles = (x.kv_len + kPageTile - 1) / kPageTile;
     const int chunks = max(1, (key_tiles + chunk - 1) / chunk);
     int units_to = tiles * chunks, tiles_to = tiles;
-    if (p.num_requests > 1) {
-      units_to = inclusive_scan(units_to, lane);
-      if constexpr (kOfTiles) tiles_to = inclusive_scan(tiles_to, lane);
-    }
+    units_to = inclusive_scan(units_to);
+    if constexpr (kOfTiles) tiles_to = inclusive_scan(tiles_to);
     const int reached = kOfTiles ? tiles_before + tiles_to : units_before + units_to;
     const unsigned long long past = __builtin_amdgcn_ballot_w64(reached > index && r0 + lane < p.num_requests);
     if (past != 0) {
@@ -279,8 +292,7 @@ __device__ inline void wait_vm() {
   __builtin_amdgcn_s_waitcnt(0xF70 | (n & 15) | ((n >> 4) << 14));
 }
 
-// Few columns (16 kTiles): single tokens and short chunks, bound by reading
-// the keys and values once.  The waves of a workgroup take turns at its 32-key
+// Up to 16 columns: single tokens, bound by reading the keys and values once.  The waves of a workgroup take turns at its 32-key
 // subtiles, each through an LDS ring of its own (no barriers: a wave waits for
 // its own gathers alone), and join their results at the end.  v_mfma_f32_16x16x32,
 // lane layouts: A and B lane l element e -> row / column l % 16, k = 8 (l / 16)
@@ -307,11 +319,11 @@ struct Narrow {
   __device__ static int v_swizzle(int t) { return D >= 128 ? 2 * (t % 8) : 2 * ((t / 2) % 4); }
 };
 
-template <int D, typename E, int kTiles>
+template <int D, typename E>
 __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const PagedParams p) {
   typedef Narrow<D> N;
   typedef typename E::frag frag;
-  constexpr int kColumns = 16 * kTiles;
+  constexpr int kColumns = 16;
   constexpr int kKSteps = D / 32;
   constexpr int kBlocks = D / 16;
   constexpr int kPitch = D + 4;  // floats of a joined row: 16 lanes' 16-byte writes meet 64 banks
@@ -335,36 +347,30 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
   const int col = lane % 16;
   unsigned char *ring = rings + wave * N::kRing;
 
-  // The lane's queries: one column of each 16-column tile.
-  frag qf[kTiles][kKSteps];
-  int pos[kTiles];
-  int seen_by_all = 0x7fffffff;  // keys below it are visible to every column
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    const int column = w.tile * kColumns + 16 * n + col;
-    const int token = column / p.group;
-    const bool exists = token < w.request.q_len;
-    const int h = head * p.group + (column - token * p.group);
-    pos[n] = exists ? w.request.kv_len - w.request.q_len + token : -1;
-    const uint16_t *row = p.q + (static_cast<long long>(w.request.q_start) + token) * p.q_token + h * p.q_head + 8 * g;
+  // The lane's column and its query.
+  const int column = w.tile * kColumns + col;
+  const int token = column / p.group;
+  const bool exists = token < w.request.q_len;
+  const int pos = exists ? w.request.kv_len - w.request.q_len + token : -1;
+  // Keys below it are visible to every column (to the first one, that is).
+  const int seen_by_all = w.request.kv_len - w.request.q_len + (w.tile * kColumns) / p.group + 1;
+  frag qf[kKSteps];
+  {
+    const int q_head = head * p.group + (column - token * p.group);
+    const uint16_t *row =
+        p.q + (static_cast<long long>(w.request.q_start) + token) * p.q_token + q_head * p.q_head + 8 * g;
 #pragma unroll
     for (int ks = 0; ks < kKSteps; ++ks) {
       u32x4 bits = u32x4{0u, 0u, 0u, 0u};
       if (exists) bits = *reinterpret_cast<const u32x4 *>(row + 32 * ks);
-      qf[n][ks] = __builtin_bit_cast(frag, bits);
+      qf[ks] = __builtin_bit_cast(frag, bits);
     }
   }
-  seen_by_all = w.request.kv_len - w.request.q_len + (w.tile * kColumns) / p.group + 1;  // the first column's
 
-  float m[kTiles], l[kTiles];
-  f32x4 o[kTiles][kBlocks];
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[kBlocks];
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) o[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int b = 0; b < kBlocks; ++b) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float scale_log2 = p.scale_log2;
   const float slack = kSlack / scale_log2;
 
@@ -457,62 +463,53 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
         asm volatile("" ::: "memory");
       }
 
-      f32x4 s[kTiles][2];
+      f32x4 s[2];
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n)
+      for (int rb = 0; rb < 2; ++rb) s[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) s[n][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < kKSteps; ++ks) {
+      for (int ks = 0; ks < kKSteps; ++ks)
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
           const frag kf = *reinterpret_cast<const frag *>(rows + k_off[ks] + rb * 16 * N::kRowBytes);
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) s[n][rb] = E::mfma16(kf, qf[n][ks], s[n][rb]);
+          s[rb] = E::mfma16(kf, qf[ks], s[rb]);
         }
-      }
-      frag pb[kTiles];
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        if (!whole) {
-#pragma unroll
-          for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int rel = 16 * rb + 4 * g + r;
-              const bool visible = ((valid >> rel) & 1u) != 0 && key0 + rel <= pos[n];
-              s[n][rb][r] = visible ? s[n][rb][r] : -INFINITY;
-            }
-        }
-        float top = -INFINITY;
+      if (!whole) {
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[n][rb][r]);
-        top = max_of_groups(top);
-        const bool raise = top > m[n] + slack;
-        const float m_new = raise ? top : m[n];
-        const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[n][rb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][rb][r], scale_log2, bias));
-        if (__builtin_amdgcn_ballot_w64(raise) != 0) {
-          const float alpha = raise ? __builtin_amdgcn_exp2f((m[n] - m_new) * scale_log2) : 1.f;
-          l[n] *= alpha;
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) o[n][b] *= alpha;
-        }
-        m[n] = m_new;
-        u32x4 bits;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          bits[j] = E::pack(s[n][j / 2][2 * (j % 2)], s[n][j / 2][2 * (j % 2) + 1]);
-          l[n] = E::dot2_ones(bits[j], l[n]);  // the weights that the value product sees
-        }
-        pb[n] = __builtin_bit_cast(frag, bits);
+          for (int r = 0; r < 4; ++r) {
+            const int rel = 16 * rb + 4 * g + r;
+            const bool visible = ((valid >> rel) & 1u) != 0 && key0 + rel <= pos;
+            s[rb][r] = visible ? s[rb][r] : -INFINITY;
+          }
       }
+      float top = -INFINITY;
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[rb][r]);
+      top = max_of_groups(top);
+      const bool raise = top > m + slack;
+      const float m_new = raise ? top : m;
+      const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[rb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][r], scale_log2, bias));
+      if (__builtin_amdgcn_ballot_w64(raise) != 0) {
+        const float alpha = raise ? __builtin_amdgcn_exp2f((m - m_new) * scale_log2) : 1.f;
+        l *= alpha;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) o[b] *= alpha;
+      }
+      m = m_new;
+      u32x4 weights;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        weights[j] = E::pack(s[j / 2][2 * (j % 2)], s[j / 2][2 * (j % 2) + 1]);
+        l = E::dot2_ones(weights[j], l);  // the weights that the value product sees
+      }
+      const frag pb = __builtin_bit_cast(frag, weights);
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
         const unsigned at = ring_lds + stage * N::kStage + v_off[b];
@@ -524,8 +521,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
         va[1] = __builtin_bit_cast(u32x2, lo)[1];
         va[2] = __builtin_bit_cast(u32x2, hi)[0];
         va[3] = __builtin_bit_cast(u32x2, hi)[1];
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) o[n][b] = E::mfma16(__builtin_bit_cast(frag, va), pb[n], o[n][b]);
+        o[b] = E::mfma16(__builtin_bit_cast(frag, va), pb, o[b]);
       }
       while (odd != 0) {
         const int rel = __builtin_ctz(odd);
@@ -534,9 +530,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
           const f32x4 x = nonfinite_only<E>(*reinterpret_cast<const u32x2 *>(row + 32 * b));
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n)
-            if (key0 + rel <= pos[n]) o[n][b] += x;
+          if (key0 + rel <= pos) o[b] += x;
           __builtin_amdgcn_sched_barrier(0);  // (rare: few registers rather than loads in flight)
         }
       }
@@ -547,51 +541,46 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
     }
   }
 
-  // The waves' results joined, 16 columns at a time.
+  // The waves' results joined.
   const bool direct = w.chunks == 1;
   float *partial = direct ? nullptr : partial_of<D>(p, kColumns, unit, head);
   float *joined = reinterpret_cast<float *>(rings);
+  __syncthreads();  // the rings are read
+  const float total = sum_of_groups(l);
+  if (g == 0) {
+    stats[wave][col][0] = m == -INFINITY ? -INFINITY : m * scale_log2;
+    stats[wave][col][1] = total;
+  }
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    __syncthreads();  // the rings (or the tile before) are read
-    const float total = sum_of_groups(l[n]);
-    if (g == 0) {
-      stats[wave][16 * n + col][0] = m[n] == -INFINITY ? -INFINITY : m[n] * scale_log2;
-      stats[wave][16 * n + col][1] = total;
+  for (int b = 0; b < kBlocks; ++b)
+    *reinterpret_cast<f32x4 *>(joined + (wave * 16 + col) * kPitch + 16 * b + 4 * g) = o[b];
+  __syncthreads();
+  for (int i = tid; i < 16 * (D / 4); i += N::kThreads) {
+    const int c = i / (D / 4);
+    const int quad = i % (D / 4);
+    if ((w.tile * kColumns + c) / p.group >= w.request.q_len) continue;
+    float top = stats[0][c][0];
+#pragma unroll
+    for (int v = 1; v < N::kWaves; ++v) top = fmaxf(top, stats[v][c][0]);
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < N::kWaves; ++v) {
+      const float weight = joined_weight(stats[v][c][0], top);
+      sum += weight * stats[v][c][1];
+      acc += weight * *reinterpret_cast<const f32x4 *>(joined + (v * 16 + c) * kPitch + 4 * quad);
     }
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-      *reinterpret_cast<f32x4 *>(joined + (wave * 16 + col) * kPitch + 16 * b + 4 * g) = o[n][b];
-    __syncthreads();
-    for (int i = tid; i < 16 * (D / 4); i += N::kThreads) {
-      const int c = i / (D / 4);
-      const int quad = i % (D / 4);
-      const int column = w.tile * kColumns + 16 * n + c;
-      if (column / p.group >= w.request.q_len) continue;
-      float top = stats[0][16 * n + c][0];
-#pragma unroll
-      for (int v = 1; v < N::kWaves; ++v) top = fmaxf(top, stats[v][16 * n + c][0]);
-      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-      float sum = 0.f;
-#pragma unroll
-      for (int v = 0; v < N::kWaves; ++v) {
-        const float own = stats[v][16 * n + c][0];
-        const float weight = joined_weight(own, top);
-        sum += weight * stats[v][16 * n + c][1];
-        acc += weight * *reinterpret_cast<const f32x4 *>(joined + (v * 16 + c) * kPitch + 4 * quad);
-      }
-      if (direct) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
-        u32x2 packed;
-        packed[0] = E::pack(acc[0] * inv, acc[1] * inv);
-        packed[1] = E::pack(acc[2] * inv, acc[3] * inv);
-        *reinterpret_cast<u32x2 *>(output_row(p, w, head, column, D) + 4 * quad) = packed;
-      } else {
-        *reinterpret_cast<f32x4 *>(partial + (16 * n + c) * D + 4 * quad) = acc;
-        if (quad == 0) {
-          partial[kColumns * D + 2 * (16 * n + c)] = top;
-          partial[kColumns * D + 2 * (16 * n + c) + 1] = sum;
-        }
+    if (direct) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+      u32x2 packed;
+      packed[0] = E::pack(acc[0] * inv, acc[1] * inv);
+      packed[1] = E::pack(acc[2] * inv, acc[3] * inv);
+      *reinterpret_cast<u32x2 *>(output_row(p, w, head, w.tile * kColumns + c, D) + 4 * quad) = packed;
+    } else {
+      *reinterpret_cast<f32x4 *>(partial + c * D + 4 * quad) = acc;
+      if (quad == 0) {
+        partial[kColumns * D + 2 * c] = top;
+        partial[kColumns * D + 2 * c + 1] = sum;
       }
     }
   }
@@ -750,11 +739,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   // the scores of the next (stage k_stage) into s.  Fragments are read one batch
   // ahead of the MFMAs that take them: eight transposed reads (every dim block of a
   // 16-key step; keys 16 step + 4 h .. + 3 and, 8 further, the second read), or
-  // four rows' chunks (two 16-dim steps of both 32-key blocks).
-  // Four waves: before(i) is called ahead of the reads of batch i, after(i) behind
-  // its MFMAs.
+  // four rows' chunks (two 16-dim steps of both 32-key blocks).  before(i) is called
+  // ahead of the reads of batch i, after(i) behind its MFMAs.
   auto products = [&](int v_stage, int k_stage, auto values_tag, auto before, auto after) __attribute__((always_inline)) {
-    auto fence = [] { if constexpr (W::kWaves == 4) __builtin_amdgcn_sched_barrier(0); };
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };  // the order below, kept
     constexpr bool values = decltype(values_tag)::value;  // else scores alone
     constexpr int kBatches = kKSteps / 2;
     const unsigned char *rows = k_ring + k_stage * W::kStage;
@@ -814,24 +802,6 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
         for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma32(kf[batch % 2][2 * j + kb], qf[2 * batch + j], s[kb]);
       after(4 + batch);
       fence();
-    }
-    if constexpr (W::kWaves == 4) return;
-    // The order above, kept: reads (0x100) and MFMAs (0x008) in turn.
-    if constexpr (values) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 2 * kBlocks, 0);
-#pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        if (step + 1 < 4) __builtin_amdgcn_sched_group_barrier(0x100, 2 * kBlocks, 0);
-        else __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, kBlocks, 0);
-      }
-    } else {
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-    }
-#pragma unroll
-    for (int batch = 0; batch < kBatches; ++batch) {
-      if (batch + 1 < kBatches) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
   };
   // The weights of the scores in s, into pb; the sums so far rescaled where the maximum rises.
@@ -915,14 +885,19 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     const int last = tiles - 1;
 #pragma unroll
     for (int t = 0; t < kLead; ++t) {
+      int slots[W::kGathers];
 #pragma unroll
-      for (int j = 0; j < W::kGathers; ++j) {
-        const int slot = slot_of(min(t, last), j);
-        gather_k(slot, t % W::kStages, j);
-        if (t + 1 < kLead) gather_v(slot, t, j);
+      for (int j = 0; j < W::kGathers; ++j) slots[j] = slot_of(min(t, last), j);
+#pragma unroll
+      for (int j = 0; j < W::kGathers; ++j) gather_k(slots[j], t % W::kStages, j);
+      if (t + 1 < kLead) {
+#pragma unroll
+        for (int j = 0; j < W::kGathers; ++j) gather_v(slots[j], t, j);
       }
     }
-    wait_vm<0>();
+    // K tile 0 is there once the rest, issued after it, is all that is outstanding
+    // (kLead - 1 tiles of each).
+    wait_vm<2 * W::kGathers * (kLead - 1)>();
     workgroup_barrier();
     if (behind) workgroup_barrier();
     const auto nothing = [](int) {};
@@ -957,37 +932,46 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
         }
       }
     };
-    // Eight waves, one half a phase behind the other.
+    // Eight waves, one half a phase behind the other.  What a tile needs from the
+    // slot list is read during the softmax before it: between the products and the
+    // barrier behind them a wave only waits.
+    int k_slots[W::kGathers], v_slots[W::kGathers];
+    unsigned long long valid = valid_keys(0);
     auto iteration = [&](const int t, auto stage_tag) __attribute__((always_inline)) {
       constexpr int stage = decltype(stage_tag)::value;  // t % kStages
       const int key0 = list_begin + t * W::kKeys;
       const bool computes = key0 < wave_stop;
-      // The next gathers' slots are read ahead of the barrier that they wait for.
-      int k_slots[W::kGathers], v_slots[W::kGathers];
-#pragma unroll
-      for (int j = 0; j < W::kGathers; ++j) {
-        k_slots[j] = slot_of(min(t + kLead, last), j);
-        v_slots[j] = slot_of(min(t + kLead - 1, last), j);
-      }
       // The share of K tile t + 1 and V tile t: all but what the last kLead - 2
       // iterations issued.
       wait_vm<2 * W::kGathers * (kLead - 2)>();
-      const unsigned long long valid = valid_keys(t);
       settle_values(t, stage, valid);
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's reads and writes of the stages are done
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
 #pragma unroll
       for (int j = 0; j < W::kGathers; ++j) {
-        gather_k(k_slots[j], (stage + kLead) % W::kStages, j);
-        gather_v(v_slots[j], (stage + kLead - 1) % W::kStages, j);
+        k_slots[j] = slot_of(min(t + kLead, last), j);
+        v_slots[j] = slot_of(min(t + kLead - 1, last), j);
       }
+      const unsigned long long next_valid = valid_keys(min(t + 1, last));
       if (computes) weigh_tile(key0, valid);
+      valid = next_valid;
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
+      // The gathers between the steps of the values, in the shadow of their MFMAs.
+      auto gather_turn = [&](int i) __attribute__((always_inline)) {
+        if (i >= 2 * W::kGathers) return;
+        if (i % 2 == 0) gather_k(k_slots[i / 2], (stage + kLead) % W::kStages, i / 2);
+        else gather_v(v_slots[i / 2], (stage + kLead - 1) % W::kStages, i / 2);
+      };
       __builtin_amdgcn_s_setprio(1);
       // (Behind the wave's last tile the scores are of an old stage, and not used.)
-      if (computes) products(stage, (stage + 1) % W::kStages, std::true_type{}, nothing, nothing);
+      if (computes) {
+        products(stage, (stage + 1) % W::kStages, std::true_type{}, nothing, gather_turn);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * W::kGathers; ++i) gather_turn(i);
+      }
       __builtin_amdgcn_s_setprio(0);
     };
     // Four waves, alone on their SIMDs: one barrier a tile, and the gathers of K
@@ -997,10 +981,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       constexpr int stage = decltype(stage_tag)::value;  // t % kStages
       const int key0 = list_begin + t * W::kKeys;
       const bool computes = key0 < wave_stop;
-      const unsigned long long valid = valid_keys(t);
-      if (computes) weigh_tile(key0, valid);
+      const unsigned long long tile_keys = valid_keys(t);
+      if (computes) weigh_tile(key0, tile_keys);
       wait_vm<0>();  // the share of K tile t + 1 and V tile t
-      settle_values(t, stage, valid);
+      settle_values(t, stage, tile_keys);
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
@@ -1110,20 +1094,21 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
 }
 
 // Joins the partial results of tiles of more than one chunk.  A lane holds four
-// values of a column, so a wave 256 / D columns; a workgroup 16 columns or, with
-// kSplit 4 (few tiles of many chunks each, whose latency adds up), the columns of
-// one wave, the four waves taking turns at their chunks.  A batch's loads are in
-// flight together.
+// values of a column, so a wave 256 / D columns; a workgroup of four waves 16
+// columns or, with kSplit waves (few tiles of many chunks each, whose latency adds
+// up), the columns of one wave, the waves taking turns at their chunks.  A batch's
+// loads are in flight together.
 template <int D, int kSplit>
 struct Combine {
   static constexpr int kPerWave = 256 / D;
   static constexpr int kColumns = kSplit == 1 ? 16 : kPerWave;  // of a workgroup
   static constexpr int kTurns = kSplit == 1 ? kColumns / (4 * kPerWave) : 1;
   static constexpr int kBatch = kSplit == 1 ? 4 : 8;
+  static constexpr int kThreads = kSplit == 1 ? 256 : kSplit * kWave;
 };
 
 template <int D, typename E, int kSplit>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p, int columns) {
+__global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_kernel(const PagedParams p, int columns) {
   typedef Combine<D, kSplit> C;
   const int groups = columns / C::kColumns;
   const int tile_head = blockIdx.x / groups;
@@ -1214,11 +1199,14 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   Launch x;
   const long long group = a->num_q_heads / a->num_kv_heads;
   const long long queries = a->num_queries, requests = a->num_requests;
-  // Columns by the average request: whole chunks in as few tiles as they fill.
+  // By the average request's columns: up to 16 on the narrow kernel, more on the
+  // wide one (16 requests of 4 tokens over 4,000 keys, 64/8 heads: 47 us there, 68
+  // on a narrow kernel of 32 columns a wave; 20 columns each of 32 requests 90 and
+  // 83 us).
   const long long average = queries == 0 ? 1 : (queries + requests - 1) / requests;
   const long long wanted = average * group;
-  x.wide = wanted > (a->head_dim == 256 ? 32 : 64);
-  x.columns = x.wide ? (a->head_dim == 256 ? 128 : 256) : wanted <= 16 ? 16 : wanted <= 32 ? 32 : 64;
+  x.wide = wanted > 16;
+  x.columns = x.wide ? (a->head_dim == 256 ? 128 : 256) : 16;
   const long long tiles = a->query_starts == nullptr
                               ? requests * ((group + x.columns - 1) / x.columns)
                               : queries * group / x.columns + requests;
@@ -1291,27 +1279,26 @@ int check_args(const ll_paged_attention_args *a) {
 }
 
 template <int D, typename E>
-void launch_narrow(const PagedParams &p, const Launch &x, unsigned grid, hipStream_t s) {
-  constexpr int kThreads = Narrow<D>::kThreads;
-  if (x.columns == 16) paged_narrow_kernel<D, E, 1><<<grid, kThreads, 0, s>>>(p);
-  else if (x.columns == 32) paged_narrow_kernel<D, E, 2><<<grid, kThreads, 0, s>>>(p);
-  else if constexpr (D != 256) paged_narrow_kernel<D, E, 4><<<grid, kThreads, 0, s>>>(p);
-}
-
-template <int D, typename E>
 int launch_all(const PagedParams &p, const Launch &x, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(x.max_units) * static_cast<unsigned>(p.hkv);
   if (x.wide) paged_wide_kernel<D, E><<<grid, Wide<D>::kThreads, 0, s>>>(p);
-  else launch_narrow<D, E>(p, x, grid, s);
+  else paged_narrow_kernel<D, E><<<grid, Narrow<D>::kThreads, 0, s>>>(p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   if (!x.splits) return LL_OK;
   const unsigned tile_heads = static_cast<unsigned>(x.max_tiles) * static_cast<unsigned>(p.hkv);
   const unsigned columns = static_cast<unsigned>(x.columns);
-  if (x.target >= 8 * x.max_tiles && !x.wide)
-    paged_combine_kernel<D, E, 4><<<tile_heads * (columns / Combine<D, 4>::kColumns), 256, 0, s>>>(p, x.columns);
-  else
+  // Few tiles of many chunks: a column's chunks on several waves, eight where there
+  // may be more than 32 (64 chunks: 6.0 us on eight, 7.2 on four; 16 chunks: 4.9 and
+  // 4.4).  Elsewhere a wave for all chunks of its columns: workgroups that mostly
+  // find no column cost more than they save (16 requests on tiles of 256 columns).
+  const unsigned split_groups = tile_heads * (columns / Combine<D, 4>::kColumns);
+  if (x.target < 8 * x.max_tiles || split_groups > 4 * kComputeUnits)
     paged_combine_kernel<D, E, 1><<<tile_heads * (columns / Combine<D, 1>::kColumns), 256, 0, s>>>(p, x.columns);
+  else if (p.max_keys <= 32 * x.min_chunk * kPageTile)
+    paged_combine_kernel<D, E, 4><<<split_groups, 4 * kWave, 0, s>>>(p, x.columns);
+  else
+    paged_combine_kernel<D, E, 8><<<split_groups, 8 * kWave, 0, s>>>(p, x.columns);
   err = hipGetLastError();
   if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   return LL_OK;
