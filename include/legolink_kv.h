@@ -701,14 +701,15 @@ int64_t ll_head_rotary_args_size(void);
  *
  * The lengths, starts and pages are read on the device, so that one captured
  * call serves any lengths that its shapes hold: lengths are held to [0,
- * page_table_columns * page_size], starts to [0, num_queries] and to growing
- * order.  Keys of a page outside the pool are invisible (never read), as is
- * everything behind a request's length, whatever it holds.  Queries of no
- * request keep their output rows.
+ * page_table_columns * page_size] and starts to [0, num_queries], and a request
+ * that ends before it begins has no queries.  (Starts that do not grow, so that
+ * requests share queries, leave those rows undefined.)  Keys of a page outside
+ * the pool are invisible (never read), as is everything behind a request's
+ * length, whatever it holds.  Queries of no request keep their output rows.
  *
  * Workspace: ll_paged_attention_workspace_bytes(args), a bound that follows from
- * the shapes alone.  Calls that share one must not overlap; nothing in it
- * outlives the call.  One launch, and a second where a table row holds more than
+ * the shapes alone (70 MB at 4 KV heads of 128, whatever the lengths).  Calls
+ * that share one must not overlap; nothing in it outlives the call.  One launch, and a second where a table row holds more than
  * 128 keys (it joins the parts of requests whose keys were split).
  */
 typedef struct ll_paged_attention_args {

@@ -150,9 +150,9 @@ __global__ void __launch_bounds__(kThreads) head_rotary_vec_kernel(const RotaryP
   constexpr int kHeads = kWave / kGroup;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kThreads / kWave) + wave;
-  const long long t = unit / p.steps;
-  const int step = static_cast<int>(unit - t * p.steps);
+  const unsigned unit = blockIdx.x * (kThreads / kWave) + wave;  // (a launch holds fewer than 2^26)
+  const long long t = unit / static_cast<unsigned>(p.steps);
+  const int step = static_cast<int>(unit % static_cast<unsigned>(p.steps));
   if (t >= p.num_tokens) return;
 
   if (step >= p.turn_steps) {
@@ -266,9 +266,9 @@ __global__ void __launch_bounds__(kThreads) head_rotary_element_kernel(const Rot
   constexpr int kPer = kMaxDim / kWave;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kThreads / kWave) + wave;
-  const long long t = unit / p.steps;
-  const int row = static_cast<int>(unit - t * p.steps);
+  const unsigned unit = blockIdx.x * (kThreads / kWave) + wave;
+  const long long t = unit / static_cast<unsigned>(p.steps);
+  const int row = static_cast<int>(unit % static_cast<unsigned>(p.steps));
   if (t >= p.num_tokens) return;
   const Token token = token_at(p, t, row == 0);
   if (!token.turned) return;

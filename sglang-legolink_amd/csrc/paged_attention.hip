@@ -64,7 +64,7 @@ struct PagedParams {
   int num_queries, num_requests, hq, hkv, group;
   int lengths64, starts64;
   int min_chunk;  // key tiles
-  int max_units, max_tiles;
+  int max_partials;
   float scale_log2;
 };
 
@@ -134,7 +134,8 @@ struct Work {
   Request request;
   int index;  // of the request; -1: none
   int tile, chunk, chunk_keys;
-  int first_unit, unit_step, chunks;  // the tile's chunk c is unit first_unit + c unit_step
+  int chunks;                        // of the tile
+  int first_partial, partial_step;   // its chunk c leaves partial first_partial + c partial_step
   int key_end;             // keys that some column of the tile sees
 };
 
@@ -147,7 +148,9 @@ __device__ inline int tiles_of(const PagedParams &p, int q_len, int columns) {
 // itself: two passes over the requests, 64 at a time, the first for the call's
 // work in key tiles times column tiles.  With L = max(min_chunk, work / target)
 // key tiles a chunk, the units number at most work / L + tiles <= target +
-// tiles, which the launch holds.
+// tiles, which the launch holds.  Those of requests of more than one chunk, which
+// may leave partial results, number below 2 work / L <= 2 target + 2: a request of
+// k > L key tiles has fewer than k / L + 1 < 2 k / L chunks.
 template <bool kOfTiles>
 __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
   const int lane = threadIdx.x % kWave;
@@ -167,7 +170,7 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
   Work w;
   w.index = -1;
   w.chunk_keys = min(chunk, 33554431) * kPageTile;
-  int units_before = 0, tiles_before = 0;
+  int units_before = 0, tiles_before = 0, partials_before = 0;
   for (int r0 = 0; r0 < p.num_requests; r0 += kWave) {
     Request x = mine;
     if (r0 > 0) {
@@ -177,9 +180,9 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
     const int tiles = tiles_of(p, x.q_len, columns);
     const int key_tiles = (x.kv_len + kPageTile - 1) / kPageTile;
     const int chunks = max(1, (key_tiles + chunk - 1) / chunk);
-    int units_to = tiles * chunks, tiles_to = tiles;
-    units_to = inclusive_scan(units_to);
-    if constexpr (kOfTiles) tiles_to = inclusive_scan(tiles_to);
+    const int units_to = inclusive_scan(tiles * chunks);
+    const int partials_to = inclusive_scan(chunks > 1 ? tiles * chunks : 0);
+    const int tiles_to = kOfTiles ? inclusive_scan(tiles) : 0;
     const int reached = kOfTiles ? tiles_before + tiles_to : units_before + units_to;
     const unsigned long long past = __builtin_amdgcn_ballot_w64(reached > index && r0 + lane < p.num_requests);
     if (past != 0) {
@@ -203,8 +206,8 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
         nth = (index - first_unit) - w.chunk * own_tiles;
       }
       w.tile = own_tiles - 1 - nth;
-      w.first_unit = first_unit + nth;
-      w.unit_step = own_tiles;
+      w.first_partial = partials_before + __builtin_amdgcn_readlane(partials_to, at) - own_tiles * own_chunks + nth;
+      w.partial_step = own_tiles;
       // The tile's last query and its position bound the keys.
       const int last_query = min(w.request.q_len - 1, ((w.tile + 1) * columns - 1) / p.group);
       w.key_end = max(0, w.request.kv_len - w.request.q_len + last_query + 1);
@@ -212,16 +215,21 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
       break;
     }
     units_before += __builtin_amdgcn_readlane(units_to, kWave - 1);
+    partials_before += __builtin_amdgcn_readlane(partials_to, kWave - 1);
     if constexpr (kOfTiles) tiles_before += __builtin_amdgcn_readlane(tiles_to, kWave - 1);
   }
   return w;
 }
 
-// Partial result of a unit's KV head: `columns` rows of D floats (the sum of
-// the weighted values, unnormalised), then (maximum, sum) pairs.
+// A partial result of one KV head: `columns` rows of D floats (the sum of the
+// weighted values, unnormalised), then (maximum, sum) pairs.
 template <int D>
-__device__ inline float *partial_of(const PagedParams &p, int columns, int unit, int head) {
-  return p.ws + (static_cast<long long>(unit) * p.hkv + head) * columns * (D + 2);
+__device__ inline float *partial_of(const PagedParams &p, int columns, int partial, int head) {
+  return p.ws + (static_cast<long long>(partial) * p.hkv + head) * columns * (D + 2);
+}
+__device__ inline bool partials_fit(const PagedParams &p, const Work &w) {  // (always, by the bound above)
+  return w.first_partial >= 0 &&
+         w.first_partial + static_cast<long long>(w.chunks - 1) * w.partial_step < p.max_partials;
 }
 
 __device__ inline uint16_t *output_row(const PagedParams &p, const Work &w, int head, int column, int dim) {
@@ -335,7 +343,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
   const int head = blockIdx.x % p.hkv;
   const int unit = blockIdx.x / p.hkv;
   const Work w = find_work<false>(p, kColumns, unit);
-  if (w.index < 0 || w.chunk >= w.chunks) return;
+  if (w.index < 0 || w.chunk >= w.chunks || (w.chunks > 1 && !partials_fit(p, w))) return;
   const int key_begin = w.chunk * w.chunk_keys;  // below the tile's key_end, or 0
   int key_end = key_begin + min(w.chunk_keys, w.key_end - key_begin);
   if (p.num_pages == 0) key_end = key_begin;  // no row that may be read
@@ -543,7 +551,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 
   // The waves' results joined.
   const bool direct = w.chunks == 1;
-  float *partial = direct ? nullptr : partial_of<D>(p, kColumns, unit, head);
+  float *partial = direct ? nullptr : partial_of<D>(p, kColumns, w.first_partial + w.chunk * w.partial_step, head);
   float *joined = reinterpret_cast<float *>(rings);
   __syncthreads();  // the rings are read
   const float total = sum_of_groups(l);
@@ -641,7 +649,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   const int head = blockIdx.x % p.hkv;
   const int unit = blockIdx.x / p.hkv;
   const Work w = find_work<false>(p, W::kColumns, unit);
-  if (w.index < 0 || w.chunk >= w.chunks) return;
+  if (w.index < 0 || w.chunk >= w.chunks || (w.chunks > 1 && !partials_fit(p, w))) return;
   const int key_begin = w.chunk * w.chunk_keys;  // below the tile's key_end, or 0
   int key_end = key_begin + min(w.chunk_keys, w.key_end - key_begin);
   if (p.num_pages == 0) key_end = key_begin;  // no row that may be read
@@ -1075,7 +1083,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       }
     return;
   }
-  float *partial = partial_of<D>(p, W::kColumns, unit, head);
+  float *partial = partial_of<D>(p, W::kColumns, w.first_partial + w.chunk * w.partial_step, head);
   const int c = 32 * wave + col;
   if (h == 0) {
     partial[W::kColumns * D + 2 * c] = m == -INFINITY ? -INFINITY : m * scale_log2;
@@ -1114,9 +1122,7 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
   const int tile_head = blockIdx.x / groups;
   const int head = tile_head % p.hkv;
   const Work w = find_work<true>(p, columns, tile_head / p.hkv);
-  if (w.index < 0 || w.chunks <= 1 || w.first_unit < 0 ||
-      w.first_unit + static_cast<long long>(w.chunks - 1) * w.unit_step >= p.max_units)
-    return;
+  if (w.index < 0 || w.chunks <= 1 || !partials_fit(p, w)) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int quad = lane % (D / 4);
 #pragma unroll
@@ -1136,7 +1142,7 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
         // Past the last chunk: the last again, dropped.  (Columns that do not exist
         // are within the partial, and dropped too.)
         const int chunk = min(s0 + i * kSplit, w.chunks - 1);
-        const float *part = partial_of<D>(p, columns, w.first_unit + chunk * w.unit_step, head);
+        const float *part = partial_of<D>(p, columns, w.first_partial + chunk * w.partial_step, head);
         tops[i] = part[columns * D + 2 * c];
         sums[i] = part[columns * D + 2 * c + 1];
         rows[i] = *reinterpret_cast<const f32x4 *>(part + c * D + 4 * quad);
@@ -1188,7 +1194,7 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
 // How a call is launched: known from sizes that the host has.
 struct Launch {
   int columns;
-  int max_tiles, max_units, target, min_chunk;
+  int max_tiles, max_units, max_partials, target, min_chunk;
   bool wide, splits;
   long long ws_floats;
 };
@@ -1222,7 +1228,8 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   x.splits = max_keys > x.min_chunk * kPageTile;
   const long long units = tiles + (x.splits ? x.target + 1 : 0);
   x.max_units = static_cast<int>(std::min(units, 0x7fffffffll));
-  x.ws_floats = x.splits ? units * a->num_kv_heads * x.columns * (a->head_dim + 2) : 0;
+  x.max_partials = x.splits ? 2 * x.target + 2 : 0;
+  x.ws_floats = x.max_partials * a->num_kv_heads * x.columns * (a->head_dim + 2);
   return x;
 }
 
@@ -1271,9 +1278,10 @@ int check_args(const ll_paged_attention_args *a) {
       !aligned(a->value_buffer, 16))
     return fail(LL_ERR_INVALID_ARGUMENT, "query, output and KV buffers must be 16-byte aligned");
   const Launch x = plan_launch(a);
-  // A launch holds fewer than 2^32 threads.
-  if (static_cast<long long>(x.max_units) * a->num_kv_heads > 0xffffffll ||
-      static_cast<long long>(x.max_tiles) * a->num_kv_heads * x.columns > 0xffffffll)
+  // A launch holds fewer than 2^32 threads: at most 512 a unit and KV head, 16 a
+  // column.
+  if (static_cast<long long>(x.max_units) * a->num_kv_heads > 0x7fffffll ||
+      static_cast<long long>(x.max_tiles) * a->num_kv_heads * x.columns > 0xfffffffll)
     return fail(LL_ERR_INVALID_ARGUMENT, "too many queries for one launch");
   return LL_OK;
 }
@@ -1356,8 +1364,7 @@ int ll_paged_attention(const ll_paged_attention_args *a, ll_stream_t stream) {
   p.starts64 = a->query_starts_dtype == LL_DTYPE_INT64 ? 1 : 0;
   p.min_chunk = x.splits ? x.min_chunk : 33554431;  // one chunk of any length
   p.inv_target = 1.0 / x.target;
-  p.max_units = x.max_units;
-  p.max_tiles = x.max_tiles;
+  p.max_partials = x.max_partials;
   p.scale_log2 = static_cast<float>(a->softmax_scale * 1.4426950408889634);  // log2(e)
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = a->kv_dtype == LL_DTYPE_FLOAT16;

@@ -78,8 +78,8 @@ def _check_marked(got, case):
             seen = max(0, length - (starts[request + 1] - 1 - i))
             counts = torch.bincount(torch.arange(seen) % dim, minlength=dim).double()
             read = got[i] * max(seen, 1) / 64.0
-            # counts are at most seen / dim + 1: half a step of bf16 (2^-8) below half a key
-            assert int(counts.max()) <= 100
+            # half a step of the output (2^-8 and 2^-11 of it) below half a key
+            assert int(counts.max()) <= (100 if case["query"].dtype == torch.bfloat16 else 800)
             assert torch.equal(read.round(), counts.expand_as(read)), (request, i, seen)
 
 
@@ -123,6 +123,17 @@ def test_chunks(gpu_device, chunks, heads, dim, page, dtype):
     lengths, queries = CHUNKS[chunks]
     case = _case(gpu_device, lengths, queries, heads=heads, dim=dim, page=page, dtype=dtype, counts=torch.int64)
     _check(paged_attention(**case), case)
+    _check_marked(paged_attention(**_marked(case)), case)
+
+
+@pytest.mark.parametrize("queries", [None, [40]])
+@pytest.mark.parametrize("heads,dim,length", [((64, 64), 64, 30000), ((128, 128), 256, 16001), ((300, 300), 64, 9000)])
+def test_chunks_longer_than_the_slot_list(gpu_device, queries, heads, dim, length):
+    """With many KV heads a workgroup takes thousands of keys, and refills its list
+    of slots on the way."""
+
+    report(f"long chunks, heads {heads} dim {dim} length {length} queries {queries}")
+    case = _case(gpu_device, [length], queries, heads=heads, dim=dim, page=16, dtype=torch.float16)
     _check_marked(paged_attention(**_marked(case)), case)
 
 

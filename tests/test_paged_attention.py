@@ -152,5 +152,10 @@ def test_the_workspace_follows_from_the_shapes():
     small = _native.paged_attention_workspace_bytes(_block())
     assert small > 0 and _native.paged_attention_workspace_bytes(_block(page_table_columns=2 ** 20)) == small
     assert _native.paged_attention_workspace_bytes(_block(num_queries=500, num_requests=500)) > small
+    # Long prompts need no more than what is split: about 70 MB, whatever the lengths and heads.
+    for heads, dim in ((1, 128), (4, 128), (8, 64), (2, 256), (300, 64)):
+        prompt = dict(num_queries=100000, num_requests=1, query_starts=64, query_starts_dtype=_native.DTYPE_INT64,
+                      num_q_heads=heads, num_kv_heads=heads, head_dim=dim, page_table_columns=2 ** 20)
+        assert 0 < _native.paged_attention_workspace_bytes(_block(**prompt)) < 85 * 10 ** 6 * max(1, heads / 256)
     with pytest.raises(_native.NativeCallError):
         _native.paged_attention_workspace_bytes(_block(head_dim=96))
