@@ -689,7 +689,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     }
   }
 
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY;
+  float l4[4] = {0.f, 0.f, 0.f, 0.f};  // the weights' sum, in four chains: a dot product waits for the one before
   f32x16 o[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
@@ -847,7 +848,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], scale_log2, bias));
     if (__builtin_amdgcn_ballot_w64(raise) != 0) {
       const float alpha = raise ? __builtin_amdgcn_exp2f((m - m_new) * scale_log2) : 1.f;
-      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l4[i] *= alpha;
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) o[b] *= alpha;
     }
@@ -860,7 +862,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           bits[j] = E::pack(s[kb][8 * st + 2 * j], s[kb][8 * st + 2 * j + 1]);
-          l = E::dot2_ones(bits[j], l);  // the weights that the value product sees
+          l4[j] = E::dot2_ones(bits[j], l4[j]);  // the weights that the value product sees
         }
         pb[2 * kb + st] = __builtin_bit_cast(frag, bits);
       }
@@ -910,9 +912,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     if (behind) workgroup_barrier();
     const auto nothing = [](int) {};
     if (list_begin < wave_stop) products(0, 0, std::false_type{}, nothing, nothing);
-    // Tile t's bits of keys with a row.
-    auto valid_keys = [&](int t) __attribute__((always_inline)) {
-      const unsigned long long bits = tile_valid[t];
+    // Bits of keys with a row, the same in every lane.
+    auto uniform = [](unsigned long long bits) __attribute__((always_inline)) {
       // readfirstlane returns int: each half goes through unsigned.
       const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits))));
       const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<unsigned>(bits >> 32))));
@@ -944,7 +945,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     // slot list is read during the softmax before it: between the products and the
     // barrier behind them a wave only waits.
     int k_slots[W::kGathers], v_slots[W::kGathers];
-    unsigned long long valid = valid_keys(0);
+    unsigned long long valid = uniform(tile_valid[0]);
     auto iteration = [&](const int t, auto stage_tag) __attribute__((always_inline)) {
       constexpr int stage = decltype(stage_tag)::value;  // t % kStages
       const int key0 = list_begin + t * W::kKeys;
@@ -961,9 +962,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
         k_slots[j] = slot_of(min(t + kLead, last), j);
         v_slots[j] = slot_of(min(t + kLead - 1, last), j);
       }
-      const unsigned long long next_valid = valid_keys(min(t + 1, last));
+      const unsigned long long next_bits = tile_valid[min(t + 1, last)];
       if (computes) weigh_tile(key0, valid);
-      valid = next_valid;
+      valid = uniform(next_bits);
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
       // The gathers between the steps of the values, in the shadow of their MFMAs.
@@ -989,7 +990,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       constexpr int stage = decltype(stage_tag)::value;  // t % kStages
       const int key0 = list_begin + t * W::kKeys;
       const bool computes = key0 < wave_stop;
-      const unsigned long long tile_keys = valid_keys(t);
+      const unsigned long long tile_keys = uniform(tile_valid[t]);
       if (computes) weigh_tile(key0, tile_keys);
       wait_vm<0>();  // the share of K tile t + 1 and V tile t
       settle_values(t, stage, tile_keys);
@@ -1062,6 +1063,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     }
   }
 
+  float l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
   {  // the column's other half (lane l ^ 32) summed the other keys
     unsigned a = __builtin_bit_cast(unsigned, l), b = a;
     permlane32_swap(a, b);
