@@ -710,17 +710,18 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   unsigned g_k = 16 * ((lane % W::kChunksPerRow) ^ W::k_swizzle(g_token));  // the lane's bytes of a row
   unsigned g_v = 16 * ((lane % W::kChunksPerRow) ^ W::v_swizzle(g_token));
   const int share = W::kGathers * wave * kWave * 16;  // the wave's first byte of a stage
+  // (Not yet held at 0, which would wait for the read.)
   auto slot_of = [&](int tile, int j) __attribute__((always_inline)) {
-    return max(slot_list[tile * W::kKeys + g_token + j * kRows], 0);
+    return slot_list[tile * W::kKeys + g_token + j * kRows];
   };
   auto gather_k = [&](int slot, int stage, int j) __attribute__((always_inline)) {
     asm volatile("" : "+v"(g_k));  // (made per use: fewer registers over the loop)
-    dma_row(row_at(p, k_base, slot) + (g_k ^ (16u * W::k_swizzle(j * kRows))),
+    dma_row(row_at(p, k_base, max(slot, 0)) + (g_k ^ (16u * W::k_swizzle(j * kRows))),
             k_ring + stage * W::kStage + share + j * kWave * 16);
   };
   auto gather_v = [&](int slot, int stage, int j) __attribute__((always_inline)) {
     asm volatile("" : "+v"(g_v));
-    dma_row(row_at(p, v_base, slot) + (g_v ^ (16u * W::v_swizzle(j * kRows))),
+    dma_row(row_at(p, v_base, max(slot, 0)) + (g_v ^ (16u * W::v_swizzle(j * kRows))),
             v_ring + stage * W::kStage + share + j * kWave * 16);
   };
 
@@ -745,12 +746,15 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   frag pb[4];
 
   // The products: the values of the tile that pb weighs (stage v_stage) onto O^T,
-  // the scores of the next (stage k_stage) into s.  Fragments are read one batch
-  // ahead of the MFMAs that take them: eight transposed reads (every dim block of a
-  // 16-key step; keys 16 step + 4 h .. + 3 and, 8 further, the second read), or
-  // four rows' chunks (two 16-dim steps of both 32-key blocks).  before(i) is called
-  // ahead of the reads of batch i, after(i) behind its MFMAs.
-  auto products = [&](int v_stage, int k_stage, auto values_tag, auto before, auto after) __attribute__((always_inline)) {
+  // the scores of the next (stage k_stage) into s.  A wave's instructions issue in
+  // order and an MFMA takes 32 cycles, so everything else goes between them, a
+  // little behind each: fragments are read one batch ahead of the MFMAs that take
+  // them (of the values two transposed reads a dim block of a 16-key step, keys 16
+  // step + 4 h .. + 3 and, 8 further, the second read; of the scores a chunk of
+  // each 32-key block's rows for each of two 16-dim steps), and beside(i) is called
+  // behind MFMA i.
+  constexpr int kMfmas = 4 * kBlocks + 2 * kKSteps;
+  auto products = [&](int v_stage, int k_stage, auto values_tag, auto beside) __attribute__((always_inline)) {
     auto fence = [] { __builtin_amdgcn_sched_barrier(0); };  // the order below, kept
     constexpr bool values = decltype(values_tag)::value;  // else scores alone
     constexpr int kBatches = kKSteps / 2;
@@ -759,59 +763,54 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     asm volatile("" : "+v"(k_at));  // the steps' offsets made per tile: eight registers fewer over the loop
     u32x4 vf[2][kBlocks];
     frag kf[2][4];
-    auto load_v = [&](int step) __attribute__((always_inline)) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const unsigned at = v_off[b] + v_stage * W::kStage + 16 * step * W::kRowBytes;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at)));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at + 8 * W::kRowBytes)));
-        vf[step % 2][b][0] = __builtin_bit_cast(u32x2, lo)[0];
-        vf[step % 2][b][1] = __builtin_bit_cast(u32x2, lo)[1];
-        vf[step % 2][b][2] = __builtin_bit_cast(u32x2, hi)[0];
-        vf[step % 2][b][3] = __builtin_bit_cast(u32x2, hi)[1];
-      }
+    auto load_v = [&](int step, int b) __attribute__((always_inline)) {
+      const unsigned at = v_off[b] + v_stage * W::kStage + 16 * step * W::kRowBytes;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at)));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          reinterpret_cast<lds_i16x4 *>(static_cast<uintptr_t>(at + 8 * W::kRowBytes)));
+      vf[step % 2][b][0] = __builtin_bit_cast(u32x2, lo)[0];
+      vf[step % 2][b][1] = __builtin_bit_cast(u32x2, lo)[1];
+      vf[step % 2][b][2] = __builtin_bit_cast(u32x2, hi)[0];
+      vf[step % 2][b][3] = __builtin_bit_cast(u32x2, hi)[1];
     };
-    auto load_k = [&](int batch) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          kf[batch % 2][2 * j + kb] =
-              *reinterpret_cast<const frag *>(rows + (k_at ^ (32 * (2 * batch + j))) + kb * 32 * W::kRowBytes);
+    auto load_k = [&](int batch, int i) __attribute__((always_inline)) {
+      kf[batch % 2][i] = *reinterpret_cast<const frag *>(rows + (k_at ^ (32 * (2 * batch + i / 2))) + (i % 2) * 32 * W::kRowBytes);
     };
     if constexpr (values) {
-      load_v(0);
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        before(step);
-        if (step + 1 < 4) load_v(step + 1);
-        else load_k(0);
-        fence();
+      for (int b = 0; b < kBlocks; ++b) load_v(0, b);
+      fence();
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) o[b] = E::mfma32(__builtin_bit_cast(frag, vf[step % 2][b]), pb[step], o[b]);
-        after(step);
-        fence();
-      }
+      for (int step = 0; step < 4; ++step)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+          o[b] = E::mfma32(__builtin_bit_cast(frag, vf[step % 2][b]), pb[step], o[b]);
+          if (step + 1 < 4) {
+            load_v(step + 1, b);
+          } else {
+#pragma unroll
+            for (int i = 4 * b / kBlocks; i < 4 * (b + 1) / kBlocks; ++i) load_k(0, i);
+          }
+          beside(kBlocks * step + b);
+          fence();
+        }
     } else {
-      load_k(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load_k(0, i);
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
-    for (int batch = 0; batch < kBatches; ++batch) {
-      before(4 + batch);
-      if (batch + 1 < kBatches) load_k(batch + 1);
-      fence();
+    for (int batch = 0; batch < kBatches; ++batch)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) s[kb] = E::mfma32(kf[batch % 2][2 * j + kb], qf[2 * batch + j], s[kb]);
-      after(4 + batch);
-      fence();
-    }
+      for (int i = 0; i < 4; ++i) {  // (dims 16 (2 batch + i / 2) on of block i % 2)
+        s[i % 2] = E::mfma32(kf[batch % 2][i], qf[2 * batch + i / 2], s[i % 2]);
+        if (batch + 1 < kBatches) load_k(batch + 1, i);
+        beside(4 * kBlocks + 4 * batch + i);
+        fence();
+      }
   };
   // The weights of the scores in s, into pb; the sums so far rescaled where the maximum rises.
   auto weigh_tile = [&](int key0, unsigned long long valid) __attribute__((always_inline)) {
@@ -910,8 +909,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     wait_vm<2 * W::kGathers * (kLead - 1)>();
     workgroup_barrier();
     if (behind) workgroup_barrier();
-    const auto nothing = [](int) {};
-    if (list_begin < wave_stop) products(0, 0, std::false_type{}, nothing, nothing);
+    if (list_begin < wave_stop) products(0, 0, std::false_type{}, [](int) {});
     // Bits of keys with a row, the same in every lane.
     auto uniform = [](unsigned long long bits) __attribute__((always_inline)) {
       // readfirstlane returns int: each half goes through unsigned.
@@ -967,19 +965,20 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       valid = uniform(next_bits);
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
-      // The gathers between the steps of the values, in the shadow of their MFMAs.
-      auto gather_turn = [&](int i) __attribute__((always_inline)) {
-        if (i >= 2 * W::kGathers) return;
+      auto gather = [&](int i) __attribute__((always_inline)) {
         if (i % 2 == 0) gather_k(k_slots[i / 2], (stage + kLead) % W::kStages, i / 2);
         else gather_v(v_slots[i / 2], (stage + kLead - 1) % W::kStages, i / 2);
       };
+      constexpr int kApart = kMfmas / (2 * W::kGathers);  // MFMAs from one gather to the next
       __builtin_amdgcn_s_setprio(1);
       // (Behind the wave's last tile the scores are of an old stage, and not used.)
       if (computes) {
-        products(stage, (stage + 1) % W::kStages, std::true_type{}, nothing, gather_turn);
+        products(stage, (stage + 1) % W::kStages, std::true_type{}, [&](int i) __attribute__((always_inline)) {
+          if (i % kApart == kApart / 2) gather(i / kApart);
+        });
       } else {
 #pragma unroll
-        for (int i = 0; i < 2 * W::kGathers; ++i) gather_turn(i);
+        for (int i = 0; i < 2 * W::kGathers; ++i) gather(i);
       }
       __builtin_amdgcn_s_setprio(0);
     };
@@ -997,28 +996,24 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
-      // Turn i of 12: the gathers 4 i / 3 .. 4 (i + 1) / 3 - 1 of the 16; their
-      // slots first.
-      int slots[2];
-      auto slots_turn = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-        for (int g = 4 * i / 3; g < 4 * (i + 1) / 3; ++g)
-          slots[g - 4 * i / 3] = slot_of(min(t + (g % 2 == 0 ? 1 : 2), last), g / 2);
+      // The gathers, V and K in turn, each behind the read of its slot.
+      int slot = 0;
+      auto read_slot = [&](int i) __attribute__((always_inline)) { slot = slot_of(min(t + 1 + i % 2, last), i / 2); };
+      auto gather = [&](int i) __attribute__((always_inline)) {
+        if (i % 2 == 0) gather_v(slot, (stage + 1) % W::kStages, i / 2);
+        else gather_k(slot, stage, i / 2);
       };
-      auto gather_turn = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-        for (int g = 4 * i / 3; g < 4 * (i + 1) / 3; ++g) {
-          if (g % 2 == 0) gather_v(slots[g - 4 * i / 3], (stage + 1) % W::kStages, g / 2);
-          else gather_k(slots[g - 4 * i / 3], stage, g / 2);
-        }
-      };
+      constexpr int kApart = kMfmas / (2 * W::kGathers);  // MFMAs from one gather to the next
       if (computes) {
-        products(stage, (stage + 1) % W::kStages, std::true_type{}, slots_turn, gather_turn);
+        products(stage, (stage + 1) % W::kStages, std::true_type{}, [&](int i) __attribute__((always_inline)) {
+          if (i % kApart == 0) read_slot(i / kApart);
+          if (i % kApart == kApart - 1) gather(i / kApart);
+        });
       } else {
 #pragma unroll
-        for (int i = 0; i < 12; ++i) {
-          slots_turn(i);
-          gather_turn(i);
+        for (int i = 0; i < 2 * W::kGathers; ++i) {
+          read_slot(i);
+          gather(i);
         }
       }
     };
