@@ -119,21 +119,21 @@ __device__ inline void dma_pair(const void *src0, void *lds0, const void *src1, 
       : "memory");
 }
 
-// One of them.
-__device__ inline void dma_row(const void *src, void *lds) {
-  const unsigned base = __builtin_amdgcn_readfirstlane(
-      static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds)));
-  unsigned saved;
+// The LDS address of what a generic pointer into LDS points to.
+__device__ inline unsigned lds_offset(void *lds) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds));
+}
+
+// One of them, to the LDS address `base` (the same in every lane).  M0 is the
+// compiler's to restore.
+__device__ inline void dma_row(const void *src, unsigned base) {
   asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %2\n\t"
+      "s_mov_b32 m0, %1\n\t"
       "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off\n\t"
-      "s_nop 0\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
+      "global_load_lds_dwordx4 %0, off"
+      :
       : "v"(src), "s"(base)
-      : "memory");
+      : "memory", "m0");
 }
 
 // dma_pair with 32-bit byte offsets into the K and V buffers (buffer loads:

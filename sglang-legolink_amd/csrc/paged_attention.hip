@@ -714,15 +714,28 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   auto slot_of = [&](int tile, int j) __attribute__((always_inline)) {
     return slot_list[tile * W::kKeys + g_token + j * kRows];
   };
+  // Gather j of a tile, in three steps that can go between MFMAs: the row's address,
+  // the lane's part of it, the load.
+  const unsigned k_lds = lds_offset(k_ring) + share, v_lds = lds_offset(v_ring) + share;
+  const unsigned char *gather_from;
+  auto gather_step = [&](int step, auto values_tag, int slot, int stage, int j) __attribute__((always_inline)) {
+    constexpr bool values = decltype(values_tag)::value;
+    unsigned &g = values ? g_v : g_k;
+    if (step == 0) gather_from = row_at(p, values ? v_base : k_base, max(slot, 0));
+    if (step == 1) {
+      asm volatile("" : "+v"(g));  // (made per use: fewer registers over the loop)
+      gather_from += g ^ (16u * (values ? W::v_swizzle(j * kRows) : W::k_swizzle(j * kRows)));
+    }
+    if (step == 2) dma_row(gather_from, (values ? v_lds : k_lds) + stage * W::kStage + j * kWave * 16);
+    else asm volatile("" : "+v"(gather_from));  // (made here)
+  };
   auto gather_k = [&](int slot, int stage, int j) __attribute__((always_inline)) {
-    asm volatile("" : "+v"(g_k));  // (made per use: fewer registers over the loop)
-    dma_row(row_at(p, k_base, max(slot, 0)) + (g_k ^ (16u * W::k_swizzle(j * kRows))),
-            k_ring + stage * W::kStage + share + j * kWave * 16);
+#pragma unroll
+    for (int step = 0; step < 3; ++step) gather_step(step, std::false_type{}, slot, stage, j);
   };
   auto gather_v = [&](int slot, int stage, int j) __attribute__((always_inline)) {
-    asm volatile("" : "+v"(g_v));
-    dma_row(row_at(p, v_base, max(slot, 0)) + (g_v ^ (16u * W::v_swizzle(j * kRows))),
-            v_ring + stage * W::kStage + share + j * kWave * 16);
+#pragma unroll
+    for (int step = 0; step < 3; ++step) gather_step(step, std::true_type{}, slot, stage, j);
   };
 
   // Offsets of the lane's fragments within a stage.
@@ -732,13 +745,11 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   const int k_off = col * W::kRowBytes + ((h ^ W::k_swizzle(col)) * 16);
   const int li = lane % 16;
   const int v_token = 4 * h + li / 4;
-  const unsigned v_lds =
-      static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char *)v_ring));
   unsigned v_off[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
     const int chunk = 4 * b + 2 * ((lane / 16) % 2) + (li % 4) / 2;
-    v_off[b] = v_lds + v_token * W::kRowBytes + (chunk ^ W::v_swizzle(v_token)) * 16 + 8 * (li % 2);
+    v_off[b] = lds_offset(v_ring) + v_token * W::kRowBytes + (chunk ^ W::v_swizzle(v_token)) * 16 + 8 * (li % 2);
     asm volatile("" : "+v"(v_off[b]));
   }
 
@@ -965,20 +976,20 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       valid = uniform(next_bits);
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
-      auto gather = [&](int i) __attribute__((always_inline)) {
-        if (i % 2 == 0) gather_k(k_slots[i / 2], (stage + kLead) % W::kStages, i / 2);
-        else gather_v(v_slots[i / 2], (stage + kLead - 1) % W::kStages, i / 2);
+      auto gather = [&](int step, int i) __attribute__((always_inline)) {
+        if (i % 2 == 0) gather_step(step, std::false_type{}, k_slots[i / 2], (stage + kLead) % W::kStages, i / 2);
+        else gather_step(step, std::true_type{}, v_slots[i / 2], (stage + kLead - 1) % W::kStages, i / 2);
       };
       constexpr int kApart = kMfmas / (2 * W::kGathers);  // MFMAs from one gather to the next
       __builtin_amdgcn_s_setprio(1);
       // (Behind the wave's last tile the scores are of an old stage, and not used.)
       if (computes) {
         products(stage, (stage + 1) % W::kStages, std::true_type{}, [&](int i) __attribute__((always_inline)) {
-          if (i % kApart == kApart / 2) gather(i / kApart);
+          if (i % kApart < 3) gather(i % kApart, i / kApart);
         });
       } else {
 #pragma unroll
-        for (int i = 0; i < 2 * W::kGathers; ++i) gather(i);
+        for (int i = 0; i < 6 * W::kGathers; ++i) gather(i % 3, i / 3);
       }
       __builtin_amdgcn_s_setprio(0);
     };
@@ -996,25 +1007,26 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
       __builtin_amdgcn_sched_barrier(0);
       workgroup_barrier();
-      // The gathers, V and K in turn, each behind the read of its slot.
-      int slot = 0;
-      auto read_slot = [&](int i) __attribute__((always_inline)) { slot = slot_of(min(t + 1 + i % 2, last), i / 2); };
-      auto gather = [&](int i) __attribute__((always_inline)) {
-        if (i % 2 == 0) gather_v(slot, (stage + 1) % W::kStages, i / 2);
-        else gather_k(slot, stage, i / 2);
+      // The gathers, V and K in turn; their slots are read two gathers ahead.
+      int slots[2];
+      auto read_slot = [&](int i) __attribute__((always_inline)) {
+        if (i < 2 * W::kGathers) slots[i % 2] = slot_of(min(t + 1 + i % 2, last), i / 2);
+      };
+      auto gather = [&](int step, int i) __attribute__((always_inline)) {
+        if (i % 2 == 0) gather_step(step, std::true_type{}, slots[0], (stage + 1) % W::kStages, i / 2);
+        else gather_step(step, std::false_type{}, slots[1], stage, i / 2);
+        if (step == 0) read_slot(i + 2);
       };
       constexpr int kApart = kMfmas / (2 * W::kGathers);  // MFMAs from one gather to the next
+      read_slot(0);
+      read_slot(1);
       if (computes) {
         products(stage, (stage + 1) % W::kStages, std::true_type{}, [&](int i) __attribute__((always_inline)) {
-          if (i % kApart == 0) read_slot(i / kApart);
-          if (i % kApart == kApart - 1) gather(i / kApart);
+          if (i % kApart < 3) gather(i % kApart, i / kApart);
         });
       } else {
 #pragma unroll
-        for (int i = 0; i < 2 * W::kGathers; ++i) {
-          read_slot(i);
-          gather(i);
-        }
+        for (int i = 0; i < 6 * W::kGathers; ++i) gather(i % 3, i / 3);
       }
     };
     if constexpr (W::kWaves == 8) {
