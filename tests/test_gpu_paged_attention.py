@@ -148,6 +148,18 @@ def test_more_requests_than_a_wave_scans_at_once(gpu_device):
     _check_marked(paged_attention(**_marked(case)), case)
 
 
+@pytest.mark.parametrize("heads,dim", [((8, 1), 64), ((8, 1), 128), ((16, 2), 256)])
+def test_chunks_of_more_requests_than_a_wave_orders_at_once(gpu_device, heads, dim):
+    """150 requests of 0 to 30 queries over 0 to 449 keys, among them ones without
+    queries, without keys, and many of the same length."""
+
+    queries = [(7 * r) % 31 for r in range(150)]
+    lengths = [0 if r % 23 == 5 else (3 * r if r < 150 // 2 else 64 * (r % 8)) for r in range(150)]
+    lengths = [max(length, n) if length else 0 for length, n in zip(lengths, queries)]
+    case = _marked(_case(gpu_device, lengths, queries, heads=heads, dim=dim, page=5))
+    _check_marked(paged_attention(**case), case)
+
+
 @pytest.mark.parametrize("queries", [None, [3, 1, 2], [200, 5, 90]])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_rows_that_are_not_seen_may_hold_anything(gpu_device, queries, dtype):
