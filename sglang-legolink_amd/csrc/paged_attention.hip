@@ -742,7 +742,6 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   unsigned g_k = 16 * ((lane % W::kChunksPerRow) ^ W::k_swizzle(g_token));  // the lane's bytes of a row
   unsigned g_v = 16 * ((lane % W::kChunksPerRow) ^ W::v_swizzle(g_token));
   const int share = W::kGathers * wave * kWave * 16;  // the wave's first byte of a stage
-  // (Not yet held at 0, which would wait for the read.)
   auto slot_of = [&](int tile, int j) __attribute__((always_inline)) {
     return slot_list[tile * W::kKeys + g_token + j * kRows];
   };
@@ -753,7 +752,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   auto gather_step = [&](int step, auto values_tag, int slot, int stage, int j) __attribute__((always_inline)) {
     constexpr bool values = decltype(values_tag)::value;
     unsigned &g = values ? g_v : g_k;
-    if (step == 0) gather_from = row_at(p, values ? v_base : k_base, max(slot, 0));
+    if (step == 0) gather_from = row_at(p, values ? v_base : k_base, slot);
     if (step == 1) {
       asm volatile("" : "+v"(g));  // (made per use: fewer registers over the loop)
       gather_from += g ^ (16u * (values ? W::v_swizzle(j * kRows) : W::k_swizzle(j * kRows)));
@@ -921,7 +920,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
       const unsigned page = static_cast<unsigned>((key * p.page_magic) >> p.page_shift);
       const int entry = pages[page];
       const bool valid = i < listed && static_cast<unsigned>(entry) < static_cast<unsigned>(p.num_pages);
-      slot_list[i] = valid ? entry * p.page_size + static_cast<int>(key - page * p.page_size) : -1;
+      // (A key without a row: slot 0, which the tile's bits keep out.)
+      slot_list[i] = valid ? entry * p.page_size + static_cast<int>(key - page * p.page_size) : 0;
       const unsigned long long bits = __builtin_amdgcn_ballot_w64(valid);  // whole tiles: the loop strides by waves
       if (lane == 0) tile_valid[i / W::kKeys] = bits;
     }
