@@ -144,7 +144,9 @@ __device__ inline Token token_at(const RotaryParams &p, long long t, bool first)
 // aligned.  A wave is one step of one token: kGroup lanes a head (the next
 // power of two of D / 16, so that the norm's sum is kGroup's xor shuffles;
 // lanes past D / 16 idle), 64 / kGroup heads a step, queries first, then keys;
-// the steps behind them copy the values, 128 chunks of 8 at a time.
+// the steps behind them copy the values, 128 chunks of 8 at a time.  8,192 tokens
+// of 64 + 8 normed heads of 128: 64.4 us, 4.7 TB/s read and written (a copy of as
+// many bytes 62 us); one token 3.6 us, the time of its three dependent loads.
 template <typename E, int kGroup>
 __global__ void __launch_bounds__(kThreads) head_rotary_vec_kernel(const RotaryParams p) {
   constexpr int kHeads = kWave / kGroup;
@@ -259,8 +261,11 @@ __global__ void __launch_bounds__(kThreads) head_rotary_vec_kernel(const RotaryP
 }
 
 // Every other shape: a wave is one row of one token (queries, keys, then
-// values), a lane every 64th value.  All of a row's loads come before its
-// stores, so that it may be rotated in place.
+// values), a lane every 64th of its rotary pairs and of the values behind them.
+// All of a row's loads come before its stores, so that it may be rotated in
+// place, and those of the row do not wait for the position.  Bound by its 2-byte
+// loads and stores: the rows above, one value off their alignment, take 296 us
+// (1.0 TB/s; 393 with a lane per value, each loading its partner too).
 template <typename E>
 __global__ void __launch_bounds__(kThreads) head_rotary_element_kernel(const RotaryParams p) {
   constexpr int kPer = kMaxDim / kWave;
@@ -270,14 +275,19 @@ __global__ void __launch_bounds__(kThreads) head_rotary_element_kernel(const Rot
   const long long t = unit / static_cast<unsigned>(p.steps);
   const int row = static_cast<int>(unit % static_cast<unsigned>(p.steps));
   if (t >= p.num_tokens) return;
-  const Token token = token_at(p, t, row == 0);
-  if (!token.turned) return;
   if (row >= p.turn_steps) {
     const int head = row - p.turn_steps;
-    if (!token.written) return;
     const uint16_t *src = p.value.base + t * p.value.token + head * p.value.head;
+    uint16_t values[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (lane + k * kWave < p.value_dim) values[k] = src[lane + k * kWave];
+    const Token token = token_at(p, t, false);
+    if (!token.written) return;
     uint16_t *dst = p.value_buffer + (token.slot * p.hkv + head) * p.value_dim;
-    for (int d = lane; d < p.value_dim; d += kWave) dst[d] = src[d];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (lane + k * kWave < p.value_dim) dst[lane + k * kWave] = values[k];
     return;
   }
   const bool is_key = row >= p.hq;
@@ -285,22 +295,36 @@ __global__ void __launch_bounds__(kThreads) head_rotary_element_kernel(const Rot
   const Rows &in = is_key ? p.key : p.query;
   const uint16_t *src = in.base + t * in.token + head * in.head;
   const void *weight = is_key ? p.key_weight : p.query_weight;
+  // Item i below `half` is the pair (first, second), the others a value each.
   const int half = p.rotary / 2;
-  float x[kPer], other[kPer];
+  const int items = half + p.dim - p.rotary;
+  auto first_of = [&](int i) { return i >= half ? i + half : p.neox ? i : 2 * i; };
+  auto second_of = [&](int i) { return p.neox ? i + half : 2 * i + 1; };
+  float x[kPer], y[kPer];
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int d = lane + k * kWave;
-    x[k] = other[k] = 0.f;
-    if (d < p.dim) x[k] = E::unpack(src[d])[0];
-    if (d < p.rotary) other[k] = E::unpack(src[p.neox ? (d < half ? d + half : d - half) : d ^ 1])[0];
-    sum += x[k] * x[k];
+    const int i = lane + k * kWave;
+    x[k] = y[k] = 0.f;
+    if (k * kWave >= items) continue;  // (of no lane)
+    if (i < items) x[k] = E::unpack(src[first_of(i)])[0];
+    if (i < half) y[k] = E::unpack(src[second_of(i)])[0];
   }
-  float scale = 1.f;
+  const Token token = token_at(p, t, row == 0);
+  if (!token.turned) return;
   if (weight != nullptr) {
 #pragma unroll
+    for (int k = 0; k < kPer; ++k) sum += x[k] * x[k] + y[k] * y[k];
+#pragma unroll
     for (int step_lanes = 1; step_lanes < kWave; step_lanes *= 2) sum += __shfl_xor(sum, step_lanes);
-    scale = rsqrtf(sum / static_cast<float>(p.dim) + p.eps);
+    const float scale = rsqrtf(sum / static_cast<float>(p.dim) + p.eps);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (k * kWave >= items) continue;
+      const int i = lane + k * kWave;
+      if (i < items) x[k] = x[k] * scale * value_at(weight, p.weight_dtype, first_of(i));
+      if (i < half) y[k] = y[k] * scale * value_at(weight, p.weight_dtype, second_of(i));
+    }
   }
   uint16_t *dst;
   if (!is_key) {
@@ -313,21 +337,16 @@ __global__ void __launch_bounds__(kThreads) head_rotary_element_kernel(const Rot
   }
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int d = lane + k * kWave;
-    if (d >= p.dim) continue;
-    float y = x[k];
-    if (weight != nullptr) y = y * scale * value_at(weight, p.weight_dtype, d);
-    if (d < p.rotary) {
-      const bool is_first = p.neox ? d < half : d % 2 == 0;
-      const int pair = p.neox ? (d < half ? d : d - half) : d / 2;
-      const int partner = p.neox ? (d < half ? d + half : d - half) : d ^ 1;
-      float z = other[k];
-      if (weight != nullptr) z = z * scale * value_at(weight, p.weight_dtype, partner);
-      const float c = value_at(p.table, p.table_dtype, token.position * p.table_stride + pair);
-      const float s = value_at(p.table, p.table_dtype, token.position * p.table_stride + half + pair);
-      y = is_first ? y * c - z * s : y * c + z * s;
+    if (k * kWave >= items) continue;
+    const int i = lane + k * kWave;
+    if (i < half) {
+      const float c = value_at(p.table, p.table_dtype, token.position * p.table_stride + i);
+      const float s = value_at(p.table, p.table_dtype, token.position * p.table_stride + half + i);
+      dst[first_of(i)] = static_cast<uint16_t>(E::pack(x[k] * c - y[k] * s, 0.f));
+      dst[second_of(i)] = static_cast<uint16_t>(E::pack(y[k] * c + x[k] * s, 0.f));
+    } else if (i < items) {
+      dst[first_of(i)] = static_cast<uint16_t>(E::pack(x[k], 0.f));
     }
-    dst[d] = static_cast<uint16_t>(E::pack(y, 0.f));
   }
 }
 

