@@ -146,7 +146,8 @@ __device__ inline Token token_at(const RotaryParams &p, long long t, bool first)
 // lanes past D / 16 idle), 64 / kGroup heads a step, queries first, then keys;
 // the steps behind them copy the values, 128 chunks of 8 at a time.  8,192 tokens
 // of 64 + 8 normed heads of 128: 64.4 us, 4.7 TB/s read and written (a copy of as
-// many bytes 62 us); one token 3.6 us, the time of its three dependent loads.
+// many bytes 62 us); one token 3.6 us, the latency of its position, the table row
+// behind it and the stores.
 template <typename E, int kGroup>
 __global__ void __launch_bounds__(kThreads) head_rotary_vec_kernel(const RotaryParams p) {
   constexpr int kHeads = kWave / kGroup;
