@@ -152,13 +152,20 @@ __device__ inline int tiles_of(const PagedParams &p, int q_len, int columns) {
 // may leave partial results, number below 2 work / L <= 2 target + 2: a request of
 // k > L key tiles has fewer than k / L + 1 < 2 k / L chunks.
 //
-// kByLength orders the units of 64 requests at a time by falling length, as far as
-// it is known before the columns' positions: the chunks of full length, then the
-// requests' last chunks, the longest first.  Workgroups start in that order, so the
-// short units fill the last round (six chunks of 5 to 701 queries, 14/2 heads of 64,
-// over 300 to 9,000 keys: 85 us, 98 request by request).
-template <bool kOfTiles, bool kByLength = false>
+// The units of 64 requests at a time come in order of falling length, as far as it
+// is known before the columns' positions: the chunks of full length, then the
+// requests' last chunks, the longest first (kByLength), or by the quarter of a full
+// chunk that they fill (kByQuarter, whose cost does not grow with the requests).
+// Workgroups start in that order, so the short units fill the last round.  Six
+// chunks of 5 to 701 queries, 14/2 heads of 64, over 300 to 9,000 keys: 85 us by
+// length, 88 by quarter, 98 request by request; 64 and 128 uneven requests of
+// single tokens, 64/8 heads of 128: 390 and 212 us by quarter, 389 and 242 by
+// length, 406 and 224 request by request.
+enum class Order { kTiles, kByLength, kByQuarter };  // (kTiles: tiles, request by request)
+
+template <Order kOrder>
 __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
+  constexpr bool kOfTiles = kOrder == Order::kTiles;
   const int lane = threadIdx.x % kWave;
   Request mine = Request{0, 0, 0};
   double work = 0.0;  // (exact below 2^53)
@@ -191,31 +198,43 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
     const int tiles_to = kOfTiles ? inclusive_scan(tiles) : 0;
     const bool listed = r0 + lane < p.num_requests;
     // The request whose units hold `index`, the index within them.
-    unsigned long long past;
-    int within = 0;       // of the lane's request
-    bool is_last = false;  // a last chunk (kByLength)
-    if constexpr (kByLength) {
+    int within;
+    bool is_last = false;  // a last chunk
+    bool holds;
+    if constexpr (kOfTiles) {
+      within = index - tiles_before - tiles_to + tiles;
+      holds = within >= 0 && within < tiles;
+    } else {
       const int full_to = inclusive_scan(tiles * (chunks - 1));
       const int full = __builtin_amdgcn_readlane(full_to, kWave - 1);
       is_last = index - units_before >= full;
-      if (is_last) {
+      if (!is_last) {
+        within = index - units_before - full_to + tiles * (chunks - 1);
+        holds = within >= 0 && within < tiles * (chunks - 1);
+      } else {
         const int length = key_tiles - (chunks - 1) * chunk;
         int before = 0;  // tiles of last chunks in front of the lane's
-        for (int j = 0; j < min(kWave, p.num_requests - r0); ++j) {
-          const int other = __builtin_amdgcn_readlane(length, j);
-          const int count = __builtin_amdgcn_readlane(tiles, j);
-          before += other > length || (other == length && j < lane) ? count : 0;
+        if constexpr (kOrder == Order::kByLength) {
+          for (int j = 0; j < min(kWave, p.num_requests - r0); ++j) {
+            const int other = __builtin_amdgcn_readlane(length, j);
+            const int count = __builtin_amdgcn_readlane(tiles, j);
+            before += other > length || (other == length && j < lane) ? count : 0;
+          }
+        } else {
+          const int quarter = min(3, 4 * (chunk - length) / chunk);  // 0: the longest
+          int of_former = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int to = inclusive_scan(quarter == q ? tiles : 0);
+            if (quarter == q) before = of_former + to - tiles;
+            of_former += __builtin_amdgcn_readlane(to, kWave - 1);
+          }
         }
         within = index - units_before - full - before;
-        past = __builtin_amdgcn_ballot_w64(listed && within >= 0 && within < tiles);
-      } else {
-        within = index - units_before - full_to + tiles * (chunks - 1);
-        past = __builtin_amdgcn_ballot_w64(listed && full_to > index - units_before);
+        holds = within >= 0 && within < tiles;
       }
-    } else {
-      within = kOfTiles ? index - tiles_before - tiles_to + tiles : index - units_before - units_to + tiles * chunks;
-      past = __builtin_amdgcn_ballot_w64(listed && within < (kOfTiles ? tiles : tiles * chunks));
     }
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(listed && holds);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       w.index = r0 + at;
@@ -230,7 +249,7 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
       int nth = own_within;
       w.chunk = 0;
       if constexpr (!kOfTiles) {
-        if (kByLength && is_last) {
+        if (is_last) {
           w.chunk = own_chunks - 1;
         } else {
           w.chunk = own_within / own_tiles;
@@ -336,12 +355,12 @@ __device__ inline void wait_vm() {
 // waves of a workgroup take turns at its 32-key subtiles, each through an LDS ring
 // of its own (no barriers: a wave waits for its own gathers alone), and join their
 // results at the end.  131,072 keys of 4 heads of 128: 47 us, 5.7 TB/s (a read-only
-// pass reaches 6.0); 64 uneven requests, 2.13 GB: 406 us, 5.2 TB/s; 2,048 keys
-// 6.5 us, the latencies of the lengths, the pages, the rows and the join.  v_mfma_f32_16x16x32,
-// lane layouts: A and B lane l element e -> row / column l % 16, k = 8 (l / 16)
-// + e; accumulator register r -> row 4 (l / 16) + r, column l % 16.  The value
-// product's k order is the scores' register order: k = 8 g + e is token 4 g + e
-// (e < 4) or 16 + 4 g + e - 4.
+// pass reaches 6.0); 64 uneven requests, 2.13 GB: 387 us, 5.5 TB/s; 2,048 keys
+// 6.5 us, the latencies of the lengths, the pages, the rows and the join.
+// v_mfma_f32_16x16x32, lane layouts: A and B lane l element e -> row / column
+// l % 16, k = 8 (l / 16) + e; accumulator register r -> row 4 (l / 16) + r, column
+// l % 16.  The value product's k order is the scores' register order: k = 8 g + e
+// is token 4 g + e (e < 4) or 16 + 4 g + e - 4.
 // LDS rows are token-major with their 16-byte chunks swizzled by token, so that
 // the 16 lanes of a K read (16 tokens, one chunk) and the 32 lanes of a
 // transposed V read (8 tokens x 32 bytes) each cover the 64 banks once.
@@ -377,7 +396,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 
   const int head = blockIdx.x % p.hkv;
   const int unit = blockIdx.x / p.hkv;
-  const Work w = find_work<false>(p, kColumns, unit);
+  const Work w = find_work<Order::kByQuarter>(p, kColumns, unit);
   if (w.index < 0 || w.chunk >= w.chunks || (w.chunks > 1 && !partials_fit(p, w))) return;
   const int key_begin = w.chunk * w.chunk_keys;  // below the tile's key_end, or 0
   int key_end = key_begin + min(w.chunk_keys, w.key_end - key_begin);
@@ -687,7 +706,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
 
   const int head = blockIdx.x % p.hkv;
   const int unit = blockIdx.x / p.hkv;
-  const Work w = find_work<false, true>(p, W::kColumns, unit);
+  const Work w = find_work<Order::kByLength>(p, W::kColumns, unit);
   if (w.index < 0 || w.chunk >= w.chunks || (w.chunks > 1 && !partials_fit(p, w))) return;
   const int key_begin = w.chunk * w.chunk_keys;  // below the tile's key_end, or 0
   int key_end = key_begin + min(w.chunk_keys, w.key_end - key_begin);
@@ -803,6 +822,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   // each 32-key block's rows for each of two 16-dim steps), and beside(i) is called
   // behind MFMA i.
   constexpr int kMfmas = 4 * kBlocks + 2 * kKSteps;
+  static_assert(kMfmas % (2 * W::kGathers) == 0 && kMfmas / (2 * W::kGathers) >= 3, "a place for every step of a gather");
   auto products = [&](int v_stage, int k_stage, auto values_tag, auto beside) __attribute__((always_inline)) {
     auto fence = [] { __builtin_amdgcn_sched_barrier(0); };  // the order below, kept
     constexpr bool values = decltype(values_tag)::value;  // else scores alone
@@ -1169,7 +1189,7 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
   const int groups = columns / C::kColumns;
   const int tile_head = blockIdx.x / groups;
   const int head = tile_head % p.hkv;
-  const Work w = find_work<true>(p, columns, tile_head / p.hkv);
+  const Work w = find_work<Order::kTiles>(p, columns, tile_head / p.hkv);
   if (w.index < 0 || w.chunks <= 1 || !partials_fit(p, w)) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int quad = lane % (D / 4);
@@ -1269,9 +1289,10 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   // A workgroup fills a compute unit (its LDS rings), so `places` units of every
   // KV head run at once.  Chunks: as many units as places, the longest first, leave
   // the least over.  Single tokens: where the tiles are few, as many units as run
-  // at once; where they are many, their lengths average out over four rounds.
+  // at once; where they are many, two rounds, whose second the short ones fill (64
+  // and 128 uneven requests: 390 and 212 us; one round 403 and 214, four 391 and 218).
   const int places = std::max(1, kComputeUnits / static_cast<int>(a->num_kv_heads));
-  x.target = x.wide ? places : 2 * x.max_tiles <= places ? places - x.max_tiles + 1 : 4 * places;
+  x.target = x.wide ? places : 2 * x.max_tiles <= places ? places - x.max_tiles + 1 : 2 * places;
   const long long max_keys = a->page_table_columns * a->page_size;
   x.splits = max_keys > x.min_chunk * kPageTile;
   const long long units = tiles + (x.splits ? x.target + 1 : 0);
