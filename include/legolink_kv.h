@@ -709,8 +709,10 @@ int64_t ll_head_rotary_args_size(void);
  *
  * Workspace: ll_paged_attention_workspace_bytes(args), a bound that follows from
  * the shapes alone (70 MB at 4 KV heads of 128, whatever the lengths).  Calls
- * that share one must not overlap; nothing in it outlives the call.  One launch, and a second where a table row holds more than
- * 128 keys (it joins the parts of requests whose keys were split).
+ * that share one must not overlap; nothing in it outlives the call.  One launch,
+ * a second where a table row holds more than 128 keys (it joins the parts of
+ * requests whose keys were split), and one in front of more than 128 requests (it
+ * sums what each holds).
  */
 typedef struct ll_paged_attention_args {
   int64_t struct_size;             /* sizeof(ll_paged_attention_args) */

@@ -56,6 +56,7 @@ struct PagedParams {
   const int *pages;
   const void *kv_lengths, *query_starts;  // query_starts NULL: one query each
   float *ws;
+  int *plan;  // of many requests (NULL: every workgroup makes its own)
   long long q_token, q_head, pages_stride;
   unsigned long long page_magic;
   double inv_target;
@@ -144,9 +145,67 @@ __device__ inline int tiles_of(const PagedParams &p, int q_len, int columns) {
   return (q_len * p.group + columns - 1) >> (31 - __builtin_clz(columns));  // (a power of two)
 }
 
+__device__ inline int key_tiles_of(const Request &x) { return (x.kv_len + kPageTile - 1) / kPageTile; }
+
+// A chunk's key tiles, of a call with this work (in key tiles times column tiles).
+__device__ inline int chunk_of(const PagedParams &p, double work) {
+  // (2^25 key tiles are more than any length; readfirstlane: uniform to the compiler too)
+  return __builtin_amdgcn_readfirstlane(
+      max(p.min_chunk, static_cast<int>(min(ceil(work * p.inv_target - 1e-6), 33554432.0))));
+}
+
+// Many requests: chunk_of, and what lies up to the end of every 64 of them, once for
+// the call (one workgroup), so that the others need not scan them all.
+// plan[0] is the chunk; plan[1 + 3 b ..] units, partial results and tiles of the
+// requests up to 64 (b + 1).
+constexpr int kPlanThreads = 1024;
+__host__ __device__ inline long long plan_ints(long long requests) { return 1 + 3 * ((requests + kWave - 1) / kWave); }
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedParams p, int columns) {
+  constexpr int kWaves = kPlanThreads / kWave;
+  __shared__ double work_of[kWaves];
+  __shared__ int sums[2][kWaves][3];
+  const int lane = threadIdx.x % kWave;
+  const int wave = threadIdx.x / kWave;
+  double work = 0.0;  // (exact below 2^53, in any order)
+  for (int r = threadIdx.x; r < p.num_requests; r += kPlanThreads) {
+    const Request x = request_at(p, r);
+    work += static_cast<double>(tiles_of(p, x.q_len, columns)) * key_tiles_of(x);
+  }
+  work = sum_of_wave(work);
+  if (lane == 0) work_of[wave] = work;
+  __syncthreads();
+  work = 0.0;
+  for (int v = 0; v < kWaves; ++v) work += work_of[v];
+  const int chunk = chunk_of(p, work);
+  if (threadIdx.x == 0) p.plan[0] = chunk;
+  int before[3] = {0, 0, 0};
+  for (int r0 = 0, turn = 0; r0 < p.num_requests; r0 += kPlanThreads, turn ^= 1) {
+    const int r = r0 + static_cast<int>(threadIdx.x);
+    Request x = Request{0, 0, 0};
+    if (r < p.num_requests) x = request_at(p, r);
+    const int tiles = tiles_of(p, x.q_len, columns);
+    const int chunks = max(1, (key_tiles_of(x) + chunk - 1) / chunk);
+    const int of_wave[3] = {inclusive_scan(tiles * chunks), inclusive_scan(chunks > 1 ? tiles * chunks : 0),
+                            inclusive_scan(tiles)};
+    if (lane == kWave - 1)
+      for (int i = 0; i < 3; ++i) sums[turn][wave][i] = of_wave[i];
+    __syncthreads();  // (the other turn's sums may still be read behind it)
+    int up_to[3] = {before[0], before[1], before[2]};
+    for (int v = 0; v < kWaves; ++v)
+      for (int i = 0; i < 3; ++i) {
+        before[i] += sums[turn][v][i];
+        if (v == wave) up_to[i] = before[i];
+      }
+    if (lane == 0 && r < p.num_requests)
+      for (int i = 0; i < 3; ++i) p.plan[1 + 3 * (r / kWave) + i] = up_to[i];
+  }
+}
+
 // Unit `index` of the call (kOfTiles: tile `index`).  Every wave finds it for
 // itself: two passes over the requests, 64 at a time, the first for the call's
-// work in key tiles times column tiles.  With L = max(min_chunk, work / target)
+// work in key tiles times column tiles (or, with a plan, over its entries, and one
+// of 64 requests).  With L = max(min_chunk, work / target)
 // key tiles a chunk, the units number at most work / L + tiles <= target +
 // tiles, which the launch holds.  Those of requests of more than one chunk, which
 // may leave partial results, number below 2 work / L <= 2 target + 2: a request of
@@ -168,30 +227,52 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
   constexpr bool kOfTiles = kOrder == Order::kTiles;
   const int lane = threadIdx.x % kWave;
   Request mine = Request{0, 0, 0};
-  double work = 0.0;  // (exact below 2^53)
-  for (int r0 = 0; r0 < p.num_requests; r0 += kWave) {
-    Request x = Request{0, 0, 0};
-    if (r0 + lane < p.num_requests) x = request_at(p, r0 + lane);
-    if (r0 == 0) mine = x;
-    work += static_cast<double>(tiles_of(p, x.q_len, columns)) * ((x.kv_len + kPageTile - 1) / kPageTile);
-  }
-  const double share = sum_of_wave(work) * p.inv_target;
-  // (2^25 key tiles are more than any length; readfirstlane: uniform to the compiler too)
-  const int chunk = __builtin_amdgcn_readfirstlane(
-      max(p.min_chunk, static_cast<int>(min(ceil(share - 1e-6), 33554432.0))));
-
   Work w;
   w.index = -1;
-  w.chunk_keys = min(chunk, 33554431) * kPageTile;
+  int chunk, first = 0, stop = p.num_requests;  // the requests to look at
   int units_before = 0, tiles_before = 0, partials_before = 0;
-  for (int r0 = 0; r0 < p.num_requests; r0 += kWave) {
+  if (p.plan == nullptr) {
+    double work = 0.0;  // (exact below 2^53)
+    for (int r0 = 0; r0 < p.num_requests; r0 += kWave) {
+      Request x = Request{0, 0, 0};
+      if (r0 + lane < p.num_requests) x = request_at(p, r0 + lane);
+      if (r0 == 0) mine = x;
+      work += static_cast<double>(tiles_of(p, x.q_len, columns)) * key_tiles_of(x);
+    }
+    chunk = chunk_of(p, sum_of_wave(work));
+  } else {
+    chunk = __builtin_amdgcn_readfirstlane(p.plan[0]);
+    const int *ends = p.plan + 1;
+    const int blocks = (p.num_requests + kWave - 1) / kWave;
+    int block = 0;
+    for (; block < blocks; block += kWave) {
+      const bool reaches = block + lane < blocks && ends[3 * (block + lane) + (kOfTiles ? 2 : 0)] > index;
+      const unsigned long long past = __builtin_amdgcn_ballot_w64(reaches);
+      if (past != 0) {
+        block += __builtin_ctzll(past);
+        break;
+      }
+    }
+    if (block >= blocks) return w;
+    first = block * kWave;
+    stop = min(stop, first + kWave);
+    if (block > 0) {
+      units_before = __builtin_amdgcn_readfirstlane(ends[3 * block - 3]);
+      partials_before = __builtin_amdgcn_readfirstlane(ends[3 * block - 2]);
+      tiles_before = __builtin_amdgcn_readfirstlane(ends[3 * block - 1]);
+    }
+    if (first + lane < stop) mine = request_at(p, first + lane);
+  }
+
+  w.chunk_keys = min(chunk, 33554431) * kPageTile;
+  for (int r0 = first; r0 < stop; r0 += kWave) {
     Request x = mine;
-    if (r0 > 0) {
+    if (r0 > first) {
       x = Request{0, 0, 0};
       if (r0 + lane < p.num_requests) x = request_at(p, r0 + lane);
     }
     const int tiles = tiles_of(p, x.q_len, columns);
-    const int key_tiles = (x.kv_len + kPageTile - 1) / kPageTile;
+    const int key_tiles = key_tiles_of(x);
     const int chunks = max(1, (key_tiles + chunk - 1) / chunk);
     const int units_to = inclusive_scan(tiles * chunks);
     const int partials_to = inclusive_scan(chunks > 1 ? tiles * chunks : 0);
@@ -1260,11 +1341,16 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
 }
 
 // How a call is launched: known from sizes that the host has.
+// More requests than this have a plan made before the call's kernels (single tokens
+// over 800 to 1,200 keys, 28/4 heads of 128: 128 requests 61 us with a plan, 60
+// without; 256 117 and 127; 1,024 422 and 577; 2,048 818 and 1,477).
+constexpr long long kPlanned = 128;
+
 struct Launch {
   int columns;
   int max_tiles, max_units, max_partials, target, min_chunk;
   bool wide, splits;
-  long long ws_floats;
+  long long ws_floats, plan_at;  // of the workspace; where the plan begins in it (ws_floats: none)
 };
 
 constexpr int kComputeUnits = 256;  // MI355X
@@ -1298,7 +1384,8 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   const long long units = tiles + (x.splits ? x.target + 1 : 0);
   x.max_units = static_cast<int>(std::min(units, 0x7fffffffll));
   x.max_partials = x.splits ? 2 * x.target + 2 : 0;
-  x.ws_floats = x.max_partials * a->num_kv_heads * x.columns * (a->head_dim + 2);
+  x.plan_at = x.max_partials * a->num_kv_heads * x.columns * (a->head_dim + 2);
+  x.ws_floats = x.plan_at + (requests > kPlanned ? plan_ints(requests) : 0);
   return x;
 }
 
@@ -1358,6 +1445,7 @@ int check_args(const ll_paged_attention_args *a) {
 template <int D, typename E>
 int launch_all(const PagedParams &p, const Launch &x, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(x.max_units) * static_cast<unsigned>(p.hkv);
+  if (p.plan != nullptr) paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, x.columns);
   if (x.wide) paged_wide_kernel<D, E><<<grid, Wide<D>::kThreads, 0, s>>>(p);
   else paged_narrow_kernel<D, E><<<grid, Narrow<D>::kThreads, 0, s>>>(p);
   hipError_t err = hipGetLastError();
@@ -1398,7 +1486,7 @@ int ll_paged_attention(const ll_paged_attention_args *a, ll_stream_t stream) {
   const int rc = check_args(a);
   if (rc != LL_OK || a->num_queries == 0 || a->num_requests == 0) return rc;
   const Launch x = plan_launch(a);
-  if (x.splits && (a->workspace == nullptr || a->workspace_bytes < x.ws_floats * 4 || !aligned(a->workspace, 16)))
+  if (x.ws_floats > 0 && (a->workspace == nullptr || a->workspace_bytes < x.ws_floats * 4 || !aligned(a->workspace, 16)))
     return fail(LL_ERR_INVALID_ARGUMENT, "the call needs a 16-byte aligned workspace of %lld bytes",
                 static_cast<long long>(x.ws_floats * 4));
   PagedParams p;
@@ -1411,6 +1499,7 @@ int ll_paged_attention(const ll_paged_attention_args *a, ll_stream_t stream) {
   p.kv_lengths = a->kv_lengths;
   p.query_starts = a->query_starts;
   p.ws = static_cast<float *>(a->workspace);
+  if (x.ws_floats > x.plan_at) p.plan = reinterpret_cast<int *>(p.ws + x.plan_at);
   p.q_token = a->query_token_stride;
   p.q_head = a->query_head_stride;
   p.pages_stride = a->page_table_stride;

@@ -160,6 +160,21 @@ def test_chunks_of_more_requests_than_a_wave_orders_at_once(gpu_device, heads, d
     _check_marked(paged_attention(**case), case)
 
 
+@pytest.mark.parametrize("count,queries_of", [
+    (257, lambda r: 1), (1100, lambda r: 1), (2600, lambda r: r % 3), (300, lambda r: (7 * r) % 31),
+    (1300, lambda r: 40 if r % 64 == 63 else 0)])
+def test_requests_past_the_plan_s_threshold(gpu_device, count, queries_of):
+    """Calls of many requests: short and long ones, ones without queries or keys."""
+
+    queries = [queries_of(r) for r in range(count)]
+    lengths = [0 if r % 53 == 17 else 1 + (29 * r) % 300 for r in range(count)]
+    lengths[count // 2], lengths[count - 1] = 4097, 1500
+    lengths = [max(length, n) if length else 0 for length, n in zip(lengths, queries)]
+    single = all(n == 1 for n in queries)
+    case = _marked(_case(gpu_device, lengths, None if single else queries, heads=(8, 2), dim=64, page=8))
+    _check_marked(paged_attention(**case), case)
+
+
 @pytest.mark.parametrize("queries", [None, [3, 1, 2], [200, 5, 90]])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_rows_that_are_not_seen_may_hold_anything(gpu_device, queries, dtype):
