@@ -392,6 +392,26 @@ def test_a_captured_call_serves_other_lengths(gpu_device, queries):
         _check(got, case)
 
 
+def test_a_captured_call_of_many_requests_serves_other_lengths(gpu_device):
+    """The sums over 200 requests are the replay's own, not the capture's."""
+
+    count = 200
+    case = _case(gpu_device, [600] * count, heads=(8, 2), dim=64, page=16)
+    paged_attention(**case)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = paged_attention(**case)
+    for step in range(3):
+        case["kv_lengths"].copy_(torch.tensor([(97 * r * (step + 1)) % 601 for r in range(count)]))
+        captured.fill_(9)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = captured.clone()
+        assert torch.equal(got, paged_attention(**case))
+        _check(got, case)
+
+
 def test_two_streams_at_once(gpu_device):
     """Calls in flight on two streams have workspaces of their own."""
 
