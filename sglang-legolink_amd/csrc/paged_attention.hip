@@ -1457,8 +1457,11 @@ int launch_all(const PagedParams &p, const Launch &x, hipStream_t s) {
   // may be more than 32 (64 chunks: 6.0 us on eight, 7.2 on four; 16 chunks: 4.9 and
   // 4.4).  Elsewhere a wave for all chunks of its columns: workgroups that mostly
   // find no column cost more than they save (16 requests on tiles of 256 columns).
+  // Between the two, by the chunks a tile may have (behind 32,768 keys: 64 tokens of
+  // 16/2 heads of 256, 25 chunks a tile, 69 us split and 93 not; 128 of 28/4 heads of
+  // 128, 16 chunks, 97 and 89).
   const unsigned split_groups = tile_heads * (columns / Combine<D, 4>::kColumns);
-  if (x.target < 8 * x.max_tiles || split_groups > 4 * kComputeUnits)
+  if (x.target < (split_groups > 4 * kComputeUnits ? 24 : 8) * x.max_tiles)
     paged_combine_kernel<D, E, 1><<<tile_heads * (columns / Combine<D, 1>::kColumns), 256, 0, s>>>(p, x.columns);
   else if (p.max_keys <= 32 * x.min_chunk * kPageTile)
     paged_combine_kernel<D, E, 4><<<split_groups, 4 * kWave, 0, s>>>(p, x.columns);
