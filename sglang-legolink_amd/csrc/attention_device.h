@@ -96,7 +96,7 @@ typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 // bytes land at the LDS base in M0 + 16 l).  They are issued from inline
 // assembly so that the compiler, which cannot tell the ring's stages apart,
 // does not add waits for every outstanding gather before each LDS access:
-// the loop below orders the stages itself with explicit vmcnt waits and
+// the kernels' loops order the stages themselves with explicit vmcnt waits and
 // barriers.  M0 is saved and restored around them.
 __device__ inline void dma_pair(const void *src0, void *lds0, const void *src1, void *lds1) {
   const unsigned base0 = __builtin_amdgcn_readfirstlane(
