@@ -22,6 +22,7 @@
 #include <c10/core/GradMode.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -114,10 +115,30 @@ struct Target {
 
 PyObject *none() { Py_RETURN_NONE; }
 
+// The tensors of a call that are not its rows: read, but for the counter.
+struct Beside {
+  std::array<const at::Tensor *, 4> read{};  // positions, table, norm weights (or null)
+  const at::Tensor *skipped = nullptr;
+
+  bool meets(const at::Tensor &written) const {
+    for (const at::Tensor *other : read)
+      if (other != nullptr && overlap(written, *other)) return true;
+    return skipped != nullptr && overlap(written, *skipped);
+  }
+  bool counter_apart(std::initializer_list<const at::Tensor *> rows) const {
+    if (skipped == nullptr) return true;
+    for (const at::Tensor *other : read)
+      if (other != nullptr && overlap(*skipped, *other)) return false;
+    for (const at::Tensor *other : rows)
+      if (overlap(*skipped, *other)) return false;
+    return true;
+  }
+};
+
 // What rotate_heads and append_rotated_kv_inplace have in common: query, key,
 // positions, cos_sin_cache, rotary_dim, neox, query norm, key norm, eps, skipped.
 bool read_rotary(PyObject *const *a, ll_head_rotary_args *args, const at::Tensor **query_out,
-                 const at::Tensor **key_out) {
+                 const at::Tensor **key_out, Beside *beside) {
   const at::Tensor *query = plain(a[0]), *key = plain(a[1]), *positions = plain(a[2]), *table = plain(a[3]);
   if (query == nullptr || query->dim() != 3) return false;
   const at::Device device = query->device();
@@ -148,7 +169,10 @@ bool read_rotary(PyObject *const *a, ll_head_rotary_args *args, const at::Tensor
     if (code < 0 || (args->norm_weight_dtype != 0 && args->norm_weight_dtype != code)) return false;
     args->norm_weight_dtype = code;
     *weights[i] = weight->data_ptr();
+    beside->read[2 + i] = weight;
   }
+  beside->read[0] = positions;
+  beside->read[1] = table;
   if (!number(a[8], &args->norm_eps) || !(args->norm_eps >= 0.0)) return false;
   args->skipped_rows = nullptr;
   if (a[9] != Py_None) {
@@ -157,6 +181,7 @@ bool read_rotary(PyObject *const *a, ll_head_rotary_args *args, const at::Tensor
         skipped->device() != device)
       return false;
     args->skipped_rows = static_cast<int64_t *>(skipped->data_ptr());
+    beside->skipped = skipped;
   }
   args->struct_size = sizeof(ll_head_rotary_args);
   args->num_tokens = tokens;
@@ -181,12 +206,13 @@ bool read_rotary(PyObject *const *a, ll_head_rotary_args *args, const at::Tensor
   return true;
 }
 
-// An output that is the input itself (the same Python object): its rows must lie
-// apart, and not meet the call's other tensors.
-bool in_place(const at::Tensor &rows, std::initializer_list<const at::Tensor *> others) {
-  if (!apart(rows)) return false;
+// An output that is its own input (the same Python object): its rows must lie
+// apart, and not meet the call's other tensors.  The others go by their role: one
+// that is the same object as the output is read by other waves while it is written.
+bool in_place(const at::Tensor &rows, std::initializer_list<const at::Tensor *> others, const Beside &beside) {
+  if (!apart(rows) || beside.meets(rows)) return false;
   for (const at::Tensor *other : others)
-    if (other != &rows && overlap(rows, *other)) return false;
+    if (overlap(rows, *other)) return false;
   return true;
 }
 
@@ -207,10 +233,13 @@ PyObject *rotate_heads(PyObject *const *a, Py_ssize_t n) {
   ll_head_rotary_args args;
   memset(&args, 0, sizeof(args));
   const at::Tensor *query, *key;
-  if (n != 15 || !target.read(a) || !read_rotary(a + 3, &args, &query, &key) || !target.takes(*query)) return none();
+  Beside beside;
+  if (n != 15 || !target.read(a) || !read_rotary(a + 3, &args, &query, &key, &beside) || !target.takes(*query) ||
+      !beside.counter_apart({query, key}))
+    return none();
   const bool query_in_place = a[13] != Py_None, key_in_place = a[14] != Py_None;
-  if (query_in_place && (a[13] != a[3] || !in_place(*query, {key}))) return none();
-  if (key_in_place && (a[14] != a[4] || !in_place(*key, {query}))) return none();
+  if (query_in_place && (a[13] != a[3] || !in_place(*query, {key}, beside))) return none();
+  if (key_in_place && (a[14] != a[4] || !in_place(*key, {query}, beside))) return none();
   if (target.entry == 0) Py_RETURN_TRUE;
   const at::Tensor query_output = query_in_place ? *query : empty_like_rows(*query);
   const at::Tensor key_output = key_in_place ? *key : empty_like_rows(*key);
@@ -233,10 +262,13 @@ PyObject *append(PyObject *const *a, Py_ssize_t n) {
   ll_head_rotary_args args;
   memset(&args, 0, sizeof(args));
   const at::Tensor *query, *key;
-  if (n != 18 || !target.read(a) || !read_rotary(a + 3, &args, &query, &key) || !target.takes(*query)) return none();
+  Beside beside;
+  if (n != 18 || !target.read(a) || !read_rotary(a + 3, &args, &query, &key, &beside) || !target.takes(*query))
+    return none();
   const at::Tensor *value = plain(a[14]), *keys = plain(a[15]), *values = plain(a[16]), *slots = plain(a[17]);
   if (args.num_tokens == 0 || !rows_ok(value, args.num_tokens, *query) || value->size(1) != key->size(1) ||
-      value->size(2) > 256 || !vector_ok(slots, args.num_tokens, query->device()))
+      value->size(2) > 256 || !vector_ok(slots, args.num_tokens, query->device()) ||
+      !beside.counter_apart({query, key, value, slots}))
     return none();
   args.destination_slots_dtype = index_code(slots->scalar_type());
   if (args.destination_slots_dtype < 0) return none();
@@ -246,12 +278,13 @@ PyObject *append(PyObject *const *a, Py_ssize_t n) {
     if (buffer == nullptr || buffer->dim() != 3 || buffer->size(0) != keys->size(0) ||
         buffer->size(1) != rows[i]->size(1) || buffer->size(2) != rows[i]->size(2) ||
         buffer->scalar_type() != query->scalar_type() || buffer->device() != query->device() ||
-        !buffer->is_contiguous() || overlap(*buffer, *query) || overlap(*buffer, *key) || overlap(*buffer, *value))
+        !buffer->is_contiguous() || overlap(*buffer, *query) || overlap(*buffer, *key) || overlap(*buffer, *value) ||
+        overlap(*buffer, *slots) || beside.meets(*buffer))
       return none();
   }
   if (overlap(*keys, *values)) return none();
   const bool query_in_place = a[13] != Py_None;
-  if (query_in_place && (a[13] != a[3] || !in_place(*query, {key, value, keys, values}))) return none();
+  if (query_in_place && (a[13] != a[3] || !in_place(*query, {key, value, keys, values, slots}, beside))) return none();
   if (target.entry == 0) Py_RETURN_TRUE;
   const at::Tensor query_output = query_in_place ? *query : empty_like_rows(*query);
   set_output(query_output, &args.query_output, &args.query_output_token_stride, &args.query_output_head_stride);

@@ -51,7 +51,7 @@ def _span(tensor: torch.Tensor) -> tuple[int, int]:
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Do two sets of rows [tokens, heads, dim] share bytes?  Exact for dense
-    heads of one token stride (views of one fused projection); other sets whose
+    heads of one token stride (views of one fused projection); other tensors whose
     spans meet count as overlapping."""
 
     if a.numel() == 0 or b.numel() == 0:
@@ -88,7 +88,10 @@ def _check_rows(name: str, rows: torch.Tensor, tokens: int, dtype: torch.dtype, 
         raise HeadRotaryError(f"{name}'s rows must be dense")
 
 
-def _check_output(name: str, output: torch.Tensor, source: torch.Tensor, inputs: Sequence[torch.Tensor]) -> None:
+def _check_output(name: str, output: torch.Tensor, source: torch.Tensor, others: Sequence[torch.Tensor]) -> None:
+    """An output is its own source or meets nothing of it, and meets none of the
+    call's other tensors, be they the source's own object in another role."""
+
     if output.shape != source.shape:
         raise HeadRotaryError(f"{name} must have the shape {tuple(source.shape)}, got {tuple(output.shape)}")
     _check_rows(name, output, int(source.shape[0]), source.dtype, source.device)
@@ -98,9 +101,8 @@ def _check_output(name: str, output: torch.Tensor, source: torch.Tensor, inputs:
     by_head = (tokens == 1 or token >= dim) and (heads == 1 or head >= (tokens - 1) * token + dim)
     if not (by_token or by_head):
         raise HeadRotaryError(f"{name}'s rows must not overlap each other")
-    for rows in inputs:
-        if not (rows is source and _same_view(output, source)) and _overlap(output, rows):
-            raise HeadRotaryError(f"{name} must be its input itself or not overlap the call's tensors")
+    if (not _same_view(output, source) and _overlap(output, source)) or any(_overlap(output, t) for t in others):
+        raise HeadRotaryError(f"{name} must be its input itself or not overlap the call's tensors")
 
 
 def _check_vector(name: str, values: torch.Tensor, count: int, device: torch.device) -> None:
@@ -171,6 +173,11 @@ def _rotary_args(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     return args
 
 
+def _check_counter(skipped_rows: Optional[torch.Tensor], others: Sequence[torch.Tensor]) -> None:
+    if skipped_rows is not None and any(_overlap(skipped_rows, tensor) for tensor in others):
+        raise HeadRotaryError("skipped_rows must not overlap the call's other tensors")
+
+
 def _launch(args: _native.HeadRotaryArgs, device: torch.device) -> None:
     if device.type != "cuda":
         raise HeadRotaryError("device tensors are required")
@@ -193,7 +200,8 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, *, positions: torch.Ten
     normed for each head by the given weights and turned to ``positions``.
 
     The table is the link's (``rope.build_cos_sin_cache``).  ``query_output`` and
-    ``key_output`` may be the inputs themselves (in place); they are new dense
+    ``key_output`` may be the inputs themselves (in place, each its own; what is
+    written overlaps none of the call's other tensors); they are new dense
     tensors by default.  A token whose position is outside the table is left
     out: its output rows keep what they held (undefined in a new tensor), and
     ``skipped_rows`` counts it.
@@ -212,14 +220,18 @@ def rotate_heads(query: torch.Tensor, key: torch.Tensor, *, positions: torch.Ten
     _refuse_gradients(query, key, query_norm_weight, key_norm_weight, cos_sin_cache, query_output, key_output)
     args = _rotary_args(query, key, positions, cos_sin_cache, rotary_dim, is_neox_style, query_norm_weight,
                         key_norm_weight, norm_eps, skipped_rows)
+    beside = [t for t in (positions, cos_sin_cache, query_norm_weight, key_norm_weight) if t is not None]
+    _check_counter(skipped_rows, (query, key, *beside))
+    if skipped_rows is not None:
+        beside.append(skipped_rows)
     if query_output is None:
         query_output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     else:
-        _check_output("query_output", query_output, query, (query, key))
+        _check_output("query_output", query_output, query, (key, *beside))
     if key_output is None:
         key_output = torch.empty(key.shape, dtype=key.dtype, device=key.device)
     else:
-        _check_output("key_output", key_output, key, (key, query))
+        _check_output("key_output", key_output, key, (query, *beside))
         if _overlap(key_output, query_output):
             raise HeadRotaryError("query_output and key_output must not overlap")
     args.query_output = query_output.data_ptr()
@@ -272,19 +284,24 @@ def append_rotated_kv_inplace(*, key_buffer: torch.Tensor, value_buffer: torch.T
         raise HeadRotaryError("key and value must have the same heads")
     if int(value.shape[2]) > 256:
         raise HeadRotaryError("head dims are at most 256")
+    beside = [t for t in (positions, cos_sin_cache, query_norm_weight, key_norm_weight, destination_slots)
+              if t is not None]
+    _check_counter(skipped_rows, (query, key, value, *beside))
+    if skipped_rows is not None:
+        beside.append(skipped_rows)
     for name, buffer, rows in (("key_buffer", key_buffer, key), ("value_buffer", value_buffer, value)):
         if buffer.ndim != 3 or buffer.shape[1:] != rows.shape[1:] or buffer.shape[0] != key_buffer.shape[0]:
             raise HeadRotaryError(f"{name} must be [slots, kv heads, dim] as the rows, got {tuple(buffer.shape)}")
         if buffer.dtype != query.dtype or buffer.device != query.device or not buffer.is_contiguous():
             raise HeadRotaryError(f"{name} must be a contiguous {query.dtype} tensor on the query's device")
-        if any(_overlap(buffer, other) for other in (query, key, value)):
-            raise HeadRotaryError(f"{name} must not overlap the call's rows")
+        if any(_overlap(buffer, other) for other in (query, key, value, *beside)):
+            raise HeadRotaryError(f"{name} must not overlap the call's other tensors")
     if _overlap(key_buffer, value_buffer):
         raise HeadRotaryError("key_buffer and value_buffer must not overlap")
     if query_output is None:
         query_output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     else:
-        _check_output("query_output", query_output, query, (query, key, value, key_buffer, value_buffer))
+        _check_output("query_output", query_output, query, (key, value, key_buffer, value_buffer, *beside))
     args.query_output = query_output.data_ptr()
     args.query_output_token_stride, args.query_output_head_stride = query_output.stride(0), query_output.stride(1)
     args.value = value.data_ptr()

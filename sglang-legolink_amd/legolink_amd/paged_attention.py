@@ -111,7 +111,8 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
     elif output.shape != query.shape or output.dtype != dtype or output.device != device or (
             not output.is_contiguous() or output.data_ptr() % 16):
         raise PagedAttentionError("output must be contiguous, 16-byte aligned and of the query's shape, dtype and device")
-    elif any(_meets(output, other) for other in (query, key_buffer, value_buffer, page_table, kv_lengths)):
+    elif any(_meets(output, other) for other in (query, key_buffer, value_buffer, page_table, kv_lengths, query_starts)
+             if other is not None):
         raise PagedAttentionError("output must not overlap the call's other tensors")
     if device.type != "cuda":
         raise PagedAttentionError("device tensors are required")
