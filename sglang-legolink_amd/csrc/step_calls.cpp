@@ -10,8 +10,9 @@
 // with nothing allocated or launched: the caller then runs the Python checks,
 // which name the reason (or take the call: only plain tensors on the current
 // device, and outputs that are new or the input itself, are taken here).  A
-// non-zero status of the library's entry comes back as an int.  With entry 0 the
-// checks run alone, on tensors of any device, and True comes back.
+// non-zero status of the library's entry comes back as an int.  Whatever fails once
+// the entry was called is raised: the call must not be made again.  With entry 0
+// the checks run alone, on tensors of any device, and True comes back.
 //
 // The module names the torch version and the block sizes that it was built for:
 // the caller uses it only where they are its own.
@@ -108,8 +109,29 @@ bool number(PyObject *object, double *out) {
 struct Target {
   int64_t entry = 0, stream = 0, device = 0;
   bool read(PyObject *const *a) { return integer(a[0], &entry) && integer(a[1], &stream) && integer(a[2], &device); }
-  bool takes(const at::Tensor &query) const {
-    return entry == 0 || (query.is_cuda() && query.device().index() == device);
+  // (Tensors in host memory have the index -1, which is no current device's.)
+  bool takes(const at::Tensor &query) const { return entry == 0 || query.device().index() == device; }
+
+  // The entry's status.  The call's result is made before it: behind it nothing is
+  // left that could fail.
+  template <typename Args>
+  int call(const Args *args, bool *launched) const {
+    typedef int (*Entry)(const Args *, ll_stream_t);
+    *launched = true;
+    return reinterpret_cast<Entry>(entry)(args, reinterpret_cast<ll_stream_t>(stream));
+  }
+};
+
+// An owned reference.
+struct Object {
+  PyObject *held;
+  explicit Object(PyObject *object) : held(object) {}
+  Object(const Object &) = delete;
+  ~Object() { Py_XDECREF(held); }
+  PyObject *release() {
+    PyObject *object = held;
+    held = nullptr;
+    return object;
   }
 };
 
@@ -224,11 +246,9 @@ void set_output(const at::Tensor &t, void **base, int64_t *token, int64_t *head)
   *head = t.stride(1);
 }
 
-typedef int (*RotaryEntry)(const ll_head_rotary_args *, ll_stream_t);
-
 // (entry, stream, device, query, key, positions, table, rotary_dim, neox, query
 // norm, key norm, eps, skipped, query_output, key_output) -> (query, key)
-PyObject *rotate_heads(PyObject *const *a, Py_ssize_t n) {
+PyObject *rotate_heads(PyObject *const *a, Py_ssize_t n, bool *launched) {
   Target target;
   ll_head_rotary_args args;
   memset(&args, 0, sizeof(args));
@@ -245,19 +265,18 @@ PyObject *rotate_heads(PyObject *const *a, Py_ssize_t n) {
   const at::Tensor key_output = key_in_place ? *key : empty_like_rows(*key);
   set_output(query_output, &args.query_output, &args.query_output_token_stride, &args.query_output_head_stride);
   set_output(key_output, &args.key_output, &args.key_output_token_stride, &args.key_output_head_stride);
-  const int status = reinterpret_cast<RotaryEntry>(target.entry)(&args, reinterpret_cast<ll_stream_t>(target.stream));
-  if (status != LL_OK) return PyLong_FromLong(status);
-  PyObject *first = THPVariable_Wrap(query_output), *second = THPVariable_Wrap(key_output);
-  PyObject *both = first != nullptr && second != nullptr ? PyTuple_Pack(2, first, second) : nullptr;
-  Py_XDECREF(first);
-  Py_XDECREF(second);
-  return both;
+  Object first(THPVariable_Wrap(query_output)), second(THPVariable_Wrap(key_output));
+  if (first.held == nullptr || second.held == nullptr) return nullptr;
+  Object both(PyTuple_Pack(2, first.held, second.held));
+  if (both.held == nullptr) return nullptr;
+  const int status = target.call(&args, launched);
+  return status != LL_OK ? PyLong_FromLong(status) : both.release();
 }
 
 // (entry, stream, device, query, key, positions, table, rotary_dim, neox, query
 // norm, key norm, eps, skipped, query_output, value, key_buffer, value_buffer,
 // slots) -> query
-PyObject *append(PyObject *const *a, Py_ssize_t n) {
+PyObject *append(PyObject *const *a, Py_ssize_t n, bool *launched) {
   Target target;
   ll_head_rotary_args args;
   memset(&args, 0, sizeof(args));
@@ -296,16 +315,17 @@ PyObject *append(PyObject *const *a, Py_ssize_t n) {
   args.value_buffer = values->data_ptr();
   args.num_slots = keys->size(0);
   args.destination_slots = slots->data_ptr();
-  const int status = reinterpret_cast<RotaryEntry>(target.entry)(&args, reinterpret_cast<ll_stream_t>(target.stream));
-  return status != LL_OK ? PyLong_FromLong(status) : THPVariable_Wrap(query_output);
+  Object result(THPVariable_Wrap(query_output));
+  if (result.held == nullptr) return nullptr;
+  const int status = target.call(&args, launched);
+  return status != LL_OK ? PyLong_FromLong(status) : result.release();
 }
 
-typedef int (*AttentionEntry)(const ll_paged_attention_args *, ll_stream_t);
 typedef int64_t (*WorkspaceEntry)(const ll_paged_attention_args *);
 
 // (entry, stream, device, workspace entry, query, key_buffer, value_buffer,
 // page_table, kv_lengths, page_size, query_starts, scale) -> output
-PyObject *paged_attention(PyObject *const *a, Py_ssize_t n) {
+PyObject *paged_attention(PyObject *const *a, Py_ssize_t n, bool *launched) {
   Target target;
   int64_t workspace_entry = 0, page_size = 0;
   if (n != 12 || !target.read(a) || !integer(a[3], &workspace_entry)) return none();
@@ -376,28 +396,37 @@ PyObject *paged_attention(PyObject *const *a, Py_ssize_t n) {
     args.workspace = workspace.data_ptr();
     args.workspace_bytes = needed;
   }
-  const int status =
-      reinterpret_cast<AttentionEntry>(target.entry)(&args, reinterpret_cast<ll_stream_t>(target.stream));
-  return status != LL_OK ? PyLong_FromLong(status) : THPVariable_Wrap(output);
+  Object result(THPVariable_Wrap(output));
+  if (result.held == nullptr) return nullptr;
+  const int status = target.call(&args, launched);
+  return status != LL_OK ? PyLong_FromLong(status) : result.release();
 }
 
-// No C++ exception leaves a call: an allocation that failed, say, is left to the
-// Python path, which meets it again.
-template <PyObject *(*kCall)(PyObject *const *, Py_ssize_t)>
+// No C++ exception leaves a call.  What fails before the library's entry is called,
+// an allocation say, is left to the Python path, which meets it again; from there
+// on it is raised.
+typedef PyObject *Call(PyObject *const *, Py_ssize_t, bool *);
+
+template <Call *kCall>
 PyObject *guarded(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
   PyObject *result = nullptr;
+  bool launched = false;
   try {
-    result = kCall(arguments, count);
+    result = kCall(arguments, count, &launched);
   } catch (...) {
     result = nullptr;
   }
   if (result != nullptr && !PyErr_Occurred()) return result;
   Py_XDECREF(result);
-  PyErr_Clear();
-  Py_RETURN_NONE;
+  if (!launched) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "a step call failed behind its launch");
+  return nullptr;
 }
 
-template <PyObject *(*kCall)(PyObject *const *, Py_ssize_t)>
+template <Call *kCall>
 PyCFunction entry() {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&guarded<kCall>));
 }
