@@ -32,11 +32,14 @@
 
 namespace {
 
+// A strided tensor that needs no gradient and has no forward-mode tangent (which
+// no_grad does not switch off).
 const at::Tensor *plain(PyObject *object) {
   if (object == nullptr || !THPVariable_CheckExact(object)) return nullptr;
   const at::Tensor &t = THPVariable_Unpack(object);
   if (t.layout() != at::kStrided || (t.requires_grad() && c10::GradMode::is_enabled()) || t.is_conj() || t.is_neg())
     return nullptr;
+  if (t._fw_grad(/*level=*/0).defined()) return nullptr;
   return &t;
 }
 

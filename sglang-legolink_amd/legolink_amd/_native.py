@@ -692,6 +692,16 @@ def paged_attention(args: PagedAttentionArgs, stream: int) -> None:
     _check(load_library().ll_paged_attention(ctypes.byref(args), _ptr(int(stream))))
 
 
+def differentiated(*tensors) -> bool:
+    """Does one of them (or None) need a gradient here, or carry a forward-mode
+    tangent (which ``no_grad`` does not switch off)?"""
+
+    present = [tensor for tensor in tensors if tensor is not None]
+    if torch.is_grad_enabled() and any(tensor.requires_grad for tensor in present):
+        return True
+    return any(torch.autograd.forward_ad.unpack_dual(tensor).tangent is not None for tensor in present)
+
+
 def step_calls():
     """The native module that makes a step's calls from their tensors, or None
     where it is not built or was built for another torch or other argument

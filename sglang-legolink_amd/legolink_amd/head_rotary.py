@@ -15,8 +15,8 @@ one after another (patched_sglang_files/python/sglang/srt/models/qwen2.py:
 
 Everything is computed in fp32 and rounded once; the calls are enqueued on the
 current stream, allocate nothing but the outputs they return, and may be
-captured into a HIP graph.  Inference only: tensors that need a gradient are
-refused.
+captured into a HIP graph.  Inference only: tensors that need a gradient or carry
+a forward-mode tangent are refused.
 """
 
 from __future__ import annotations
@@ -186,7 +186,7 @@ def _launch(args: _native.HeadRotaryArgs, device: torch.device) -> None:
 
 
 def _refuse_gradients(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(tensor is not None and tensor.requires_grad for tensor in tensors):
+    if _native.differentiated(*tensors):
         raise HeadRotaryError("these operators have no gradient: call them under torch.no_grad()")
 
 

@@ -75,7 +75,7 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
             _native.check_status(done)
         elif done is not None:
             return done
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (query, key_buffer, value_buffer)):
+    if _native.differentiated(query, key_buffer, value_buffer, output):
         raise PagedAttentionError("paged attention has no gradient: call it under torch.no_grad()")
     device, dtype = query.device, query.dtype
     if dtype not in _DTYPES:
