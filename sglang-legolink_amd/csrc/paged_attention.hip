@@ -34,6 +34,7 @@
 #include "attention_device.h"
 #include "legolink_kv.h"
 #include "ll_internal.h"
+#include "paged_units.h"
 
 namespace {
 
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
     Request x = Request{0, 0, 0};
     if (r < p.num_requests) x = request_at(p, r);
     const int tiles = tiles_of(p, x.q_len, columns);
-    const int chunks = max(1, (key_tiles_of(x) + chunk - 1) / chunk);
+    const int chunks = parts_of(key_tiles_of(x), chunk);
     const int of_wave[3] = {inclusive_scan(tiles * chunks), inclusive_scan(chunks > 1 ? tiles * chunks : 0),
                             inclusive_scan(tiles)};
     if (lane == kWave - 1)
@@ -264,7 +265,7 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
     if (first + lane < stop) mine = request_at(p, first + lane);
   }
 
-  w.chunk_keys = min(chunk, 33554431) * kPageTile;
+  w.chunk_keys = min(chunk, kOneChunk) * kPageTile;
   for (int r0 = first; r0 < stop; r0 += kWave) {
     Request x = mine;
     if (r0 > first) {
@@ -273,7 +274,7 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
     }
     const int tiles = tiles_of(p, x.q_len, columns);
     const int key_tiles = key_tiles_of(x);
-    const int chunks = max(1, (key_tiles + chunk - 1) / chunk);
+    const int chunks = parts_of(key_tiles, chunk);
     const int units_to = inclusive_scan(tiles * chunks);
     const int partials_to = inclusive_scan(chunks > 1 ? tiles * chunks : 0);
     const int tiles_to = kOfTiles ? inclusive_scan(tiles) : 0;
@@ -343,7 +344,7 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
       // The tile's last query and its position bound the keys.
       const int last_query = min(w.request.q_len - 1, ((w.tile + 1) * columns - 1) / p.group);
       w.key_end = max(0, w.request.kv_len - w.request.q_len + last_query + 1);
-      w.chunks = max(1, (w.key_end + w.chunk_keys - 1) / w.chunk_keys);
+      w.chunks = parts_of(w.key_end, w.chunk_keys);
       break;
     }
     units_before += __builtin_amdgcn_readlane(units_to, kWave - 1);
@@ -1348,7 +1349,8 @@ constexpr long long kPlanned = 128;
 
 struct Launch {
   int columns;
-  int max_tiles, max_units, max_partials, target, min_chunk;
+  long long max_tiles, max_units;
+  int max_partials, target, min_chunk;
   bool wide, splits;
   long long ws_floats, plan_at;  // of the workspace; where the plan begins in it (ws_floats: none)
 };
@@ -1367,10 +1369,8 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   const long long wanted = average * group;
   x.wide = wanted > 16;
   x.columns = x.wide ? (a->head_dim == 256 ? 128 : 256) : 16;
-  const long long tiles = a->query_starts == nullptr
-                              ? requests * ((group + x.columns - 1) / x.columns)
-                              : queries * group / x.columns + requests;
-  x.max_tiles = static_cast<int>(std::min(tiles, 0x7fffffffll));
+  x.max_tiles = a->query_starts == nullptr ? requests * ((group + x.columns - 1) / x.columns)
+                                           : queries * group / x.columns + requests;
   x.min_chunk = 2;
   // A workgroup fills a compute unit (its LDS rings), so `places` units of every
   // KV head run at once.  Chunks: as many units as places, the longest first, leave
@@ -1378,11 +1378,12 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   // at once; where they are many, two rounds, whose second the short ones fill (64
   // and 128 uneven requests: 390 and 212 us; one round 403 and 214, four 391 and 218).
   const int places = std::max(1, kComputeUnits / static_cast<int>(a->num_kv_heads));
-  x.target = x.wide ? places : 2 * x.max_tiles <= places ? places - x.max_tiles + 1 : 2 * places;
+  x.target = x.wide                           ? places
+             : 2 * x.max_tiles <= places ? places - static_cast<int>(x.max_tiles) + 1
+                                         : 2 * places;
   const long long max_keys = a->page_table_columns * a->page_size;
   x.splits = max_keys > x.min_chunk * kPageTile;
-  const long long units = tiles + (x.splits ? x.target + 1 : 0);
-  x.max_units = static_cast<int>(std::min(units, 0x7fffffffll));
+  x.max_units = x.max_tiles + (x.splits ? x.target + 1 : 0);
   x.max_partials = x.splits ? 2 * x.target + 2 : 0;
   x.plan_at = x.max_partials * a->num_kv_heads * x.columns * (a->head_dim + 2);
   x.ws_floats = x.plan_at + (requests > kPlanned ? plan_ints(requests) : 0);
@@ -1436,8 +1437,8 @@ int check_args(const ll_paged_attention_args *a) {
   const Launch x = plan_launch(a);
   // A launch holds fewer than 2^32 threads: at most 512 a unit and KV head, 16 a
   // column.
-  if (static_cast<long long>(x.max_units) * a->num_kv_heads > 0x7fffffll ||
-      static_cast<long long>(x.max_tiles) * a->num_kv_heads * x.columns > 0xfffffffll)
+  if (x.max_units * a->num_kv_heads > 0x7fffffll ||
+      x.max_tiles * a->num_kv_heads * x.columns > 0xfffffffll)
     return fail(LL_ERR_INVALID_ARGUMENT, "too many queries for one launch");
   return LL_OK;
 }
@@ -1523,7 +1524,7 @@ int ll_paged_attention(const ll_paged_attention_args *a, ll_stream_t stream) {
   p.group = p.hq / p.hkv;
   p.lengths64 = a->kv_lengths_dtype == LL_DTYPE_INT64 ? 1 : 0;
   p.starts64 = a->query_starts_dtype == LL_DTYPE_INT64 ? 1 : 0;
-  p.min_chunk = x.splits ? x.min_chunk : 33554431;  // one chunk of any length
+  p.min_chunk = x.splits ? x.min_chunk : kOneChunk;
   p.inv_target = 1.0 / x.target;
   p.max_partials = x.max_partials;
   p.scale_log2 = static_cast<float>(a->softmax_scale * 1.4426950408889634);  // log2(e)
