@@ -728,7 +728,7 @@ typedef struct ll_paged_attention_args {
   int64_t num_kv_heads;
   int64_t head_dim;                /* 64, 128 or 256 */
   int64_t kv_dtype;                /* LL_DTYPE_BFLOAT16 or LL_DTYPE_FLOAT16 */
-  double softmax_scale;            /* positive */
+  double softmax_scale;            /* in [1e-37, 1e30) */
   const int32_t *page_table;       /* device int32 [num_requests, page_table_columns] */
   int64_t page_table_stride;       /* of a request's row, in entries */
   int64_t page_table_columns;      /* times page_size: below 2^30 */

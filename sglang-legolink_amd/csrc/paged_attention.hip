@@ -1404,8 +1404,10 @@ int check_args(const ll_paged_attention_args *a) {
     return fail(LL_ERR_HEAD_DIMENSION_OUT_OF_RANGE, "head_dim must be 64, 128 or 256");
   if (a->kv_dtype != LL_DTYPE_FLOAT16 && a->kv_dtype != LL_DTYPE_BFLOAT16)
     return fail(LL_ERR_FP16_OR_BF16_REQUIRED, "kv_dtype must be fp16 or bf16");
-  if (!(a->softmax_scale > 0.0) || !(a->softmax_scale < 1e30))
-    return fail(LL_ERR_INVALID_ARGUMENT, "softmax_scale must be positive and finite");
+  // (In fp32 the scale and kSlack over it are normal numbers: with a scale of 0 the
+  // score of a hidden key, -inf, would weigh exp2(-inf * 0).)
+  if (!(a->softmax_scale >= 1e-37) || !(a->softmax_scale < 1e30))
+    return fail(LL_ERR_INVALID_ARGUMENT, "softmax_scale must be in [1e-37, 1e30)");
   const long long group = a->num_q_heads / a->num_kv_heads;
   if (a->num_queries < 0 || a->num_requests < 0 || a->num_requests > 0x3fffffff ||
       a->num_queries > 0x3fffffff / group)

@@ -367,7 +367,7 @@ PyObject *paged_attention(PyObject *const *a, Py_ssize_t n, bool *launched) {
   }
   if (a[11] == Py_None) args.softmax_scale = 1.0 / std::sqrt(static_cast<double>(dim));
   else if (!number(a[11], &args.softmax_scale)) return none();
-  if (!(args.softmax_scale > 0.0 && args.softmax_scale < 1e30)) return none();
+  if (!(args.softmax_scale >= 1e-37 && args.softmax_scale < 1e30)) return none();
   if (query->stride(2) != 1 || query->stride(0) % 8 != 0 || query->stride(1) % 8 != 0 ||
       reinterpret_cast<uintptr_t>(query->data_ptr()) % 16 != 0)
     return none();

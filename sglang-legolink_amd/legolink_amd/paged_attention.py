@@ -104,8 +104,8 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
     elif queries != requests:
         raise PagedAttentionError("without query_starts every request has one query")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise PagedAttentionError("scale must be positive and finite")
+    if not 1e-37 <= scale < 1e30:  # a normal number in the kernels' fp32
+        raise PagedAttentionError("scale must be in [1e-37, 1e30)")
     if output is None:
         output = torch.empty((queries, q_heads, dim), dtype=dtype, device=device)
     elif output.shape != query.shape or output.dtype != dtype or output.device != device or (

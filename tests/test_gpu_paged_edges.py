@@ -22,3 +22,10 @@ def test_tables_of_at_most_128_keys(gpu_device, queries, heads, dim, page):
     assert case["page_table"].shape[1] * page == 128
     _check(paged_attention(**case), case)
     _check_marked(paged_attention(**_marked(case)), case)
+
+
+@pytest.mark.parametrize("queries", [None, [200, 1]])
+@pytest.mark.parametrize("scale", [1e-37, 1e-30])
+def test_the_smallest_scales_weigh_all_keys_alike(gpu_device, queries, scale):
+    case = _case(gpu_device, [300, 64], queries, heads=(4, 2), dim=64, dtype=torch.bfloat16)
+    _check(paged_attention(**case, scale=scale), case, scale=scale)

@@ -10,8 +10,10 @@ import sys
 import pytest
 
 from legolink_amd import _native, build
+from legolink_amd.paged_attention import PagedAttentionError, paged_attention
 from tests import test_host_sanitizer as sanitizer
-from tests.test_paged_attention import _block
+from tests.test_paged_attention import _arguments, _block
+from tests.test_step_calls import _attend
 
 
 @pytest.mark.parametrize("requests", [2 ** 30 - 1, 2 ** 29 + 1])
@@ -56,3 +58,23 @@ def test_the_step_entries_are_clean_under_asan_and_ubsan():
     assert "AddressSanitizer" not in output and "runtime error:" not in output, output[-6000:]
     assert result.returncode == 0, output[-6000:]
     assert " passed" in result.stdout, output[-3000:]
+
+
+@pytest.mark.parametrize("scale", [5e-324, 1e-46, 1e-40, 9e-38])
+def test_scales_that_fp32_does_not_hold_are_refused(scale):
+    """The kernels' scale and the maximum's slack over it are normal fp32 numbers."""
+
+    with pytest.raises(_native.NativeCallError, match="softmax_scale") as error:
+        _native.paged_attention_workspace_bytes(_block(softmax_scale=scale))
+    assert error.value.reason == "invalid_argument"
+    with pytest.raises(PagedAttentionError, match="scale"):
+        paged_attention(**_arguments(), scale=scale)
+    assert _attend({**_arguments(), "scale": scale}) is None
+
+
+@pytest.mark.parametrize("scale", [1e-37, 1e-30, 9e29])
+def test_scales_that_it_holds_are_taken(scale):
+    assert _native.paged_attention_workspace_bytes(_block(softmax_scale=scale)) > 0
+    with pytest.raises(PagedAttentionError, match="device tensors are required"):
+        paged_attention(**_arguments(), scale=scale)
+    assert _attend({**_arguments(), "scale": scale}) is True
