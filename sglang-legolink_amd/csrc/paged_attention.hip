@@ -355,7 +355,8 @@ __device__ inline Work find_work(const PagedParams &p, int columns, int index) {
 }
 
 // A partial result of one KV head: `columns` rows of D floats (the sum of the
-// weighted values, unnormalised), then (maximum, sum) pairs.
+// weighted values, unnormalised), then (maximum of the scores before their scale,
+// sum) pairs.
 template <int D>
 __device__ inline float *partial_of(const PagedParams &p, int columns, int partial, int head) {
   return p.ws + (static_cast<long long>(partial) * p.hkv + head) * columns * (D + 2);
@@ -405,9 +406,17 @@ __device__ inline f32x4 nonfinite_only(u32x2 bits) {  // four values, the finite
   return out;
 }
 
-// The weight, under the maximum `top` of several, of a result with the maximum `own`.
-__device__ inline float joined_weight(float own, float top) {
-  return own == -INFINITY && top == -INFINITY ? 1.f : exp2f(own - top);  // (sums of nothing seen are 0)
+// The exponent of a score s under the maximum m is s * scale - m * scale, one fma,
+// whose second term is rounded: by up to 2^-5 below this limit, which is the same
+// factor for every weight of the row, but by more than the weights' range holds where
+// it is far beyond.  A wave with such a row subtracts first: (s - m) * scale.
+constexpr float kLarge = 1048576.f;
+__device__ inline bool is_large(float bias) { return fabsf(bias) >= kLarge; }
+
+// The weight, under the maximum `top` of several, of a result with the maximum `own`
+// (of scores without their scale).
+__device__ inline float joined_weight(float own, float top, float scale_log2) {
+  return own == -INFINITY && top == -INFINITY ? 1.f : exp2f((own - top) * scale_log2);  // (sums of nothing seen are 0)
 }
 
 // Column statistics across the four lane groups of a 16-column MFMA.
@@ -512,6 +521,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
   }
 
   float m = -INFINITY, l = 0.f;
+  bool large = false;  // of a column of the wave
   f32x4 o[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -636,17 +646,21 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
       const bool raise = top > m + slack;
       const float m_new = raise ? top : m;
       const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[rb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][r], scale_log2, bias));
       if (__builtin_amdgcn_ballot_w64(raise) != 0) {
         const float alpha = raise ? __builtin_amdgcn_exp2f((m - m_new) * scale_log2) : 1.f;
         l *= alpha;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) o[b] *= alpha;
+        large = __builtin_amdgcn_ballot_w64(is_large(bias)) != 0;
       }
       m = m_new;
+      const float top_seen = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[rb][r] = __builtin_amdgcn_exp2f(large ? (s[rb][r] - top_seen) * scale_log2
+                                                  : __builtin_fmaf(s[rb][r], scale_log2, bias));
       u32x4 weights;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -692,7 +706,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
   __syncthreads();  // the rings are read
   const float total = sum_of_groups(l);
   if (g == 0) {
-    stats[wave][col][0] = m == -INFINITY ? -INFINITY : m * scale_log2;
+    stats[wave][col][0] = m;
     stats[wave][col][1] = total;
   }
 #pragma unroll
@@ -710,7 +724,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < N::kWaves; ++v) {
-      const float weight = joined_weight(stats[v][c][0], top);
+      const float weight = joined_weight(stats[v][c][0], top, scale_log2);
       sum += weight * stats[v][c][1];
       acc += weight * *reinterpret_cast<const f32x4 *>(joined + (v * 16 + c) * kPitch + 4 * quad);
     }
@@ -830,6 +844,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   }
 
   float m = -INFINITY;
+  bool large = false;  // of a column of the wave
   float l4[4] = {0.f, 0.f, 0.f, 0.f};  // the weights' sum, in four chains: a dot product waits for the one before
   f32x16 o[kBlocks];
 #pragma unroll
@@ -992,18 +1007,31 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     const bool raise = top > m + slack;
     const float m_new = raise ? top : m;
     const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], scale_log2, bias));
     if (__builtin_amdgcn_ballot_w64(raise) != 0) {
       const float alpha = raise ? __builtin_amdgcn_exp2f((m - m_new) * scale_log2) : 1.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) l4[i] *= alpha;
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) o[b] *= alpha;
+      large = __builtin_amdgcn_ballot_w64(is_large(bias)) != 0;
     }
     m = m_new;
+    if (!large) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], scale_log2, bias);
+    } else {
+      const float top_seen = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = (s[kb][r] - top_seen) * scale_log2;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_amdgcn_exp2f(s[kb][r]);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -1236,7 +1264,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
   float *partial = partial_of<D>(p, W::kColumns, w.first_partial + w.chunk * w.partial_step, head);
   const int c = 32 * wave + col;
   if (h == 0) {
-    partial[W::kColumns * D + 2 * c] = m == -INFINITY ? -INFINITY : m * scale_log2;
+    partial[W::kColumns * D + 2 * c] = m;
     partial[W::kColumns * D + 2 * c + 1] = l;
   }
   float *dst = partial + c * D + 4 * h;
@@ -1301,14 +1329,14 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
 #pragma unroll
       for (int i = 0; i < C::kBatch; ++i)
         if (s0 + i * kSplit < w.chunks) high = fmaxf(high, tops[i]);
-      const float old = joined_weight(top, high);
+      const float old = joined_weight(top, high, p.scale_log2);
       sum *= old;
       acc *= old;
       top = high;
 #pragma unroll
       for (int i = 0; i < C::kBatch; ++i)
         if (s0 + i * kSplit < w.chunks) {
-          const float weight = joined_weight(tops[i], top);
+          const float weight = joined_weight(tops[i], top, p.scale_log2);
           sum += weight * sums[i];
           acc += weight * rows[i];
         }
@@ -1327,7 +1355,7 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
       acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int v = 0; v < kSplit; ++v) {
-        const float weight = joined_weight(tops[v][lane], top);
+        const float weight = joined_weight(tops[v][lane], top, p.scale_log2);
         sum += weight * sums[v][lane];
         acc += weight * parts[v][lane];
       }

@@ -29,3 +29,29 @@ def test_tables_of_at_most_128_keys(gpu_device, queries, heads, dim, page):
 def test_the_smallest_scales_weigh_all_keys_alike(gpu_device, queries, scale):
     case = _case(gpu_device, [300, 64], queries, heads=(4, 2), dim=64, dtype=torch.bfloat16)
     _check(paged_attention(**case, scale=scale), case, scale=scale)
+
+
+@pytest.mark.parametrize("queries", [None, [130], [9]])
+@pytest.mark.parametrize("length", [140, 900])
+@pytest.mark.parametrize("dim,dtype", [(64, torch.bfloat16), (128, torch.float16), (256, torch.bfloat16)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_of_any_size_that_fp32_holds(gpu_device, queries, length, dim, dtype, sign):
+    """Keys of equal largest scores share the weight alike, the others have none,
+    whatever the scores: products that are exact in fp32, from 2^12 to 2^126 (fp16: to
+    2^36), and scaled ones past its largest number."""
+
+    report(f"score sizes, queries {queries} length {length} dim {dim} {dtype} sign {sign}")
+    case = _case(gpu_device, [length], queries, heads=(4, 2), dim=dim, dtype=dtype, page=1)
+    slots = case["page_table"][0, :length].long()
+    tied = torch.tensor([0, 3, 5, 9], device=gpu_device)  # seen by every query
+    keys = torch.full((length,), 0.75 if sign > 0 else 1.25, device=gpu_device)
+    keys[tied] = 1.0
+    want = case["value_buffer"][slots[tied]].double().mean(0).repeat_interleave(2, dim=0)  # [q heads, dim]
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + 8 * 2.0 ** -24 * 8  # the rounding, and sums in fp32
+    # 2^power a query and a key: scores of dim 2^(2 power) scale.
+    for power, scale in ((3, 1 / 3), (8, 1 / 3), (11, 1 / 3), (14, 1 / 3), *(
+            ((30, 1 / 3), (59, 1 / 3), (59, 100.0)) if dtype == torch.bfloat16 else ((14, 1e28),))):
+        case["query"].fill_(2.0 ** power)
+        case["key_buffer"][slots] = (sign * 2.0 ** power * keys).to(dtype)[:, None, None]
+        off = (paged_attention(**case, scale=scale).double() - want).abs()
+        assert bool((off <= bound).all()), (power, scale, off.max().item())
