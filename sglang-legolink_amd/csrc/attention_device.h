@@ -26,6 +26,7 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 struct Bf16 {
   typedef bf16x8 frag;
   static constexpr uint32_t kOnes = 0x3F803F80u;  // two 1.0s
+  static constexpr float kWeightShift = 0.f;      // log2 of what paged attention scales its weights by
   __device__ static uint32_t pack(float lo, float hi) {  // one v_cvt_pk_bf16_f32
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
   }
@@ -48,6 +49,7 @@ struct Bf16 {
 struct F16 {
   typedef f16x8 frag;
   static constexpr uint32_t kOnes = 0x3C003C00u;
+  static constexpr float kWeightShift = 7.f;
   __device__ static uint32_t pack(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, f16x2));
   }

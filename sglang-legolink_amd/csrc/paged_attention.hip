@@ -406,12 +406,24 @@ __device__ inline f32x4 nonfinite_only(u32x2 bits) {  // four values, the finite
   return out;
 }
 
+// Weights are 2^kWeightShift times what they are of the maximum, and so are their
+// sums: they go to the value product in the KV type, where fp16 ends at 2^-25.  With
+// the shift, a weight counts down to 2^-32 of the maximum, so that those lost beside
+// one large key weigh less than 2^-15 over 131,072 keys (unshifted, 2^-8 and eight
+// times the output's rounding); the largest, at kSlack above the maximum, is 2^15.
+// (bf16 has fp32's range.)
+//
 // The exponent of a score s under the maximum m is s * scale - m * scale, one fma,
 // whose second term is rounded: by up to 2^-5 below this limit, which is the same
 // factor for every weight of the row, but by more than the weights' range holds where
 // it is far beyond.  A wave with such a row subtracts first: (s - m) * scale.
 constexpr float kLarge = 1048576.f;
 __device__ inline bool is_large(float bias) { return fabsf(bias) >= kLarge; }
+
+template <typename E>
+__device__ inline float weight_bias(float m, float scale_log2) {
+  return __builtin_fmaf(-m, scale_log2, E::kWeightShift);
+}
 
 // The weight, under the maximum `top` of several, of a result with the maximum `own`
 // (of scores without their scale).
@@ -645,7 +657,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
       top = max_of_groups(top);
       const bool raise = top > m + slack;
       const float m_new = raise ? top : m;
-      const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
+      const float bias = m_new == -INFINITY ? 0.f : weight_bias<E>(m_new, scale_log2);  // nothing seen yet: all weights 0
       if (__builtin_amdgcn_ballot_w64(raise) != 0) {
         const float alpha = raise ? __builtin_amdgcn_exp2f((m - m_new) * scale_log2) : 1.f;
         l *= alpha;
@@ -659,7 +671,7 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
       for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          s[rb][r] = __builtin_amdgcn_exp2f(large ? (s[rb][r] - top_seen) * scale_log2
+          s[rb][r] = __builtin_amdgcn_exp2f(large ? __builtin_fmaf(s[rb][r] - top_seen, scale_log2, E::kWeightShift)
                                                   : __builtin_fmaf(s[rb][r], scale_log2, bias));
       u32x4 weights;
 #pragma unroll
@@ -1006,7 +1018,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
     }
     const bool raise = top > m + slack;
     const float m_new = raise ? top : m;
-    const float bias = m_new == -INFINITY ? 0.f : -m_new * scale_log2;  // nothing seen yet: all weights 0
+    const float bias = m_new == -INFINITY ? 0.f : weight_bias<E>(m_new, scale_log2);  // nothing seen yet: all weights 0
     if (__builtin_amdgcn_ballot_w64(raise) != 0) {
       const float alpha = raise ? __builtin_amdgcn_exp2f((m - m_new) * scale_log2) : 1.f;
 #pragma unroll
@@ -1026,7 +1038,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads) paged_wide_kernel(const Pag
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][r] = (s[kb][r] - top_seen) * scale_log2;
+        for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r] - top_seen, scale_log2, E::kWeightShift);
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)

@@ -55,3 +55,32 @@ def test_scores_of_any_size_that_fp32_holds(gpu_device, queries, length, dim, dt
         case["key_buffer"][slots] = (sign * 2.0 ** power * keys).to(dtype)[:, None, None]
         off = (paged_attention(**case, scale=scale).double() - want).abs()
         assert bool((off <= bound).all()), (power, scale, off.max().item())
+
+
+@pytest.mark.parametrize("queries", [None, [40]])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_small_weights_beside_a_large_one(gpu_device, queries, dtype):
+    """20,000 keys of weight 2^-26 beside one of weight 1, with values 64 times its:
+    2 % of the result.  (256 KV heads: a workgroup takes all keys of one.)"""
+
+    length, heads, dim = 20001, 256, 64
+    case = _case(gpu_device, [length], queries, heads=(heads, heads), dim=dim, dtype=dtype, page=16)
+    slot = int(case["page_table"][0, 0]) * 16  # key 0
+    for name, first, rest in (("key_buffer", 0.0, -2.25), ("value_buffer", 1.0, 64.0)):
+        case[name].fill_(rest)
+        case[name][slot] = first
+    case["query"].fill_(1.0)
+    got = paged_attention(**case, scale=0.125).double()
+    rows = got.shape[0]
+    others = torch.arange(length - rows, length, dtype=torch.float64, device=gpu_device)  # that a query sees
+    small = torch.exp(torch.tensor(-dim * 2.25 * 0.125, dtype=torch.float64, device=gpu_device))
+    want = ((1.0 + small * others * 64.0) / (1.0 + small * others))[:, None, None]
+    # The output's rounding; fp32 sums over the keys; of the small weights' part a
+    # score's error (67 roundings of 18) and exp2's, and a weight's rounding: relative,
+    # half a step, or in fp16's subnormal range 2^-25 on weights of up to 2^7.
+    info = torch.finfo(dtype)
+    bound = info.eps / 2 * want + (length + 64) * 2.0 ** -24 * want
+    bound = bound + (want - 1.0) * (67 * 2.0 ** -24 * 18 + 2.0 ** -20 + info.eps / 2)
+    if dtype == torch.float16:
+        bound = bound + length * 2.0 ** -32 * 64.0
+    assert bool(((got - want).abs() <= bound).all()), ((got - want).abs() / bound).max().item()
