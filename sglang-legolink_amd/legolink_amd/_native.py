@@ -692,6 +692,16 @@ def paged_attention(args: PagedAttentionArgs, stream: int) -> None:
     _check(load_library().ll_paged_attention(ctypes.byref(args), _ptr(int(stream))))
 
 
+def whole_number(value):
+    """``value`` as an int, or None where it is no whole number."""
+
+    try:
+        number = int(value)
+    except (TypeError, ValueError, OverflowError):
+        return None
+    return number if number == value else None
+
+
 def differentiated(*tensors) -> bool:
     """Does one of them (or None) need a gradient here, or carry a forward-mode
     tangent (which ``no_grad`` does not switch off)?"""

@@ -127,8 +127,8 @@ def _rotary_args(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
         raise HeadRotaryError("query and key must have one head dim")
     if dim > 256:
         raise HeadRotaryError("head dims are at most 256")
-    rotary_dim = int(rotary_dim)
-    if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > dim:
+    rotary_dim = _native.whole_number(rotary_dim)
+    if rotary_dim is None or rotary_dim < 2 or rotary_dim % 2 or rotary_dim > dim:
         raise HeadRotaryError("rotary_dim must be even and in [2, head dim]")
     _check_vector("positions", positions, tokens, device)
     if positions.dtype not in _INDEX_DTYPES:

@@ -96,8 +96,9 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
             page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise PagedAttentionError("page_table must be int32 [requests, pages] with dense rows on the query's device")
     requests, pages = page_table.shape
-    if int(page_size) < 1:
-        raise PagedAttentionError("page_size must be positive")
+    page_size = _native.whole_number(page_size)
+    if page_size is None or page_size < 1:
+        raise PagedAttentionError("page_size must be positive and whole")
     _check_counts("kv_lengths", kv_lengths, requests, device)
     if query_starts is not None:
         _check_counts("query_starts", query_starts, requests + 1, device)
@@ -130,7 +131,7 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
     args.softmax_scale = scale
     args.page_table = page_table.data_ptr()
     args.page_table_stride, args.page_table_columns = page_table.stride(0), pages
-    args.page_size = int(page_size)
+    args.page_size = page_size
     args.kv_lengths, args.kv_lengths_dtype = kv_lengths.data_ptr(), _INDEX_DTYPES[kv_lengths.dtype]
     if query_starts is not None:
         args.query_starts, args.query_starts_dtype = query_starts.data_ptr(), _INDEX_DTYPES[query_starts.dtype]
