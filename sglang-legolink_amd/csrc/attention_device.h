@@ -30,7 +30,7 @@ struct Bf16 {
   __device__ static uint32_t pack(float lo, float hi) {  // one v_cvt_pk_bf16_f32
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
   }
-  static constexpr uint32_t kExponent = 0x7F80u, kFraction = 0x007Fu, kOne = 0x3F80u;  // of one value's bits
+  static constexpr uint32_t kExponent = 0x7F80u;  // of one value's bits
   __device__ static f32x16 mfma32(frag a, frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -53,7 +53,7 @@ struct F16 {
   __device__ static uint32_t pack(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, f16x2));
   }
-  static constexpr uint32_t kExponent = 0x7C00u, kFraction = 0x03FFu, kOne = 0x3C00u;
+  static constexpr uint32_t kExponent = 0x7C00u;
   __device__ static f32x16 mfma32(frag a, frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
