@@ -697,7 +697,8 @@ int64_t ll_head_rotary_args_size(void);
  * h / (num_q_heads / num_kv_heads):
  *     output[i][h] = sum_j softmax_j(softmax_scale * q . K_j) V_j
  * with the softmax in fp32, its weights rounded to the KV type for the value
- * product and the output rounded once.  A query that sees no key gets zeros.
+ * product (in fp16 those below 2^-32 of the largest may count as 0) and the output
+ * rounded once.  A query that sees no key gets zeros.
  *
  * The lengths, starts and pages are read on the device, so that one captured
  * call serves any lengths that its shapes hold: lengths are held to [0,
@@ -706,6 +707,14 @@ int64_t ll_head_rotary_args_size(void);
  * requests share queries, leave those rows undefined.)  Keys of a page outside
  * the pool are invisible (never read), as is everything behind a request's
  * length, whatever it holds.  Queries of no request keep their output rows.
+ *
+ * One kernel takes the whole call, chosen by its average request, num_queries /
+ * num_requests: by up to 16 (query, head) pairs a KV head one for single tokens,
+ * else one for chunks.  A chunk among many single tokens, or beside many requests
+ * without queries, is right but slow there (it reads its keys once for every 16
+ * pairs): make two calls, and leave padding requests out.
+ *
+ * Scores of any size that fp32 holds are told apart as fp32 does.
  *
  * Workspace: ll_paged_attention_workspace_bytes(args), a bound that follows from
  * the shapes alone (70 MB at 4 KV heads of 128, whatever the lengths).  Calls

@@ -145,8 +145,8 @@ __device__ inline Token token_at(const RotaryParams &p, long long t, bool first)
 // power of two of D / 16, so that the norm's sum is kGroup's xor shuffles;
 // lanes past D / 16 idle), 64 / kGroup heads a step, queries first, then keys;
 // the steps behind them copy the values, 128 chunks of 8 at a time.  8,192 tokens
-// of 64 + 8 normed heads of 128: 64.4 us, 4.7 TB/s read and written (a copy of as
-// many bytes 62 us); one token 3.6 us, the latency of its position, the table row
+// of 64 + 8 normed heads of 128: 64.6 us, 4.7 TB/s read and written (a copy of as
+// many bytes 62 us); one token 3.1 us, the latency of its position, the table row
 // behind it and the stores.
 template <typename E, int kGroup>
 __global__ void __launch_bounds__(kThreads) head_rotary_vec_kernel(const RotaryParams p) {
@@ -265,8 +265,9 @@ __global__ void __launch_bounds__(kThreads) head_rotary_vec_kernel(const RotaryP
 // values), a lane every 64th of its rotary pairs and of the values behind them.
 // All of a row's loads come before its stores, so that it may be rotated in
 // place, and those of the row do not wait for the position.  Bound by its 2-byte
-// loads and stores: the rows above, one value off their alignment, take 296 us
-// (1.0 TB/s; 393 with a lane per value, each loading its partner too).
+// loads and stores: the rows above, one value off their alignment, take 285 us
+// (1.1 TB/s; 393 with a lane per value, each loading its partner too), 8,192 tokens
+// of 72 heads of 40 and of 200 values 177 and 358 us (0.5 and 1.3 TB/s).
 template <typename E>
 __global__ void __launch_bounds__(kThreads) head_rotary_element_kernel(const RotaryParams p) {
   constexpr int kPer = kMaxDim / kWave;

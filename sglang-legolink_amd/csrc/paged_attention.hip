@@ -21,7 +21,13 @@
 // are gathered by slot straight into LDS; the softmax runs in fp32 with exp2
 // and a maximum that is only raised where a score passes it by 8 (in log2);
 // the probabilities go from the S^T accumulators to the value product rounded
-// to the KV type, V^T through transposed LDS reads.
+// to the KV type, V^T through transposed LDS reads.  That rounding is the price of
+// the matrix unit, which takes both operands of one 16-bit type: a second product
+// with what the rounding leaves would be half as many MFMAs again (and 0 times an
+// infinity a NaN).  The sums are of the rounded weights, so a constant comes back as
+// it is; of random values the results are 1.1 to 1.4 times as far from 64 bits as a
+// single rounding of the output (bf16 0.0018-0.0024 of their norm against 0.0017,
+// fp16 0.00029 against 0.00021).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdarg.h>
@@ -217,8 +223,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
 // requests' last chunks, the longest first (kByLength), or by the quarter of a full
 // chunk that they fill (kByQuarter, whose cost does not grow with the requests).
 // Workgroups start in that order, so the short units fill the last round.  Six
-// chunks of 5 to 701 queries, 14/2 heads of 64, over 300 to 9,000 keys: 85 us by
-// length, 88 by quarter, 98 request by request; 64 and 128 uneven requests of
+// chunks of 5 to 701 queries, 14/2 heads of 64, over 300 to 9,000 keys: 80 us by
+// length, 84 by quarter, 98 request by request; 64 and 128 uneven requests of
 // single tokens, 64/8 heads of 128: 390 and 212 us by quarter, 389 and 242 by
 // length, 406 and 224 request by request.
 enum class Order { kTiles, kByLength, kByQuarter };  // (kTiles: tiles, request by request)
@@ -457,9 +463,9 @@ __device__ inline void wait_vm() {
 // Up to 16 columns: single tokens, bound by reading the keys and values once.  The
 // waves of a workgroup take turns at its 32-key subtiles, each through an LDS ring
 // of its own (no barriers: a wave waits for its own gathers alone), and join their
-// results at the end.  131,072 keys of 4 heads of 128: 47 us, 5.7 TB/s (a read-only
-// pass reaches 6.0); 64 uneven requests, 2.13 GB: 387 us, 5.5 TB/s; 2,048 keys
-// 6.5 us, the latencies of the lengths, the pages, the rows and the join.
+// results at the end.  131,072 keys of 4 heads of 128: 47.5 us, 5.65 TB/s (a read-only
+// pass reaches 6.0); 64 uneven requests, 2.13 GB: 391 us, 5.5 TB/s; 2,048 keys
+// 7.7 us, the latencies of the lengths, the pages, the rows and the join.
 // v_mfma_f32_16x16x32, lane layouts: A and B lane l element e -> row / column
 // l % 16, k = 8 (l / 16) + e; accumulator register r -> row 4 (l / 16) + r, column
 // l % 16.  The value product's k order is the scores' register order: k = 8 g + e
@@ -758,14 +764,16 @@ __global__ void __launch_bounds__(Narrow<D>::kThreads) paged_narrow_kernel(const
 
 // Many columns: chunks, bound by the matrix products.  Eight waves of 32 columns
 // each (four at head dim 256, whose registers do not leave room for a second wave
-// per SIMD) share every gathered tile of 64 keys.  Bound by the matrix unit's power
-// at head dim 128 (2,048 queries over 32,768 keys, 28/4 heads: 820 us, 1.13
-// PFLOP/s, a library product of 8192^3 reaches 1.17), by the softmax next to half
-// as many products at 64, by one wave's issue of products, reads and softmax at 256
-// (4,099 queries of 16/2 heads over themselves: 0.85 PFLOP/s).  v_mfma_f32_32x32x16, lane
-// layouts: A and B lane l element e -> row / column l % 32, k = 8 (l / 32) + e;
-// accumulator register r -> row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.
-// The value product's k order is the scores' register order.
+// per SIMD) share every gathered tile of 64 keys.  2,048 queries behind 4,096 to
+// 32,768 keys take, per tile of 64 keys (from the difference of two lengths), 1.82 us
+// at head dim 128, the matrix unit's rate in a library product of 8192^3 (1.17
+// PFLOP/s), 1.91 at 256 (1.13 PFLOP/s) and 1.23 at 64 (0.87 PFLOP/s; the products
+// alone would be 0.92, and what the rest is has not been found); 27 to 39 us a call do
+// not grow with the keys (starts of the units, their unevenness, the join).  28/4 heads
+// of 128 over 32,768 keys: 812 us.  v_mfma_f32_32x32x16, lane layouts: A and B lane l
+// element e -> row / column l % 32, k = 8 (l / 32) + e; accumulator register r -> row
+// 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.  The value product's k order is the
+// scores' register order.
 //
 // A tile is two phases, the products (the values of tile t - 1, the scores of
 // tile t) and the softmax, about as long as each other: the products keep the
@@ -1383,8 +1391,8 @@ __global__ void __launch_bounds__((Combine<D, kSplit>::kThreads)) paged_combine_
 
 // How a call is launched: known from sizes that the host has.
 // More requests than this have a plan made before the call's kernels (single tokens
-// over 800 to 1,200 keys, 28/4 heads of 128: 128 requests 61 us with a plan, 60
-// without; 256 117 and 127; 1,024 422 and 577; 2,048 818 and 1,477).
+// over 800 to 1,200 keys, 28/4 heads of 128: 128 requests 62 us with a plan, 61
+// without; 256 117 and 128; 1,024 428 and 571; 2,048 837 and 1,507).
 constexpr long long kPlanned = 128;
 
 struct Launch {
@@ -1401,10 +1409,15 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   Launch x;
   const long long group = a->num_q_heads / a->num_kv_heads;
   const long long queries = a->num_queries, requests = a->num_requests;
-  // By the average request's columns: up to 16 on the narrow kernel, more on the
-  // wide one (16 requests of 4 tokens over 4,000 keys, 64/8 heads: 47 us there, 68
-  // on a narrow kernel of 32 columns a wave; 20 columns each of 32 requests 90 and
-  // 83 us).
+  // By the average request's columns, since the host knows no more: up to 16 on the
+  // narrow kernel, more on the wide one.  Of equal requests over 4,000 keys, heads of
+  // 128: 16 of 32 columns (64/8 heads) 59 us wide, 68 narrow; 32 of 20 (8/8) 123 and
+  // 139; 16 of 21 (28/4) 36 and 55.  (One request alone may be faster on the narrow
+  // one: 32 columns over 32,768 keys of one head 22 and 17 us, 56 over 2,048 15 and
+  // 14.)  Where the requests differ the average may fit none: 127 single tokens over
+  // 2,000 keys and a chunk of 128 over 8,000 (28/4 heads, 14 columns on average) take
+  // 204 us, in two calls 113 and 41; 63 single tokens and a chunk of 2,048 take 310,
+  // in two calls 108 and 212.
   const long long average = queries == 0 ? 1 : (queries + requests - 1) / requests;
   const long long wanted = average * group;
   x.wide = wanted > 16;
@@ -1412,11 +1425,11 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   x.max_tiles = a->query_starts == nullptr ? requests * ((group + x.columns - 1) / x.columns)
                                            : queries * group / x.columns + requests;
   x.min_chunk = 2;
-  // A workgroup fills a compute unit (its LDS rings), so `places` units of every
-  // KV head run at once.  Chunks: as many units as places, the longest first, leave
+  // A workgroup fills a compute unit (by its LDS: rings and slot list), so `places`
+  // units of every KV head run at once.  Chunks: as many units as places, the longest first, leave
   // the least over.  Single tokens: where the tiles are few, as many units as run
   // at once; where they are many, two rounds, whose second the short ones fill (64
-  // and 128 uneven requests: 390 and 212 us; one round 403 and 214, four 391 and 218).
+  // and 128 uneven requests: 390 and 212 us; one round 404 and 214, four 391 and 218).
   const int places = std::max(1, kComputeUnits / static_cast<int>(a->num_kv_heads));
   x.target = x.wide                           ? places
              : 2 * x.max_tiles <= places ? places - static_cast<int>(x.max_tiles) + 1
@@ -1501,8 +1514,8 @@ int launch_all(const PagedParams &p, const Launch &x, hipStream_t s) {
   // 4.4).  Elsewhere a wave for all chunks of its columns: workgroups that mostly
   // find no column cost more than they save (16 requests on tiles of 256 columns).
   // Between the two, by the chunks a tile may have (behind 32,768 keys: 64 tokens of
-  // 16/2 heads of 256, 25 chunks a tile, 69 us split and 93 not; 128 of 28/4 heads of
-  // 128, 16 chunks, 97 and 89).
+  // 16/2 heads of 256, 25 chunks a tile, 64 us split and 84 not; 128 of 28/4 heads of
+  // 128, 16 chunks, 92 and 83).
   const unsigned split_groups = tile_heads * (columns / Combine<D, 4>::kColumns);
   if (x.target < (split_groups > 4 * kComputeUnits ? 24 : 8) * x.max_tiles)
     paged_combine_kernel<D, E, 1><<<tile_heads * (columns / Combine<D, 1>::kColumns), 256, 0, s>>>(p, x.columns);

@@ -60,7 +60,9 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
 
     Returns (or fills, with ``output``) [queries, q heads, dim].  A query that
     sees no key gets zeros; rows of no request keep what they held (undefined in
-    a new tensor).  Pages outside the pool are invisible.  Work goes to the
+    a new tensor).  Pages outside the pool are invisible.  A call suits its average
+    request: a chunk among many single tokens, or beside many rows without queries,
+    is faster in a call of its own.  Work goes to the
     current stream; the call's workspace comes from torch's allocator and belongs
     to that stream (or to the graph that captures the call).
     """
