@@ -56,7 +56,7 @@ def paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, value_buffer:
     each request's keys, its new ones among them.  ``query_starts`` [requests +
     1] says where each request's queries begin; without it each request has one.
     Query i of a request's n sees its keys up to position length - n + i, itself
-    included.
+    included.  ``scale`` is 1 / sqrt(dim) by default, and in [1e-37, 1e30).
 
     Returns (or fills, with ``output``) [queries, q heads, dim].  A query that
     sees no key gets zeros; rows of no request keep what they held (undefined in
