@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define LL_ABI_VERSION 18
+#define LL_ABI_VERSION 19
 
 /* hipStream_t, declared without pulling in the HIP headers. */
 struct ihipStream_t;
@@ -755,6 +755,168 @@ typedef struct ll_paged_attention_args {
 int64_t ll_paged_attention_workspace_bytes(const ll_paged_attention_args *args);
 int ll_paged_attention(const ll_paged_attention_args *args, ll_stream_t stream);
 int64_t ll_paged_attention_args_size(void);
+
+/*
+ * One layer's pool held in 8 bits (ABI 19).  The reference's pool holds its model's
+ * own type (srt/pic_runtime.py:6283-6289); this one takes half of it, and a step
+ * reads half as much.
+ *
+ * Keys and values are codes of e4m3 (1 sign, 4 exponent, 3 fraction bits, bias 7,
+ * largest 448, no infinity, NaN 0x7f) with a scale of e8m0 for each head of every
+ * scale_block slots: row s, head h, dim d is
+ *     code[s][h][d] * 2^(scale[s / scale_block][h] - 127)        (scale 255: NaN)
+ * A pool that holds nothing is zeros in both.
+ *
+ * Where a call writes rows y to a block, with need the least scale byte under which
+ * every finite |y| is at most 448: the block's scale becomes need where the call
+ * writes every one of its rows, and else the larger of need and what it was, under
+ * which its other rows' codes are then rounded again.  So a scale only grows while
+ * rows are added; who gives a block to another request sets its scale bytes to 0,
+ * lest the new rows be rounded under the old ones' scale.  Codes are rounded to
+ * nearest even from results of more than 24 bits (keys) or exact ones; values that are
+ * not finite become NaN.
+ */
+typedef struct ll_quantized_pool {
+  void *key_buffer;                /* device e4m3 [num_slots, num_kv_heads, head_dim], dense, 16-byte aligned */
+  void *value_buffer;              /* device e4m3, the same shape */
+  void *key_scales;                /* device e8m0 [num_slots / scale_block, num_kv_heads], dense */
+  void *value_scales;              /* device e8m0, the same shape */
+  int64_t num_slots;               /* whole blocks, below 2^31 */
+  int64_t scale_block;             /* slots under one scale: a power of two, at most 128 */
+  int64_t num_kv_heads;            /* 1 .. 65535 */
+  int64_t head_dim;                /* a multiple of 16, at most 256 */
+} ll_quantized_pool;
+
+/*
+ * A step's new tokens into the pool: ll_head_rotary's norms and rotation, with the
+ * keys and values written to the rows destination_slots[t] of an 8-bit pool and the
+ * queries to query_output (which may be the queries themselves).
+ *
+ * A token whose position lies outside the table is left out; one whose slot is
+ * negative is padding (its queries are turned), and so is one whose slot is
+ * num_slots or more.  skipped_rows counts positions outside the table and slots past
+ * the pool, a token once.  The slots that are written are pairwise distinct, and
+ * those of one block stand next to each other in the call (in any order, no padding
+ * between them), as a request's new tokens do; what a block holds whose slots do not
+ * is not defined.  Strides are in elements, multiples of 8; rows, norm weights and
+ * their heads begin at multiples of 16 bytes.  One launch.
+ */
+typedef struct ll_quantized_append_args {
+  int64_t struct_size;             /* sizeof(ll_quantized_append_args) */
+  ll_quantized_pool pool;
+  int64_t num_tokens;              /* 0: nothing is launched */
+  int64_t num_q_heads;             /* 1 .. 65535 */
+  int64_t dtype;                   /* LL_DTYPE_FLOAT16 or LL_DTYPE_BFLOAT16: queries, keys and values */
+  const void *query;               /* device [num_tokens, num_q_heads, head_dim], strided */
+  int64_t query_token_stride;
+  int64_t query_head_stride;
+  void *query_output;
+  int64_t query_output_token_stride;
+  int64_t query_output_head_stride;
+  const void *key;                 /* device [num_tokens, num_kv_heads, head_dim], strided */
+  int64_t key_token_stride;
+  int64_t key_head_stride;
+  const void *value;               /* device [num_tokens, num_kv_heads, head_dim], strided */
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  const void *destination_slots;   /* device int32/int64 [num_tokens] */
+  int64_t destination_slots_dtype;
+  const void *positions;           /* device int32/int64 [num_tokens] */
+  int64_t positions_dtype;
+  const void *cos_sin_cache;       /* device [cos_sin_rows, cos_sin_cols], columns dense */
+  int64_t cos_sin_dtype;           /* fp16, bf16 or fp32 */
+  int64_t cos_sin_rows;
+  int64_t cos_sin_cols;            /* >= rotary_dim */
+  int64_t cos_sin_stride_row;
+  int64_t rotary_dim;              /* a multiple of 16, at most head_dim */
+  int64_t is_neox_style;
+  const void *query_norm_weight;   /* device [head_dim], or NULL: no norm */
+  const void *key_norm_weight;
+  int64_t norm_weight_dtype;       /* fp16, bf16 or fp32, of both weights */
+  double norm_eps;
+  int64_t *skipped_rows;           /* device counter, added to; or NULL */
+} ll_quantized_append_args;
+
+int ll_quantized_append(const ll_quantized_append_args *args, ll_stream_t stream);
+int64_t ll_quantized_append_args_size(void);
+
+/*
+ * The link within an 8-bit pool: row source_slots[t] goes to row
+ * destination_slots[t], its key turned from local_positions[t] to
+ * global_positions[t] (t >= prefix_token_count; below it the key is only moved).
+ * Tokens of repair_mask are left to the repair pass.  The angle is that of the
+ * table's rows, cos = c' c + s' s, sin = s' c - c' s.
+ *
+ * A negative destination is padding.  Tokens whose destination is past the pool,
+ * whose source is outside it or whose positions (where they are used) are outside
+ * the table are left out and counted in skipped_rows, unless masked.  The
+ * destinations are as an append's; no source lies in a block that the call writes
+ * (not checked).  One launch.
+ */
+typedef struct ll_quantized_link_args {
+  int64_t struct_size;             /* sizeof(ll_quantized_link_args) */
+  ll_quantized_pool pool;
+  int64_t num_tokens;              /* 0: nothing is launched */
+  const void *source_slots;        /* device int32/int64 [num_tokens] */
+  const void *destination_slots;   /* device, the same type */
+  int64_t slots_dtype;
+  const void *local_positions;     /* device int32/int64 [num_tokens] */
+  const void *global_positions;    /* device, the same type */
+  int64_t positions_dtype;
+  const uint8_t *repair_mask;      /* device uint8 or bool [num_tokens], or NULL */
+  int64_t prefix_token_count;
+  const void *cos_sin_cache;       /* device [cos_sin_rows, cos_sin_cols], columns dense */
+  int64_t cos_sin_dtype;           /* fp16, bf16 or fp32 */
+  int64_t cos_sin_rows;
+  int64_t cos_sin_cols;            /* >= rotary_dim */
+  int64_t cos_sin_stride_row;
+  int64_t rotary_dim;              /* a multiple of 16, at most head_dim */
+  int64_t is_neox_style;
+  int64_t *skipped_rows;           /* device counter, added to; or NULL */
+} ll_quantized_link_args;
+
+int ll_quantized_link(const ll_quantized_link_args *args, ll_stream_t stream);
+int64_t ll_quantized_link_args_size(void);
+
+/*
+ * Rows of an 8-bit pool as the values they stand for, rounded once to dtype: row i
+ * of the outputs is row slots[i] (without slots, row i), zeros where that is outside
+ * the pool.  One launch.
+ */
+typedef struct ll_quantized_load_args {
+  int64_t struct_size;             /* sizeof(ll_quantized_load_args) */
+  ll_quantized_pool pool;
+  int64_t num_rows;                /* 0: nothing is launched */
+  const void *slots;               /* device int32/int64 [num_rows], or NULL */
+  int64_t slots_dtype;
+  void *key_output;                /* device [num_rows, num_kv_heads, head_dim], dense, 16-byte aligned */
+  void *value_output;
+  int64_t dtype;                   /* fp16, bf16 or fp32 */
+} ll_quantized_load_args;
+
+int ll_quantized_load(const ll_quantized_load_args *args, ll_stream_t stream);
+int64_t ll_quantized_load_args_size(void);
+
+/*
+ * ll_paged_attention over the pages of an 8-bit pool.  Its block is `paged`, with
+ * the pool's buffers in it (e4m3) and kv_dtype the type of the queries and the
+ * output; what is said there holds here.  Keys and values are taken as
+ * ll_quantized_load gives them in kv_dtype (bf16 holds every value of the pool
+ * exactly; fp16 rounds those below 2^-14, and has infinities past 65504).
+ * page_size is a multiple of scale_block, and scale_block at least 16.
+ */
+typedef struct ll_quantized_attention_args {
+  int64_t struct_size;             /* sizeof(ll_quantized_attention_args) */
+  ll_paged_attention_args paged;   /* its struct_size is checked too */
+  const void *key_scales;          /* device e8m0 [num_slots / scale_block, num_kv_heads], dense */
+  const void *value_scales;
+  int64_t scale_block;             /* 16, 32, 64 or 128 */
+} ll_quantized_attention_args;
+
+/* Bytes of workspace that the call needs (negative: an LL_ERR_* code). */
+int64_t ll_quantized_attention_workspace_bytes(const ll_quantized_attention_args *args);
+int ll_quantized_attention(const ll_quantized_attention_args *args, ll_stream_t stream);
+int64_t ll_quantized_attention_args_size(void);
 
 /* Which kernel and launch shape ll_kv_link would use (no GPU work). */
 typedef struct ll_launch_info {

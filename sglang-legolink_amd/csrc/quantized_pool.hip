@@ -1,0 +1,883 @@
+// Writing, linking and reading a pool held in 8 bits, on gfx950 (MI355X).
+//
+// One layer's keys (and values) are codes c[slot][head][d] of e4m3 and bytes
+// x[block][head] of e8m0, block = slot / B: a value is c * 2^(x - 127).  The scales
+// are powers of two: codes times scale are exact in bf16 and fp32, and a scale that
+// grows costs the rows under it nothing but the bits that fall below e4m3's least
+// number (2^-9 of the scale).
+//
+// Rows y (computed before any rounding to 8 bits) that a call writes to block b:
+//   need = the least byte with max |y| <= 448 * 2^(need - 127), y finite
+//   x'   = need where the call writes all of b's rows, else max(x, need)
+//   c(written) = e4m3(y * 2^(127 - x')), to nearest even; inf and NaN become NaN
+//   c(others)  = e4m3(c * 2^(x - x')) where x' > x
+//
+// append: y = a new token's key, normed and rotated, and its value.
+// link:   y = the value of another row of the pool, a key turned by the angle from
+//         its old to its new position: cos = c' c + s' s, sin = s' c - c' s with rows
+//         (c, s) of the table at the old and (c', s') at the new position.
+//
+// A call's rows of one block are neighbours in the call (a run), so that one wave,
+// or the waves of one workgroup for blocks over 16 rows, holds them all, one head of
+// the keys or values: their maximum is known before the first code is written, and
+// every row is read once.  Keys are turned in 64 bits: a code changes by up to 1/8 of
+// itself where a value lies at the border of two, which 32 bits meet some hundred
+// times in a call of 32,768 tokens, and the calls are bound by memory all the same.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "legolink_kv.h"
+#include "ll_internal.h"
+#include "quantized_device.h"
+
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWave = 64;
+constexpr int kThreads = 256;
+constexpr int kMaxDim = 256;
+constexpr int kMaxBlock = 128;
+constexpr int kHeldRows = 16;  // of a run, in one wave's registers
+
+int fail(int code, const char *fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  const int rc = ll_record_error(code, fmt, ap);
+  va_end(ap);
+  return rc;
+}
+
+struct Rows {
+  const uint16_t *base;
+  long long token, head;
+};
+
+// One of the pool's two halves.
+struct Half {
+  uint8_t *codes;  // [slots][heads][dim]
+  uint8_t *scales;  // [blocks][heads]
+};
+
+struct PoolParams {
+  Half key, value;
+  const void *slots;  // where the rows go
+  unsigned long long *skipped;
+  long long num_tokens, num_slots;
+  int block_shift, hkv, dim;
+  int slots64;
+  int window;       // tokens whose runs a workgroup looks for
+  int pair_groups;  // workgroups for the heads' keys and values of a window
+  // The table and the keys' positions in it.
+  const void *table, *positions, *old_positions;  // (old: of a link)
+  long long table_rows, table_stride;
+  int table_dtype, rotary, neox, positions64;
+  bool table_chunks;  // rows of whole 16-byte chunks
+  // append
+  Rows query, new_key, new_value;
+  uint16_t *query_output;
+  long long query_output_token, query_output_head;
+  const void *query_weight, *key_weight;
+  int weight_dtype, hq, query_steps;
+  float eps;
+  long long query_groups;  // workgroups of the queries, behind the others
+  // link
+  const void *sources;
+  const uint8_t *masked;
+  long long prefix;
+};
+
+struct Bf16 {
+  __device__ static f32x2 unpack(uint32_t pair) {
+    return f32x2{__uint_as_float(pair << 16), __uint_as_float(pair & 0xffff0000u)};
+  }
+  __device__ static uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+  }
+  __device__ static uint32_t decode(uint32_t codes, float scale, bool high) {
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
+  }
+};
+struct F16 {
+  __device__ static f32x2 unpack(uint32_t pair) {
+    return __builtin_convertvector(__builtin_bit_cast(f16x2, pair), f32x2);
+  }
+  __device__ static uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, f16x2));
+  }
+  __device__ static uint32_t decode(uint32_t codes, float scale, bool high) {
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, false));
+  }
+};
+
+__device__ inline long long index_at(const void *values, int is64, long long i) {
+  return is64 ? static_cast<const int64_t *>(values)[i] : static_cast<const int32_t *>(values)[i];
+}
+
+__device__ inline float value_at(const void *values, int dtype, long long i) {
+  if (dtype == LL_DTYPE_FLOAT32) return static_cast<const float *>(values)[i];
+  const uint32_t bits = static_cast<const uint16_t *>(values)[i];
+  return dtype == LL_DTYPE_BFLOAT16 ? Bf16::unpack(bits)[0] : F16::unpack(bits)[0];
+}
+
+// Eight neighbouring values of a table or weight.
+__device__ inline void values8(const void *values, int dtype, bool chunks, long long i, float *out) {
+  if (!chunks) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = value_at(values, dtype, i + j);
+  } else if (dtype == LL_DTYPE_FLOAT32) {
+    const f32x4 *v = reinterpret_cast<const f32x4 *>(static_cast<const float *>(values) + i);
+    const f32x4 lo = v[0], hi = v[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      out[j] = lo[j];
+      out[4 + j] = hi[j];
+    }
+  } else {
+    const u32x4 bits = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(values) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 two = dtype == LL_DTYPE_BFLOAT16 ? Bf16::unpack(bits[j]) : F16::unpack(bits[j]);
+      out[2 * j] = two[0];
+      out[2 * j + 1] = two[1];
+    }
+  }
+}
+
+// A double as a float whose last bit says whether something was lost, so that a
+// rounding of it to fewer bits falls where that of the double falls.
+__device__ inline float to_odd(double x) {
+  unsigned long long bits = __builtin_bit_cast(unsigned long long, x);
+  const unsigned long long lost = bits & 0x1fffffffull;
+  bits = (bits & ~0x1fffffffull) | (lost != 0 ? 0x20000000ull : 0ull);
+  return static_cast<float>(__builtin_bit_cast(double, bits));
+}
+
+// A lane's two chunks of a row: its rotary pairs' halves (neox), or neighbours.
+struct Lane {
+  int i, first, second;
+  bool active, rotates;
+};
+template <int kGroup>
+__device__ inline Lane lane_of(const PoolParams &p) {
+  Lane l;
+  l.i = static_cast<int>(threadIdx.x) % kGroup;
+  l.active = l.i < p.dim / 16;
+  const int rotary_lanes = p.rotary / 16;
+  l.rotates = l.i < rotary_lanes;
+  l.first = l.rotates && p.neox ? 8 * l.i : 16 * l.i;
+  l.second = l.rotates && p.neox ? 8 * (l.i + rotary_lanes) : 16 * l.i + 8;
+  return l;
+}
+
+template <typename E>
+__device__ inline void load_row(const uint16_t *row, const Lane &l, float *a, float *b) {
+  const u32x4 x = *reinterpret_cast<const u32x4 *>(row + l.first), y = *reinterpret_cast<const u32x4 *>(row + l.second);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const f32x2 u = E::unpack(x[j]), v = E::unpack(y[j]);
+    a[2 * j] = u[0];
+    a[2 * j + 1] = u[1];
+    b[2 * j] = v[0];
+    b[2 * j + 1] = v[1];
+  }
+}
+
+// Turned by angles of these cosines and sines, pairs across the chunks or within.
+template <typename T>
+__device__ inline void turn(bool neox, const T *c, const T *s, T *a, T *b) {
+  if (neox) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const T lo = a[j], hi = b[j];
+      a[j] = lo * c[j] - hi * s[j];
+      b[j] = hi * c[j] + lo * s[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const T a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
+      a[2 * j] = a0 * c[j] - a1 * s[j];
+      a[2 * j + 1] = a1 * c[j] + a0 * s[j];
+      b[2 * j] = b0 * c[4 + j] - b1 * s[4 + j];
+      b[2 * j + 1] = b1 * c[4 + j] + b0 * s[4 + j];
+    }
+  }
+}
+
+// A row normed by its kGroup lanes.
+template <int kGroup, typename T>
+__device__ inline void norm(const PoolParams &p, const void *weight, const Lane &l, T *a, T *b) {
+  T sum = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum += a[j] * a[j] + b[j] * b[j];
+#pragma unroll
+  for (int step = 1; step < kGroup; step *= 2) sum += __shfl_xor(sum, step);
+  if (!l.active) return;
+  const T mean = sum / static_cast<T>(p.dim) + static_cast<T>(p.eps);
+  const T scale = sizeof(T) == 8 ? static_cast<T>(1.0 / sqrt(static_cast<double>(mean)))
+                                 : static_cast<T>(rsqrtf(static_cast<float>(mean)));
+  float w[8];
+  values8(weight, p.weight_dtype, true, l.first, w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = a[j] * scale * static_cast<T>(w[j]);
+  values8(weight, p.weight_dtype, true, l.second, w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = b[j] * scale * static_cast<T>(w[j]);
+}
+
+__device__ inline bool in_table(const PoolParams &p, long long position) {
+  return position >= 0 && position < p.table_rows;
+}
+
+// The rows of append: a step's new tokens.
+template <typename E>
+struct NewTokens {
+  // What token t writes is there.
+  __device__ static bool exists(const PoolParams &p, long long t) {
+    return in_table(p, index_at(p.positions, p.positions64, t));
+  }
+  __device__ static bool masked(const PoolParams &, long long) { return false; }
+
+  // Row t of one head into a and b.
+  template <int kGroup>
+  __device__ static void row(const PoolParams &p, bool is_key, int head, long long t, bool there, const Lane &l,
+                             float *a, float *b) {
+    const Rows &in = is_key ? p.new_key : p.new_value;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
+    const bool reads = there && l.active;
+    if (reads) load_row<E>(in.base + t * in.token + head * in.head, l, a, b);
+    if (!is_key) return;
+    double x[8], y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = a[j];
+      y[j] = b[j];
+    }
+    float c[8], s[8];
+    if (reads && l.rotates) {
+      const long long at = index_at(p.positions, p.positions64, t) * p.table_stride + 8 * l.i;
+      values8(p.table, p.table_dtype, p.table_chunks, at, c);
+      values8(p.table, p.table_dtype, p.table_chunks, at + p.rotary / 2, s);
+    }
+    if (p.key_weight != nullptr) norm<kGroup>(p, p.key_weight, l, x, y);
+    if (reads && l.rotates) {
+      double cd[8], sd[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cd[j] = c[j];
+        sd[j] = s[j];
+      }
+      turn(p.neox != 0, cd, sd, x, y);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      a[j] = to_odd(x[j]);
+      b[j] = to_odd(y[j]);
+    }
+  }
+};
+
+__device__ inline void decode8(u32x2 codes, float scale, float *out) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(codes[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(codes[j], true);
+    out[4 * j] = lo[0] * scale;
+    out[4 * j + 1] = lo[1] * scale;
+    out[4 * j + 2] = hi[0] * scale;
+    out[4 * j + 3] = hi[1] * scale;
+  }
+}
+__device__ inline u32x2 encode8(const float *values, float inverse) {
+  u32x2 codes;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    int word = __builtin_amdgcn_cvt_pk_fp8_f32(values[4 * j] * inverse, values[4 * j + 1] * inverse, 0, false);
+    codes[j] = static_cast<uint32_t>(
+        __builtin_amdgcn_cvt_pk_fp8_f32(values[4 * j + 2] * inverse, values[4 * j + 3] * inverse, word, true));
+  }
+  return codes;
+}
+
+// The rows of a link: the pool's own.
+struct CachedRows {
+  __device__ static bool turned(const PoolParams &p, long long t) { return t >= p.prefix; }
+  __device__ static bool exists(const PoolParams &p, long long t) {
+    const long long source = index_at(p.sources, p.slots64, t);
+    if (source < 0 || source >= p.num_slots) return false;
+    return !turned(p, t) || (in_table(p, index_at(p.old_positions, p.positions64, t)) &&
+                             in_table(p, index_at(p.positions, p.positions64, t)));
+  }
+  __device__ static bool masked(const PoolParams &p, long long t) { return p.masked != nullptr && p.masked[t] != 0; }
+
+  template <int kGroup>
+  __device__ static void row(const PoolParams &p, bool is_key, int head, long long t, bool there, const Lane &l,
+                             float *a, float *b) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
+    if (!there || !l.active) return;
+    const Half &half = is_key ? p.key : p.value;
+    const long long source = index_at(p.sources, p.slots64, t);
+    const uint8_t *codes = half.codes + (source * p.hkv + head) * p.dim;
+    const u32x2 x = *reinterpret_cast<const u32x2 *>(codes + l.first);
+    const u32x2 y = *reinterpret_cast<const u32x2 *>(codes + l.second);
+    const float scale = scale_of(half.scales[(source >> p.block_shift) * p.hkv + head]);
+    const bool turns = is_key && l.rotates && turned(p, t);
+    float c[8], s[8], from_c[8], from_s[8];
+    if (turns) {
+      const long long to = index_at(p.positions, p.positions64, t) * p.table_stride + 8 * l.i;
+      const long long from = index_at(p.old_positions, p.positions64, t) * p.table_stride + 8 * l.i;
+      values8(p.table, p.table_dtype, p.table_chunks, to, c);
+      values8(p.table, p.table_dtype, p.table_chunks, to + p.rotary / 2, s);
+      values8(p.table, p.table_dtype, p.table_chunks, from, from_c);
+      values8(p.table, p.table_dtype, p.table_chunks, from + p.rotary / 2, from_s);
+    }
+    decode8(x, scale, a);
+    decode8(y, scale, b);
+    if (!turns) return;
+    double cd[8], sd[8], u[8], v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      cd[j] = static_cast<double>(c[j]) * from_c[j] + static_cast<double>(s[j]) * from_s[j];
+      sd[j] = static_cast<double>(s[j]) * from_c[j] - static_cast<double>(c[j]) * from_s[j];
+      u[j] = a[j];
+      v[j] = b[j];
+    }
+    turn(p.neox != 0, cd, sd, u, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      a[j] = to_odd(u[j]);
+      b[j] = to_odd(v[j]);
+    }
+  }
+};
+
+__device__ inline float finite_size(float x) {
+  const float size = fabsf(x);
+  return size < INFINITY ? size : 0.f;  // (and of NaN)
+}
+
+// The queries of append: kGroup lanes a head, 64 / kGroup heads of one token a wave.
+template <typename E, int kGroup>
+__device__ inline void turn_queries(const PoolParams &p, long long unit) {
+  constexpr int kHeads = kWave / kGroup;
+  const int lane = threadIdx.x % kWave;
+  const long long t = unit / p.query_steps;
+  const int step = static_cast<int>(unit - t * p.query_steps);
+  if (t >= p.num_tokens) return;
+  const Lane l = lane_of<kGroup>(p);
+  const int head = step * kHeads + lane / kGroup;
+  const bool active = l.active && head < p.hq;
+  float a[8], b[8], c[8], s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
+  if (active) load_row<E>(p.query.base + t * p.query.token + head * p.query.head, l, a, b);
+  const long long position = index_at(p.positions, p.positions64, t);
+  const bool turned = in_table(p, position);
+  if (step == 0 && lane == 0 && p.skipped != nullptr && (!turned || index_at(p.slots, p.slots64, t) >= p.num_slots))
+    atomicAdd(p.skipped, 1ull);
+  if (!turned) return;
+  if (active && l.rotates) {
+    const long long at = position * p.table_stride + 8 * l.i;
+    values8(p.table, p.table_dtype, p.table_chunks, at, c);
+    values8(p.table, p.table_dtype, p.table_chunks, at + p.rotary / 2, s);
+  }
+  if (p.query_weight != nullptr) norm<kGroup>(p, p.query_weight, l, a, b);
+  if (!active) return;
+  if (l.rotates) turn(p.neox != 0, c, s, a, b);
+  u32x4 out_a, out_b;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    out_a[j] = E::pack(a[2 * j], a[2 * j + 1]);
+    out_b[j] = E::pack(b[2 * j], b[2 * j + 1]);
+  }
+  uint16_t *dst = p.query_output + t * p.query_output_token + head * p.query_output_head;
+  *reinterpret_cast<u32x4 *>(dst + l.first) = out_a;
+  *reinterpret_cast<u32x4 *>(dst + l.second) = out_b;
+}
+
+// Writes runs of rows.  A pair is one head's keys or values; kParts waves of a
+// workgroup hold a pair's run, up to kHeldRows rows each (block sizes up to 16 kParts).
+template <typename Source, typename E, int kGroup, int kParts, bool kQueries>
+__global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads) quantized_write_kernel(const PoolParams p) {
+  constexpr int kWaves = kParts > 4 ? kParts : kThreads / kWave;
+  constexpr int kPairs = kWaves / kParts;  // of a workgroup
+  constexpr int kRows = kWave / kGroup;    // of a step
+  constexpr int kSteps = kHeldRows / kRows;
+  constexpr int kWords = (kParts * kHeldRows + kWave - 1) / kWave;
+  __shared__ float most_of[kPairs][kParts];
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int lane = threadIdx.x % kWave;
+  unsigned group = blockIdx.x;
+  if constexpr (kQueries) {
+    // (The queries come first: a run's waves take longer to start than they do.)
+    if (group < p.query_groups) {
+      turn_queries<E, kGroup>(p, static_cast<long long>(group) * kWaves + wave);
+      return;
+    }
+    group -= static_cast<unsigned>(p.query_groups);
+  }
+  const long long t0 = static_cast<long long>(group / static_cast<unsigned>(p.pair_groups)) * p.window;
+  const int pair = static_cast<int>(group % static_cast<unsigned>(p.pair_groups)) * kPairs + wave / kParts;
+  const int part = wave % kParts;
+  const bool has_pair = pair < 2 * p.hkv;
+  const bool is_key = pair < p.hkv;
+  const int head = is_key ? pair : pair - p.hkv;
+  const Half half = is_key ? p.key : p.value;
+  const int block_rows = 1 << p.block_shift;
+  const Lane l = lane_of<kGroup>(p);
+
+  // A token's block (-1: none).
+  auto block_of = [&](long long t) -> long long {
+    if (t < 0 || t >= p.num_tokens) return -1;
+    const long long slot = index_at(p.slots, p.slots64, t);
+    return slot < 0 || slot >= p.num_slots ? -1 : slot >> p.block_shift;
+  };
+  // Lane l: token t0 - 1 + l.  A run begins where the block changes.
+  const long long mine = block_of(t0 - 1 + lane);
+  const long long former = __shfl_up(mine, 1);
+  unsigned long long begins =
+      __builtin_amdgcn_ballot_w64(lane >= 1 && lane <= p.window && mine >= 0 && mine != former);
+  if constexpr (!kQueries) {
+    if (p.skipped != nullptr && pair == 0 && part == 0) {
+      const long long t = t0 - 1 + lane;
+      const bool listed = lane >= 1 && lane <= p.window && t < p.num_tokens && !Source::masked(p, t);
+      const bool bad = listed && (index_at(p.slots, p.slots64, t) >= p.num_slots ||
+                                  (mine >= 0 && !Source::exists(p, t)));
+      const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(bad));
+      if (lane == 0 && count > 0) atomicAdd(p.skipped, static_cast<unsigned long long>(count));
+    }
+  }
+  while (begins != 0) {
+    const int at = __builtin_ctzll(begins);
+    begins &= begins - 1;
+    const long long start = t0 - 1 + at;
+    const long long block = __shfl(mine, at);
+    // Its rows, and those of them that are written.
+    int rows = 0;
+    unsigned long long written[kWords];
+    int count = 0;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      written[w] = 0;
+      if (rows < w * kWave) continue;
+      const long long t = start + w * kWave + lane;
+      const bool own = w * kWave + lane < block_rows && block_of(t) == block;
+      const unsigned long long same = __builtin_amdgcn_ballot_w64(own);
+      const int length = same == ~0ull ? kWave : __builtin_ctzll(~same);
+      rows += length;
+      written[w] = __builtin_amdgcn_ballot_w64(own && lane < length && !Source::masked(p, t) && Source::exists(p, t));
+      count += __builtin_popcountll(written[w]);
+    }
+    if (count == 0) continue;
+    uint8_t *scale_at = half.scales + block * p.hkv + head;
+    unsigned old = has_pair ? *scale_at : 0u;
+    // The 16 rows of this part that are written.
+    auto part_of = [&](const unsigned long long *words) {
+      unsigned bits = 0;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        if (part * kHeldRows / kWave == w) bits = static_cast<unsigned>(words[w] >> (part * kHeldRows % kWave)) & 0xffffu;
+      return bits;
+    };
+    const unsigned own_rows = part_of(written);
+
+    float a[kSteps][8], b[kSteps][8];
+    float most = 0.f;
+    auto held_of = [&](int step) { return step * kRows + lane / kGroup; };  // of the part's rows
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      const bool there = has_pair && ((own_rows >> held_of(step)) & 1u) != 0;
+      if (__builtin_amdgcn_ballot_w64(there) == 0) continue;
+      Source::template row<kGroup>(p, is_key, head, start + part * kHeldRows + held_of(step), there, l, a[step],
+                                   b[step]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(finite_size(a[step][j]), finite_size(b[step][j])));
+    }
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
+    if constexpr (kParts > 1) {
+      if (lane == 0) most_of[wave / kParts][part] = most;
+      asm volatile("" : "+v"(old));  // read before part 0 may write it
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < kParts; ++v) most = fmaxf(most, most_of[wave / kParts][v]);
+      __syncthreads();  // (the next run writes it)
+    }
+    if (!has_pair) continue;
+    const unsigned need = byte_for(most);
+    const unsigned byte = count == block_rows ? need : max(old, need);
+    if (part == 0 && lane == 0 && byte != old) *scale_at = static_cast<uint8_t>(byte);
+    const float inverse = inverse_of(byte);
+    auto codes_at = [&](long long slot) { return half.codes + (slot * p.hkv + head) * p.dim; };
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      if (((own_rows >> held_of(step)) & 1u) == 0 || !l.active) continue;
+      uint8_t *dst = codes_at(index_at(p.slots, p.slots64, start + part * kHeldRows + held_of(step)));
+      *reinterpret_cast<u32x2 *>(dst + l.first) = encode8(a[step], inverse);
+      *reinterpret_cast<u32x2 *>(dst + l.second) = encode8(b[step], inverse);
+    }
+    if (byte <= old || count == block_rows) continue;
+    // The block's other rows, under the scale that has grown.
+    unsigned long long taken[kWords];
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) taken[w] = 0;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      if (w * kWave >= rows) continue;
+      const bool own = ((written[w] >> lane) & 1ull) != 0;
+      const int offset =
+          own ? static_cast<int>(index_at(p.slots, p.slots64, start + w * kWave + lane)) & (block_rows - 1) : 0;
+#pragma unroll
+      for (int v = 0; v < kWords; ++v) {
+        unsigned long long bits = own && offset / kWave == v ? 1ull << (offset % kWave) : 0ull;
+#pragma unroll
+        for (int step = 1; step < kWave; step *= 2) bits |= __shfl_xor(bits, step);
+        taken[v] |= bits;
+      }
+    }
+    const unsigned grown = byte - old;
+    const float ratio = grown < 127u ? __uint_as_float((127u - grown) << 23) : 0.f;
+    const unsigned own_taken = part_of(taken);
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      const int offset = part * kHeldRows + held_of(step);
+      if (offset >= block_rows || ((own_taken >> held_of(step)) & 1u) != 0 || !l.active) continue;
+      uint8_t *row = codes_at((block << p.block_shift) + offset);
+      u32x2 *chunks[2] = {reinterpret_cast<u32x2 *>(row + l.first), reinterpret_cast<u32x2 *>(row + l.second)};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float values[8];
+        decode8(*chunks[k], ratio, values);
+        *chunks[k] = encode8(values, 1.f);
+      }
+    }
+  }
+}
+
+// Rows of the pool in 16 or 32 bits: a lane takes chunks of eight codes, several in
+// flight, of the workgroup's tokens.
+struct LoadParams {
+  const uint8_t *key, *value, *key_scales, *value_scales;
+  void *key_output, *value_output;  // [tokens][heads][dim]
+  const void *slots;                // NULL: the pool's own order
+  long long num_slots, num_rows;
+  int slots64, block_shift, hkv, dim_chunks, row_chunks, dtype;
+  int group_rows;  // of a workgroup
+};
+constexpr int kLoadChunks = 4;
+
+__global__ void __launch_bounds__(kThreads) quantized_load_kernel(const LoadParams p) {
+  const bool is_key = blockIdx.y == 0;
+  const uint8_t *codes = is_key ? p.key : p.value, *scales = is_key ? p.key_scales : p.value_scales;
+  const long long t0 = static_cast<long long>(blockIdx.x) * p.group_rows;
+  const unsigned row_chunks = static_cast<unsigned>(p.row_chunks);
+  const unsigned total = static_cast<unsigned>(min(static_cast<long long>(p.group_rows), p.num_rows - t0)) * row_chunks;
+  const long long first = t0 * p.row_chunks;  // of the outputs' chunks
+  void *output = is_key ? p.key_output : p.value_output;
+  for (unsigned begin = threadIdx.x; begin < total; begin += kThreads * kLoadChunks) {
+    u32x2 bits[kLoadChunks];
+    unsigned byte[kLoadChunks];
+#pragma unroll
+    for (int k = 0; k < kLoadChunks; ++k) {
+      const unsigned c = begin + k * kThreads;
+      bits[k] = u32x2{0u, 0u};
+      byte[k] = 0;
+      if (c >= total) continue;
+      const unsigned row = c / row_chunks, within = c - row * row_chunks;
+      const long long slot = p.slots == nullptr ? t0 + row : index_at(p.slots, p.slots64, t0 + row);
+      if (slot < 0 || slot >= p.num_slots) continue;  // a row of zeros
+      bits[k] = *reinterpret_cast<const u32x2 *>(codes + (slot * p.row_chunks + within) * 8);
+      byte[k] = scales[(slot >> p.block_shift) * p.hkv + within / static_cast<unsigned>(p.dim_chunks)];
+    }
+#pragma unroll
+    for (int k = 0; k < kLoadChunks; ++k) {
+      const unsigned c = begin + k * kThreads;
+      if (c >= total) continue;
+      const float scale = scale_of(byte[k]);
+      if (p.dtype == LL_DTYPE_FLOAT32) {
+        float values[8];
+        decode8(bits[k], scale, values);
+        f32x4 *dst = reinterpret_cast<f32x4 *>(output) + 2 * (first + c);
+        dst[0] = f32x4{values[0], values[1], values[2], values[3]};
+        dst[1] = f32x4{values[4], values[5], values[6], values[7]};
+      } else {
+        u32x4 out;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            out[2 * j + h] = p.dtype == LL_DTYPE_BFLOAT16 ? Bf16::decode(bits[k][j], scale, h != 0)
+                                                          : F16::decode(bits[k][j], scale, h != 0);
+        reinterpret_cast<u32x4 *>(output)[first + c] = out;
+      }
+    }
+  }
+}
+
+bool aligned(const void *p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+bool float_code(int64_t dtype) {
+  return dtype == LL_DTYPE_FLOAT16 || dtype == LL_DTYPE_BFLOAT16 || dtype == LL_DTYPE_FLOAT32;
+}
+bool index_code(int64_t dtype) { return dtype == LL_DTYPE_INT32 || dtype == LL_DTYPE_INT64; }
+
+int check_pool(const ll_quantized_pool *pool) {
+  if (pool->scale_block < 1 || pool->scale_block > kMaxBlock || (pool->scale_block & (pool->scale_block - 1)) != 0)
+    return fail(LL_ERR_INVALID_ARGUMENT, "scale_block must be a power of two, at most %d", kMaxBlock);
+  if (pool->num_slots < 0 || pool->num_slots > 0x7fffffff || pool->num_slots % pool->scale_block != 0)
+    return fail(LL_ERR_INVALID_ARGUMENT, "num_slots must be whole blocks, below 2^31");
+  if (pool->num_kv_heads < 1 || pool->num_kv_heads > 65535)
+    return fail(LL_ERR_KV_HEAD_LAYOUT_MISMATCH, "num_kv_heads must be in [1, 65535]");
+  if (pool->head_dim < 16 || pool->head_dim > kMaxDim || pool->head_dim % 16 != 0)
+    return fail(LL_ERR_HEAD_DIMENSION_OUT_OF_RANGE, "head_dim must be a multiple of 16, at most %d", kMaxDim);
+  if (pool->num_slots > 0 && (pool->key_buffer == nullptr || pool->value_buffer == nullptr ||
+                              pool->key_scales == nullptr || pool->value_scales == nullptr))
+    return fail(LL_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
+  if (!aligned(pool->key_buffer, 16) || !aligned(pool->value_buffer, 16))
+    return fail(LL_ERR_INVALID_ARGUMENT, "the pool's buffers must be 16-byte aligned");
+  return LL_OK;
+}
+
+int check_table(int64_t dtype, int64_t rows, int64_t cols, int64_t stride, int64_t rotary, int64_t dim) {
+  if (rotary < 2 || rotary % 2 != 0) return fail(LL_ERR_EVEN_ROTARY_DIM_REQUIRED, "rotary_dim must be positive and even");
+  if (rotary > dim) return fail(LL_ERR_ROTARY_DIM_EXCEEDS_HEAD_DIM, "rotary_dim exceeds head_dim");
+  if (rotary % 16 != 0) return fail(LL_ERR_INVALID_ARGUMENT, "rotary_dim must be a multiple of 16");
+  if (!float_code(dtype)) return fail(LL_ERR_UNSUPPORTED_COS_SIN_DTYPE, "cos/sin dtype");
+  if (rows < 0 || cols < rotary || stride < 0)
+    return fail(LL_ERR_UNSUPPORTED_COS_SIN_CACHE, "the cos/sin table needs rotary_dim columns");
+  return LL_OK;
+}
+
+bool whole_chunks(const void *base, int64_t token, int64_t head) {
+  return aligned(base, 16) && token % 8 == 0 && head % 8 == 0;
+}
+
+void fill_pool(const ll_quantized_pool &pool, PoolParams *p) {
+  p->key = Half{static_cast<uint8_t *>(pool.key_buffer), static_cast<uint8_t *>(pool.key_scales)};
+  p->value = Half{static_cast<uint8_t *>(pool.value_buffer), static_cast<uint8_t *>(pool.value_scales)};
+  p->num_slots = pool.num_slots;
+  p->hkv = static_cast<int>(pool.num_kv_heads);
+  p->dim = static_cast<int>(pool.head_dim);
+  p->block_shift = 0;
+  while ((1ll << p->block_shift) < pool.scale_block) ++p->block_shift;
+}
+
+void fill_table(const void *table, int64_t dtype, int64_t rows, int64_t stride, int64_t rotary, bool neox,
+                PoolParams *p) {
+  p->table = table;
+  p->table_dtype = static_cast<int>(dtype);
+  p->table_rows = rows;
+  p->table_stride = stride;
+  p->rotary = static_cast<int>(rotary);
+  p->neox = neox ? 1 : 0;
+  p->table_chunks = aligned(table, 16) && stride * (dtype == LL_DTYPE_FLOAT32 ? 4 : 2) % 16 == 0;
+}
+
+template <typename Source, typename E, int kGroup, int kParts, bool kQueries>
+int launch_write(PoolParams &p, hipStream_t s) {
+  constexpr int kWaves = kParts > 4 ? kParts : kThreads / kWave;
+  constexpr int kPairs = kWaves / kParts;
+  p.pair_groups = (2 * p.hkv + kPairs - 1) / kPairs;
+  // A window's runs are written one after another: single tokens are a run each, and
+  // a window each where that makes fewer waves than the card holds (16 a CU).
+  const long long waves = p.num_tokens * 2 * p.hkv * kParts;
+  p.window = 1;
+  while (p.window < 16 && waves / p.window > 256 * 16) p.window *= 2;
+  long long groups = (p.num_tokens + p.window - 1) / p.window * p.pair_groups;
+  if constexpr (kQueries) {
+    constexpr int kHeads = kWave / kGroup;
+    p.query_steps = (p.hq + kHeads - 1) / kHeads;
+    p.query_groups = (p.num_tokens * p.query_steps + kWaves - 1) / kWaves;
+    groups += p.query_groups;
+  }
+  if (groups * (kWaves * kWave) > 0xffffffffll)  // a launch holds fewer than 2^32 threads
+    return fail(LL_ERR_INVALID_ARGUMENT, "too many rows for one launch");
+  quantized_write_kernel<Source, E, kGroup, kParts, kQueries>
+      <<<static_cast<unsigned>(groups), kWaves * kWave, 0, s>>>(p);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return LL_OK;
+}
+
+template <typename Source, typename E, int kGroup, bool kQueries>
+int launch_by_block(PoolParams &p, hipStream_t s) {
+  if (p.block_shift <= 4) return launch_write<Source, E, kGroup, 1, kQueries>(p, s);
+  if (p.block_shift == 5) return launch_write<Source, E, kGroup, 2, kQueries>(p, s);
+  if (p.block_shift == 6) return launch_write<Source, E, kGroup, 4, kQueries>(p, s);
+  return launch_write<Source, E, kGroup, 8, kQueries>(p, s);
+}
+
+template <typename Source, typename E, bool kQueries>
+int launch_by_dim(PoolParams &p, hipStream_t s) {
+  if (p.dim <= 64) return launch_by_block<Source, E, 4, kQueries>(p, s);
+  if (p.dim <= 128) return launch_by_block<Source, E, 8, kQueries>(p, s);
+  return launch_by_block<Source, E, 16, kQueries>(p, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ll_quantized_append_args_size(void) { return static_cast<int64_t>(sizeof(ll_quantized_append_args)); }
+int64_t ll_quantized_link_args_size(void) { return static_cast<int64_t>(sizeof(ll_quantized_link_args)); }
+int64_t ll_quantized_load_args_size(void) { return static_cast<int64_t>(sizeof(ll_quantized_load_args)); }
+
+int ll_quantized_append(const ll_quantized_append_args *a, ll_stream_t stream) {
+  if (a == nullptr) return fail(LL_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->struct_size != static_cast<int64_t>(sizeof(*a)))
+    return fail(LL_ERR_INVALID_ARGUMENT, "struct_size %lld, expected %lld", static_cast<long long>(a->struct_size),
+                static_cast<long long>(sizeof(*a)));
+  int rc = check_pool(&a->pool);
+  if (rc != LL_OK) return rc;
+  if (a->num_tokens < 0 || a->num_tokens > 0x7fffffff)
+    return fail(LL_ERR_INVALID_ARGUMENT, "num_tokens must be in [0, 2^31)");
+  if (a->num_q_heads < 1 || a->num_q_heads > 65535)
+    return fail(LL_ERR_KV_HEAD_LAYOUT_MISMATCH, "num_q_heads must be in [1, 65535]");
+  if (a->dtype != LL_DTYPE_FLOAT16 && a->dtype != LL_DTYPE_BFLOAT16)
+    return fail(LL_ERR_FP16_OR_BF16_REQUIRED, "dtype must be fp16 or bf16");
+  rc = check_table(a->cos_sin_dtype, a->cos_sin_rows, a->cos_sin_cols, a->cos_sin_stride_row, a->rotary_dim,
+                   a->pool.head_dim);
+  if (rc != LL_OK) return rc;
+  if (!index_code(a->positions_dtype) || !index_code(a->destination_slots_dtype))
+    return fail(LL_ERR_INTEGER_TOKEN_MAPS_REQUIRED, "positions and slots must be int32 or int64");
+  const bool normed = a->query_norm_weight != nullptr || a->key_norm_weight != nullptr;
+  if (normed && !float_code(a->norm_weight_dtype))
+    return fail(LL_ERR_INVALID_ARGUMENT, "norm weights must be fp16, bf16 or fp32");
+  if (normed && !(a->norm_eps >= 0.0)) return fail(LL_ERR_INVALID_ARGUMENT, "norm_eps must not be negative");
+  if (a->num_tokens == 0) return LL_OK;
+  if (a->query == nullptr || a->query_output == nullptr || a->key == nullptr || a->value == nullptr ||
+      a->positions == nullptr || a->cos_sin_cache == nullptr || a->destination_slots == nullptr)
+    return fail(LL_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
+  if (!whole_chunks(a->query, a->query_token_stride, a->query_head_stride) ||
+      !whole_chunks(a->query_output, a->query_output_token_stride, a->query_output_head_stride) ||
+      !whole_chunks(a->key, a->key_token_stride, a->key_head_stride) ||
+      !whole_chunks(a->value, a->value_token_stride, a->value_head_stride) || !aligned(a->query_norm_weight, 16) ||
+      !aligned(a->key_norm_weight, 16))
+    return fail(LL_ERR_INVALID_ARGUMENT, "rows and norm weights must begin at multiples of 16 bytes");
+  PoolParams p;
+  memset(&p, 0, sizeof(p));
+  fill_pool(a->pool, &p);
+  fill_table(a->cos_sin_cache, a->cos_sin_dtype, a->cos_sin_rows, a->cos_sin_stride_row, a->rotary_dim,
+             a->is_neox_style != 0, &p);
+  p.slots = a->destination_slots;
+  p.slots64 = a->destination_slots_dtype == LL_DTYPE_INT64 ? 1 : 0;
+  p.positions = a->positions;
+  p.positions64 = a->positions_dtype == LL_DTYPE_INT64 ? 1 : 0;
+  p.skipped = reinterpret_cast<unsigned long long *>(a->skipped_rows);
+  p.num_tokens = a->num_tokens;
+  p.query = Rows{static_cast<const uint16_t *>(a->query), a->query_token_stride, a->query_head_stride};
+  p.new_key = Rows{static_cast<const uint16_t *>(a->key), a->key_token_stride, a->key_head_stride};
+  p.new_value = Rows{static_cast<const uint16_t *>(a->value), a->value_token_stride, a->value_head_stride};
+  p.query_output = static_cast<uint16_t *>(a->query_output);
+  p.query_output_token = a->query_output_token_stride;
+  p.query_output_head = a->query_output_head_stride;
+  p.query_weight = a->query_norm_weight;
+  p.key_weight = a->key_norm_weight;
+  p.weight_dtype = static_cast<int>(a->norm_weight_dtype);
+  p.eps = static_cast<float>(a->norm_eps);
+  p.hq = static_cast<int>(a->num_q_heads);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return a->dtype == LL_DTYPE_FLOAT16 ? launch_by_dim<NewTokens<F16>, F16, true>(p, s)
+                                      : launch_by_dim<NewTokens<Bf16>, Bf16, true>(p, s);
+}
+
+int ll_quantized_link(const ll_quantized_link_args *a, ll_stream_t stream) {
+  if (a == nullptr) return fail(LL_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->struct_size != static_cast<int64_t>(sizeof(*a)))
+    return fail(LL_ERR_INVALID_ARGUMENT, "struct_size %lld, expected %lld", static_cast<long long>(a->struct_size),
+                static_cast<long long>(sizeof(*a)));
+  int rc = check_pool(&a->pool);
+  if (rc != LL_OK) return rc;
+  if (a->num_tokens < 0 || a->num_tokens > 0x7fffffff)
+    return fail(LL_ERR_INVALID_ARGUMENT, "num_tokens must be in [0, 2^31)");
+  rc = check_table(a->cos_sin_dtype, a->cos_sin_rows, a->cos_sin_cols, a->cos_sin_stride_row, a->rotary_dim,
+                   a->pool.head_dim);
+  if (rc != LL_OK) return rc;
+  if (!index_code(a->slots_dtype) || !index_code(a->positions_dtype))
+    return fail(LL_ERR_INTEGER_TOKEN_MAPS_REQUIRED, "slots and positions must be int32 or int64");
+  if (a->prefix_token_count < 0 || a->prefix_token_count > a->num_tokens)
+    return fail(LL_ERR_INVALID_ARGUMENT, "prefix_token_count must be in [0, num_tokens]");
+  if (a->num_tokens == 0) return LL_OK;
+  if (a->source_slots == nullptr || a->destination_slots == nullptr || a->local_positions == nullptr ||
+      a->global_positions == nullptr || a->cos_sin_cache == nullptr)
+    return fail(LL_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
+  PoolParams p;
+  memset(&p, 0, sizeof(p));
+  fill_pool(a->pool, &p);
+  fill_table(a->cos_sin_cache, a->cos_sin_dtype, a->cos_sin_rows, a->cos_sin_stride_row, a->rotary_dim,
+             a->is_neox_style != 0, &p);
+  p.slots = a->destination_slots;
+  p.sources = a->source_slots;
+  p.slots64 = a->slots_dtype == LL_DTYPE_INT64 ? 1 : 0;
+  p.positions = a->global_positions;
+  p.old_positions = a->local_positions;
+  p.positions64 = a->positions_dtype == LL_DTYPE_INT64 ? 1 : 0;
+  p.skipped = reinterpret_cast<unsigned long long *>(a->skipped_rows);
+  p.num_tokens = a->num_tokens;
+  p.masked = static_cast<const uint8_t *>(a->repair_mask);
+  p.prefix = a->prefix_token_count;
+  return launch_by_dim<CachedRows, Bf16, false>(p, reinterpret_cast<hipStream_t>(stream));
+}
+
+int ll_quantized_load(const ll_quantized_load_args *a, ll_stream_t stream) {
+  if (a == nullptr) return fail(LL_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->struct_size != static_cast<int64_t>(sizeof(*a)))
+    return fail(LL_ERR_INVALID_ARGUMENT, "struct_size %lld, expected %lld", static_cast<long long>(a->struct_size),
+                static_cast<long long>(sizeof(*a)));
+  const int rc = check_pool(&a->pool);
+  if (rc != LL_OK) return rc;
+  if (a->num_rows < 0 || a->num_rows > 0x7fffffff)
+    return fail(LL_ERR_INVALID_ARGUMENT, "num_rows must be in [0, 2^31)");
+  if (!float_code(a->dtype)) return fail(LL_ERR_INVALID_ARGUMENT, "dtype must be fp16, bf16 or fp32");
+  if (a->slots != nullptr && !index_code(a->slots_dtype))
+    return fail(LL_ERR_INTEGER_TOKEN_MAPS_REQUIRED, "slots must be int32 or int64");
+  if (a->num_rows == 0) return LL_OK;
+  if (a->key_output == nullptr || a->value_output == nullptr)
+    return fail(LL_ERR_INVALID_ARGUMENT, "a device pointer is NULL");
+  if (!aligned(a->key_output, 16) || !aligned(a->value_output, 16))
+    return fail(LL_ERR_INVALID_ARGUMENT, "the outputs must be 16-byte aligned");
+  PoolParams pool;
+  memset(&pool, 0, sizeof(pool));
+  fill_pool(a->pool, &pool);
+  LoadParams p;
+  memset(&p, 0, sizeof(p));
+  p.key = pool.key.codes;
+  p.value = pool.value.codes;
+  p.key_scales = pool.key.scales;
+  p.value_scales = pool.value.scales;
+  p.key_output = a->key_output;
+  p.value_output = a->value_output;
+  p.slots = a->slots;
+  p.slots64 = a->slots_dtype == LL_DTYPE_INT64 ? 1 : 0;
+  p.num_slots = pool.num_slots;
+  p.block_shift = pool.block_shift;
+  p.hkv = pool.hkv;
+  p.dim_chunks = pool.dim / 8;
+  p.row_chunks = pool.hkv * p.dim_chunks;
+  p.num_rows = a->num_rows;
+  p.group_rows = std::max(1, kThreads * kLoadChunks / p.row_chunks);
+  p.dtype = static_cast<int>(a->dtype);
+  const long long groups = (p.num_rows + p.group_rows - 1) / p.group_rows;
+  if (groups * 2 * kThreads > 0xffffffffll)
+    return fail(LL_ERR_INVALID_ARGUMENT, "too many rows for one launch");
+  quantized_load_kernel<<<dim3(static_cast<unsigned>(groups), 2), kThreads, 0,
+                          reinterpret_cast<hipStream_t>(stream)>>>(p);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return LL_OK;
+}
+
+}  // extern "C"

@@ -24,7 +24,7 @@ LIB_DIR = Path(__file__).resolve().parent / "lib"
 # LEGOLINK_KV_LIBRARY names another build of the library (the host-sanitized
 # one of the CPU sanitizer test).
 LIB_PATH = Path(os.environ.get("LEGOLINK_KV_LIBRARY") or LIB_DIR / "liblegolink_kv.so")
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 # Element type codes (include/legolink_kv.h).
 DTYPE_FLOAT16 = 1
@@ -81,6 +81,15 @@ EXPORTED_SYMBOLS = (
     "ll_paged_attention",
     "ll_paged_attention_workspace_bytes",
     "ll_paged_attention_args_size",
+    "ll_quantized_append",
+    "ll_quantized_append_args_size",
+    "ll_quantized_link",
+    "ll_quantized_link_args_size",
+    "ll_quantized_load",
+    "ll_quantized_load_args_size",
+    "ll_quantized_attention",
+    "ll_quantized_attention_workspace_bytes",
+    "ll_quantized_attention_args_size",
 )
 
 _i64 = ctypes.c_int64
@@ -390,6 +399,114 @@ class PagedAttentionArgs(ctypes.Structure):
     ]
 
 
+class QuantizedPool(ctypes.Structure):
+    """Mirror of ``ll_quantized_pool``."""
+
+    _fields_ = [
+        ("key_buffer", _ptr),
+        ("value_buffer", _ptr),
+        ("key_scales", _ptr),
+        ("value_scales", _ptr),
+        ("num_slots", _i64),
+        ("scale_block", _i64),
+        ("num_kv_heads", _i64),
+        ("head_dim", _i64),
+    ]
+
+
+class QuantizedAppendArgs(ctypes.Structure):
+    """Mirror of ``ll_quantized_append_args``."""
+
+    _fields_ = [
+        ("struct_size", _i64),
+        ("pool", QuantizedPool),
+        ("num_tokens", _i64),
+        ("num_q_heads", _i64),
+        ("dtype", _i64),
+        ("query", _ptr),
+        ("query_token_stride", _i64),
+        ("query_head_stride", _i64),
+        ("query_output", _ptr),
+        ("query_output_token_stride", _i64),
+        ("query_output_head_stride", _i64),
+        ("key", _ptr),
+        ("key_token_stride", _i64),
+        ("key_head_stride", _i64),
+        ("value", _ptr),
+        ("value_token_stride", _i64),
+        ("value_head_stride", _i64),
+        ("destination_slots", _ptr),
+        ("destination_slots_dtype", _i64),
+        ("positions", _ptr),
+        ("positions_dtype", _i64),
+        ("cos_sin_cache", _ptr),
+        ("cos_sin_dtype", _i64),
+        ("cos_sin_rows", _i64),
+        ("cos_sin_cols", _i64),
+        ("cos_sin_stride_row", _i64),
+        ("rotary_dim", _i64),
+        ("is_neox_style", _i64),
+        ("query_norm_weight", _ptr),
+        ("key_norm_weight", _ptr),
+        ("norm_weight_dtype", _i64),
+        ("norm_eps", ctypes.c_double),
+        ("skipped_rows", _ptr),
+    ]
+
+
+class QuantizedLinkArgs(ctypes.Structure):
+    """Mirror of ``ll_quantized_link_args``."""
+
+    _fields_ = [
+        ("struct_size", _i64),
+        ("pool", QuantizedPool),
+        ("num_tokens", _i64),
+        ("source_slots", _ptr),
+        ("destination_slots", _ptr),
+        ("slots_dtype", _i64),
+        ("local_positions", _ptr),
+        ("global_positions", _ptr),
+        ("positions_dtype", _i64),
+        ("repair_mask", _ptr),
+        ("prefix_token_count", _i64),
+        ("cos_sin_cache", _ptr),
+        ("cos_sin_dtype", _i64),
+        ("cos_sin_rows", _i64),
+        ("cos_sin_cols", _i64),
+        ("cos_sin_stride_row", _i64),
+        ("rotary_dim", _i64),
+        ("is_neox_style", _i64),
+        ("skipped_rows", _ptr),
+    ]
+
+
+class QuantizedLoadArgs(ctypes.Structure):
+    """Mirror of ``ll_quantized_load_args``."""
+
+    _fields_ = [
+        ("struct_size", _i64),
+        ("pool", QuantizedPool),
+        ("num_rows", _i64),
+        ("slots", _ptr),
+        ("slots_dtype", _i64),
+        ("key_output", _ptr),
+        ("value_output", _ptr),
+        ("dtype", _i64),
+    ]
+
+
+class QuantizedAttentionArgs(ctypes.Structure):
+    """Mirror of ``ll_quantized_attention_args``."""
+
+    _fields_ = [
+        ("struct_size", _i64),
+        ("paged", PagedAttentionArgs),
+        ("key_scales", _ptr),
+        ("value_scales", _ptr),
+        ("scale_block", _i64),
+    ]
+
+
 REPAIR_ITEM_INTS = 86
 REPAIR_ITEM_HEADER = 6  # kv_offset, kv_begin, kv_end, tiles, first pair's head, pair count
 REPAIR_TILE_INTS = 5   # per tile of an item: first query, lowest position, count, partial, key end
@@ -504,6 +621,13 @@ def load_library() -> ctypes.CDLL:
         lib.ll_paged_attention_workspace_bytes.restype = _i64
         lib.ll_paged_attention_args_size.argtypes = []
         lib.ll_paged_attention_args_size.restype = _i64
+        for name, args in (("append", QuantizedAppendArgs), ("link", QuantizedLinkArgs), ("load", QuantizedLoadArgs),
+                           ("attention", QuantizedAttentionArgs)):
+            entry, size = getattr(lib, f"ll_quantized_{name}"), getattr(lib, f"ll_quantized_{name}_args_size")
+            entry.argtypes, entry.restype = [ctypes.POINTER(args), _ptr], ctypes.c_int
+            size.argtypes, size.restype = [], _i64
+        lib.ll_quantized_attention_workspace_bytes.argtypes = [ctypes.POINTER(QuantizedAttentionArgs)]
+        lib.ll_quantized_attention_workspace_bytes.restype = _i64
         if lib.ll_abi_version() != ABI_VERSION:
             raise NativeLibraryUnavailable(
                 f"{LIB_PATH} has ABI {lib.ll_abi_version()}, expected {ABI_VERSION}; rebuild it"
@@ -514,7 +638,11 @@ def load_library() -> ctypes.CDLL:
                 or lib.ll_order_maps_args_size() != ctypes.sizeof(OrderMapsArgs)
                 or lib.ll_repair_attention_args_size() != ctypes.sizeof(RepairAttentionArgs)
                 or lib.ll_head_rotary_args_size() != ctypes.sizeof(HeadRotaryArgs)
-                or lib.ll_paged_attention_args_size() != ctypes.sizeof(PagedAttentionArgs)):
+                or lib.ll_paged_attention_args_size() != ctypes.sizeof(PagedAttentionArgs)
+                or lib.ll_quantized_append_args_size() != ctypes.sizeof(QuantizedAppendArgs)
+                or lib.ll_quantized_link_args_size() != ctypes.sizeof(QuantizedLinkArgs)
+                or lib.ll_quantized_load_args_size() != ctypes.sizeof(QuantizedLoadArgs)
+                or lib.ll_quantized_attention_args_size() != ctypes.sizeof(QuantizedAttentionArgs)):
             raise NativeLibraryUnavailable(f"{LIB_PATH} struct layout differs; rebuild it")
         _lib = lib
         return lib
@@ -690,6 +818,35 @@ def paged_attention_workspace_bytes(args: PagedAttentionArgs) -> int:
 def paged_attention(args: PagedAttentionArgs, stream: int) -> None:
     args.struct_size = ctypes.sizeof(PagedAttentionArgs)
     _check(load_library().ll_paged_attention(ctypes.byref(args), _ptr(int(stream))))
+
+
+def quantized_append(args: QuantizedAppendArgs, stream: int) -> None:
+    args.struct_size = ctypes.sizeof(QuantizedAppendArgs)
+    _check(load_library().ll_quantized_append(ctypes.byref(args), _ptr(int(stream))))
+
+
+def quantized_link(args: QuantizedLinkArgs, stream: int) -> None:
+    args.struct_size = ctypes.sizeof(QuantizedLinkArgs)
+    _check(load_library().ll_quantized_link(ctypes.byref(args), _ptr(int(stream))))
+
+
+def quantized_load(args: QuantizedLoadArgs, stream: int) -> None:
+    args.struct_size = ctypes.sizeof(QuantizedLoadArgs)
+    _check(load_library().ll_quantized_load(ctypes.byref(args), _ptr(int(stream))))
+
+
+def quantized_attention_workspace_bytes(args: QuantizedAttentionArgs) -> int:
+    args.struct_size = ctypes.sizeof(QuantizedAttentionArgs)
+    args.paged.struct_size = ctypes.sizeof(PagedAttentionArgs)
+    needed = load_library().ll_quantized_attention_workspace_bytes(ctypes.byref(args))
+    _check(min(needed, LL_OK))
+    return needed
+
+
+def quantized_attention(args: QuantizedAttentionArgs, stream: int) -> None:
+    args.struct_size = ctypes.sizeof(QuantizedAttentionArgs)
+    args.paged.struct_size = ctypes.sizeof(PagedAttentionArgs)
+    _check(load_library().ll_quantized_attention(ctypes.byref(args), _ptr(int(stream))))
 
 
 def whole_number(value):

@@ -21,9 +21,11 @@ from pathlib import Path
 PACKAGE_DIR = Path(__file__).resolve().parent
 SOURCE = PACKAGE_DIR.parent / "csrc" / "legolink_kv.hip"
 # Translation units of liblegolink_kv.so: the link kernels, the repair
-# attention, the norms and rotation of a step's heads, and its attention.
+# attention, the norms and rotation of a step's heads, its attention, and both over
+# a pool held in 8 bits.
 SOURCES = (SOURCE, *(PACKAGE_DIR.parent / "csrc" / name
-                     for name in ("repair_attention.hip", "head_rotary.hip", "paged_attention.hip")))
+                     for name in ("repair_attention.hip", "head_rotary.hip", "paged_attention.hip",
+                                  "quantized_pool.hip", "quantized_attention.hip")))
 INCLUDE_DIR = PACKAGE_DIR.parents[1] / "include"
 OUTPUT = PACKAGE_DIR / "lib" / "liblegolink_kv.so"
 # The row-access calibration kernels of bench.py's sweep (measurement only,
@@ -52,11 +54,11 @@ SANITIZE_FLAGS = ["-g", "-fno-omit-frame-pointer", "-shared-libsan",
 OFFLOAD_ARCH = "gfx950"
 
 
-# Flags of one translation unit.  paged_attention.hip: MFMA results in vector
+# Flags of one translation unit.  Paged attention: MFMA results in vector
 # registers (the compiler otherwise keeps them in accumulator registers where a
 # kernel may use more than 256, and copies them for every vector instruction: a
 # 4,099-token prompt at head dim 256 takes 255 us instead of 225).
-SOURCE_FLAGS = {"paged_attention": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("paged_attention", "quantized_attention")}
 
 
 def hipcc_path() -> str:
