@@ -22,7 +22,7 @@
 // the keys or values: their maximum is known before the first code is written, and
 // every row is read once.  Keys are turned in 64 bits: a code changes by up to 1/8 of
 // itself where a value lies at the border of two, which 32 bits meet some hundred
-// times in a call of 32,768 tokens, and the calls are bound by memory all the same.
+// times in a call of 32,768 tokens.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdarg.h>
@@ -48,7 +48,9 @@ constexpr int kWave = 64;
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int kMaxBlock = 128;
-constexpr int kHeldRows = 16;  // of a run, in one wave's registers
+constexpr int kMostWindow = 16;
+constexpr int kHeldSteps = 2;  // of 64 / kGroup rows, in a wave's registers
+constexpr long long kMostTogether = 4096;  // waves of queries that go with the runs
 
 int fail(int code, const char *fmt, ...) {
   va_list ap;
@@ -78,6 +80,7 @@ struct PoolParams {
   int slots64;
   int window;       // tokens whose runs a workgroup looks for
   int pair_groups;  // workgroups for the heads' keys and values of a window
+  unsigned run_groups;  // workgroups of all windows; those of the queries come behind them
   // The table and the keys' positions in it.
   const void *table, *positions, *old_positions;  // (old: of a link)
   long long table_rows, table_stride;
@@ -89,8 +92,7 @@ struct PoolParams {
   long long query_output_token, query_output_head;
   const void *query_weight, *key_weight;
   int weight_dtype, hq, query_steps;
-  float eps;
-  long long query_groups;  // workgroups of the queries, behind the others
+  double eps;
   // link
   const void *sources;
   const uint8_t *masked;
@@ -195,101 +197,9 @@ __device__ inline void load_row(const uint16_t *row, const Lane &l, float *a, fl
   }
 }
 
-// Turned by angles of these cosines and sines, pairs across the chunks or within.
-template <typename T>
-__device__ inline void turn(bool neox, const T *c, const T *s, T *a, T *b) {
-  if (neox) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const T lo = a[j], hi = b[j];
-      a[j] = lo * c[j] - hi * s[j];
-      b[j] = hi * c[j] + lo * s[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const T a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
-      a[2 * j] = a0 * c[j] - a1 * s[j];
-      a[2 * j + 1] = a1 * c[j] + a0 * s[j];
-      b[2 * j] = b0 * c[4 + j] - b1 * s[4 + j];
-      b[2 * j + 1] = b1 * c[4 + j] + b0 * s[4 + j];
-    }
-  }
-}
-
-// A row normed by its kGroup lanes.
-template <int kGroup, typename T>
-__device__ inline void norm(const PoolParams &p, const void *weight, const Lane &l, T *a, T *b) {
-  T sum = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) sum += a[j] * a[j] + b[j] * b[j];
-#pragma unroll
-  for (int step = 1; step < kGroup; step *= 2) sum += __shfl_xor(sum, step);
-  if (!l.active) return;
-  const T mean = sum / static_cast<T>(p.dim) + static_cast<T>(p.eps);
-  const T scale = sizeof(T) == 8 ? static_cast<T>(1.0 / sqrt(static_cast<double>(mean)))
-                                 : static_cast<T>(rsqrtf(static_cast<float>(mean)));
-  float w[8];
-  values8(weight, p.weight_dtype, true, l.first, w);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = a[j] * scale * static_cast<T>(w[j]);
-  values8(weight, p.weight_dtype, true, l.second, w);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) b[j] = b[j] * scale * static_cast<T>(w[j]);
-}
-
 __device__ inline bool in_table(const PoolParams &p, long long position) {
   return position >= 0 && position < p.table_rows;
 }
-
-// The rows of append: a step's new tokens.
-template <typename E>
-struct NewTokens {
-  // What token t writes is there.
-  __device__ static bool exists(const PoolParams &p, long long t) {
-    return in_table(p, index_at(p.positions, p.positions64, t));
-  }
-  __device__ static bool masked(const PoolParams &, long long) { return false; }
-
-  // Row t of one head into a and b.
-  template <int kGroup>
-  __device__ static void row(const PoolParams &p, bool is_key, int head, long long t, bool there, const Lane &l,
-                             float *a, float *b) {
-    const Rows &in = is_key ? p.new_key : p.new_value;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
-    const bool reads = there && l.active;
-    if (reads) load_row<E>(in.base + t * in.token + head * in.head, l, a, b);
-    if (!is_key) return;
-    double x[8], y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = a[j];
-      y[j] = b[j];
-    }
-    float c[8], s[8];
-    if (reads && l.rotates) {
-      const long long at = index_at(p.positions, p.positions64, t) * p.table_stride + 8 * l.i;
-      values8(p.table, p.table_dtype, p.table_chunks, at, c);
-      values8(p.table, p.table_dtype, p.table_chunks, at + p.rotary / 2, s);
-    }
-    if (p.key_weight != nullptr) norm<kGroup>(p, p.key_weight, l, x, y);
-    if (reads && l.rotates) {
-      double cd[8], sd[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        cd[j] = c[j];
-        sd[j] = s[j];
-      }
-      turn(p.neox != 0, cd, sd, x, y);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[j] = to_odd(x[j]);
-      b[j] = to_odd(y[j]);
-    }
-  }
-};
 
 __device__ inline void decode8(u32x2 codes, float scale, float *out) {
 #pragma unroll
@@ -312,55 +222,132 @@ __device__ inline u32x2 encode8(const float *values, float inverse) {
   return codes;
 }
 
+// What a workgroup knows of a token: where it goes (-1: nowhere), where it comes from
+// (of a link; -1: it is not written), its positions (-1: it is not turned).
+struct Token {
+  int slot, from, position, old_position;
+};
+
+// A pair's cosine and sine.
+struct Angle {
+  double cos, sin;
+};
+
+// Four neighbouring values of the table.
+__device__ inline void values4(const PoolParams &p, long long i, float *out) {
+  if (p.table_chunks && p.table_dtype == LL_DTYPE_FLOAT32) {
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p.table) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = v[j];
+  } else if (p.table_chunks) {  // (rows of whole 16-byte chunks: four values are at 8 bytes)
+    const u32x2 bits = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p.table) + i);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x2 two = p.table_dtype == LL_DTYPE_BFLOAT16 ? Bf16::unpack(bits[j]) : F16::unpack(bits[j]);
+      out[2 * j] = two[0];
+      out[2 * j + 1] = two[1];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = value_at(p.table, p.table_dtype, i + j);
+  }
+}
+
+// The rows of append: a step's new tokens.
+template <typename E>
+struct NewTokens {
+  struct Raw {
+    u32x4 x, y;
+  };
+  static constexpr bool kNorms = true;
+
+  __device__ static Token token(const PoolParams &p, long long t, bool *bad) {
+    Token k{-1, -1, -1, -1};
+    const long long slot = index_at(p.slots, p.slots64, t), position = index_at(p.positions, p.positions64, t);
+    if (slot >= 0 && slot < p.num_slots) k.slot = static_cast<int>(slot);
+    if (in_table(p, position)) {
+      k.position = static_cast<int>(position);
+      k.from = k.slot;
+    }
+    *bad = false;  // (counted with the queries)
+    return k;
+  }
+  __device__ static Raw fetch(const PoolParams &p, const Half &, bool is_key, int head, long long t, const Token &,
+                              const Lane &l) {
+    const Rows &in = is_key ? p.new_key : p.new_value;
+    const uint16_t *row = in.base + t * in.token + head * in.head;
+    return Raw{*reinterpret_cast<const u32x4 *>(row + l.first), *reinterpret_cast<const u32x4 *>(row + l.second)};
+  }
+  __device__ static void unpack(const Raw &raw, float *a, float *b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 u = E::unpack(raw.x[j]), v = E::unpack(raw.y[j]);
+      a[2 * j] = u[0];
+      a[2 * j + 1] = u[1];
+      b[2 * j] = v[0];
+      b[2 * j + 1] = v[1];
+    }
+  }
+  // Pairs i to i + 3 of a token.
+  __device__ static void angles(const PoolParams &p, const Token &k, int i, Angle *out) {
+    float c[4], s[4];
+    const long long at = k.position * p.table_stride + i;
+    values4(p, at, c);
+    values4(p, at + p.rotary / 2, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = Angle{c[j], s[j]};
+  }
+};
+
 // The rows of a link: the pool's own.
 struct CachedRows {
-  __device__ static bool turned(const PoolParams &p, long long t) { return t >= p.prefix; }
-  __device__ static bool exists(const PoolParams &p, long long t) {
-    const long long source = index_at(p.sources, p.slots64, t);
-    if (source < 0 || source >= p.num_slots) return false;
-    return !turned(p, t) || (in_table(p, index_at(p.old_positions, p.positions64, t)) &&
-                             in_table(p, index_at(p.positions, p.positions64, t)));
-  }
-  __device__ static bool masked(const PoolParams &p, long long t) { return p.masked != nullptr && p.masked[t] != 0; }
+  struct Raw {
+    u32x2 x, y;
+    float scale;
+  };
+  static constexpr bool kNorms = false;
 
-  template <int kGroup>
-  __device__ static void row(const PoolParams &p, bool is_key, int head, long long t, bool there, const Lane &l,
-                             float *a, float *b) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
-    if (!there || !l.active) return;
-    const Half &half = is_key ? p.key : p.value;
-    const long long source = index_at(p.sources, p.slots64, t);
-    const uint8_t *codes = half.codes + (source * p.hkv + head) * p.dim;
-    const u32x2 x = *reinterpret_cast<const u32x2 *>(codes + l.first);
-    const u32x2 y = *reinterpret_cast<const u32x2 *>(codes + l.second);
-    const float scale = scale_of(half.scales[(source >> p.block_shift) * p.hkv + head]);
-    const bool turns = is_key && l.rotates && turned(p, t);
-    float c[8], s[8], from_c[8], from_s[8];
-    if (turns) {
-      const long long to = index_at(p.positions, p.positions64, t) * p.table_stride + 8 * l.i;
-      const long long from = index_at(p.old_positions, p.positions64, t) * p.table_stride + 8 * l.i;
-      values8(p.table, p.table_dtype, p.table_chunks, to, c);
-      values8(p.table, p.table_dtype, p.table_chunks, to + p.rotary / 2, s);
-      values8(p.table, p.table_dtype, p.table_chunks, from, from_c);
-      values8(p.table, p.table_dtype, p.table_chunks, from + p.rotary / 2, from_s);
+  __device__ static Token token(const PoolParams &p, long long t, bool *bad) {
+    Token k{-1, -1, -1, -1};
+    const long long slot = index_at(p.slots, p.slots64, t), source = index_at(p.sources, p.slots64, t);
+    const long long position = index_at(p.positions, p.positions64, t);
+    const long long old_position = index_at(p.old_positions, p.positions64, t);
+    const bool masked = p.masked != nullptr && p.masked[t] != 0;
+    const bool turned = t >= p.prefix;
+    const bool there = source >= 0 && source < p.num_slots &&
+                       (!turned || (in_table(p, position) && in_table(p, old_position)));
+    if (slot >= 0 && slot < p.num_slots) k.slot = static_cast<int>(slot);
+    if (there && !masked && k.slot >= 0) {
+      k.from = static_cast<int>(source);
+      if (turned) {
+        k.position = static_cast<int>(position);
+        k.old_position = static_cast<int>(old_position);
+      }
     }
-    decode8(x, scale, a);
-    decode8(y, scale, b);
-    if (!turns) return;
-    double cd[8], sd[8], u[8], v[8];
+    *bad = !masked && (slot >= p.num_slots || (slot >= 0 && !there));
+    return k;
+  }
+  __device__ static Raw fetch(const PoolParams &p, const Half &half, bool, int head, long long, const Token &k,
+                              const Lane &l) {
+    const uint8_t *codes = half.codes + (static_cast<long long>(k.from) * p.hkv + head) * p.dim;
+    return Raw{*reinterpret_cast<const u32x2 *>(codes + l.first), *reinterpret_cast<const u32x2 *>(codes + l.second),
+               scale_of(half.scales[static_cast<long long>(k.from >> p.block_shift) * p.hkv + head])};
+  }
+  __device__ static void unpack(const Raw &raw, float *a, float *b) {
+    decode8(raw.x, raw.scale, a);
+    decode8(raw.y, raw.scale, b);
+  }
+  __device__ static void angles(const PoolParams &p, const Token &k, int i, Angle *out) {
+    float c[4], s[4], from_c[4], from_s[4];
+    const long long to = k.position * p.table_stride + i, from = k.old_position * p.table_stride + i;
+    values4(p, to, c);
+    values4(p, to + p.rotary / 2, s);
+    values4(p, from, from_c);
+    values4(p, from + p.rotary / 2, from_s);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      cd[j] = static_cast<double>(c[j]) * from_c[j] + static_cast<double>(s[j]) * from_s[j];
-      sd[j] = static_cast<double>(s[j]) * from_c[j] - static_cast<double>(c[j]) * from_s[j];
-      u[j] = a[j];
-      v[j] = b[j];
-    }
-    turn(p.neox != 0, cd, sd, u, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[j] = to_odd(u[j]);
-      b[j] = to_odd(v[j]);
+    for (int j = 0; j < 4; ++j) {
+      out[j].cos = static_cast<double>(c[j]) * from_c[j] + static_cast<double>(s[j]) * from_s[j];
+      out[j].sin = static_cast<double>(s[j]) * from_c[j] - static_cast<double>(c[j]) * from_s[j];
     }
   }
 };
@@ -372,11 +359,11 @@ __device__ inline float finite_size(float x) {
 
 // The queries of append: kGroup lanes a head, 64 / kGroup heads of one token a wave.
 template <typename E, int kGroup>
-__device__ inline void turn_queries(const PoolParams &p, long long unit) {
+__device__ inline void turn_queries(const PoolParams &p, unsigned unit) {
   constexpr int kHeads = kWave / kGroup;
   const int lane = threadIdx.x % kWave;
-  const long long t = unit / p.query_steps;
-  const int step = static_cast<int>(unit - t * p.query_steps);
+  const long long t = unit / static_cast<unsigned>(p.query_steps);
+  const int step = static_cast<int>(unit % static_cast<unsigned>(p.query_steps));
   if (t >= p.num_tokens) return;
   const Lane l = lane_of<kGroup>(p);
   const int head = step * kHeads + lane / kGroup;
@@ -395,9 +382,41 @@ __device__ inline void turn_queries(const PoolParams &p, long long unit) {
     values8(p.table, p.table_dtype, p.table_chunks, at, c);
     values8(p.table, p.table_dtype, p.table_chunks, at + p.rotary / 2, s);
   }
-  if (p.query_weight != nullptr) norm<kGroup>(p, p.query_weight, l, a, b);
+  if (p.query_weight != nullptr) {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += a[j] * a[j] + b[j] * b[j];
+#pragma unroll
+    for (int lanes_apart = 1; lanes_apart < kGroup; lanes_apart *= 2) sum += __shfl_xor(sum, lanes_apart);
+    if (active) {
+      const float scale = rsqrtf(sum / static_cast<float>(p.dim) + static_cast<float>(p.eps));
+      float w[8];
+      values8(p.query_weight, p.weight_dtype, true, l.first, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = a[j] * scale * w[j];
+      values8(p.query_weight, p.weight_dtype, true, l.second, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = b[j] * scale * w[j];
+    }
+  }
   if (!active) return;
-  if (l.rotates) turn(p.neox != 0, c, s, a, b);
+  if (l.rotates && p.neox) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float lo = a[j], hi = b[j];
+      a[j] = lo * c[j] - hi * s[j];
+      b[j] = hi * c[j] + lo * s[j];
+    }
+  } else if (l.rotates) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
+      a[2 * j] = a0 * c[j] - a1 * s[j];
+      a[2 * j + 1] = a1 * c[j] + a0 * s[j];
+      b[2 * j] = b0 * c[4 + j] - b1 * s[4 + j];
+      b[2 * j + 1] = b1 * c[4 + j] + b0 * s[4 + j];
+    }
+  }
   u32x4 out_a, out_b;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -409,29 +428,50 @@ __device__ inline void turn_queries(const PoolParams &p, long long unit) {
   *reinterpret_cast<u32x4 *>(dst + l.second) = out_b;
 }
 
+template <typename E, int kGroup>
+__global__ void __launch_bounds__(kThreads) quantized_query_kernel(const PoolParams p) {
+  turn_queries<E, kGroup>(p, blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+}
+
 // Writes runs of rows.  A pair is one head's keys or values; kParts waves of a
-// workgroup hold a pair's run, up to kHeldRows rows each (block sizes up to 16 kParts).
+// workgroup hold a pair's run, two steps of 64 / kGroup rows each.
+//
+// A call is bound by memory, or for few rows by the chain slot -> row and angle -> code.
+// So what there is to know of the window's tokens is read at once, each row's loads do
+// not wait for its angles, and a run's angles are made once for the workgroup's heads
+// and kept in LDS (a link's are four table rows' worth of products; every head by
+// itself would read 1 KB of table for 256 bytes of codes).  LDS has the angles of
+// lane i's pair j as element 9 R row + R j + i, R = rotary lanes of a row, so that 16
+// lanes' 16-byte reads meet every bank once.
 template <typename Source, typename E, int kGroup, int kParts, bool kQueries>
-__global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads) quantized_write_kernel(const PoolParams p) {
+__global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts <= 2 ? 4 : kParts <= 8 ? 3 : 1) quantized_write_kernel(const PoolParams p) {
   constexpr int kWaves = kParts > 4 ? kParts : kThreads / kWave;
   constexpr int kPairs = kWaves / kParts;  // of a workgroup
   constexpr int kRows = kWave / kGroup;    // of a step
-  constexpr int kSteps = kHeldRows / kRows;
-  constexpr int kWords = (kParts * kHeldRows + kWave - 1) / kWave;
+  constexpr int kSteps = kHeldSteps;
+  constexpr int kHeldRows = kSteps * kRows;  // of a run, in one wave's registers
+  constexpr int kRunRows = kParts * kHeldRows;
+  constexpr int kWords = (kRunRows + kWave - 1) / kWave;
+  constexpr bool kShares = kPairs > 1;
+  constexpr int kTokens = 1 + kMostWindow + kRunRows;  // the one before the window, the window, a run from its last on
   __shared__ float most_of[kPairs][kParts];
+  __shared__ Token tokens[kTokens];
+  __shared__ Angle shared_angles[kShares ? kRunRows * 9 * kGroup : 1];
+  __shared__ float key_weights[Source::kNorms ? 16 * kGroup : 1];
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave;
-  unsigned group = blockIdx.x;
+  const unsigned group = blockIdx.x;
   if constexpr (kQueries) {
-    // (The queries come first: a run's waves take longer to start than they do.)
-    if (group < p.query_groups) {
-      turn_queries<E, kGroup>(p, static_cast<long long>(group) * kWaves + wave);
+    // (The runs, which take longer, come first.)
+    if (group >= p.run_groups) {
+      turn_queries<E, kGroup>(p, (group - p.run_groups) * kWaves + wave);
       return;
     }
-    group -= static_cast<unsigned>(p.query_groups);
   }
-  const long long t0 = static_cast<long long>(group / static_cast<unsigned>(p.pair_groups)) * p.window;
-  const int pair = static_cast<int>(group % static_cast<unsigned>(p.pair_groups)) * kPairs + wave / kParts;
+  const unsigned window = group / static_cast<unsigned>(p.pair_groups);
+  const int pair_group = static_cast<int>(group % static_cast<unsigned>(p.pair_groups));
+  const long long t0 = static_cast<long long>(window) * p.window - 1;  // of tokens[0]
+  const int pair = pair_group * kPairs + wave / kParts;
   const int part = wave % kParts;
   const bool has_pair = pair < 2 * p.hkv;
   const bool is_key = pair < p.hkv;
@@ -440,72 +480,147 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads) quanti
   const int block_rows = 1 << p.block_shift;
   const Lane l = lane_of<kGroup>(p);
 
-  // A token's block (-1: none).
-  auto block_of = [&](long long t) -> long long {
-    if (t < 0 || t >= p.num_tokens) return -1;
-    const long long slot = index_at(p.slots, p.slots64, t);
-    return slot < 0 || slot >= p.num_slots ? -1 : slot >> p.block_shift;
-  };
-  // Lane l: token t0 - 1 + l.  A run begins where the block changes.
-  const long long mine = block_of(t0 - 1 + lane);
-  const long long former = __shfl_up(mine, 1);
+  for (int i = threadIdx.x; i < 1 + p.window + kRunRows; i += kWaves * kWave) {
+    Token k{-1, -1, -1, -1};
+    bool bad = false;
+    if (t0 + i >= 0 && t0 + i < p.num_tokens) k = Source::token(p, t0 + i, &bad);
+    tokens[i] = k;
+    if (bad && i >= 1 && i <= p.window && pair_group == 0 && p.skipped != nullptr) atomicAdd(p.skipped, 1ull);
+  }
+  if constexpr (Source::kNorms)
+    for (int i = threadIdx.x; i < p.dim; i += kWaves * kWave)
+      key_weights[i] = p.key_weight != nullptr ? value_at(p.key_weight, p.weight_dtype, i) : 1.f;
+  __syncthreads();
+  // A run begins where the block changes.
+  auto block_of = [&](int i) { return tokens[i].slot < 0 ? -1 : tokens[i].slot >> p.block_shift; };
+  const int in_window = min(lane, p.window);
+  const int mine = block_of(in_window), former = block_of(max(in_window - 1, 0));
   unsigned long long begins =
       __builtin_amdgcn_ballot_w64(lane >= 1 && lane <= p.window && mine >= 0 && mine != former);
-  if constexpr (!kQueries) {
-    if (p.skipped != nullptr && pair == 0 && part == 0) {
-      const long long t = t0 - 1 + lane;
-      const bool listed = lane >= 1 && lane <= p.window && t < p.num_tokens && !Source::masked(p, t);
-      const bool bad = listed && (index_at(p.slots, p.slots64, t) >= p.num_slots ||
-                                  (mine >= 0 && !Source::exists(p, t)));
-      const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(bad));
-      if (lane == 0 && count > 0) atomicAdd(p.skipped, static_cast<unsigned long long>(count));
-    }
-  }
   while (begins != 0) {
-    const int at = __builtin_ctzll(begins);
+    const int start = __builtin_ctzll(begins);
     begins &= begins - 1;
-    const long long start = t0 - 1 + at;
-    const long long block = __shfl(mine, at);
-    // Its rows, and those of them that are written.
-    int rows = 0;
+    const int block = __builtin_amdgcn_readlane(mine, start);
+    // Its rows that are written.
     unsigned long long written[kWords];
     int count = 0;
+    bool more = true;
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
-      written[w] = 0;
-      if (rows < w * kWave) continue;
-      const long long t = start + w * kWave + lane;
-      const bool own = w * kWave + lane < block_rows && block_of(t) == block;
+      const int row = w * kWave + lane;
+      const bool own = row < block_rows && block_of(start + min(row, kRunRows - 1)) == block;
       const unsigned long long same = __builtin_amdgcn_ballot_w64(own);
-      const int length = same == ~0ull ? kWave : __builtin_ctzll(~same);
-      rows += length;
-      written[w] = __builtin_amdgcn_ballot_w64(own && lane < length && !Source::masked(p, t) && Source::exists(p, t));
+      const int length = !more ? 0 : same == ~0ull ? kWave : __builtin_ctzll(~same);
+      more = length == kWave;
+      written[w] = __builtin_amdgcn_ballot_w64(own && lane < length && tokens[start + min(row, kRunRows - 1)].from >= 0);
       count += __builtin_popcountll(written[w]);
     }
     if (count == 0) continue;
-    uint8_t *scale_at = half.scales + block * p.hkv + head;
+    uint8_t *scale_at = half.scales + static_cast<long long>(block) * p.hkv + head;
     unsigned old = has_pair ? *scale_at : 0u;
-    // The 16 rows of this part that are written.
+    // The rows of this part that are written (kHeldRows bits).
     auto part_of = [&](const unsigned long long *words) {
       unsigned bits = 0;
 #pragma unroll
       for (int w = 0; w < kWords; ++w)
-        if (part * kHeldRows / kWave == w) bits = static_cast<unsigned>(words[w] >> (part * kHeldRows % kWave)) & 0xffffu;
+        if (part * kHeldRows / kWave == w) bits = static_cast<unsigned>(words[w] >> (part * kHeldRows % kWave));
       return bits;
     };
     const unsigned own_rows = part_of(written);
-
-    float a[kSteps][8], b[kSteps][8];
-    float most = 0.f;
     auto held_of = [&](int step) { return step * kRows + lane / kGroup; };  // of the part's rows
+    auto token_of = [&](int step) { return start + part * kHeldRows + held_of(step); };
+    auto has_row = [&](int step) { return has_pair && l.active && ((own_rows >> held_of(step)) & 1u) != 0; };
+
+    typename Source::Raw raw[kSteps];
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      const bool there = has_pair && ((own_rows >> held_of(step)) & 1u) != 0;
-      if (__builtin_amdgcn_ballot_w64(there) == 0) continue;
-      Source::template row<kGroup>(p, is_key, head, start + part * kHeldRows + held_of(step), there, l, a[step],
-                                   b[step]);
+      raw[step] = typename Source::Raw{};
+      if (has_row(step)) raw[step] = Source::fetch(p, half, is_key, head, t0 + token_of(step), tokens[token_of(step)], l);
+    }
+    const int lanes = p.rotary / 16;
+    if constexpr (kShares) {
+      if (pair_group * kPairs < p.hkv) {  // (keys among its pairs)
+        const int quads = 2 * lanes;  // of four pairs, a row's
+        for (int i = threadIdx.x; i < kRunRows * quads; i += kWaves * kWave) {
+          const int row = i / quads, quad = i - row * quads;
+          if (((written[kWords - 1] >> row) & 1ull) == 0 || tokens[start + row].position < 0) continue;
+          Angle four[4];
+          Source::angles(p, tokens[start + row], 4 * quad, four);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(finite_size(a[step][j]), finite_size(b[step][j])));
+          for (int j = 0; j < 4; ++j)
+            shared_angles[(9 * row + 4 * (quad % 2) + j) * lanes + quad / 2] = four[j];
+        }
+      }
+      __syncthreads();
+    }
+    float a[kSteps][8], b[kSteps][8];
+    float most = 0.f;
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      if (__builtin_amdgcn_ballot_w64(has_row(step)) == 0) continue;
+      Source::unpack(raw[step], a[step], b[step]);
+      if (is_key) {
+        const bool normed = Source::kNorms && p.key_weight != nullptr;
+        double scale = 1.0;
+        if (normed) {
+          double sum = 0.0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sum += static_cast<double>(a[step][j]) * a[step][j];
+            sum += static_cast<double>(b[step][j]) * b[step][j];
+          }
+#pragma unroll
+          for (int apart = 1; apart < kGroup; apart *= 2) sum += __shfl_xor(sum, apart);
+          scale = 1.0 / sqrt(sum / static_cast<double>(p.dim) + p.eps);
+        }
+        const Token &k = tokens[token_of(step)];
+        const bool turns = has_row(step) && l.rotates && k.position >= 0;
+        Angle made[kShares ? 1 : 8];
+        const Angle *from = shared_angles + 9 * (part * kHeldRows + held_of(step)) * lanes + l.i;
+        if constexpr (!kShares) {
+          if (turns) {
+            Source::angles(p, k, 8 * l.i, made);
+            Source::angles(p, k, 8 * l.i + 4, made + 4);
+          }
+        }
+        // A pair of dims, at these places of the row: normed, turned and rounded.
+        auto pair_of = [&](int j, float &first, float &second, int at, int other, bool turned) {
+          double x = first, y = second;
+          if (Source::kNorms) {  // (weights of 1 under a scale of 1 without a norm)
+            x = x * scale * key_weights[at];
+            y = y * scale * key_weights[other];
+          }
+          if (turned) {
+            const Angle angle = kShares ? from[j * lanes] : made[kShares ? 0 : j];
+            const double lo = x, hi = y;
+            x = lo * angle.cos - hi * angle.sin;
+            y = hi * angle.cos + lo * angle.sin;
+          }
+          first = to_odd(x);
+          second = to_odd(y);
+          if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (few doubles at a time)
+        };
+        if (turns && p.neox != 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pair_of(j, a[step][j], b[step][j], l.first + j, l.second + j, true);
+        } else if (turns || normed) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = 2 * j;
+            if (turns) {
+              pair_of(j, a[step][at], a[step][at + 1], l.first + at, l.first + at + 1, true);
+              pair_of(4 + j, b[step][at], b[step][at + 1], l.second + at, l.second + at + 1, true);
+            } else {
+              pair_of(j, a[step][at], a[step][at + 1], l.first + at, l.first + at + 1, false);
+              pair_of(4 + j, b[step][at], b[step][at + 1], l.second + at, l.second + at + 1, false);
+            }
+          }
+        }
+      }
+      if (has_row(step)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(finite_size(a[step][j]), finite_size(b[step][j])));
+      }
     }
 #pragma unroll
     for (int step = 1; step < kWave; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
@@ -515,18 +630,18 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads) quanti
       __syncthreads();
 #pragma unroll
       for (int v = 0; v < kParts; ++v) most = fmaxf(most, most_of[wave / kParts][v]);
-      __syncthreads();  // (the next run writes it)
     }
+    if (begins != 0) __syncthreads();  // (the next run writes most_of and the angles)
     if (!has_pair) continue;
     const unsigned need = byte_for(most);
     const unsigned byte = count == block_rows ? need : max(old, need);
     if (part == 0 && lane == 0 && byte != old) *scale_at = static_cast<uint8_t>(byte);
     const float inverse = inverse_of(byte);
-    auto codes_at = [&](long long slot) { return half.codes + (slot * p.hkv + head) * p.dim; };
+    auto codes_at = [&](int slot) { return half.codes + (static_cast<long long>(slot) * p.hkv + head) * p.dim; };
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      if (((own_rows >> held_of(step)) & 1u) == 0 || !l.active) continue;
-      uint8_t *dst = codes_at(index_at(p.slots, p.slots64, start + part * kHeldRows + held_of(step)));
+      if (!has_row(step)) continue;
+      uint8_t *dst = codes_at(tokens[token_of(step)].slot);
       *reinterpret_cast<u32x2 *>(dst + l.first) = encode8(a[step], inverse);
       *reinterpret_cast<u32x2 *>(dst + l.second) = encode8(b[step], inverse);
     }
@@ -537,10 +652,8 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads) quanti
     for (int w = 0; w < kWords; ++w) taken[w] = 0;
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
-      if (w * kWave >= rows) continue;
       const bool own = ((written[w] >> lane) & 1ull) != 0;
-      const int offset =
-          own ? static_cast<int>(index_at(p.slots, p.slots64, start + w * kWave + lane)) & (block_rows - 1) : 0;
+      const int offset = own ? tokens[start + w * kWave + lane].slot & (block_rows - 1) : 0;
 #pragma unroll
       for (int v = 0; v < kWords; ++v) {
         unsigned long long bits = own && offset / kWave == v ? 1ull << (offset % kWave) : 0ull;
@@ -549,22 +662,29 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads) quanti
         taken[v] |= bits;
       }
     }
+    const unsigned own_taken = part_of(taken);
     const unsigned grown = byte - old;
     const float ratio = grown < 127u ? __uint_as_float((127u - grown) << 23) : 0.f;
-    const unsigned own_taken = part_of(taken);
+    u32x2 others[kSteps][2];
+    auto is_other = [&](int step) {
+      return part * kHeldRows + held_of(step) < block_rows && ((own_taken >> held_of(step)) & 1u) == 0 && l.active;
+    };
+    auto other_at = [&](int step) { return codes_at((block << p.block_shift) + part * kHeldRows + held_of(step)); };
 #pragma unroll
-    for (int step = 0; step < kSteps; ++step) {
-      const int offset = part * kHeldRows + held_of(step);
-      if (offset >= block_rows || ((own_taken >> held_of(step)) & 1u) != 0 || !l.active) continue;
-      uint8_t *row = codes_at((block << p.block_shift) + offset);
-      u32x2 *chunks[2] = {reinterpret_cast<u32x2 *>(row + l.first), reinterpret_cast<u32x2 *>(row + l.second)};
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float values[8];
-        decode8(*chunks[k], ratio, values);
-        *chunks[k] = encode8(values, 1.f);
+    for (int step = 0; step < kSteps; ++step)
+      if (is_other(step)) {
+        others[step][0] = *reinterpret_cast<const u32x2 *>(other_at(step) + l.first);
+        others[step][1] = *reinterpret_cast<const u32x2 *>(other_at(step) + l.second);
       }
-    }
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step)
+      if (is_other(step)) {
+        float values[8];
+        decode8(others[step][0], ratio, values);
+        *reinterpret_cast<u32x2 *>(other_at(step) + l.first) = encode8(values, 1.f);
+        decode8(others[step][1], ratio, values);
+        *reinterpret_cast<u32x2 *>(other_at(step) + l.second) = encode8(values, 1.f);
+      }
   }
 }
 
@@ -656,7 +776,7 @@ int check_table(int64_t dtype, int64_t rows, int64_t cols, int64_t stride, int64
   if (rotary > dim) return fail(LL_ERR_ROTARY_DIM_EXCEEDS_HEAD_DIM, "rotary_dim exceeds head_dim");
   if (rotary % 16 != 0) return fail(LL_ERR_INVALID_ARGUMENT, "rotary_dim must be a multiple of 16");
   if (!float_code(dtype)) return fail(LL_ERR_UNSUPPORTED_COS_SIN_DTYPE, "cos/sin dtype");
-  if (rows < 0 || cols < rotary || stride < 0)
+  if (rows < 0 || rows > 0x7fffffff || cols < rotary || stride < 0)
     return fail(LL_ERR_UNSUPPORTED_COS_SIN_CACHE, "the cos/sin table needs rotary_dim columns");
   return LL_OK;
 }
@@ -695,18 +815,26 @@ int launch_write(PoolParams &p, hipStream_t s) {
   // a window each where that makes fewer waves than the card holds (16 a CU).
   const long long waves = p.num_tokens * 2 * p.hkv * kParts;
   p.window = 1;
-  while (p.window < 16 && waves / p.window > 256 * 16) p.window *= 2;
-  long long groups = (p.num_tokens + p.window - 1) / p.window * p.pair_groups;
-  if constexpr (kQueries) {
-    constexpr int kHeads = kWave / kGroup;
-    p.query_steps = (p.hq + kHeads - 1) / kHeads;
-    p.query_groups = (p.num_tokens * p.query_steps + kWaves - 1) / kWaves;
-    groups += p.query_groups;
+  while (p.window < kMostWindow && waves / p.window > 256 * 16) p.window *= 2;
+  const long long run_groups = (p.num_tokens + p.window - 1) / p.window * p.pair_groups;
+  p.run_groups = static_cast<unsigned>(std::min(run_groups, 0xffffffffll));
+  const long long query_waves = p.num_tokens * p.query_steps;
+  // The queries of a small call go with its runs in one launch.  Those of a large one
+  // are bound by memory, and go by themselves: the runs' registers leave room for two
+  // waves a SIMD.
+  const bool together = kQueries && query_waves <= kMostTogether;
+  const long long groups = run_groups + (together ? (query_waves + kWaves - 1) / kWaves : 0);
+  if (groups * (kWaves * kWave) > 0xffffffffll || query_waves * kWave > 0xffffff00ll)
+    return fail(LL_ERR_INVALID_ARGUMENT, "too many rows for one launch");  // (fewer than 2^32 threads)
+  const dim3 grid(static_cast<unsigned>(groups));
+  if (together) {
+    quantized_write_kernel<Source, E, kGroup, kParts, kQueries><<<grid, kWaves * kWave, 0, s>>>(p);
+  } else {
+    if (kQueries)
+      quantized_query_kernel<E, kGroup>
+          <<<static_cast<unsigned>((query_waves + kThreads / kWave - 1) / (kThreads / kWave)), kThreads, 0, s>>>(p);
+    quantized_write_kernel<Source, E, kGroup, kParts, false><<<grid, kWaves * kWave, 0, s>>>(p);
   }
-  if (groups * (kWaves * kWave) > 0xffffffffll)  // a launch holds fewer than 2^32 threads
-    return fail(LL_ERR_INVALID_ARGUMENT, "too many rows for one launch");
-  quantized_write_kernel<Source, E, kGroup, kParts, kQueries>
-      <<<static_cast<unsigned>(groups), kWaves * kWave, 0, s>>>(p);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return fail(LL_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   return LL_OK;
@@ -714,10 +842,17 @@ int launch_write(PoolParams &p, hipStream_t s) {
 
 template <typename Source, typename E, int kGroup, bool kQueries>
 int launch_by_block(PoolParams &p, hipStream_t s) {
-  if (p.block_shift <= 4) return launch_write<Source, E, kGroup, 1, kQueries>(p, s);
-  if (p.block_shift == 5) return launch_write<Source, E, kGroup, 2, kQueries>(p, s);
-  if (p.block_shift == 6) return launch_write<Source, E, kGroup, 4, kQueries>(p, s);
-  return launch_write<Source, E, kGroup, 8, kQueries>(p, s);
+  constexpr int kHeld = kHeldSteps * kWave / kGroup;
+  const int rows = 1 << p.block_shift;
+  if (rows <= kHeld) return launch_write<Source, E, kGroup, 1, kQueries>(p, s);
+  if (rows <= 2 * kHeld) return launch_write<Source, E, kGroup, 2, kQueries>(p, s);
+  if (rows <= 4 * kHeld) return launch_write<Source, E, kGroup, 4, kQueries>(p, s);
+  if constexpr (8 * kHeld >= kMaxBlock) {
+    return launch_write<Source, E, kGroup, 8, kQueries>(p, s);
+  } else {
+    if (rows <= 8 * kHeld) return launch_write<Source, E, kGroup, 8, kQueries>(p, s);
+    return launch_write<Source, E, kGroup, 16, kQueries>(p, s);
+  }
 }
 
 template <typename Source, typename E, bool kQueries>
@@ -787,8 +922,10 @@ int ll_quantized_append(const ll_quantized_append_args *a, ll_stream_t stream) {
   p.query_weight = a->query_norm_weight;
   p.key_weight = a->key_norm_weight;
   p.weight_dtype = static_cast<int>(a->norm_weight_dtype);
-  p.eps = static_cast<float>(a->norm_eps);
+  p.eps = a->norm_eps;
   p.hq = static_cast<int>(a->num_q_heads);
+  const int query_heads = kWave / (p.dim <= 64 ? 4 : p.dim <= 128 ? 8 : 16);  // of a wave
+  p.query_steps = (p.hq + query_heads - 1) / query_heads;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return a->dtype == LL_DTYPE_FLOAT16 ? launch_by_dim<NewTokens<F16>, F16, true>(p, s)
                                       : launch_by_dim<NewTokens<Bf16>, Bf16, true>(p, s);

@@ -1,6 +1,6 @@
 // The calls of a model's step (rotate_heads, append_rotated_kv_inplace,
-// paged_attention) from their tensors: checks, outputs and the library's entry in
-// one native call.
+// paged_attention, and the four over a pool held in 8 bits) from their tensors:
+// checks, outputs and the library's entry in one native call.
 //
 // A decode step makes these calls once per layer on a few rows, where the GPU
 // takes 4 us; the checks and the argument block take Python 15 to 25 us a call,
@@ -324,85 +324,354 @@ PyObject *append(PyObject *const *a, Py_ssize_t n, bool *launched) {
   return status != LL_OK ? PyLong_FromLong(status) : result.release();
 }
 
-typedef int64_t (*WorkspaceEntry)(const ll_paged_attention_args *);
+// What attention over 16-bit and over 8-bit pools have in common: query, key_buffer,
+// value_buffer (checked by the caller beyond their shape), page_table, kv_lengths,
+// page_size, query_starts, scale.
+bool read_paged(const at::Tensor *query, const at::Tensor *keys, const at::Tensor *values, PyObject *const *a,
+                ll_paged_attention_args *args) {
+  const at::Tensor *pages = plain(a[0]), *lengths = plain(a[1]);
+  int64_t page_size = 0;
+  if (query == nullptr || keys == nullptr || values == nullptr || pages == nullptr) return false;
+  const at::Device device = query->device();
+  args->kv_dtype = half_code(query->scalar_type());
+  if (args->kv_dtype < 0 || query->dim() != 3 || keys->dim() != 3 || values->sizes() != keys->sizes()) return false;
+  const int64_t queries = query->size(0), q_heads = query->size(1), dim = query->size(2), kv_heads = keys->size(1);
+  if (keys->size(2) != dim || (dim != 64 && dim != 128 && dim != 256) || kv_heads < 1 || q_heads < 1 ||
+      q_heads % kv_heads != 0)
+    return false;
+  for (const at::Tensor *buffer : {keys, values})
+    if (buffer->device() != device || !buffer->is_contiguous() ||
+        reinterpret_cast<uintptr_t>(buffer->data_ptr()) % 16 != 0)
+      return false;
+  if (pages->dim() != 2 || pages->scalar_type() != at::kInt || pages->device() != device ||
+      (pages->size(1) > 1 && pages->stride(1) != 1))
+    return false;
+  const int64_t requests = pages->size(0);
+  if (!integer(a[2], &page_size) || page_size < 1 || !vector_ok(lengths, requests, device)) return false;
+  args->kv_lengths_dtype = index_code(lengths->scalar_type());
+  if (args->kv_lengths_dtype < 0) return false;
+  if (a[3] != Py_None) {
+    const at::Tensor *starts = plain(a[3]);
+    if (!vector_ok(starts, requests + 1, device)) return false;
+    args->query_starts = starts->data_ptr();
+    args->query_starts_dtype = index_code(starts->scalar_type());
+    if (args->query_starts_dtype < 0) return false;
+  } else if (queries != requests) {
+    return false;
+  }
+  if (a[4] == Py_None) args->softmax_scale = 1.0 / std::sqrt(static_cast<double>(dim));
+  else if (!number(a[4], &args->softmax_scale)) return false;
+  if (!(args->softmax_scale >= 1e-37 && args->softmax_scale < 1e30)) return false;
+  if (query->stride(2) != 1 || query->stride(0) % 8 != 0 || query->stride(1) % 8 != 0 ||
+      reinterpret_cast<uintptr_t>(query->data_ptr()) % 16 != 0)
+    return false;
+  args->struct_size = sizeof(*args);
+  args->query = query->data_ptr();
+  args->query_token_stride = query->stride(0);
+  args->query_head_stride = query->stride(1);
+  args->num_queries = queries;
+  args->key_buffer = keys->data_ptr();
+  args->value_buffer = values->data_ptr();
+  args->num_slots = keys->size(0);
+  args->num_q_heads = q_heads;
+  args->num_kv_heads = kv_heads;
+  args->head_dim = dim;
+  args->page_table = static_cast<const int32_t *>(pages->data_ptr());
+  args->page_table_stride = pages->stride(0);
+  args->page_table_columns = pages->size(1);
+  args->page_size = page_size;
+  args->kv_lengths = lengths->data_ptr();
+  args->num_requests = requests;
+  return true;
+}
+
+// The output and the workspace of an attention call, and the call.
+template <typename Args>
+PyObject *attend(const Target &target, int64_t workspace_entry, const at::Tensor &query, Args *args,
+                 ll_paged_attention_args *paged, bool *launched) {
+  typedef int64_t (*WorkspaceEntry)(const Args *);
+  const at::Tensor output = at::empty({query.size(0), query.size(1), query.size(2)}, query.options());
+  paged->output = output.data_ptr();
+  const int64_t needed = reinterpret_cast<WorkspaceEntry>(workspace_entry)(args);
+  if (needed < 0) return PyLong_FromLongLong(needed);
+  at::Tensor workspace;
+  if (needed > 0) {
+    workspace = at::empty({needed}, query.options().dtype(at::kByte));
+    paged->workspace = workspace.data_ptr();
+    paged->workspace_bytes = needed;
+  }
+  Object result(THPVariable_Wrap(output));
+  if (result.held == nullptr) return nullptr;
+  const int status = target.call(args, launched);
+  return status != LL_OK ? PyLong_FromLong(status) : result.release();
+}
 
 // (entry, stream, device, workspace entry, query, key_buffer, value_buffer,
 // page_table, kv_lengths, page_size, query_starts, scale) -> output
 PyObject *paged_attention(PyObject *const *a, Py_ssize_t n, bool *launched) {
   Target target;
-  int64_t workspace_entry = 0, page_size = 0;
+  int64_t workspace_entry = 0;
   if (n != 12 || !target.read(a) || !integer(a[3], &workspace_entry)) return none();
-  const at::Tensor *query = plain(a[4]), *keys = plain(a[5]), *values = plain(a[6]), *pages = plain(a[7]),
-                   *lengths = plain(a[8]);
-  if (query == nullptr || keys == nullptr || values == nullptr || pages == nullptr || !target.takes(*query))
-    return none();
+  const at::Tensor *query = plain(a[4]), *keys = plain(a[5]), *values = plain(a[6]);
   ll_paged_attention_args args;
   memset(&args, 0, sizeof(args));
-  const at::Device device = query->device();
-  args.kv_dtype = half_code(query->scalar_type());
-  if (args.kv_dtype < 0 || query->dim() != 3 || keys->dim() != 3 || values->sizes() != keys->sizes()) return none();
-  const int64_t queries = query->size(0), q_heads = query->size(1), dim = query->size(2), kv_heads = keys->size(1);
-  if (keys->size(2) != dim || (dim != 64 && dim != 128 && dim != 256) || kv_heads < 1 || q_heads < 1 ||
-      q_heads % kv_heads != 0)
-    return none();
-  for (const at::Tensor *buffer : {keys, values})
-    if (buffer->scalar_type() != query->scalar_type() || buffer->device() != device || !buffer->is_contiguous() ||
-        reinterpret_cast<uintptr_t>(buffer->data_ptr()) % 16 != 0)
-      return none();
-  if (pages->dim() != 2 || pages->scalar_type() != at::kInt || pages->device() != device ||
-      (pages->size(1) > 1 && pages->stride(1) != 1))
-    return none();
-  const int64_t requests = pages->size(0);
-  if (!integer(a[9], &page_size) || page_size < 1 || !vector_ok(lengths, requests, device)) return none();
-  args.kv_lengths_dtype = index_code(lengths->scalar_type());
-  if (args.kv_lengths_dtype < 0) return none();
-  if (a[10] != Py_None) {
-    const at::Tensor *starts = plain(a[10]);
-    if (!vector_ok(starts, requests + 1, device)) return none();
-    args.query_starts = starts->data_ptr();
-    args.query_starts_dtype = index_code(starts->scalar_type());
-    if (args.query_starts_dtype < 0) return none();
-  } else if (queries != requests) {
-    return none();
-  }
-  if (a[11] == Py_None) args.softmax_scale = 1.0 / std::sqrt(static_cast<double>(dim));
-  else if (!number(a[11], &args.softmax_scale)) return none();
-  if (!(args.softmax_scale >= 1e-37 && args.softmax_scale < 1e30)) return none();
-  if (query->stride(2) != 1 || query->stride(0) % 8 != 0 || query->stride(1) % 8 != 0 ||
-      reinterpret_cast<uintptr_t>(query->data_ptr()) % 16 != 0)
-    return none();
+  if (!read_paged(query, keys, values, a + 7, &args) || !target.takes(*query)) return none();
+  if (keys->scalar_type() != query->scalar_type() || values->scalar_type() != query->scalar_type()) return none();
   if (target.entry == 0) Py_RETURN_TRUE;
-  args.struct_size = sizeof(args);
-  args.query = query->data_ptr();
-  args.query_token_stride = query->stride(0);
-  args.query_head_stride = query->stride(1);
-  args.num_queries = queries;
-  args.key_buffer = keys->data_ptr();
-  args.value_buffer = values->data_ptr();
-  args.num_slots = keys->size(0);
-  args.num_q_heads = q_heads;
-  args.num_kv_heads = kv_heads;
-  args.head_dim = dim;
-  args.page_table = static_cast<const int32_t *>(pages->data_ptr());
-  args.page_table_stride = pages->stride(0);
-  args.page_table_columns = pages->size(1);
-  args.page_size = page_size;
-  args.kv_lengths = lengths->data_ptr();
-  args.num_requests = requests;
-  const at::Tensor output = at::empty({queries, q_heads, dim}, query->options());
-  args.output = output.data_ptr();
-  const int64_t needed = reinterpret_cast<WorkspaceEntry>(workspace_entry)(&args);
-  if (needed < 0) return PyLong_FromLongLong(needed);
-  at::Tensor workspace;
-  if (needed > 0) {
-    workspace = at::empty({needed}, query->options().dtype(at::kByte));
-    args.workspace = workspace.data_ptr();
-    args.workspace_bytes = needed;
+  return attend(target, workspace_entry, *query, &args, &args, launched);
+}
+
+// An 8-bit pool: key_buffer, value_buffer, key_scales, value_scales, scale_block.
+struct Pool {
+  std::array<const at::Tensor *, 4> tensors{};
+  ll_quantized_pool args{};
+
+  bool read(PyObject *const *a) {
+    for (int i = 0; i < 4; ++i)
+      if ((tensors[i] = plain(a[i])) == nullptr) return false;
+    const at::Tensor &keys = *tensors[0];
+    int64_t block = 0;
+    if (!integer(a[4], &block) || block < 1 || block > 128 || (block & (block - 1)) != 0 || keys.dim() != 3) return false;
+    const int64_t slots = keys.size(0), heads = keys.size(1), dim = keys.size(2);
+    if (slots % block != 0 || heads < 1 || dim < 16 || dim > 256 || dim % 16 != 0) return false;
+    for (int i = 0; i < 4; ++i) {
+      const at::Tensor &t = *tensors[i];
+      if (t.device() != keys.device() || !t.is_contiguous()) return false;
+      if (i < 2 ? t.scalar_type() != at::kFloat8_e4m3fn || t.sizes() != keys.sizes() ||
+                      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0
+                : t.scalar_type() != at::kFloat8_e8m0fnu || t.dim() != 2 || t.size(0) != slots / block ||
+                      t.size(1) != heads)
+        return false;
+    }
+    args.key_buffer = tensors[0]->data_ptr();
+    args.value_buffer = tensors[1]->data_ptr();
+    args.key_scales = tensors[2]->data_ptr();
+    args.value_scales = tensors[3]->data_ptr();
+    args.num_slots = slots;
+    args.scale_block = block;
+    args.num_kv_heads = heads;
+    args.head_dim = dim;
+    return true;
   }
+  bool meets(const at::Tensor *other) const {
+    if (other == nullptr) return false;
+    for (const at::Tensor *t : tensors)
+      if (overlap(*t, *other)) return true;
+    return false;
+  }
+  // A pool that is written.
+  bool apart() const {
+    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < i; ++j)
+        if (overlap(*tensors[i], *tensors[j])) return false;
+    return true;
+  }
+};
+
+bool in_chunks(const at::Tensor &rows) {
+  return rows.stride(2) == 1 && rows.stride(0) % 8 == 0 && rows.stride(1) % 8 == 0 &&
+         reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 == 0;
+}
+
+// (entry, stream, device, query, key, positions, table, rotary_dim, neox, query
+// norm, key norm, eps, skipped, query_output, value, slots, key_buffer,
+// value_buffer, key_scales, value_scales, scale_block) -> query
+PyObject *quantized_append(PyObject *const *a, Py_ssize_t n, bool *launched) {
+  Target target;
+  ll_head_rotary_args turn;
+  memset(&turn, 0, sizeof(turn));
+  const at::Tensor *query, *key;
+  Beside beside;
+  Pool pool;
+  if (n != 21 || !target.read(a) || !read_rotary(a + 3, &turn, &query, &key, &beside) || !target.takes(*query) ||
+      !pool.read(a + 16))
+    return none();
+  const at::Tensor *value = plain(a[14]), *slots = plain(a[15]);
+  const int64_t tokens = turn.num_tokens;
+  if (tokens == 0 || pool.tensors[0]->device() != query->device() || turn.rotary_dim % 16 != 0 ||
+      !rows_ok(value, tokens, *query) || !vector_ok(slots, tokens, query->device()))
+    return none();
+  for (const at::Tensor *rows : {key, value})
+    if (rows->size(1) != pool.args.num_kv_heads || rows->size(2) != pool.args.head_dim) return none();
+  if (!in_chunks(*query) || !in_chunks(*key) || !in_chunks(*value)) return none();
+  for (int i = 2; i < 4; ++i)
+    if (beside.read[i] != nullptr && reinterpret_cast<uintptr_t>(beside.read[i]->data_ptr()) % 16 != 0) return none();
+  if (!beside.counter_apart({query, key, value, slots}) || !pool.apart()) return none();
+  for (const at::Tensor *t : pool.tensors)
+    if (beside.meets(*t)) return none();
+  for (const at::Tensor *t : {query, key, value, slots})
+    if (pool.meets(t)) return none();
+  ll_quantized_append_args args;
+  memset(&args, 0, sizeof(args));
+  args.destination_slots_dtype = index_code(slots->scalar_type());
+  if (args.destination_slots_dtype < 0) return none();
+  const bool query_in_place = a[13] != Py_None;
+  if (query_in_place && (a[13] != a[3] || !in_place(*query, {key, value, slots}, beside))) return none();
+  if (target.entry == 0) Py_RETURN_TRUE;
+  const at::Tensor output = query_in_place ? *query : empty_like_rows(*query);
+  args.struct_size = sizeof(args);
+  args.pool = pool.args;
+  args.num_tokens = tokens;
+  args.num_q_heads = turn.num_q_heads;
+  args.dtype = turn.dtype;
+  args.query = turn.query;
+  args.query_token_stride = turn.query_token_stride;
+  args.query_head_stride = turn.query_head_stride;
+  set_output(output, &args.query_output, &args.query_output_token_stride, &args.query_output_head_stride);
+  args.key = turn.key;
+  args.key_token_stride = turn.key_token_stride;
+  args.key_head_stride = turn.key_head_stride;
+  args.value = value->data_ptr();
+  args.value_token_stride = value->stride(0);
+  args.value_head_stride = value->stride(1);
+  args.destination_slots = slots->data_ptr();
+  args.positions = turn.positions;
+  args.positions_dtype = turn.positions_dtype;
+  args.cos_sin_cache = turn.cos_sin_cache;
+  args.cos_sin_dtype = turn.cos_sin_dtype;
+  args.cos_sin_rows = turn.cos_sin_rows;
+  args.cos_sin_cols = turn.cos_sin_cols;
+  args.cos_sin_stride_row = turn.cos_sin_stride_row;
+  args.rotary_dim = turn.rotary_dim;
+  args.is_neox_style = turn.is_neox_style;
+  args.query_norm_weight = turn.query_norm_weight;
+  args.key_norm_weight = turn.key_norm_weight;
+  args.norm_weight_dtype = turn.norm_weight_dtype;
+  args.norm_eps = turn.norm_eps;
+  args.skipped_rows = turn.skipped_rows;
   Object result(THPVariable_Wrap(output));
   if (result.held == nullptr) return nullptr;
   const int status = target.call(&args, launched);
   return status != LL_OK ? PyLong_FromLong(status) : result.release();
+}
+
+// (entry, stream, device, key_buffer, value_buffer, key_scales, value_scales,
+// scale_block, source slots, destination slots, local positions, global positions,
+// table, rotary_dim, neox, prefix, repair mask, skipped) -> True
+PyObject *quantized_link(PyObject *const *a, Py_ssize_t n, bool *launched) {
+  Target target;
+  Pool pool;
+  if (n != 18 || !target.read(a) || !pool.read(a + 3) || !target.takes(*pool.tensors[0]) || !pool.apart()) return none();
+  ll_quantized_link_args args;
+  memset(&args, 0, sizeof(args));
+  const at::Device device = pool.tensors[0]->device();
+  std::array<const at::Tensor *, 4> maps{};
+  for (int i = 0; i < 4; ++i) {
+    maps[i] = plain(a[8 + i]);
+    if (maps[i] == nullptr || !vector_ok(maps[i], maps[0]->numel(), device) || pool.meets(maps[i])) return none();
+  }
+  args.slots_dtype = index_code(maps[0]->scalar_type());
+  args.positions_dtype = index_code(maps[2]->scalar_type());
+  if (args.slots_dtype < 0 || args.positions_dtype < 0 || maps[1]->scalar_type() != maps[0]->scalar_type() ||
+      maps[3]->scalar_type() != maps[2]->scalar_type())
+    return none();
+  const int64_t tokens = maps[0]->numel();
+  const at::Tensor *table = plain(a[12]);
+  int64_t rotary = 0, prefix = 0;
+  if (tokens == 0 || !integer(a[13], &rotary) || rotary < 16 || rotary % 16 != 0 || rotary > pool.args.head_dim ||
+      (a[14] != Py_True && a[14] != Py_False) || !integer(a[15], &prefix) || prefix < 0 || prefix > tokens)
+    return none();
+  if (table == nullptr || table->dim() != 2 || table->size(1) < rotary || table->device() != device ||
+      table->stride(1) != 1 || pool.meets(table))
+    return none();
+  args.cos_sin_dtype = float_code(table->scalar_type());
+  if (args.cos_sin_dtype < 0) return none();
+  const at::Tensor *mask = nullptr;
+  if (a[16] != Py_None) {
+    mask = plain(a[16]);
+    if (!vector_ok(mask, tokens, device) || (mask->scalar_type() != at::kBool && mask->scalar_type() != at::kByte) ||
+        pool.meets(mask))
+      return none();
+    args.repair_mask = static_cast<const uint8_t *>(mask->data_ptr());
+  }
+  if (a[17] != Py_None) {
+    const at::Tensor *skipped = plain(a[17]);
+    if (skipped == nullptr || skipped->scalar_type() != at::kLong || skipped->numel() != 1 ||
+        skipped->device() != device || pool.meets(skipped) || overlap(*skipped, *table) ||
+        (mask != nullptr && overlap(*skipped, *mask)))
+      return none();
+    for (const at::Tensor *map : maps)
+      if (overlap(*skipped, *map)) return none();
+    args.skipped_rows = static_cast<int64_t *>(skipped->data_ptr());
+  }
+  if (target.entry == 0) Py_RETURN_TRUE;
+  args.struct_size = sizeof(args);
+  args.pool = pool.args;
+  args.num_tokens = tokens;
+  args.source_slots = maps[0]->data_ptr();
+  args.destination_slots = maps[1]->data_ptr();
+  args.local_positions = maps[2]->data_ptr();
+  args.global_positions = maps[3]->data_ptr();
+  args.prefix_token_count = prefix;
+  args.cos_sin_cache = table->data_ptr();
+  args.cos_sin_rows = table->size(0);
+  args.cos_sin_cols = table->size(1);
+  args.cos_sin_stride_row = table->stride(0);
+  args.rotary_dim = rotary;
+  args.is_neox_style = a[14] == Py_True;
+  const int status = target.call(&args, launched);
+  if (status != LL_OK) return PyLong_FromLong(status);
+  Py_RETURN_TRUE;
+}
+
+// (entry, stream, device, key_buffer, value_buffer, key_scales, value_scales,
+// scale_block, slots, type code) -> (keys, values)
+PyObject *quantized_load(PyObject *const *a, Py_ssize_t n, bool *launched) {
+  Target target;
+  Pool pool;
+  if (n != 10 || !target.read(a) || !pool.read(a + 3) || !target.takes(*pool.tensors[0])) return none();
+  ll_quantized_load_args args;
+  memset(&args, 0, sizeof(args));
+  args.num_rows = pool.args.num_slots;
+  if (a[8] != Py_None) {
+    const at::Tensor *slots = plain(a[8]);
+    if (slots == nullptr || !vector_ok(slots, slots->numel(), pool.tensors[0]->device())) return none();
+    args.slots_dtype = index_code(slots->scalar_type());
+    if (args.slots_dtype < 0) return none();
+    args.slots = slots->data_ptr();
+    args.num_rows = slots->numel();
+  }
+  if (!integer(a[9], &args.dtype)) return none();
+  at::ScalarType type;
+  if (args.dtype == LL_DTYPE_FLOAT16) type = at::kHalf;
+  else if (args.dtype == LL_DTYPE_BFLOAT16) type = at::kBFloat16;
+  else if (args.dtype == LL_DTYPE_FLOAT32) type = at::kFloat;
+  else return none();
+  if (target.entry == 0) Py_RETURN_TRUE;
+  const auto options = pool.tensors[0]->options().dtype(type);
+  const at::Tensor keys = at::empty({args.num_rows, pool.args.num_kv_heads, pool.args.head_dim}, options);
+  const at::Tensor values = at::empty({args.num_rows, pool.args.num_kv_heads, pool.args.head_dim}, options);
+  args.struct_size = sizeof(args);
+  args.pool = pool.args;
+  args.key_output = keys.data_ptr();
+  args.value_output = values.data_ptr();
+  Object first(THPVariable_Wrap(keys)), second(THPVariable_Wrap(values));
+  if (first.held == nullptr || second.held == nullptr) return nullptr;
+  Object both(PyTuple_Pack(2, first.held, second.held));
+  if (both.held == nullptr) return nullptr;
+  const int status = target.call(&args, launched);
+  return status != LL_OK ? PyLong_FromLong(status) : both.release();
+}
+
+// (entry, stream, device, workspace entry, query, key_buffer, value_buffer,
+// key_scales, value_scales, scale_block, page_table, kv_lengths, page_size,
+// query_starts, scale) -> output
+PyObject *quantized_attention(PyObject *const *a, Py_ssize_t n, bool *launched) {
+  Target target;
+  int64_t workspace_entry = 0;
+  Pool pool;
+  if (n != 15 || !target.read(a) || !integer(a[3], &workspace_entry) || !pool.read(a + 5)) return none();
+  const at::Tensor *query = plain(a[4]);
+  ll_quantized_attention_args args;
+  memset(&args, 0, sizeof(args));
+  if (!read_paged(query, pool.tensors[0], pool.tensors[1], a + 10, &args.paged) || !target.takes(*query)) return none();
+  if (pool.args.scale_block < 16 || args.paged.page_size % pool.args.scale_block != 0) return none();
+  if (target.entry == 0) Py_RETURN_TRUE;
+  args.struct_size = sizeof(args);
+  args.key_scales = pool.args.key_scales;
+  args.value_scales = pool.args.value_scales;
+  args.scale_block = pool.args.scale_block;
+  return attend(target, workspace_entry, *query, &args, &args.paged, launched);
 }
 
 // No C++ exception leaves a call.  What fails before the library's entry is called,
@@ -438,6 +707,10 @@ PyMethodDef methods[] = {
     {"rotate_heads", entry<rotate_heads>(), METH_FASTCALL, "rotate_heads in one call, or None"},
     {"append", entry<append>(), METH_FASTCALL, "append_rotated_kv_inplace in one call, or None"},
     {"paged_attention", entry<paged_attention>(), METH_FASTCALL, "paged_attention in one call, or None"},
+    {"quantized_append", entry<quantized_append>(), METH_FASTCALL, "append_quantized_kv_inplace in one call, or None"},
+    {"quantized_link", entry<quantized_link>(), METH_FASTCALL, "link_quantized_kv_inplace in one call, or None"},
+    {"quantized_load", entry<quantized_load>(), METH_FASTCALL, "load_quantized_kv in one call, or None"},
+    {"quantized_attention", entry<quantized_attention>(), METH_FASTCALL, "quantized_paged_attention in one call, or None"},
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -451,7 +724,11 @@ PyMODINIT_FUNC PyInit__step_calls(void) {
   if (created == nullptr) return nullptr;
   if (PyModule_AddStringConstant(created, "TORCH_VERSION", TORCH_VERSION) != 0 ||
       PyModule_AddIntConstant(created, "HEAD_ROTARY_ARGS_SIZE", sizeof(ll_head_rotary_args)) != 0 ||
-      PyModule_AddIntConstant(created, "PAGED_ATTENTION_ARGS_SIZE", sizeof(ll_paged_attention_args)) != 0) {
+      PyModule_AddIntConstant(created, "PAGED_ATTENTION_ARGS_SIZE", sizeof(ll_paged_attention_args)) != 0 ||
+      PyModule_AddIntConstant(created, "QUANTIZED_APPEND_ARGS_SIZE", sizeof(ll_quantized_append_args)) != 0 ||
+      PyModule_AddIntConstant(created, "QUANTIZED_LINK_ARGS_SIZE", sizeof(ll_quantized_link_args)) != 0 ||
+      PyModule_AddIntConstant(created, "QUANTIZED_LOAD_ARGS_SIZE", sizeof(ll_quantized_load_args)) != 0 ||
+      PyModule_AddIntConstant(created, "QUANTIZED_ATTENTION_ARGS_SIZE", sizeof(ll_quantized_attention_args)) != 0) {
     Py_DECREF(created);
     return nullptr;
   }

@@ -878,9 +878,12 @@ def step_calls():
         from . import _step_calls as module
     except ImportError:
         return None
-    built_for = tuple(getattr(module, name, None)
-                      for name in ("TORCH_VERSION", "HEAD_ROTARY_ARGS_SIZE", "PAGED_ATTENTION_ARGS_SIZE"))
-    here = (torch.__version__.split("+")[0], ctypes.sizeof(HeadRotaryArgs), ctypes.sizeof(PagedAttentionArgs))
+    blocks = {"HEAD_ROTARY": HeadRotaryArgs, "PAGED_ATTENTION": PagedAttentionArgs,
+              "QUANTIZED_APPEND": QuantizedAppendArgs, "QUANTIZED_LINK": QuantizedLinkArgs,
+              "QUANTIZED_LOAD": QuantizedLoadArgs, "QUANTIZED_ATTENTION": QuantizedAttentionArgs}
+    built_for = (getattr(module, "TORCH_VERSION", None),
+                 *(getattr(module, f"{name}_ARGS_SIZE", None) for name in blocks))
+    here = (torch.__version__.split("+")[0], *(ctypes.sizeof(block) for block in blocks.values()))
     return module if built_for == here else None
 
 

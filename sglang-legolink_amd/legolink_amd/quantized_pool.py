@@ -48,8 +48,23 @@ _INDEX_DTYPES = {torch.int32: _native.DTYPE_INT32, torch.int64: _native.DTYPE_IN
 _MOST_BLOCK = 128
 
 
+# Each call in one native call where it takes it; the Python checks take the others,
+# and name the reason where a call must not run.
+_calls = _native.step_calls()
+
+
 class QuantizedPoolError(RuntimeError):
     """A call over an 8-bit pool that must not run."""
+
+
+def _native_call(call, name: str, *arguments):
+    """What the native call made of it: its result, or None where it did not take it."""
+
+    device = torch._C._cuda_getDevice()
+    done = call(_native.entry_address(name), torch._C._cuda_getCurrentRawStream(device), device, *arguments)
+    if type(done) is int:
+        _native.check_status(done)
+    return done
 
 
 def _refuse_gradients(*tensors: Optional[torch.Tensor]) -> None:
@@ -188,6 +203,13 @@ def append_quantized_kv_inplace(*, key_buffer: torch.Tensor, value_buffer: torch
     multiple of 16.
     """
 
+    if _calls is not None and query.is_cuda:
+        done = _native_call(_calls.quantized_append, "ll_quantized_append", query, key, positions, cos_sin_cache,
+                            rotary_dim, is_neox_style, query_norm_weight, key_norm_weight, norm_eps, skipped_rows,
+                            query_output, value, destination_slots, key_buffer, value_buffer, key_scales, value_scales,
+                            scale_block)
+        if done is not None:
+            return done
     _refuse_gradients(query, key, value, query_norm_weight, key_norm_weight, cos_sin_cache, query_output, key_buffer,
                       value_buffer, key_scales, value_scales)
     block = _check_pool(key_buffer, value_buffer, key_scales, value_scales, scale_block)
@@ -271,6 +293,11 @@ def link_quantized_kv_inplace(*, key_buffer: torch.Tensor, value_buffer: torch.T
     ``skipped_rows``; a negative destination is padding.
     """
 
+    if _calls is not None and key_buffer.is_cuda:
+        if _native_call(_calls.quantized_link, "ll_quantized_link", key_buffer, value_buffer, key_scales, value_scales,
+                        scale_block, source_slots, destination_slots, local_positions, global_positions, cos_sin_cache,
+                        rotary_dim, is_neox_style, prefix_token_count, repair_mask, skipped_rows) is not None:
+            return
     _refuse_gradients(key_buffer, value_buffer, key_scales, value_scales, cos_sin_cache)
     block = _check_pool(key_buffer, value_buffer, key_scales, value_scales, scale_block)
     device, tokens = key_buffer.device, int(source_slots.numel())
@@ -312,6 +339,11 @@ def load_quantized_kv(key_buffer: torch.Tensor, value_buffer: torch.Tensor, key_
     dim], new or ``key_output`` and ``value_output`` filled.  A slot outside the
     pool gives zeros."""
 
+    if _calls is not None and key_output is None and value_output is None and key_buffer.is_cuda:
+        done = _native_call(_calls.quantized_load, "ll_quantized_load", key_buffer, value_buffer, key_scales,
+                            value_scales, scale_block, slots, _FLOAT_DTYPES.get(dtype))
+        if done is not None:
+            return done
     _refuse_gradients(key_buffer, value_buffer, key_scales, value_scales, key_output, value_output)
     block = _check_pool(key_buffer, value_buffer, key_scales, value_scales, scale_block)
     device = key_buffer.device
@@ -360,6 +392,13 @@ def quantized_paged_attention(query: torch.Tensor, key_buffer: torch.Tensor, val
     captures the call).
     """
 
+    if _calls is not None and output is None and query.is_cuda:
+        done = _native_call(_calls.quantized_attention, "ll_quantized_attention",
+                            _native.entry_address("ll_quantized_attention_workspace_bytes"), query, key_buffer,
+                            value_buffer, key_scales, value_scales, scale_block, page_table, kv_lengths, page_size,
+                            query_starts, scale)
+        if done is not None:
+            return done
     _refuse_gradients(query, key_buffer, value_buffer, key_scales, value_scales, output)
     block = _check_pool(key_buffer, value_buffer, key_scales, value_scales, scale_block)
     device, dtype = key_buffer.device, query.dtype
