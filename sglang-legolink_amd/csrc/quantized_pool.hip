@@ -48,9 +48,8 @@ constexpr int kWave = 64;
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int kMaxBlock = 128;
-constexpr int kMostWindow = 16;
+constexpr int kMostWindow = 64;
 constexpr int kHeldSteps = 2;  // of 64 / kGroup rows, in a wave's registers
-constexpr long long kMostTogether = 4096;  // waves of queries that go with the runs
 
 int fail(int code, const char *fmt, ...) {
   va_list ap;
@@ -433,28 +432,101 @@ __global__ void __launch_bounds__(kThreads) quantized_query_kernel(const PoolPar
   turn_queries<E, kGroup>(p, blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
 }
 
+// Bits of rows: of up to 32 (kWords 0), 64 or 128.
+template <int kWords>
+struct RowBits {
+  unsigned long long words[kWords];
+
+  __device__ void set(int word, unsigned long long bits) { words[word] = bits; }
+  __device__ bool at(int row) const {
+    unsigned long long word = words[0];
+    if (kWords > 1 && row >= kWave) word = words[kWords - 1];
+    return ((word >> (row % kWave)) & 1ull) != 0;
+  }
+  // The last one up to `row` (0: none).
+  __device__ int last_to(int row) const {
+    const unsigned long long up_to = (2ull << (row % kWave)) - 1;
+    if (kWords > 1 && row >= kWave) {
+      const unsigned long long high = words[kWords - 1] & up_to;
+      if (high != 0) return 2 * kWave - 1 - __builtin_clzll(high);
+      return words[0] == 0 ? 0 : kWave - 1 - __builtin_clzll(words[0]);
+    }
+    const unsigned long long low = words[0] & up_to;
+    return low == 0 ? 0 : kWave - 1 - __builtin_clzll(low);
+  }
+  // The first one from `row` on (64 kWords: none).
+  __device__ int first_from(int row) const {
+    if (row >= kWords * kWave) return kWords * kWave;
+    const unsigned long long from = ~0ull << (row % kWave);
+    if (kWords > 1 && row >= kWave) {
+      const unsigned long long high = words[kWords - 1] & from;
+      return high == 0 ? 2 * kWave : kWave + __builtin_ctzll(high);
+    }
+    const unsigned long long low = words[0] & from;
+    if (low != 0) return __builtin_ctzll(low);
+    if (kWords > 1 && words[kWords - 1] != 0) return kWave + __builtin_ctzll(words[kWords - 1]);
+    return kWords * kWave;
+  }
+  // How many of [begin, end).
+  __device__ int count(int begin, int end) const {
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      const int from = max(begin - w * kWave, 0), to = min(end - w * kWave, kWave);
+      if (from >= to) continue;
+      const unsigned long long below = to == kWave ? ~0ull : (1ull << to) - 1;
+      sum += __builtin_popcountll(words[w] & below & (~0ull << from));
+    }
+    return sum;
+  }
+};
+
+template <>
+struct RowBits<0> {
+  uint32_t word;
+
+  __device__ void set(int, unsigned long long bits) { word = static_cast<uint32_t>(bits); }
+  __device__ bool at(int row) const { return ((word >> row) & 1u) != 0; }
+  __device__ int last_to(int row) const {
+    const uint32_t low = word & ((2u << row) - 1u);
+    return low == 0 ? 0 : 31 - __builtin_clz(low);
+  }
+  __device__ int first_from(int row) const {
+    const uint32_t low = row >= 32 ? 0u : word & (~0u << row);
+    return low == 0 ? 32 : __builtin_ctz(low);
+  }
+  __device__ int count(int begin, int end) const {
+    if (begin >= end) return 0;
+    return __builtin_popcount((word >> begin) & (~0u >> (32 - (end - begin))));
+  }
+};
+
 // Writes runs of rows.  A pair is one head's keys or values; kParts waves of a
-// workgroup hold a pair's run, two steps of 64 / kGroup rows each.
+// workgroup hold up to kRunRows rows of it at a time, two steps of 64 / kGroup rows
+// each: as many of the window's runs as fit whole (one of a prompt's blocks, or many
+// single tokens').
 //
 // A call is bound by memory, or for few rows by the chain slot -> row and angle -> code.
 // So what there is to know of the window's tokens is read at once, each row's loads do
-// not wait for its angles, and a run's angles are made once for the workgroup's heads
+// not wait for its angles, and the rows' angles are made once for the workgroup's heads
 // and kept in LDS (a link's are four table rows' worth of products; every head by
 // itself would read 1 KB of table for 256 bytes of codes).  LDS has the angles of
 // lane i's pair j as element 9 R row + R j + i, R = rotary lanes of a row, so that 16
 // lanes' 16-byte reads meet every bank once.
 template <typename Source, typename E, int kGroup, int kParts, bool kQueries>
-__global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts <= 2 ? 4 : kParts <= 8 ? 3 : 1) quantized_write_kernel(const PoolParams p) {
+__global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts <= 2 ? 4 : kParts <= 8 ? 3 : 1)
+    quantized_write_kernel(const PoolParams p) {
   constexpr int kWaves = kParts > 4 ? kParts : kThreads / kWave;
   constexpr int kPairs = kWaves / kParts;  // of a workgroup
   constexpr int kRows = kWave / kGroup;    // of a step
   constexpr int kSteps = kHeldSteps;
-  constexpr int kHeldRows = kSteps * kRows;  // of a run, in one wave's registers
+  constexpr int kHeldRows = kSteps * kRows;  // of a wave
   constexpr int kRunRows = kParts * kHeldRows;
   constexpr int kWords = (kRunRows + kWave - 1) / kWave;
   constexpr bool kShares = kPairs > 1;
   constexpr int kTokens = 1 + kMostWindow + kRunRows;  // the one before the window, the window, a run from its last on
-  __shared__ float most_of[kPairs][kParts];
+  typedef RowBits<kRunRows <= 32 ? 0 : kWords> Bits;
+  __shared__ unsigned most_of[kPairs][kRunRows];  // of a run, at its first row: a float's bits
   __shared__ Token tokens[kTokens];
   __shared__ Angle shared_angles[kShares ? kRunRows * 9 * kGroup : 1];
   __shared__ float key_weights[Source::kNorms ? 16 * kGroup : 1];
@@ -471,7 +543,8 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts
   const unsigned window = group / static_cast<unsigned>(p.pair_groups);
   const int pair_group = static_cast<int>(group % static_cast<unsigned>(p.pair_groups));
   const long long t0 = static_cast<long long>(window) * p.window - 1;  // of tokens[0]
-  const int pair = pair_group * kPairs + wave / kParts;
+  const int own_pair = wave / kParts;  // of the workgroup's
+  const int pair = pair_group * kPairs + own_pair;
   const int part = wave % kParts;
   const bool has_pair = pair < 2 * p.hkv;
   const bool is_key = pair < p.hkv;
@@ -491,73 +564,87 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts
     for (int i = threadIdx.x; i < p.dim; i += kWaves * kWave)
       key_weights[i] = p.key_weight != nullptr ? value_at(p.key_weight, p.weight_dtype, i) : 1.f;
   __syncthreads();
-  // A run begins where the block changes.
   auto block_of = [&](int i) { return tokens[i].slot < 0 ? -1 : tokens[i].slot >> p.block_shift; };
-  const int in_window = min(lane, p.window);
-  const int mine = block_of(in_window), former = block_of(max(in_window - 1, 0));
-  unsigned long long begins =
-      __builtin_amdgcn_ballot_w64(lane >= 1 && lane <= p.window && mine >= 0 && mine != former);
+  // A run begins where the block changes.  Bit l: token 1 + l of those here.
+  unsigned long long begins;
+  {
+    const int block = block_of(1 + min(lane, p.window - 1));
+    begins = __builtin_amdgcn_ballot_w64(lane < p.window && block >= 0 && block != block_of(min(lane, p.window - 1)));
+  }
   while (begins != 0) {
-    const int start = __builtin_ctzll(begins);
-    begins &= begins - 1;
-    const int block = __builtin_amdgcn_readlane(mine, start);
-    // Its rows that are written.
-    unsigned long long written[kWords];
-    int count = 0;
-    bool more = true;
+    const int first = 1 + __builtin_ctzll(begins);  // token of row 0
+    // The rows from there on: those of a block, those that begin a run, those written.
+    Bits member, begin, written, bounds;  // (bounds: those that belong to no run before them)
+    int stop = kRunRows;  // behind the last run that begins in the window
+    bool ends = true;     // row kRunRows, too, is of another run
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      const int row = min(w * kWave + lane, kRunRows - 1);
+      const bool exists = w * kWave + lane < kRunRows;
+      const int block = block_of(first + row);
+      const bool starts = block >= 0 && (row == 0 || block != block_of(first + row - 1));
+      member.set(w, __builtin_amdgcn_ballot_w64(exists && block >= 0));
+      begin.set(w, __builtin_amdgcn_ballot_w64(exists && starts));
+      written.set(w, __builtin_amdgcn_ballot_w64(exists && tokens[first + row].from >= 0));
+      bounds.set(w, __builtin_amdgcn_ballot_w64(exists && (starts || block < 0)));
+      const unsigned long long out =
+          __builtin_amdgcn_ballot_w64(exists && first + row > p.window && (starts || block < 0));
+      if (stop == kRunRows && out != 0) stop = w * kWave + __builtin_ctzll(out);
+    }
+    {
+      const int next = block_of(first + kRunRows), last = block_of(first + kRunRows - 1);
+      ends = next < 0 || next != last;
+    }
+    // (A run that goes on past the last row is left to the next turn, unless it is the
+    // only one: blocks have no more than kRunRows rows.)
+    if (stop == kRunRows && !ends) {
+      const int last = begin.last_to(kRunRows - 1);
+      if (last > 0) stop = last;
+    }
+    begins = first - 1 + stop >= kWave ? 0ull : begins & (~0ull << (first - 1 + stop));
+    auto end_of = [&](int row) { return min(bounds.first_from(row + 1), stop); };  // of the run of a row
+
+    // Lane r: row r's run and its scale.
+    unsigned old[kWords];
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
       const int row = w * kWave + lane;
-      const bool own = row < block_rows && block_of(start + min(row, kRunRows - 1)) == block;
-      const unsigned long long same = __builtin_amdgcn_ballot_w64(own);
-      const int length = !more ? 0 : same == ~0ull ? kWave : __builtin_ctzll(~same);
-      more = length == kWave;
-      written[w] = __builtin_amdgcn_ballot_w64(own && lane < length && tokens[start + min(row, kRunRows - 1)].from >= 0);
-      count += __builtin_popcountll(written[w]);
+      old[w] = 0u;
+      if (has_pair && row < stop && member.at(row))
+        old[w] = half.scales[static_cast<long long>(block_of(first + row)) * p.hkv + head];
     }
-    if (count == 0) continue;
-    uint8_t *scale_at = half.scales + static_cast<long long>(block) * p.hkv + head;
-    unsigned old = has_pair ? *scale_at : 0u;
-    // The rows of this part that are written (kHeldRows bits).
-    auto part_of = [&](const unsigned long long *words) {
-      unsigned bits = 0;
-#pragma unroll
-      for (int w = 0; w < kWords; ++w)
-        if (part * kHeldRows / kWave == w) bits = static_cast<unsigned>(words[w] >> (part * kHeldRows % kWave));
-      return bits;
-    };
-    const unsigned own_rows = part_of(written);
-    auto held_of = [&](int step) { return step * kRows + lane / kGroup; };  // of the part's rows
-    auto token_of = [&](int step) { return start + part * kHeldRows + held_of(step); };
-    auto has_row = [&](int step) { return has_pair && l.active && ((own_rows >> held_of(step)) & 1u) != 0; };
+    if (part == 0)
+      for (int row = lane; row < kRunRows; row += kWave) most_of[own_pair][row] = 0u;
 
+    auto held_of = [&](int step) { return part * kHeldRows + step * kRows + lane / kGroup; };
+    auto token_of = [&](int step) { return first + held_of(step); };
+    bool has[kSteps];
     typename Source::Raw raw[kSteps];
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
+      has[step] = has_pair && l.active && held_of(step) < stop && written.at(held_of(step));
       raw[step] = typename Source::Raw{};
-      if (has_row(step)) raw[step] = Source::fetch(p, half, is_key, head, t0 + token_of(step), tokens[token_of(step)], l);
+      if (has[step]) raw[step] = Source::fetch(p, half, is_key, head, t0 + token_of(step), tokens[token_of(step)], l);
     }
     const int lanes = p.rotary / 16;
     if constexpr (kShares) {
       if (pair_group * kPairs < p.hkv) {  // (keys among its pairs)
-        const int quads = 2 * lanes;  // of four pairs, a row's
-        for (int i = threadIdx.x; i < kRunRows * quads; i += kWaves * kWave) {
+        const int quads = 2 * lanes;      // of four pairs, a row's
+        for (int i = threadIdx.x; i < stop * quads; i += kWaves * kWave) {
           const int row = i / quads, quad = i - row * quads;
-          if (((written[kWords - 1] >> row) & 1ull) == 0 || tokens[start + row].position < 0) continue;
+          if (!written.at(row) || tokens[first + row].position < 0) continue;
           Angle four[4];
-          Source::angles(p, tokens[start + row], 4 * quad, four);
+          Source::angles(p, tokens[first + row], 4 * quad, four);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            shared_angles[(9 * row + 4 * (quad % 2) + j) * lanes + quad / 2] = four[j];
+          for (int j = 0; j < 4; ++j) shared_angles[(9 * row + 4 * (quad % 2) + j) * lanes + quad / 2] = four[j];
         }
       }
-      __syncthreads();
     }
+    __syncthreads();
     float a[kSteps][8], b[kSteps][8];
-    float most = 0.f;
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      if (__builtin_amdgcn_ballot_w64(has_row(step)) == 0) continue;
+      if (__builtin_amdgcn_ballot_w64(has[step]) == 0) continue;
       Source::unpack(raw[step], a[step], b[step]);
       if (is_key) {
         const bool normed = Source::kNorms && p.key_weight != nullptr;
@@ -574,9 +661,9 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts
           scale = 1.0 / sqrt(sum / static_cast<double>(p.dim) + p.eps);
         }
         const Token &k = tokens[token_of(step)];
-        const bool turns = has_row(step) && l.rotates && k.position >= 0;
+        const bool turns = has[step] && l.rotates && k.position >= 0;
         Angle made[kShares ? 1 : 8];
-        const Angle *from = shared_angles + 9 * (part * kHeldRows + held_of(step)) * lanes + l.i;
+        const Angle *from = shared_angles + 9 * held_of(step) * lanes + l.i;
         if constexpr (!kShares) {
           if (turns) {
             Source::angles(p, k, 8 * l.i, made);
@@ -584,8 +671,8 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts
           }
         }
         // A pair of dims, at these places of the row: normed, turned and rounded.
-        auto pair_of = [&](int j, float &first, float &second, int at, int other, bool turned) {
-          double x = first, y = second;
+        auto pair_of = [&](int j, float &one, float &two, int at, int other, bool turned) {
+          double x = one, y = two;
           if (Source::kNorms) {  // (weights of 1 under a scale of 1 without a norm)
             x = x * scale * key_weights[at];
             y = y * scale * key_weights[other];
@@ -596,8 +683,8 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts
             x = lo * angle.cos - hi * angle.sin;
             y = hi * angle.cos + lo * angle.sin;
           }
-          first = to_odd(x);
-          second = to_odd(y);
+          one = to_odd(x);
+          two = to_odd(y);
           if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // (few doubles at a time)
         };
         if (turns && p.neox != 0) {
@@ -617,74 +704,97 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts
           }
         }
       }
-      if (has_row(step)) {
+      float most = 0.f;
+      if (has[step]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(finite_size(a[step][j]), finite_size(b[step][j])));
       }
+#pragma unroll
+      for (int apart = 1; apart < kGroup; apart *= 2) most = fmaxf(most, __shfl_xor(most, apart));
+      if (has[step] && l.i == 0)
+        atomicMax(&most_of[own_pair][begin.last_to(held_of(step))], __float_as_uint(most));
     }
 #pragma unroll
-    for (int step = 1; step < kWave; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
-    if constexpr (kParts > 1) {
-      if (lane == 0) most_of[wave / kParts][part] = most;
-      asm volatile("" : "+v"(old));  // read before part 0 may write it
-      __syncthreads();
+    for (int w = 0; w < kWords; ++w) asm volatile("" : "+v"(old[w]));  // read before another wave may write it
+    if constexpr (kParts > 1) __syncthreads();
+    unsigned byte[kWords];
+    Bits grown;
 #pragma unroll
-      for (int v = 0; v < kParts; ++v) most = fmaxf(most, most_of[wave / kParts][v]);
+    for (int w = 0; w < kWords; ++w) {
+      const int row = min(w * kWave + lane, kRunRows - 1);
+      const bool exists = has_pair && w * kWave + lane < stop && member.at(row);
+      const int from = begin.last_to(row);
+      const int count = exists ? written.count(from, end_of(row)) : 0;
+      const unsigned need = byte_for(__uint_as_float(most_of[own_pair][from]));
+      byte[w] = count == 0 ? old[w] : count == block_rows ? need : max(old[w], need);
+      if (exists && part == 0 && row == from && byte[w] != old[w])
+        half.scales[static_cast<long long>(block_of(first + row)) * p.hkv + head] = static_cast<uint8_t>(byte[w]);
+      grown.set(w, __builtin_amdgcn_ballot_w64(exists && row == from && count < block_rows && byte[w] > old[w]));
     }
-    if (begins != 0) __syncthreads();  // (the next run writes most_of and the angles)
-    if (!has_pair) continue;
-    const unsigned need = byte_for(most);
-    const unsigned byte = count == block_rows ? need : max(old, need);
-    if (part == 0 && lane == 0 && byte != old) *scale_at = static_cast<uint8_t>(byte);
-    const float inverse = inverse_of(byte);
+    auto of_row = [&](const unsigned *values, int row) {  // lane r's value
+      unsigned value = static_cast<unsigned>(__shfl(static_cast<int>(values[0]), row % kWave));
+      if (kWords > 1) {
+        const unsigned high = static_cast<unsigned>(__shfl(static_cast<int>(values[kWords - 1]), row % kWave));
+        value = row >= kWave ? high : value;
+      }
+      return value;
+    };
     auto codes_at = [&](int slot) { return half.codes + (static_cast<long long>(slot) * p.hkv + head) * p.dim; };
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      if (!has_row(step)) continue;
+      const float inverse = inverse_of(of_row(byte, held_of(step)));
+      if (!has[step]) continue;
       uint8_t *dst = codes_at(tokens[token_of(step)].slot);
       *reinterpret_cast<u32x2 *>(dst + l.first) = encode8(a[step], inverse);
       *reinterpret_cast<u32x2 *>(dst + l.second) = encode8(b[step], inverse);
     }
-    if (byte <= old || count == block_rows) continue;
-    // The block's other rows, under the scale that has grown.
-    unsigned long long taken[kWords];
+    // The other rows of blocks whose scale has grown.
+    for (int run = grown.first_from(0); run < kRunRows; run = grown.first_from(run + 1)) {
+      const int run_end = end_of(run), block = block_of(first + run);
+      unsigned long long offsets[kWords];  // that are written
 #pragma unroll
-    for (int w = 0; w < kWords; ++w) taken[w] = 0;
+      for (int w = 0; w < kWords; ++w) offsets[w] = 0;
 #pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      const bool own = ((written[w] >> lane) & 1ull) != 0;
-      const int offset = own ? tokens[start + w * kWave + lane].slot & (block_rows - 1) : 0;
+      for (int w = 0; w < kWords; ++w) {
+        const int row = w * kWave + lane;
+        const bool own = row >= run && row < run_end && written.at(min(row, kRunRows - 1));
+        const int offset = own ? tokens[first + min(row, kRunRows - 1)].slot & (block_rows - 1) : 0;
 #pragma unroll
-      for (int v = 0; v < kWords; ++v) {
-        unsigned long long bits = own && offset / kWave == v ? 1ull << (offset % kWave) : 0ull;
+        for (int v = 0; v < kWords; ++v) {
+          unsigned long long bits = own && offset / kWave == v ? 1ull << (offset % kWave) : 0ull;
 #pragma unroll
-        for (int step = 1; step < kWave; step *= 2) bits |= __shfl_xor(bits, step);
-        taken[v] |= bits;
+          for (int apart = 1; apart < kWave; apart *= 2) bits |= __shfl_xor(bits, apart);
+          offsets[v] |= bits;
+        }
       }
+      Bits taken;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) taken.set(w, offsets[w]);
+      const unsigned rise = of_row(byte, run) - of_row(old, run);
+      const float ratio = rise < 127u ? __uint_as_float((127u - rise) << 23) : 0.f;
+      u32x2 others[kSteps][2];
+      auto is_other = [&](int step) {
+        const int offset = held_of(step);
+        return offset < block_rows && l.active && !taken.at(min(offset, kRunRows - 1));
+      };
+      auto other_at = [&](int step) { return codes_at((block << p.block_shift) + held_of(step)); };
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+        if (is_other(step)) {
+          others[step][0] = *reinterpret_cast<const u32x2 *>(other_at(step) + l.first);
+          others[step][1] = *reinterpret_cast<const u32x2 *>(other_at(step) + l.second);
+        }
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+        if (is_other(step)) {
+          float values[8];
+          decode8(others[step][0], ratio, values);
+          *reinterpret_cast<u32x2 *>(other_at(step) + l.first) = encode8(values, 1.f);
+          decode8(others[step][1], ratio, values);
+          *reinterpret_cast<u32x2 *>(other_at(step) + l.second) = encode8(values, 1.f);
+        }
     }
-    const unsigned own_taken = part_of(taken);
-    const unsigned grown = byte - old;
-    const float ratio = grown < 127u ? __uint_as_float((127u - grown) << 23) : 0.f;
-    u32x2 others[kSteps][2];
-    auto is_other = [&](int step) {
-      return part * kHeldRows + held_of(step) < block_rows && ((own_taken >> held_of(step)) & 1u) == 0 && l.active;
-    };
-    auto other_at = [&](int step) { return codes_at((block << p.block_shift) + part * kHeldRows + held_of(step)); };
-#pragma unroll
-    for (int step = 0; step < kSteps; ++step)
-      if (is_other(step)) {
-        others[step][0] = *reinterpret_cast<const u32x2 *>(other_at(step) + l.first);
-        others[step][1] = *reinterpret_cast<const u32x2 *>(other_at(step) + l.second);
-      }
-#pragma unroll
-    for (int step = 0; step < kSteps; ++step)
-      if (is_other(step)) {
-        float values[8];
-        decode8(others[step][0], ratio, values);
-        *reinterpret_cast<u32x2 *>(other_at(step) + l.first) = encode8(values, 1.f);
-        decode8(others[step][1], ratio, values);
-        *reinterpret_cast<u32x2 *>(other_at(step) + l.second) = encode8(values, 1.f);
-      }
+    if (begins != 0) __syncthreads();  // (the next rows take most_of and the angles)
   }
 }
 
@@ -811,18 +921,22 @@ int launch_write(PoolParams &p, hipStream_t s) {
   constexpr int kWaves = kParts > 4 ? kParts : kThreads / kWave;
   constexpr int kPairs = kWaves / kParts;
   p.pair_groups = (2 * p.hkv + kPairs - 1) / kPairs;
-  // A window's runs are written one after another: single tokens are a run each, and
-  // a window each where that makes fewer waves than the card holds (16 a CU).
+  // A window's runs share a workgroup's turns.  It is as wide as a block (a prompt's
+  // runs then begin in one window each), or less where that makes fewer waves than one
+  // a SIMD (1,024 tokens linked: 7.0 us, and 10.7 with four waves a SIMD).
   const long long waves = p.num_tokens * 2 * p.hkv * kParts;
+  const int widest = std::min(kMostWindow, std::max(16, 1 << p.block_shift));
   p.window = 1;
-  while (p.window < kMostWindow && waves / p.window > 256 * 16) p.window *= 2;
+  while (p.window < widest && waves / p.window > 256 * 4) p.window *= 2;
   const long long run_groups = (p.num_tokens + p.window - 1) / p.window * p.pair_groups;
   p.run_groups = static_cast<unsigned>(std::min(run_groups, 0xffffffffll));
   const long long query_waves = p.num_tokens * p.query_steps;
   // The queries of a small call go with its runs in one launch.  Those of a large one
-  // are bound by memory, and go by themselves: the runs' registers leave room for two
-  // waves a SIMD.
-  const bool together = kQueries && query_waves <= kMostTogether;
+  // are bound by memory, and go by themselves: the runs' registers leave room for three
+  // or four waves a SIMD.  28/4 heads of 128, blocks of 16: 4,096 tokens (16,384 waves
+  // of queries) 23 us together and 32 apart, 8,192 44 and 48, 16,384 95 and 85; blocks
+  // of 64: 4,096 tokens 20 and 25, 8,192 49 and 46.
+  const bool together = kQueries && query_waves <= (kParts <= 2 ? 32768 : 16384);
   const long long groups = run_groups + (together ? (query_waves + kWaves - 1) / kWaves : 0);
   if (groups * (kWaves * kWave) > 0xffffffffll || query_waves * kWave > 0xffffff00ll)
     return fail(LL_ERR_INVALID_ARGUMENT, "too many rows for one launch");  // (fewer than 2^32 threads)
