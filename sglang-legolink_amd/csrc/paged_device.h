@@ -557,7 +557,8 @@ struct Launch {
 
 constexpr int kComputeUnits = 256;  // MI355X
 
-Launch plan_launch(const ll_paged_attention_args *a) {
+// `together`: KV heads that a workgroup of the narrow kernel takes.
+Launch plan_launch(const ll_paged_attention_args *a, int together = 1) {
   Launch x;
   const long long group = a->num_q_heads / a->num_kv_heads;
   const long long queries = a->num_queries, requests = a->num_requests;
@@ -582,7 +583,8 @@ Launch plan_launch(const ll_paged_attention_args *a) {
   // the least over.  Single tokens: where the tiles are few, as many units as run
   // at once; where they are many, two rounds, whose second the short ones fill (64
   // and 128 uneven requests: 390 and 212 us; one round 404 and 214, four 391 and 218).
-  const int places = std::max(1, kComputeUnits / static_cast<int>(a->num_kv_heads));
+  const int heads = static_cast<int>(a->num_kv_heads) / (x.wide ? 1 : together);
+  const int places = std::max(1, kComputeUnits / heads);
   x.target = x.wide                           ? places
              : 2 * x.max_tiles <= places ? places - static_cast<int>(x.max_tiles) + 1
                                          : 2 * places;

@@ -56,23 +56,30 @@ __device__ inline u32x2 decode4(uint32_t codes, float scale) {
 }
 
 // The keys of a list, by groups: the group's first row (-1: of no page of the pool),
-// and the scales of its keys and values for the head (bytes 0 and 1).
+// and the scales of its keys and values for each of the workgroup's heads (bytes 0 and 1).
+template <int kHeads>
 struct Group {
   int slot;
-  unsigned scales;
+  int scales[kHeads];
+  __device__ void clear() {
+    slot = -1;
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) scales[h] = 0x7f7f;
+  }
 };
 
-__device__ inline Group group_at(const QuantizedParams &p, const int *pages, int head, int key) {
+template <int kHeads>
+__device__ inline Group<kHeads> group_at(const QuantizedParams &p, const int *pages, int head, int key) {
   const unsigned first = static_cast<unsigned>(key);
   const unsigned page = static_cast<unsigned>((first * p.page_magic) >> p.page_shift);
   const int entry = pages[page];
-  Group g;
-  g.slot = -1;
-  g.scales = 0x7f7fu;
+  Group<kHeads> g;
+  g.clear();
   if (static_cast<unsigned>(entry) < static_cast<unsigned>(p.num_pages)) {
     g.slot = entry * p.page_size + static_cast<int>(first - page * p.page_size);
     const long long at = static_cast<long long>(g.slot >> p.block_shift) * p.hkv + head;
-    g.scales = p.k_scales[at] | static_cast<unsigned>(p.v_scales[at]) << 8;
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) g.scales[h] = p.k_scales[at + h] | p.v_scales[at + h] << 8;
   }
   return g;
 }
@@ -115,21 +122,22 @@ struct Narrow8 {
   }
 };
 
-template <int D, typename E>
+template <int D, typename E, int kHeads>
 __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(const QuantizedParams p) {
   typedef Narrow8<D> N;
   typedef typename E::frag frag;
   constexpr int kColumns = 16;
   constexpr int kPairs = D / 64;  // of the scores' steps
   constexpr int kBlocks = D / 16;
+  constexpr int kTurns = N::kWaves / kHeads;  // waves of a head
   constexpr int kPitch = D + 4;  // floats of a joined row: 16 lanes' 16-byte writes meet 64 banks
   constexpr int kShared = N::kWaves * (N::kRing > 16 * kPitch * 4 ? N::kRing : 16 * kPitch * 4);
   __shared__ __attribute__((aligned(16))) unsigned char rings[kShared];
-  __shared__ Group groups[N::kList / kGroupKeys];
+  __shared__ Group<kHeads> groups[N::kList / kGroupKeys];
   __shared__ float stats[N::kWaves][kColumns][2];
 
-  const int head = blockIdx.x % p.hkv;
-  const int unit = blockIdx.x / p.hkv;
+  const int first_head = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.hkv / kHeads)) * kHeads;
+  const int unit = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.hkv / kHeads));
   const Work w = find_work<Order::kByQuarter>(p, kColumns, unit);
   if (w.index < 0 || w.chunk >= w.chunks || (w.chunks > 1 && !partials_fit(p, w))) return;
   const int key_begin = w.chunk * w.chunk_keys;  // below the tile's key_end, or 0
@@ -141,6 +149,8 @@ __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(
   const int lane = tid % kWave;
   const int g = lane / 16;
   const int col = lane % 16;
+  const int own_head = wave / kTurns;  // of the workgroup's
+  const int head = first_head + own_head;
   unsigned char *ring = rings + wave * N::kRing;
 
   // The lane's column and its query.
@@ -208,10 +218,9 @@ __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(
     const int subs = (listed + N::kKeys - 1) / N::kKeys;
     __syncthreads();  // every wave is past the former list
     for (int i = tid; i < 2 * subs; i += N::kThreads) {
-      Group x;
-      x.slot = -1;
-      x.scales = 0x7f7fu;
-      if (i * kGroupKeys < listed) x = group_at(p, pages, head, list_begin + i * kGroupKeys);
+      Group<kHeads> x;
+      x.clear();
+      if (i * kGroupKeys < listed) x = group_at<kHeads>(p, pages, first_head, list_begin + i * kGroupKeys);
       groups[i] = x;
     }
     // The compiler does not count the gathers: nothing that it waits for in the
@@ -221,18 +230,17 @@ __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(
 
 #pragma unroll
     for (int s = 0; s < N::kStages; ++s)
-      if (wave + s * N::kWaves < subs) gather(wave + s * N::kWaves, s);
+      if (wave % kTurns + s * kTurns < subs) gather(wave % kTurns + s * kTurns, s);
     int stage = 0;
-    for (int sub = wave; sub < subs; sub += N::kWaves) {
+    for (int sub = wave % kTurns; sub < subs; sub += kTurns) {
       const int key0 = list_begin + sub * N::kKeys;
-      Group two[2] = {groups[2 * sub], groups[2 * sub + 1]};
       float k_scale[2], v_scale[2];
       unsigned valid = 0;  // keys that have a row and are not behind the list's last
       bool bad_scale[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int slot = __builtin_amdgcn_readfirstlane(two[i].slot);
-        const unsigned scales = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(two[i].scales)));
+        const int slot = __builtin_amdgcn_readfirstlane(groups[2 * sub + i].slot);
+        const unsigned scales = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(groups[2 * sub + i].scales[own_head]));
         k_scale[i] = uniform_scale(scales & 0xffu);
         v_scale[i] = uniform_scale(scales >> 8);
         bad_scale[i] = (scales >> 8) == 255u;
@@ -240,7 +248,7 @@ __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(
         if (slot >= 0) valid |= ((1u << rows) - 1u) << (16 * i);
       }
       // This stage's gathers are complete when at most the later stages' are outstanding.
-      const int later = min(N::kStages - 1, (subs - 1 - sub) / N::kWaves);
+      const int later = min(N::kStages - 1, (subs - 1 - sub) / kTurns);
       if (N::kStages == 4 && later == 3) wait_vm<3 * 2 * N::kGathers % 64>();
       else if (N::kStages == 4 && later == 2) wait_vm<2 * 2 * N::kGathers % 64>();
       else if (later >= 1) wait_vm<2 * N::kGathers>();
@@ -360,9 +368,8 @@ __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(
       while (odd != 0) {
         const int rel = __builtin_ctz(odd);
         odd &= odd - 1;
-        const Group x = groups[2 * sub + rel / 16];
-        const unsigned char *row = row_at(p, v_base, x.slot + rel % 16) + 4 * g;
-        const float scale = scale_of(x.scales >> 8);
+        const unsigned char *row = row_at(p, v_base, groups[2 * sub + rel / 16].slot + rel % 16) + 4 * g;
+        const float scale = scale_of(static_cast<unsigned>(groups[2 * sub + rel / 16].scales[own_head]) >> 8);
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
           const f32x4 x4 = nonfinite_only<E>(decode4<E>(*reinterpret_cast<const uint32_t *>(row + 16 * b), scale));
@@ -372,14 +379,13 @@ __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(
       }
       // The stage's reads are done: the gather kStages turns ahead takes it.
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (sub + N::kStages * N::kWaves < subs) gather(sub + N::kStages * N::kWaves, stage);
+      if (sub + N::kStages * kTurns < subs) gather(sub + N::kStages * kTurns, stage);
       stage = stage + 1 == N::kStages ? 0 : stage + 1;
     }
   }
 
   // The waves' results joined.
   const bool direct = w.chunks == 1;
-  float *partial = direct ? nullptr : partial_of<D>(p, kColumns, w.first_partial + w.chunk * w.partial_step, head);
   float *joined = reinterpret_cast<float *>(rings);
   __syncthreads();  // the rings are read
   const float total = sum_of_groups(l);
@@ -391,28 +397,32 @@ __global__ void __launch_bounds__(Narrow8<D>::kThreads) quantized_narrow_kernel(
   for (int b = 0; b < kBlocks; ++b)
     *reinterpret_cast<f32x4 *>(joined + (wave * 16 + col) * kPitch + 16 * b + 4 * g) = o[b];
   __syncthreads();
-  for (int i = tid; i < 16 * (D / 4); i += N::kThreads) {
-    const int c = i / (D / 4);
+  for (int i = tid; i < kHeads * 16 * (D / 4); i += N::kThreads) {
+    const int of_head = i / (16 * (D / 4));
+    const int first = of_head * kTurns;  // of the head's waves
+    const int c = i / (D / 4) % 16;
     const int quad = i % (D / 4);
     if ((w.tile * kColumns + c) / p.group >= w.request.q_len) continue;
-    float top = stats[0][c][0];
+    float top = stats[first][c][0];
 #pragma unroll
-    for (int v = 1; v < N::kWaves; ++v) top = fmaxf(top, stats[v][c][0]);
+    for (int v = 1; v < kTurns; ++v) top = fmaxf(top, stats[first + v][c][0]);
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
 #pragma unroll
-    for (int v = 0; v < N::kWaves; ++v) {
-      const float weight = joined_weight(stats[v][c][0], top, scale_log2);
-      sum += weight * stats[v][c][1];
-      acc += weight * *reinterpret_cast<const f32x4 *>(joined + (v * 16 + c) * kPitch + 4 * quad);
+    for (int v = 0; v < kTurns; ++v) {
+      const float weight = joined_weight(stats[first + v][c][0], top, scale_log2);
+      sum += weight * stats[first + v][c][1];
+      acc += weight * *reinterpret_cast<const f32x4 *>(joined + ((first + v) * 16 + c) * kPitch + 4 * quad);
     }
     if (direct) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
       u32x2 packed;
       packed[0] = E::pack(acc[0] * inv, acc[1] * inv);
       packed[1] = E::pack(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<u32x2 *>(output_row(p, w, head, w.tile * kColumns + c, D) + 4 * quad) = packed;
+      *reinterpret_cast<u32x2 *>(output_row(p, w, first_head + of_head, w.tile * kColumns + c, D) + 4 * quad) = packed;
     } else {
+      float *partial =
+          partial_of<D>(p, kColumns, w.first_partial + w.chunk * w.partial_step, first_head + of_head);
       *reinterpret_cast<f32x4 *>(partial + c * D + 4 * quad) = acc;
       if (quad == 0) {
         partial[kColumns * D + 2 * c] = top;
@@ -450,7 +460,9 @@ struct Wide8 {
   static constexpr int kList = 7168;                        // keys held at a time
   static_assert(kRows <= kGroupKeys && kGroupKeys % kRows == 0, "a share lies in one group");
   __host__ __device__ static constexpr int k_swizzle(int t) { return D >= 128 ? t % 16 : (t / 2) % 8; }
-  __host__ __device__ static constexpr int v_swizzle(int t) { return D >= 128 ? 4 * (t % 4) : 4 * ((t / 2) % 2); }
+  // (Of values, the last bit for the writes: two neighbouring rows' even chunks meet no
+  // bank twice.)
+  __host__ __device__ static constexpr int v_swizzle(int t) { return D >= 128 ? 4 * (t % 4) + t % 2 : 4 * ((t / 2) % 2); }
 };
 
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
@@ -463,7 +475,7 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
   constexpr int kBlocks = D / 32;
   __shared__ __attribute__((aligned(512))) unsigned char k_ring[W::kStages * W::kStage];
   __shared__ __attribute__((aligned(512))) unsigned char v_ring[W::kStages * W::kStage];
-  __shared__ Group groups[W::kList / kGroupKeys];
+  __shared__ Group<1> groups[W::kList / kGroupKeys];
   __shared__ int tile_groups[W::kList / W::kKeys];  // a bit for each of a tile's four groups: it has rows
   __shared__ unsigned odd_rows[W::kList / 32];  // a bit per key: values that are not all finite
 
@@ -537,19 +549,19 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
   codes_t k_codes[W::kPieces], v_codes[W::kPieces];
   float k_scale = 1.f, v_scale = 1.f;  // of the codes above
   auto group_of = [&](int tile) __attribute__((always_inline)) {
-    const Group x = groups[tile * (W::kKeys / kGroupKeys) + share_row / kGroupKeys];
-    Group u;
+    const Group<1> x = groups[tile * (W::kKeys / kGroupKeys) + share_row / kGroupKeys];
+    Group<1> u;
     u.slot = __builtin_amdgcn_readfirstlane(x.slot);
-    u.scales = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(x.scales)));
+    u.scales[0] = __builtin_amdgcn_readfirstlane(x.scales[0]);
     return u;
   };
-  auto load_piece = [&](auto values_tag, const Group &x, int j) __attribute__((always_inline)) {
+  auto load_piece = [&](auto values_tag, const Group<1> &x, int j) __attribute__((always_inline)) {
     constexpr bool values = decltype(values_tag)::value;
     const int slot = max(x.slot, 0) + share_row % kGroupKeys + j * W::kRowsApart;
     (values ? v_codes : k_codes)[j] =
         *reinterpret_cast<const codes_t *>(row_at(p, values ? v_base : k_base, slot) + piece_from);
     // (Behind the last piece of the tile before.)
-    if (j == W::kPieces - 1) (values ? v_scale : k_scale) = scale_of(values ? x.scales >> 8 : x.scales & 0xffu);
+    if (j == W::kPieces - 1) (values ? v_scale : k_scale) = scale_of((values ? x.scales[0] >> 8 : x.scales[0]) & 0xff);
   };
   // The words of a piece's values, two codes each.
   uint32_t words[W::kPiece / 2];
@@ -752,10 +764,9 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
     const int tiles = (listed + W::kKeys - 1) / W::kKeys;
     __syncthreads();  // every wave is past the former list and its tiles
     for (int i = tid; i < tiles * (W::kKeys / kGroupKeys); i += W::kThreads) {
-      Group x;
-      x.slot = -1;
-      x.scales = 0x7f7fu;
-      if (i * kGroupKeys < listed) x = group_at(p, pages, head, list_begin + i * kGroupKeys);
+      Group<1> x;
+      x.clear();
+      if (i * kGroupKeys < listed) x = group_at<1>(p, pages, head, list_begin + i * kGroupKeys);
       groups[i] = x;
     }
     for (int i = tid; i < 2 * tiles; i += W::kThreads) odd_rows[i] = 0;
@@ -775,7 +786,7 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
     const int last = tiles - 1;
     int v_slot;  // of the V codes held
     auto load_tile = [&](auto values_tag, int t) __attribute__((always_inline)) {
-      const Group x = group_of(min(t, last));
+      const Group<1> x = group_of(min(t, last));
       if (decltype(values_tag)::value) v_slot = x.slot;
 #pragma unroll
       for (int j = 0; j < W::kPieces; ++j) load_piece(values_tag, x, j);
@@ -805,7 +816,7 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
     // and K tile t + 2, held in registers, to their stages, then V tile t + 2 and K
     // tile t + 3 from memory.  Their stages held V tile t - 1 and K tile t, which all
     // waves have left.
-    Group next_v, next_k;
+    Group<1> next_v, next_k;
     auto staging = [&](int step, int t, auto stage_tag) __attribute__((always_inline)) {
       constexpr int stage = decltype(stage_tag)::value;
       const int j = step / 4 % W::kPieces, what = step % 4;
@@ -884,9 +895,9 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
           words &= words - 1;
           for (unsigned bits = __builtin_amdgcn_readlane(word, at); bits != 0; bits &= bits - 1) {
             const int key = (base + at) * 32 + __builtin_ctz(bits);  // of the list
-            const Group x = groups[key / kGroupKeys];
+            const Group<1> x = groups[key / kGroupKeys];
             const unsigned char *row = row_at(p, v_base, x.slot + key % kGroupKeys) + 4 * h;
-            const float scale = scale_of(x.scales >> 8);
+            const float scale = scale_of(x.scales[0] >> 8);
             if (list_begin + key > pos) continue;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
@@ -944,12 +955,32 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
     }
 }
 
+// KV heads that a workgroup of the narrow kernel takes together: what they read of a
+// row is one piece of 256 bytes where the heads' count allows it.
+// Heads of 128, one at a time and two: 32 requests over 32,768 keys of 4 KV heads
+// 290 and 215 us, 16 requests of 8 KV heads 323 and 224; what few requests read comes
+// from the memory-side cache either way, and their splits cost more (one over 131,072
+// keys 36 and 38 us, 4 over 4,000 14 and 15).
+int heads_together(const ll_paged_attention_args &a) {
+  if (a.head_dim == 256 || a.num_requests * a.num_kv_heads < 32) return 1;
+  if (a.head_dim == 64 && a.num_kv_heads % 4 == 0) return 4;
+  return a.num_kv_heads % 2 == 0 ? 2 : 1;
+}
+
 template <int D, typename E>
-int launch_all(const QuantizedParams &p, const Launch &x, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(x.max_units) * static_cast<unsigned>(p.hkv);
+int launch_all(const QuantizedParams &p, const Launch &x, int heads, hipStream_t s) {
+  const unsigned units = static_cast<unsigned>(x.max_units);
   launch_plan(p, x, s);
-  if (x.wide) quantized_wide_kernel<D, E><<<grid, Wide8<D>::kThreads, 0, s>>>(p);
-  else quantized_narrow_kernel<D, E><<<grid, Narrow8<D>::kThreads, 0, s>>>(p);
+  if (x.wide) {
+    quantized_wide_kernel<D, E><<<units * static_cast<unsigned>(p.hkv), Wide8<D>::kThreads, 0, s>>>(p);
+  } else {
+    const unsigned grid = units * static_cast<unsigned>(p.hkv / heads);
+    if (heads == 1) quantized_narrow_kernel<D, E, 1><<<grid, Narrow8<D>::kThreads, 0, s>>>(p);
+    if constexpr (D < 256)
+      if (heads == 2) quantized_narrow_kernel<D, E, 2><<<grid, Narrow8<D>::kThreads, 0, s>>>(p);
+    if constexpr (D == 64)
+      if (heads == 4) quantized_narrow_kernel<D, E, 4><<<grid, Narrow8<D>::kThreads, 0, s>>>(p);
+  }
   return launch_join<D, E>(p, x, s);
 }
 
@@ -980,13 +1011,13 @@ int64_t ll_quantized_attention_workspace_bytes(const ll_quantized_attention_args
   const int rc = check_quantized(a);
   if (rc != LL_OK) return rc;
   if (a->paged.num_queries == 0 || a->paged.num_requests == 0) return 0;
-  return plan_launch(&a->paged).ws_floats * 4;
+  return plan_launch(&a->paged, heads_together(a->paged)).ws_floats * 4;
 }
 
 int ll_quantized_attention(const ll_quantized_attention_args *a, ll_stream_t stream) {
   int rc = check_quantized(a);
   if (rc != LL_OK || a->paged.num_queries == 0 || a->paged.num_requests == 0) return rc;
-  const Launch x = plan_launch(&a->paged);
+  const Launch x = plan_launch(&a->paged, heads_together(a->paged));
   QuantizedParams p;
   memset(&p, 0, sizeof(p));
   rc = fill_params(&a->paged, x, &p);
@@ -999,9 +1030,11 @@ int ll_quantized_attention(const ll_quantized_attention_args *a, ll_stream_t str
   while ((1ll << p.block_shift) < a->scale_block) ++p.block_shift;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool f16 = a->paged.kv_dtype == LL_DTYPE_FLOAT16;
-  if (a->paged.head_dim == 64) return f16 ? launch_all<64, F16>(p, x, s) : launch_all<64, Bf16>(p, x, s);
-  if (a->paged.head_dim == 128) return f16 ? launch_all<128, F16>(p, x, s) : launch_all<128, Bf16>(p, x, s);
-  return f16 ? launch_all<256, F16>(p, x, s) : launch_all<256, Bf16>(p, x, s);
+  const int heads = heads_together(a->paged);
+  if (a->paged.head_dim == 64) return f16 ? launch_all<64, F16>(p, x, heads, s) : launch_all<64, Bf16>(p, x, heads, s);
+  if (a->paged.head_dim == 128)
+    return f16 ? launch_all<128, F16>(p, x, heads, s) : launch_all<128, Bf16>(p, x, heads, s);
+  return f16 ? launch_all<256, F16>(p, x, heads, s) : launch_all<256, Bf16>(p, x, heads, s);
 }
 
 }  // extern "C"
