@@ -435,48 +435,41 @@ __global__ void __launch_bounds__(kThreads) quantized_query_kernel(const PoolPar
 // Bits of rows: of up to 32 (kWords 0), 64 or 128.
 template <int kWords>
 struct RowBits {
-  unsigned long long words[kWords];
+  unsigned long long low, high;  // (members, not an array: the compiler would index it in memory)
 
-  __device__ void set(int word, unsigned long long bits) { words[word] = bits; }
+  __device__ void set(int word, unsigned long long bits) {
+    if (word == 0) low = bits;
+    else high = bits;
+  }
+  __device__ static unsigned long long up_to(int bit) { return (2ull << bit) - 1; }
   __device__ bool at(int row) const {
-    unsigned long long word = words[0];
-    if (kWords > 1 && row >= kWave) word = words[kWords - 1];
-    return ((word >> (row % kWave)) & 1ull) != 0;
+    const unsigned shifted_low = static_cast<unsigned>(low >> (row % kWave)) & 1u;
+    if (kWords == 1) return shifted_low != 0;
+    const unsigned shifted_high = static_cast<unsigned>(high >> (row % kWave)) & 1u;
+    return (row >= kWave ? shifted_high : shifted_low) != 0;
   }
   // The last one up to `row` (0: none).
   __device__ int last_to(int row) const {
-    const unsigned long long up_to = (2ull << (row % kWave)) - 1;
-    if (kWords > 1 && row >= kWave) {
-      const unsigned long long high = words[kWords - 1] & up_to;
-      if (high != 0) return 2 * kWave - 1 - __builtin_clzll(high);
-      return words[0] == 0 ? 0 : kWave - 1 - __builtin_clzll(words[0]);
-    }
-    const unsigned long long low = words[0] & up_to;
-    return low == 0 ? 0 : kWave - 1 - __builtin_clzll(low);
+    const unsigned long long in_low = kWords > 1 && row >= kWave ? low : low & up_to(row % kWave);
+    const unsigned long long in_high = kWords > 1 && row >= kWave ? high & up_to(row % kWave) : 0ull;
+    if (in_high != 0) return 2 * kWave - 1 - __builtin_clzll(in_high);
+    return in_low == 0 ? 0 : kWave - 1 - __builtin_clzll(in_low);
   }
   // The first one from `row` on (64 kWords: none).
   __device__ int first_from(int row) const {
-    if (row >= kWords * kWave) return kWords * kWave;
-    const unsigned long long from = ~0ull << (row % kWave);
-    if (kWords > 1 && row >= kWave) {
-      const unsigned long long high = words[kWords - 1] & from;
-      return high == 0 ? 2 * kWave : kWave + __builtin_ctzll(high);
-    }
-    const unsigned long long low = words[0] & from;
-    if (low != 0) return __builtin_ctzll(low);
-    if (kWords > 1 && words[kWords - 1] != 0) return kWave + __builtin_ctzll(words[kWords - 1]);
-    return kWords * kWave;
+    const unsigned long long in_low = row >= kWave ? 0ull : low & (~0ull << row);
+    if (in_low != 0) return __builtin_ctzll(in_low);
+    if (kWords == 1) return kWave;
+    const unsigned long long in_high = row >= 2 * kWave ? 0ull : row <= kWave ? high : high & (~0ull << (row - kWave));
+    return in_high == 0 ? 2 * kWave : kWave + __builtin_ctzll(in_high);
   }
   // How many of [begin, end).
   __device__ int count(int begin, int end) const {
-    int sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      const int from = max(begin - w * kWave, 0), to = min(end - w * kWave, kWave);
-      if (from >= to) continue;
-      const unsigned long long below = to == kWave ? ~0ull : (1ull << to) - 1;
-      sum += __builtin_popcountll(words[w] & below & (~0ull << from));
-    }
+    return (begin >= end) ? 0 : below(end) - below(begin);
+  }
+  __device__ int below(int end) const {
+    int sum = __builtin_popcountll(end >= kWave ? low : low & ((1ull << end) - 1));
+    if (kWords > 1 && end > kWave) sum += __builtin_popcountll(end >= 2 * kWave ? high : high & ((1ull << (end - kWave)) - 1));
     return sum;
   }
 };
@@ -501,6 +494,14 @@ struct RowBits<0> {
   }
 };
 
+// Waves a SIMD that the registers leave room for: what reads most latency away for few
+// spilled registers (32,768 tokens linked in blocks of 16: 39 us with four, 44 with
+// three; 8,192 in blocks of 128 34 and 37, but 8,192 appended 135 and 111).
+template <typename Source>
+constexpr int least_waves(int parts) {
+  return parts <= 2 || (parts == 8 && !Source::kNorms) ? 4 : parts <= 8 ? 3 : 1;
+}
+
 // Writes runs of rows.  A pair is one head's keys or values; kParts waves of a
 // workgroup hold up to kRunRows rows of it at a time, two steps of 64 / kGroup rows
 // each: as many of the window's runs as fit whole (one of a prompt's blocks, or many
@@ -514,7 +515,7 @@ struct RowBits<0> {
 // lane i's pair j as element 9 R row + R j + i, R = rotary lanes of a row, so that 16
 // lanes' 16-byte reads meet every bank once.
 template <typename Source, typename E, int kGroup, int kParts, bool kQueries>
-__global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, kParts <= 2 ? 4 : kParts <= 8 ? 3 : 1)
+__global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_waves<Source>(kParts))
     quantized_write_kernel(const PoolParams p) {
   constexpr int kWaves = kParts > 4 ? kParts : kThreads / kWave;
   constexpr int kPairs = kWaves / kParts;  // of a workgroup

@@ -199,6 +199,37 @@ def test_append_to_a_block_whose_scale_is_nan(gpu_device):
         assert bool((scales[1] == 255).all()) and bool((scales[2] < 255).all())
 
 
+@pytest.mark.parametrize("left_out", ["query_norm_weight", "key_norm_weight"])
+@pytest.mark.parametrize("neox,rotary", [(True, 64), (False, 128)])
+def test_append_with_one_norm(gpu_device, left_out, neox, rotary):
+    case = _append_case(gpu_device, list(range(30, 60)), rotary=rotary, weights=torch.float32)
+    _check_append({**case, left_out: None}, neox)
+
+
+def test_append_nothing(gpu_device):
+    case = _append_case(gpu_device, [3], slots=32)
+    before = _state(case)
+    empty = {name: case[name][:0] for name in ("query", "key", "value", "positions", "destination_slots")}
+    assert append_quantized_kv_inplace(**{**case, **empty}).shape == (0, 4, 128)
+    assert all(np.array_equal(a, b) for a, b in zip(_state(case), before))
+
+
+def test_runs_that_windows_cut(gpu_device):
+    """Runs of every length from 1 to 17 one after another, padding between some: windows
+    of all widths begin and end inside them."""
+
+    for block, tokens in ((16, 2500), (64, 2500), (128, 1500), (8, 400)):
+        slots, length, at = [], 1, 0
+        while len(slots) < tokens:
+            begin = at * block + (length % 3 if block > length + 3 else 0)
+            slots += list(range(begin, begin + min(length, block)))
+            slots += [-1] * (length % 2)
+            length, at = length % 17 + 1, at + 1
+        report(f"runs of 1 to 17, block {block}, {len(slots)} tokens")
+        case = _append_case(gpu_device, slots, q_heads=2, kv_heads=2, dim=64, block=block, slots=(at + 1) * block)
+        _check_append(case)
+
+
 def test_append_leaves_out_and_counts(gpu_device):
     slots = [3, 4, 5, 300, 301, -1, 20, 21, 22, 256]
     case = _append_case(gpu_device, slots, q_heads=28)
