@@ -14,13 +14,6 @@ __device__ inline float scale_of(unsigned byte) {
   return __builtin_bit_cast(float, bits);
 }
 
-// What values are multiplied by to become codes under a byte: 2^(127 - byte), 0 for
-// the byte of NaN.
-__device__ inline float inverse_of(unsigned byte) {
-  const unsigned bits = byte >= 254u ? (byte == 254u ? 0x00400000u : 0u) : (254u - byte) << 23;
-  return __builtin_bit_cast(float, bits);
-}
-
 // The least byte under which `most` (finite, not negative) is at most 448, e4m3's
 // largest: with most = m 2^k, 1 <= m < 2, and 448 = 1.75 * 2^8, k - 8 where m <= 1.75
 // and k - 7 elsewhere.  (Byte 0 holds everything below it.)

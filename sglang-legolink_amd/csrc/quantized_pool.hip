@@ -200,23 +200,27 @@ __device__ inline bool in_table(const PoolParams &p, long long position) {
   return position >= 0 && position < p.table_rows;
 }
 
+// Eight codes as values under a scale, exactly, and values as codes under one.
 __device__ inline void decode8(u32x2 codes, float scale, float *out) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(codes[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(codes[j], true);
-    out[4 * j] = lo[0] * scale;
-    out[4 * j + 1] = lo[1] * scale;
-    out[4 * j + 2] = hi[0] * scale;
-    out[4 * j + 3] = hi[1] * scale;
+    const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[j], scale, false);
+    const f32x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes[j], scale, true);
+    out[4 * j] = lo[0];
+    out[4 * j + 1] = lo[1];
+    out[4 * j + 2] = hi[0];
+    out[4 * j + 3] = hi[1];
   }
 }
-__device__ inline u32x2 encode8(const float *values, float inverse) {
+__device__ inline u32x2 encode8(const float *values, float scale) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
   u32x2 codes;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    int word = __builtin_amdgcn_cvt_pk_fp8_f32(values[4 * j] * inverse, values[4 * j + 1] * inverse, 0, false);
-    codes[j] = static_cast<uint32_t>(
-        __builtin_amdgcn_cvt_pk_fp8_f32(values[4 * j + 2] * inverse, values[4 * j + 3] * inverse, word, true));
+    i16x2 word = i16x2{0, 0};
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, values[4 * j], values[4 * j + 1], scale, false);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(word, values[4 * j + 2], values[4 * j + 3], scale, true);
+    codes[j] = __builtin_bit_cast(uint32_t, word);
   }
   return codes;
 }
@@ -708,7 +712,12 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
       float most = 0.f;
       if (has[step]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(finite_size(a[step][j]), finite_size(b[step][j])));
+        for (int j = 0; j < 8; ++j) most = fmaxf(fmaxf(most, fabsf(a[step][j])), fabsf(b[step][j]));  // (NaN left out)
+        if (!(most < INFINITY)) {  // (rare: infinities left out, too)
+          most = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, fmaxf(finite_size(a[step][j]), finite_size(b[step][j])));
+        }
       }
 #pragma unroll
       for (int apart = 1; apart < kGroup; apart *= 2) most = fmaxf(most, __shfl_xor(most, apart));
@@ -743,11 +752,11 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
     auto codes_at = [&](int slot) { return half.codes + (static_cast<long long>(slot) * p.hkv + head) * p.dim; };
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      const float inverse = inverse_of(of_row(byte, held_of(step)));
+      const float scale = scale_of(of_row(byte, held_of(step)));
       if (!has[step]) continue;
       uint8_t *dst = codes_at(tokens[token_of(step)].slot);
-      *reinterpret_cast<u32x2 *>(dst + l.first) = encode8(a[step], inverse);
-      *reinterpret_cast<u32x2 *>(dst + l.second) = encode8(b[step], inverse);
+      *reinterpret_cast<u32x2 *>(dst + l.first) = encode8(a[step], scale);
+      *reinterpret_cast<u32x2 *>(dst + l.second) = encode8(b[step], scale);
     }
     // The other rows of blocks whose scale has grown.
     for (int run = grown.first_from(0); run < kRunRows; run = grown.first_from(run + 1)) {
