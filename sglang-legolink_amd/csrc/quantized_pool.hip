@@ -518,6 +518,11 @@ constexpr int least_waves(int parts) {
 // itself would read 1 KB of table for 256 bytes of codes).  LDS has the angles of
 // lane i's pair j as element 9 R row + R j + i, R = rotary lanes of a row, so that 16
 // lanes' 16-byte reads meet every bank once.
+//
+// 4 heads of 128 in blocks of 16: 32,768 tokens linked 38 us (100 MB with the table's
+// rows, 2.7 TB/s: the vector units are busy for more than half of it, the rest is what
+// four waves a SIMD leave of the latencies), 1,024 6.8 us; 16,384 tokens' keys and
+// values appended 31 us, 64 single tokens 6.1 us.
 template <typename Source, typename E, int kGroup, int kParts, bool kQueries>
 __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_waves<Source>(kParts))
     quantized_write_kernel(const PoolParams p) {
@@ -809,7 +814,8 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
 }
 
 // Rows of the pool in 16 or 32 bits: a lane takes chunks of eight codes, several in
-// flight, of the workgroup's tokens.
+// flight, of the workgroup's tokens.  40,960 rows of 4 heads of 128 in bf16: 20 us,
+// 6.2 TB/s read and written (codes from the memory-side cache); 701 rows 3.9 us.
 struct LoadParams {
   const uint8_t *key, *value, *key_scales, *value_scales;
   void *key_output, *value_output;  // [tokens][heads][dim]

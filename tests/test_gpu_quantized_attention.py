@@ -190,14 +190,15 @@ def test_it_is_paged_attention_over_the_loaded_rows(gpu_device, queries, dtype):
 
 @pytest.mark.parametrize("queries", [None, [3, 1, 2], [200, 5, 90]])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("dim", [64, 128, 256])
-def test_rows_that_are_not_seen_may_hold_anything(gpu_device, queries, dtype, dim):
+@pytest.mark.parametrize("dim,heads", [(64, (4, 2)), (128, (4, 2)), (256, (4, 2)), (64, (32, 32)), (64, (22, 22)),
+                                       (128, (32, 32))])  # one, two and four heads a workgroup
+def test_rows_that_are_not_seen_may_hold_anything(gpu_device, queries, dtype, dim, heads):
     """NaN behind a request's length, in pages of no request and in later tokens of a
     query's own chunk do not reach it, in codes and in scales."""
 
-    report(f"unseen rows, queries {queries} {dtype} dim {dim}")
+    report(f"unseen rows, queries {queries} {dtype} dim {dim} heads {heads}")
     lengths = [70, 31, 300] if queries != [200, 5, 90] else [270, 31, 300]
-    case = _case(gpu_device, lengths, queries, heads=(4, 2), dim=dim, dtype=dtype)
+    case = _case(gpu_device, lengths, queries, heads=heads, dim=dim, dtype=dtype)
     want = quantized_paged_attention(**case)
     used = torch.zeros(case["key_buffer"].shape[0], dtype=torch.bool, device=gpu_device)
     for request, length in enumerate(lengths):
@@ -245,8 +246,9 @@ def test_a_scale_of_nan_reaches_those_who_see_its_block(gpu_device, queries, nam
     assert bool(torch.isnan(got[first:, 2:]).all())
 
 
-def test_single_tokens_over_a_scale_of_nan(gpu_device):
-    case = _case(gpu_device, [100, 20], heads=(4, 2), dim=128)
+@pytest.mark.parametrize("heads,dim", [((4, 2), 128), ((32, 16), 128), ((32, 16), 64), ((4, 2), 256)])
+def test_single_tokens_over_a_scale_of_nan(gpu_device, heads, dim):
+    case = _case(gpu_device, [100, 20], heads=heads, dim=dim)
     want = quantized_paged_attention(**case)
     case["value_scales"].view(torch.uint8)[case["page_table"][0, 6].long(), 0] = 255  # keys 96 to 99
     got = quantized_paged_attention(**case)
