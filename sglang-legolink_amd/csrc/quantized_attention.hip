@@ -540,11 +540,14 @@ __global__ void __launch_bounds__(Wide8<D>::kThreads) quantized_wide_kernel(cons
   const float slack = kSlack / scale_log2;
 
   // The wave's share of a tile, kRows rows of one group: piece j of a lane is its
-  // codes from byte kPiece (64 j + lane) of the share on.
+  // codes from byte kPiece * piece of row piece_row + j * kRowsApart of the share on.
+  // (Rows of 256 codes: 16 neighbouring lanes take half of each of two rows. A row's
+  // every second chunk meets each of these banks twice; two rows' swizzles differ by one.)
   const unsigned char *k_base = p.k8 + static_cast<long long>(head) * D;
   const unsigned char *v_base = p.v8 + static_cast<long long>(head) * D;
   const int share_row = wave * W::kRows;  // of a tile
-  const int piece_row = lane / W::kPiecesPerRow, piece = lane % W::kPiecesPerRow;
+  const int piece_row = W::kPiecesPerRow == 16 ? lane / 32 * 2 + lane / 8 % 2 : lane / W::kPiecesPerRow;
+  const int piece = W::kPiecesPerRow == 16 ? lane / 16 % 2 * 8 + lane % 8 : lane % W::kPiecesPerRow;
   const unsigned piece_from = static_cast<unsigned>(piece_row) * p.row_bytes + piece * W::kPiece;
   // Where a piece's values go in a stage: 16-byte chunks kChunks * piece on of row
   // share_row + piece_row + j * kRowsApart, swizzled (of j, by an xor).
