@@ -557,8 +557,9 @@ struct Launch {
 
 constexpr int kComputeUnits = 256;  // MI355X
 
-// `together`: KV heads that a workgroup of the narrow kernel takes.
-Launch plan_launch(const ll_paged_attention_args *a, int together = 1) {
+// `together`: KV heads that a workgroup of the narrow kernel takes.  `codes`: a pool of
+// 8 bits.
+Launch plan_launch(const ll_paged_attention_args *a, int together = 1, bool codes = false) {
   Launch x;
   const long long group = a->num_q_heads / a->num_kv_heads;
   const long long queries = a->num_queries, requests = a->num_requests;
@@ -585,10 +586,17 @@ Launch plan_launch(const ll_paged_attention_args *a, int together = 1) {
   // and 128 uneven requests: 390 and 212 us; one round 404 and 214, four 391 and 218).
   const int heads = static_cast<int>(a->num_kv_heads) / (x.wide ? 1 : together);
   const int places = std::max(1, kComputeUnits / heads);
-  x.target = x.wide                           ? places
-             : 2 * x.max_tiles <= places ? places - static_cast<int>(x.max_tiles) + 1
-                                         : 2 * places;
   const long long max_keys = a->page_table_columns * a->page_size;
+  // Between a quarter and half as many tiles as places, one round cuts requests of one
+  // length into chunks and small rests, two cut evenly but pay a second start.  Codes,
+  // 56/8 heads of 128, one round and two: 24 requests over 4,000 keys 57 and 63 us,
+  // 8,000 103 and 97, 32,768 380 and 335; 20 over 8,000 83 and 87, 32,768 308 and
+  // 297; 32, half the places, whose rests are next to nothing, 4,000 78 and 68, 32,768
+  // 536 and 403.  (Rows of 16 bits keep one round: unmeasured.)
+  const bool long_rows = max_keys * a->head_dim >= 8192 * 128;
+  const bool one_round = 2 * x.max_tiles <= places &&
+                         !(codes && (2 * x.max_tiles == places || (long_rows && 4 * x.max_tiles > places)));
+  x.target = x.wide ? places : one_round ? places - static_cast<int>(x.max_tiles) + 1 : 2 * places;
   x.splits = max_keys > x.min_chunk * kPageTile;
   x.max_units = x.max_tiles + (x.splits ? x.target + 1 : 0);
   x.max_partials = x.splits ? 2 * x.target + 2 : 0;

@@ -1019,13 +1019,13 @@ int64_t ll_quantized_attention_workspace_bytes(const ll_quantized_attention_args
   const int rc = check_quantized(a);
   if (rc != LL_OK) return rc;
   if (a->paged.num_queries == 0 || a->paged.num_requests == 0) return 0;
-  return plan_launch(&a->paged, heads_together(a->paged)).ws_floats * 4;
+  return plan_launch(&a->paged, heads_together(a->paged), true).ws_floats * 4;
 }
 
 int ll_quantized_attention(const ll_quantized_attention_args *a, ll_stream_t stream) {
   int rc = check_quantized(a);
   if (rc != LL_OK || a->paged.num_queries == 0 || a->paged.num_requests == 0) return rc;
-  const Launch x = plan_launch(&a->paged, heads_together(a->paged));
+  const Launch x = plan_launch(&a->paged, heads_together(a->paged), true);
   QuantizedParams p;
   memset(&p, 0, sizeof(p));
   rc = fill_params(&a->paged, x, &p);
