@@ -164,6 +164,20 @@ def test_many_requests(gpu_device, count, queries_of):
     _check_marked(quantized_paged_attention(**case), case)
 
 
+@pytest.mark.parametrize("count,spare", [(16, 600), (17, 0), (17, 600), (24, 600), (31, 600), (32, 0), (32, 600),
+                                         (33, 600)])
+@pytest.mark.parametrize("equal", [True, False])
+def test_units_of_one_round_and_of_two(gpu_device, count, spare, equal):
+    """Requests about a quarter and half of the places, in tables of few and of
+    more than 8,192 keys."""
+
+    report(f"{count} requests, {spare} spare columns, equal {equal}")
+    lengths = [700] * count if equal else [(r * 397) % 1200 for r in range(count)]
+    case = _case(gpu_device, lengths, heads=(16, 8), dim=128, spare_columns=spare)
+    _check(quantized_paged_attention(**case), case)
+    _check_marked(quantized_paged_attention(**_marked(case)), case)
+
+
 @pytest.mark.parametrize("queries", [None, [1, 40, 3, 65], [60, 128, 1, 70]])
 @pytest.mark.parametrize("heads,dim,page", [((28, 4), 128, 16), ((14, 2), 64, 32), ((7, 1), 256, 32)])
 def test_tables_of_at_most_128_keys(gpu_device, queries, heads, dim, page):
