@@ -796,9 +796,9 @@ typedef struct ll_quantized_pool {
  * negative is padding (its queries are turned), and so is one whose slot is
  * num_slots or more.  skipped_rows counts positions outside the table and slots past
  * the pool, a token once.  The slots that are written are pairwise distinct, and
- * those of one block stand next to each other in the call (in any order, no padding
- * between them), as a request's new tokens do; what a block holds whose slots do not
- * is not defined.  Strides are in elements, multiples of 8; rows, norm weights and
+ * those of one block stand next to each other in the call, as a request's new tokens
+ * do: in any order, with padding between them or not, but no row of another block.
+ * What a block holds whose slots do not is not defined.  Strides are in elements, multiples of 8; rows, norm weights and
  * their heads begin at multiples of 16 bytes.  One launch.
  */
 typedef struct ll_quantized_append_args {

@@ -17,10 +17,10 @@
 //         its old to its new position: cos = c' c + s' s, sin = s' c - c' s with rows
 //         (c, s) of the table at the old and (c', s') at the new position.
 //
-// A call's rows of one block are neighbours in the call (a run), so that one wave,
-// or the waves of one workgroup for blocks over 16 rows, holds them all, one head of
-// the keys or values: their maximum is known before the first code is written, and
-// every row is read once.  Keys are turned in 64 bits: a code changes by up to 1/8 of
+// A call's rows of one block are neighbours in the call (a run; padding between them
+// does not count), so that one wave, or the waves of one workgroup for blocks over 16
+// rows, holds them all, one head of the keys or values: their maximum is known before
+// the first code is written, and every row is read once.  Keys are turned in 64 bits: a code changes by up to 1/8 of
 // itself where a value lies at the border of two, which 32 bits meet some hundred
 // times in a call of 32,768 tokens.
 #include <hip/hip_runtime.h>
@@ -226,9 +226,10 @@ __device__ inline u32x2 encode8(const float *values, float scale) {
 }
 
 // What a workgroup knows of a token: where it goes (-1: nowhere), where it comes from
-// (of a link; -1: it is not written), its positions (-1: it is not turned).
+// (of a link; -1: it is not written), its position (-1: it is not turned), and a link's
+// position before that or an append's place in the call.
 struct Token {
-  int slot, from, position, old_position;
+  int slot, from, position, origin;
 };
 
 // A pair's cosine and sine.
@@ -268,6 +269,7 @@ struct NewTokens {
     Token k{-1, -1, -1, -1};
     const long long slot = index_at(p.slots, p.slots64, t), position = index_at(p.positions, p.positions64, t);
     if (slot >= 0 && slot < p.num_slots) k.slot = static_cast<int>(slot);
+    k.origin = static_cast<int>(t);
     if (in_table(p, position)) {
       k.position = static_cast<int>(position);
       k.from = k.slot;
@@ -275,10 +277,9 @@ struct NewTokens {
     *bad = false;  // (counted with the queries)
     return k;
   }
-  __device__ static Raw fetch(const PoolParams &p, const Half &, bool is_key, int head, long long t, const Token &,
-                              const Lane &l) {
+  __device__ static Raw fetch(const PoolParams &p, const Half &, bool is_key, int head, const Token &k, const Lane &l) {
     const Rows &in = is_key ? p.new_key : p.new_value;
-    const uint16_t *row = in.base + t * in.token + head * in.head;
+    const uint16_t *row = in.base + k.origin * in.token + head * in.head;
     return Raw{*reinterpret_cast<const u32x4 *>(row + l.first), *reinterpret_cast<const u32x4 *>(row + l.second)};
   }
   __device__ static void unpack(const Raw &raw, float *a, float *b) {
@@ -324,14 +325,13 @@ struct CachedRows {
       k.from = static_cast<int>(source);
       if (turned) {
         k.position = static_cast<int>(position);
-        k.old_position = static_cast<int>(old_position);
+        k.origin = static_cast<int>(old_position);
       }
     }
     *bad = !masked && (slot >= p.num_slots || (slot >= 0 && !there));
     return k;
   }
-  __device__ static Raw fetch(const PoolParams &p, const Half &half, bool, int head, long long, const Token &k,
-                              const Lane &l) {
+  __device__ static Raw fetch(const PoolParams &p, const Half &half, bool, int head, const Token &k, const Lane &l) {
     const uint8_t *codes = half.codes + (static_cast<long long>(k.from) * p.hkv + head) * p.dim;
     return Raw{*reinterpret_cast<const u32x2 *>(codes + l.first), *reinterpret_cast<const u32x2 *>(codes + l.second),
                scale_of(half.scales[static_cast<long long>(k.from >> p.block_shift) * p.hkv + head])};
@@ -342,7 +342,7 @@ struct CachedRows {
   }
   __device__ static void angles(const PoolParams &p, const Token &k, int i, Angle *out) {
     float c[4], s[4], from_c[4], from_s[4];
-    const long long to = k.position * p.table_stride + i, from = k.old_position * p.table_stride + i;
+    const long long to = k.position * p.table_stride + i, from = k.origin * p.table_stride + i;
     values4(p, to, c);
     values4(p, to + p.rotary / 2, s);
     values4(p, from, from_c);
@@ -506,6 +506,81 @@ constexpr int least_waves(int parts) {
   return parts <= 2 || (parts == 8 && !Source::kNorms) ? 4 : parts <= 8 ? 3 : 1;
 }
 
+// The tokens that have a slot, moved together over the padding between them: tokens[1]
+// on are then the window's, behind them the others up to the end of the last one's run
+// (as far as a workgroup holds), tokens[0] the last one in front of the window.  Padding
+// may be of any length, so the call is searched both ways, kLooks tokens a lane at a time
+// (64 single tokens padded to 2,048 at their end: 11.4 us, 3 of them for this; in 64
+// places one gap in the middle costs 1.4).  Of one wave; returns how many of the window's
+// there are (at least one).
+template <typename Source, int kRunRows>
+__device__ inline int pack_tokens(const PoolParams &p, long long t0, Token *tokens) {
+  constexpr int kLooks = 8;
+  const int lane = threadIdx.x % kWave;
+  // The first of kLooks * 64 tokens from `at` on (or back) that has a slot; that many: none.
+  auto first_of = [&](long long at, int step) {
+    auto place = [&](int i) { return at + step * (i * kWave + lane); };
+    auto exists = [&](int i) { return place(i) >= 0 && place(i) < p.num_tokens; };
+    long long slot[kLooks];  // (of one type a branch: all loads in flight)
+    if (p.slots64 != 0) {
+#pragma unroll
+      for (int i = 0; i < kLooks; ++i) slot[i] = index_at(p.slots, 1, exists(i) ? place(i) : 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLooks; ++i) slot[i] = index_at(p.slots, 0, exists(i) ? place(i) : 0);
+    }
+    int first = kLooks * kWave;
+#pragma unroll
+    for (int i = kLooks - 1; i >= 0; --i) {
+      const unsigned long long there = __builtin_amdgcn_ballot_w64(exists(i) && slot[i] >= 0 && slot[i] < p.num_slots);
+      if (there != 0) first = i * kWave + __builtin_ctzll(there);
+    }
+    return first;
+  };
+  // Those of `taken` to the places behind `to` (never past their own).
+  auto move = [&](const Token &k, unsigned long long taken, int to, int last) {
+    const int place = to + 1 + __builtin_popcountll(taken & ((1ull << lane) - 1));
+    if (((taken >> lane) & 1ull) != 0 && place <= last) tokens[place] = k;
+  };
+  const Token own = tokens[1 + min(lane, p.window - 1)];
+  const unsigned long long of_window = __builtin_amdgcn_ballot_w64(lane < p.window && own.slot >= 0);
+  const int count = __builtin_popcountll(of_window), last = count + kRunRows;
+  if (tokens[0].slot < 0) {
+    for (long long at = t0 - 1; at >= 0; at -= kLooks * kWave) {
+      const int first = first_of(at, -1);
+      if (first == kLooks * kWave) continue;
+      if (lane == 0) tokens[0].slot = static_cast<int>(index_at(p.slots, p.slots64, at - first));
+      break;
+    }
+  }
+  move(own, of_window, 0, count);
+  const int block = __builtin_amdgcn_readlane(own.slot, kWave - 1 - __builtin_clzll(of_window)) >> p.block_shift;
+  int held = count;
+  bool ended = false;  // the run; its end is the first token of another block
+  auto take = [&](const Token &k, bool exists) {
+    unsigned long long taken = __builtin_amdgcn_ballot_w64(exists && k.slot >= 0);
+    const unsigned long long others = __builtin_amdgcn_ballot_w64(exists && k.slot >= 0 && k.slot >> p.block_shift != block);
+    if (others != 0) taken &= others ^ (others - 1);  // (up to the first one)
+    move(k, taken, held, last);
+    held = min(held + static_cast<int>(__builtin_popcountll(taken)), last);
+    ended = others != 0 || held == last;
+  };
+  for (int i = p.window + 1; !ended && i <= p.window + kRunRows; i += kWave)
+    take(tokens[min(i + lane, p.window + kRunRows)], i + lane <= p.window + kRunRows);
+  for (long long t = t0 + p.window + kRunRows + 1; !ended && t < p.num_tokens;) {
+    const int first = first_of(t, 1);
+    t += first;
+    if (first == kLooks * kWave) continue;
+    Token k{-1, -1, -1, -1};
+    bool bad;
+    if (t + lane < p.num_tokens) k = Source::token(p, t + lane, &bad);
+    take(k, t + lane < p.num_tokens);
+    t += kWave;
+  }
+  for (int i = held + 1 + lane; i <= last; i += kWave) tokens[i] = Token{-1, -1, -1, -1};
+  return count;
+}
+
 // Writes runs of rows.  A pair is one head's keys or values; kParts waves of a
 // workgroup hold up to kRunRows rows of it at a time, two steps of 64 / kGroup rows
 // each: as many of the window's runs as fit whole (one of a prompt's blocks, or many
@@ -538,6 +613,7 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
   typedef RowBits<kRunRows <= 32 ? 0 : kWords> Bits;
   __shared__ unsigned most_of[kPairs][kRunRows];  // of a run, at its first row: a float's bits
   __shared__ Token tokens[kTokens];
+  __shared__ int packed;
   __shared__ Angle shared_angles[kShares ? kRunRows * 9 * kGroup : 1];
   __shared__ float key_weights[Source::kNorms ? 16 * kGroup : 1];
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -574,12 +650,50 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
     for (int i = threadIdx.x; i < p.dim; i += kWaves * kWave)
       key_weights[i] = p.key_weight != nullptr ? value_at(p.key_weight, p.weight_dtype, i) : 1.f;
   __syncthreads();
+  int own_tokens = p.window;
+  {
+    const int exist = static_cast<int>(min(p.num_tokens - t0, static_cast<long long>(1 + p.window + kRunRows)));
+    const int begin = t0 < 0 ? 1 : 0;
+    int least = 0;  // (every wave reads all of them, at once)
+#pragma unroll
+    for (int i = 0; i < kTokens; i += kWave) least = min(least, tokens[max(begin, min(i + lane, exist - 1))].slot);
+    if (__builtin_amdgcn_ballot_w64(least < 0) != 0) {
+      // It matters where a token may follow that belongs to the runs that begin here:
+      // not behind the first one of another block than the window's last, or at the end.
+      const int last_block = tokens[p.window].slot >> p.block_shift;
+      unsigned long long owns = 0;
+      int first_gap = kTokens, run_end = kTokens, last_there = -1;
+#pragma unroll
+      for (int i = 0; i < kTokens; i += kWave) {
+        const int at = i + lane, slot = tokens[min(at, exist - 1)].slot;
+        const bool in = at >= begin && at < exist;
+        const unsigned long long gaps = __builtin_amdgcn_ballot_w64(in && slot < 0);
+        const unsigned long long there = __builtin_amdgcn_ballot_w64(in && slot >= 0);
+        const unsigned long long others =
+            __builtin_amdgcn_ballot_w64(in && slot >= 0 && at > p.window && slot >> p.block_shift != last_block);
+        owns |= __builtin_amdgcn_ballot_w64(in && slot >= 0 && at >= 1 && at <= p.window);
+        if (first_gap == kTokens && gaps != 0) first_gap = i + __builtin_ctzll(gaps);
+        if (run_end == kTokens && others != 0) run_end = i + __builtin_ctzll(others);
+        if (there != 0) last_there = i + kWave - 1 - __builtin_clzll(there);
+      }
+      if (owns == 0) return;
+      if (first_gap < run_end && (last_there > first_gap || t0 + exist < p.num_tokens)) {
+        __syncthreads();
+        if (wave == 0) {
+          const int count = pack_tokens<Source, kRunRows>(p, t0, tokens);
+          if (lane == 0) packed = count;
+        }
+        __syncthreads();
+        own_tokens = __builtin_amdgcn_readfirstlane(packed);
+      }
+    }
+  }
   auto block_of = [&](int i) { return tokens[i].slot < 0 ? -1 : tokens[i].slot >> p.block_shift; };
   // A run begins where the block changes.  Bit l: token 1 + l of those here.
   unsigned long long begins;
   {
-    const int block = block_of(1 + min(lane, p.window - 1));
-    begins = __builtin_amdgcn_ballot_w64(lane < p.window && block >= 0 && block != block_of(min(lane, p.window - 1)));
+    const int block = block_of(1 + min(lane, own_tokens - 1));
+    begins = __builtin_amdgcn_ballot_w64(lane < own_tokens && block >= 0 && block != block_of(min(lane, own_tokens - 1)));
   }
   while (begins != 0) {
     const int first = 1 + __builtin_ctzll(begins);  // token of row 0
@@ -598,7 +712,7 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
       written.set(w, __builtin_amdgcn_ballot_w64(exists && tokens[first + row].from >= 0));
       bounds.set(w, __builtin_amdgcn_ballot_w64(exists && (starts || block < 0)));
       const unsigned long long out =
-          __builtin_amdgcn_ballot_w64(exists && first + row > p.window && (starts || block < 0));
+          __builtin_amdgcn_ballot_w64(exists && first + row > own_tokens && (starts || block < 0));
       if (stop == kRunRows && out != 0) stop = w * kWave + __builtin_ctzll(out);
     }
     {
@@ -634,7 +748,7 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
     for (int step = 0; step < kSteps; ++step) {
       has[step] = has_pair && l.active && held_of(step) < stop && written.at(held_of(step));
       raw[step] = typename Source::Raw{};
-      if (has[step]) raw[step] = Source::fetch(p, half, is_key, head, t0 + token_of(step), tokens[token_of(step)], l);
+      if (has[step]) raw[step] = Source::fetch(p, half, is_key, head, tokens[token_of(step)], l);
     }
     const int lanes = p.rotary / 16;
     if constexpr (kShares) {

@@ -196,7 +196,9 @@ def append_quantized_kv_inplace(*, key_buffer: torch.Tensor, value_buffer: torch
     ``query_output``, which may be the query itself).
 
     The slots that are written must be pairwise distinct, and those of one block
-    stand next to each other in the call, as a request's new tokens do.  A
+    stand next to each other in the call, as a request's new tokens do: in any
+    order, with padding between them or not, but no row of another block (not
+    checked: what a block holds whose rows do not is undefined).  A
     negative slot is padding (its queries are turned, nothing is written), a slot
     past the pool likewise and counted in ``skipped_rows``; a token whose position
     is outside the table is left out whole and counted.  ``rotary_dim`` is a

@@ -455,3 +455,72 @@ def test_calls_on_another_stream(gpu_device):
     stream.synchronize()
     slots = case["destination_slots"].tolist()
     _check_pool(case, before, 16, slots, _rows_of(case, True, "key"), _rows_of(case, True, "value"), [True] * len(slots))
+
+
+# -- padding within a block's rows ---------------------------------------------
+
+PADDED = {  # slots of a pool of 512; 512 and more are past it
+    "one": [0, -1, 1],
+    "past the pool": [0, 512, 1, 7, 2 ** 31 - 1, 3],
+    "two blocks": [133, -1, -9, 130, 600, 128, -1, 300, -1, 257],
+    "every second": [s for pair in zip(range(256, 384), [-1, 512] * 64) for s in pair],
+    "a few": [s for i in range(140) for s in ([-1] * (i % 23 == 5) + [140 + i])],
+    "long": [40, *[-1] * 700, 41, *[-5] * 1500, 47, *[-1] * 64, 200, *[512] * 3000, 207, 204],
+    "in front": [*[-1] * 1200, 384, *[-1] * 600, 385, 386],
+    "behind": [17, 18, 19, *[-1] * 2045],
+    "alone": [-1] * 1000 + [511] + [-1] * 200,
+    "nothing": [-1, 512] * 300,
+}
+
+
+@pytest.mark.parametrize("runs", list(PADDED))
+@pytest.mark.parametrize("dim,block", [(128, 16), (64, 64), (128, 32), (256, 128), (64, 128), (16, 128), (80, 8)])
+def test_append_with_padding_within_a_block(gpu_device, runs, dim, block):
+    """A block's scale and codes are of all its rows in the call, whatever padding of
+    whatever length stands between them."""
+
+    report(f"append padded {runs}, dim {dim} block {block}")
+    slots = PADDED[runs]
+    case = _append_case(gpu_device, slots, dim=dim, block=block, slots=512, kv_heads=2, q_heads=2, rotary=16)
+    case["key"].mul_(torch.linspace(0.1, 30.0, len(slots), device=gpu_device).to(case["key"].dtype)[:, None, None])
+    case["value"].mul_(torch.linspace(20.0, 0.1, len(slots), device=gpu_device).to(case["key"].dtype)[:, None, None])
+    skipped = torch.zeros(1, dtype=torch.int64, device=gpu_device)
+    _check_append(case, skipped_rows=skipped)
+    assert int(skipped) == sum(s >= 512 for s in slots)
+
+
+@pytest.mark.parametrize("runs", list(PADDED))
+@pytest.mark.parametrize("dim,block", [(128, 16), (128, 64), (64, 128), (256, 32), (256, 128)])
+def test_link_with_padding_within_a_block(gpu_device, runs, dim, block):
+    report(f"link padded {runs}, dim {dim} block {block}")
+    slots = PADDED[runs]
+    sources = [1024 + (5 * i) % 512 for i in range(len(slots))]
+    case = _link_case(gpu_device, sources, [s if s < 512 else 1536 + s for s in slots], dim=dim, block=block, slots=1536,
+                      rotary=32, repair=True, index=torch.int64)
+    skipped = torch.zeros(1, dtype=torch.int64, device=gpu_device)
+    _check_link(case, skipped_rows=skipped)
+    masked = case["repair_mask"].tolist()
+    assert int(skipped) == sum(s >= 512 and not m for s, m in zip(slots, masked))
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("tokens", [40, 700, 5000])
+def test_padding_anywhere_in_a_large_append(gpu_device, block, tokens):
+    """Windows of every width: rows of many blocks in any order within each, and padding
+    of any length between any two of them."""
+
+    report(f"padding anywhere, {tokens} tokens, block {block}")
+    generator = torch.Generator().manual_seed(tokens + block)
+
+    def draw(high):
+        return int(torch.randint(high, (1,), generator=generator))
+
+    slots, blocks = [], iter(torch.randperm(tokens, generator=generator).tolist())
+    while len(slots) < tokens:
+        base = next(blocks) * block
+        for offset in torch.randperm(block, generator=generator)[:1 + draw(block)].tolist():
+            if draw(9) == 0:
+                slots += [-1] * (1 + draw(3) * draw(3) * draw(90))
+            slots.append(base + offset)
+    case = _append_case(gpu_device, slots, q_heads=2, kv_heads=3, dim=64, block=block, slots=tokens * block)
+    _check_append(case)
