@@ -524,3 +524,63 @@ def test_padding_anywhere_in_a_large_append(gpu_device, block, tokens):
             slots.append(base + offset)
     case = _append_case(gpu_device, slots, q_heads=2, kv_heads=3, dim=64, block=block, slots=tokens * block)
     _check_append(case)
+
+
+# -- every kernel that the dispatch by dim and block sends calls to ------------------
+
+VARIANTS = [(128, 128, 32), (128, 64, 128), (256, 128, 32), (256, 256, 8), (64, 64, 64), (64, 32, 128), (144, 16, 16)]
+
+
+@pytest.mark.parametrize("runs", list(RUNS))
+@pytest.mark.parametrize("dim,rotary,block", VARIANTS)
+def test_append_other_blocks(gpu_device, runs, dim, rotary, block):
+    report(f"append {runs}, dim {dim} rotary {rotary} block {block}")
+    for neox, dtype, weights in ((True, torch.bfloat16, None), (False, torch.float16, torch.float32)):
+        case = _append_case(gpu_device, RUNS[runs], dim=dim, rotary=rotary, block=block, dtype=dtype, weights=weights,
+                            q_heads=7, kv_heads=3)
+        _check_append(case, neox)
+
+
+@pytest.mark.parametrize("dim,rotary,block", VARIANTS)
+@pytest.mark.parametrize("neox,repair,prefix", [(True, False, 0), (False, True, 7), (True, True, 60)])
+def test_link_other_blocks(gpu_device, dim, rotary, block, neox, repair, prefix):
+    report(f"link dim {dim} rotary {rotary} block {block} neox {neox} repair {repair} prefix {prefix}")
+    sources = [*range(3, 40), *range(100, 101), *range(7, 90)]
+    destinations = [*range(256, 256 + len(sources) - 20), *range(400, 420)]
+    case = _link_case(gpu_device, sources, destinations, dim=dim, rotary=rotary, block=block, repair=repair, kv_heads=3)
+    _check_link(case, neox, prefix)
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("block,tokens", [(8, 400), (32, 1500), (128, 1500)])
+def test_runs_that_windows_cut_of_other_dims(gpu_device, dim, block, tokens):
+    slots, length, at = [], 1, 0
+    while len(slots) < tokens:
+        begin = at * block + (length % 3 if block > length + 3 else 0)
+        slots += list(range(begin, begin + min(length, block)))
+        slots += [-1] * (length % 2)
+        length, at = length % 17 + 1, at + 1
+    report(f"runs of 1 to 17, dim {dim} block {block}, {len(slots)} tokens")
+    case = _append_case(gpu_device, slots, q_heads=2, kv_heads=2, dim=dim, block=block, slots=(at + 1) * block)
+    _check_append(case)
+
+
+@pytest.mark.parametrize("heads,dim,block,tokens", [
+    ((28, 1), 128, 16, 8192), ((28, 1), 128, 16, 8193), ((28, 1), 128, 64, 4096), ((28, 1), 128, 64, 4097),
+    ((33, 2), 64, 32, 11000), ((9, 1), 256, 128, 6000)])  # 32,768 waves of queries or more, 16,384 in large blocks
+def test_append_with_queries_of_either_launch(gpu_device, heads, dim, block, tokens):
+    """Padding, counting, norms and the queries' own rows as output, whichever launch turns the queries."""
+
+    report(f"append {tokens} tokens, heads {heads} of {dim}, block {block}")
+    total = (tokens // block + 2) * block
+    slots = [total - 1 - i for i in range(tokens)]
+    slots[100:103], slots[tokens - 2], slots[tokens - 1] = [-1, -7, -1], total, total + 12345
+    case = _append_case(gpu_device, slots, q_heads=heads[0], kv_heads=heads[1], dim=dim, block=block, slots=total,
+                        weights=torch.float32, rotary=32)
+    case["positions"][5], case["positions"][tokens // 2], case["positions"][101] = POSITIONS, -1, 2 ** 40
+    skipped = torch.full((1,), 3, dtype=torch.int64, device=gpu_device)
+    query = case["query"].clone()
+    got = _check_append(case, query_output=case["query"], skipped_rows=skipped)
+    assert int(skipped) == 3 + 5  # three positions, two slots past the pool
+    left_out = [5, tokens // 2, 101]
+    assert got is case["query"] and torch.equal(got[left_out], query[left_out])
