@@ -772,7 +772,8 @@ int64_t ll_paged_attention_args_size(void);
  * writes every one of its rows, and else the larger of need and what it was, under
  * which its other rows' codes are then rounded again.  So a scale only grows while
  * rows are added; who gives a block to another request sets its scale bytes to 0,
- * lest the new rows be rounded under the old ones' scale.  Codes are rounded to
+ * lest the new rows be rounded under the old ones' scale (needless only where one call
+ * writes all its rows: not a link with a repair mask, nor a prompt's partial last block).  Codes are rounded to
  * nearest even from results of more than 24 bits (keys) or exact ones; values that are
  * not finite become NaN.
  */

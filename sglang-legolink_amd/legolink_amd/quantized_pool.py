@@ -22,7 +22,9 @@ a block to another request clears its scales first::
 
     key_scales.view(torch.uint8)[blocks] = 0      # and value_scales
 
-or the new rows may be rounded under the scale of the old ones.
+or the new rows may be rounded under the scale of the old ones (and are NaN under a
+byte of 255).  Only a block that one call writes whole needs no clearing: a link with a
+repair mask leaves rows out, and a prompt's last block is mostly partial.
 
 Everything is enqueued on the current stream; no call synchronises, and all may be
 captured into a HIP graph.  Inference only: tensors that need a gradient or carry a

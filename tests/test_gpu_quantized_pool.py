@@ -584,3 +584,30 @@ def test_append_with_queries_of_either_launch(gpu_device, heads, dim, block, tok
     assert int(skipped) == 3 + 5  # three positions, two slots past the pool
     left_out = [5, tokens // 2, 101]
     assert got is case["query"] and torch.equal(got[left_out], query[left_out])
+
+
+# -- blocks of an earlier owner ------------------------------------------------------
+
+
+@pytest.mark.parametrize("block", [16, 64])
+def test_rows_added_to_used_blocks_need_cleared_scales(gpu_device, block):
+    """A link that leaves rows out, and a prompt's last block: their blocks' scales are the
+    rows' own where their bytes were cleared, and else no less than the earlier owner's."""
+
+    sources, destinations = list(range(70)), list(range(256, 326))
+    for cleared in (True, False):
+        case = _link_case(gpu_device, sources, destinations, block=block, repair=True, low=110, high=111)
+        for name in ("key_scales", "value_scales"):
+            case[name].view(torch.uint8)[256 // block:] = 0 if cleared else 200
+        assert bool(case["repair_mask"].view(torch.uint8)[:64].view(-1, block).any(1).all())  # in every block
+        _check_link(case)
+        for name in ("key_scales", "value_scales"):
+            of_blocks = case[name].view(torch.uint8)[256 // block:-(-326 // block)]
+            assert bool(((of_blocks > 0) & (of_blocks < 115)).all() if cleared else (of_blocks == 200).all())
+        case = _append_case(gpu_device, list(range(block + 3)), block=block)
+        for name in ("key_scales", "value_scales"):
+            case[name].view(torch.uint8)[:] = 0 if cleared else 200
+        _check_append(case)
+        for name in ("key_scales", "value_scales"):
+            scales = case[name].view(torch.uint8)[:2]
+            assert bool((scales[0] < 130).all()) and bool((scales[1] < 130).all() if cleared else (scales[1] == 200).all())
