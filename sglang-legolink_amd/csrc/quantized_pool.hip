@@ -608,6 +608,7 @@ __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_
   constexpr int kHeldRows = kSteps * kRows;  // of a wave
   constexpr int kRunRows = kParts * kHeldRows;
   constexpr int kWords = (kRunRows + kWave - 1) / kWave;
+  static_assert(kRunRows <= kMaxBlock, "RowBits holds two words, and no block has more rows");
   constexpr bool kShares = kPairs > 1;
   constexpr int kTokens = 1 + kMostWindow + kRunRows;  // the one before the window, the window, a run from its last on
   typedef RowBits<kRunRows <= 32 ? 0 : kWords> Bits;
@@ -1084,18 +1085,15 @@ int launch_write(PoolParams &p, hipStream_t s) {
   return LL_OK;
 }
 
-template <typename Source, typename E, int kGroup, bool kQueries>
+// As few waves of a pair as hold a block's rows.
+template <typename Source, typename E, int kGroup, bool kQueries, int kParts = 1>
 int launch_by_block(PoolParams &p, hipStream_t s) {
-  constexpr int kHeld = kHeldSteps * kWave / kGroup;
-  const int rows = 1 << p.block_shift;
-  if (rows <= kHeld) return launch_write<Source, E, kGroup, 1, kQueries>(p, s);
-  if (rows <= 2 * kHeld) return launch_write<Source, E, kGroup, 2, kQueries>(p, s);
-  if (rows <= 4 * kHeld) return launch_write<Source, E, kGroup, 4, kQueries>(p, s);
-  if constexpr (8 * kHeld >= kMaxBlock) {
-    return launch_write<Source, E, kGroup, 8, kQueries>(p, s);
+  constexpr int kHeld = kParts * kHeldSteps * kWave / kGroup;
+  if constexpr (kHeld >= kMaxBlock) {
+    return launch_write<Source, E, kGroup, kParts, kQueries>(p, s);
   } else {
-    if (rows <= 8 * kHeld) return launch_write<Source, E, kGroup, 8, kQueries>(p, s);
-    return launch_write<Source, E, kGroup, 16, kQueries>(p, s);
+    if (1 << p.block_shift <= kHeld) return launch_write<Source, E, kGroup, kParts, kQueries>(p, s);
+    return launch_by_block<Source, E, kGroup, kQueries, 2 * kParts>(p, s);
   }
 }
 
