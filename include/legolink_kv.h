@@ -773,9 +773,15 @@ int64_t ll_paged_attention_args_size(void);
  * which its other rows' codes are then rounded again.  So a scale only grows while
  * rows are added; who gives a block to another request sets its scale bytes to 0,
  * lest the new rows be rounded under the old ones' scale (needless only where one call
- * writes all its rows: not a link with a repair mask, nor a prompt's partial last block).  Codes are rounded to
- * nearest even from results of more than 24 bits (keys) or exact ones; values that are
- * not finite become NaN.
+ * writes all its rows: not a link with a repair mask, nor a prompt's partial last
+ * block).  Codes are rounded to nearest even from results of more than 24 bits (keys
+ * of at least 2^-126; smaller ones from fp32's subnormal numbers) or exact ones; values
+ * that are not finite in fp32 become NaN.
+ *
+ * Scale bytes 3 to 246 make values that bf16 holds exactly, 0 to 246 that fp32 does
+ * (fp16 those from 2^-21 up to 65504).  Under 0 to 2 bf16 rounds to its least step,
+ * 2^-133; from 247 on the largest codes are past fp32 and infinite when read: a finite
+ * row's value of at least 1.9375 * 2^127 is held as 2^128.
  */
 typedef struct ll_quantized_pool {
   void *key_buffer;                /* device e4m3 [num_slots, num_kv_heads, head_dim], dense, 16-byte aligned */
@@ -799,8 +805,9 @@ typedef struct ll_quantized_pool {
  * the pool, a token once.  The slots that are written are pairwise distinct, and
  * those of one block stand next to each other in the call, as a request's new tokens
  * do: in any order, with padding between them or not, but no row of another block.
- * What a block holds whose slots do not is not defined.  Strides are in elements, multiples of 8; rows, norm weights and
- * their heads begin at multiples of 16 bytes.  One launch.
+ * What a block holds whose slots do not is not defined.  Strides are in elements,
+ * multiples of 8; rows, norm weights and their heads begin at multiples of 16 bytes.
+ * One launch, or two where the queries are many.
  */
 typedef struct ll_quantized_append_args {
   int64_t struct_size;             /* sizeof(ll_quantized_append_args) */
@@ -902,8 +909,8 @@ int64_t ll_quantized_load_args_size(void);
  * ll_paged_attention over the pages of an 8-bit pool.  Its block is `paged`, with
  * the pool's buffers in it (e4m3) and kv_dtype the type of the queries and the
  * output; what is said there holds here.  Keys and values are taken as
- * ll_quantized_load gives them in kv_dtype (bf16 holds every value of the pool
- * exactly; fp16 rounds those below 2^-14, and has infinities past 65504).
+ * ll_quantized_load gives them in kv_dtype (exact where that type holds them; fp16
+ * rounds below 2^-21, and has infinities past 65504).
  * page_size is a multiple of scale_block, and scale_block at least 16.
  */
 typedef struct ll_quantized_attention_args {

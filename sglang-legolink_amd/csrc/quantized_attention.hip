@@ -4,11 +4,11 @@
 // joined is in paged_device.h; the pool's format in quantized_device.h.
 //
 // Codes become the queries' type before the matrix unit: code * 2^(byte - 127) is
-// exact in bf16 (and in fp16 within its range), one instruction for two values, so
-// the products and the softmax are those of a pool in that type.  (An 8-bit product
-// would need the queries and the weights in 4 significant bits, or two products of
-// the halves of each: as many cycles as one in 16 bits.)  Pages are whole blocks of at
-// least 16 tokens, so the keys come in groups of 16 neighbouring rows under one scale
+// exact in bf16 (bytes 3 to 246; in fp16 from 2^-21 up to 65504), one instruction for
+// two values, so the products and the softmax are those of a pool in that type.  (An
+// 8-bit product would need the queries and the weights in 4 significant bits, or two
+// products of the halves of each: as many cycles as one in 16 bits.)  Pages are whole
+// blocks of at least 16 tokens, so the keys come in groups of 16 neighbouring rows under one scale
 // for the head: page, row and scale are looked up once for a group.
 #include <hip/hip_runtime.h>
 #include <math.h>

@@ -2,9 +2,9 @@
 //
 // One layer's keys (and values) are codes c[slot][head][d] of e4m3 and bytes
 // x[block][head] of e8m0, block = slot / B: a value is c * 2^(x - 127).  The scales
-// are powers of two: codes times scale are exact in bf16 and fp32, and a scale that
-// grows costs the rows under it nothing but the bits that fall below e4m3's least
-// number (2^-9 of the scale).
+// are powers of two: codes times scale are exact in bf16 (x from 3 to 246) and fp32 (x up
+// to 246; beyond, the largest are infinite), and a scale that grows costs the rows under
+// it nothing but the bits that fall below e4m3's least number (2^-9 of the scale).
 //
 // Rows y (computed before any rounding to 8 bits) that a call writes to block b:
 //   need = the least byte with max |y| <= 448 * 2^(need - 127), y finite

@@ -371,3 +371,33 @@ def test_nothing_to_do_launches_nothing():
 def test_the_workspace_is_that_of_paged_attention():
     args = _attention_block()
     assert _native.quantized_attention_workspace_bytes(args) == _native.paged_attention_workspace_bytes(args.paged) > 0
+
+
+@pytest.mark.parametrize("dtype,exact", [(torch.bfloat16, range(3, 247)), (torch.float32, range(247)),
+                                         (torch.float16, range(127 - 15, 127 + 8))])
+def test_the_scales_whose_values_a_type_holds(dtype, exact):
+    """Every code under every scale byte: which bytes make values that the type holds."""
+
+    codes = torch.arange(256, dtype=torch.uint8)[:, None].expand(256, 255).contiguous().numpy()
+    scales = np.arange(255)
+    values = torch.from_numpy(qm.VALUES[codes] * np.ldexp(1.0, scales - 127))
+    held = values.to(dtype)
+    same = ((held.double() == values) | values.isnan()).all(0).tolist()
+    assert [byte for byte in range(255) if same[byte]] == list(exact)
+    # What is past the type is infinite; elsewhere a value is off by no more than half its least step.
+    past = held.isinf()
+    assert bool((values[past].abs() >= torch.finfo(dtype).max).all())
+    step = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert bool(((held.double() - values).abs()[~past & ~values.isnan()] <= step / 2).all())
+    if dtype == torch.float16:  # exact from 2^-21 on, up to the largest
+        size = values.abs()
+        assert bool((held.double() == values)[(size >= 2.0 ** -21) & (size <= 65504)].all())
+
+
+def test_the_largest_rows_are_held_as_two_to_the_128():
+    """1.9375 * 2^127 lies between the codes 240 and 256 of byte 247, and goes to the even one."""
+
+    byte = qm.least_byte(1.9375 * 2.0 ** 127)
+    assert byte == 247
+    below, at = np.float64([1.9375 * 2.0 ** 127 * (1 - 2.0 ** -50), 1.9375 * 2.0 ** 127]) * 2.0 ** -120
+    assert qm.VALUES[qm.encoded(np.array([below]))][0] == 240 and qm.VALUES[qm.encoded(np.array([at]))][0] == 256
