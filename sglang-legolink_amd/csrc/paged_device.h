@@ -58,6 +58,7 @@ struct PagedParams {
   long long q_token, q_head, pages_stride;
   unsigned long long page_magic;
   double inv_target;
+  double long_work, inv_long_target;  // of calls of so much work (in key tiles times column tiles) and more
   unsigned row_bytes;  // of one slot's K (or V) row: hkv * D values
   int page_shift, page_size, num_pages, max_keys;
   int num_queries, num_requests, hq, hkv, group;
@@ -148,8 +149,9 @@ __device__ inline int key_tiles_of(const Request &x) { return (x.kv_len + kPageT
 // A chunk's key tiles, of a call with this work (in key tiles times column tiles).
 __device__ inline int chunk_of(const PagedParams &p, double work) {
   // (2^25 key tiles are more than any length; readfirstlane: uniform to the compiler too)
+  const double inv_target = work >= p.long_work ? p.inv_long_target : p.inv_target;
   return __builtin_amdgcn_readfirstlane(
-      max(p.min_chunk, static_cast<int>(min(ceil(work * p.inv_target - 1e-6), 33554432.0))));
+      max(p.min_chunk, static_cast<int>(min(ceil(work * inv_target - 1e-6), 33554432.0))));
 }
 
 // Many requests: chunk_of, and what lies up to the end of every 64 of them, once for
@@ -550,7 +552,8 @@ constexpr long long kPlanned = 128;
 struct Launch {
   int columns;
   long long max_tiles, max_units;
-  int max_partials, target, min_chunk;
+  int max_partials, target, long_target, min_chunk;
+  double long_work;  // from here on the units are long_target (at least target), below it target
   bool wide, splits;
   long long ws_floats, plan_at;  // of the workspace; where the plan begins in it (ws_floats: none)
 };
@@ -587,19 +590,30 @@ Launch plan_launch(const ll_paged_attention_args *a, int together = 1, bool code
   const int heads = static_cast<int>(a->num_kv_heads) / (x.wide ? 1 : together);
   const int places = std::max(1, kComputeUnits / heads);
   const long long max_keys = a->page_table_columns * a->page_size;
-  // Between a quarter and half as many tiles as places, one round cuts requests of one
-  // length into chunks and small rests, two cut evenly but pay a second start.  Codes,
-  // 56/8 heads of 128, one round and two: 24 requests over 4,000 keys 57 and 63 us,
-  // 8,000 103 and 97, 32,768 380 and 335; 20 over 8,000 83 and 87, 32,768 308 and
-  // 297; 32, half the places, whose rests are next to nothing, 4,000 78 and 68, 32,768
-  // 536 and 403.  (Rows of 16 bits keep one round: unmeasured.)
-  const bool long_rows = max_keys * a->head_dim >= 8192 * 128;
-  const bool one_round = 2 * x.max_tiles <= places &&
-                         !(codes && (2 * x.max_tiles == places || (long_rows && 4 * x.max_tiles > places)));
-  x.target = x.wide ? places : one_round ? places - static_cast<int>(x.max_tiles) + 1 : 2 * places;
+  x.target = x.wide                           ? places
+             : 2 * x.max_tiles <= places ? places - static_cast<int>(x.max_tiles) + 1
+                                         : 2 * places;
+  // Up to half as many tiles as places, one round cuts requests of one length into long
+  // chunks and rests; two cut evenly, but pay a second start, which the longer rows and
+  // the more tiles make good.  Codes, one round and two, 8 KV heads of 128 (64 places):
+  // 20 requests over 8,000 keys 78 and 82 us, 32,768 291 and 282; 24 over 6,000 67 and
+  // 71, 8,000 102 and 94, 32,768 358 and 317; 28 over 4,000 55 and 59, 6,000 94 and 84;
+  // 31 over 4,000 59 and 58, 5,000 90 and 72; 32 over 2,000 36 and 40, 5,000 94 and 75,
+  // 32,768 518 and 424.  10 KV heads (51 places): 13 over 8,000 52 and 72, 22 over 4,000
+  // 53 and 58, 6,000 90 and 82.  8 of 256 (32 places): 10 over 16,000 152 and 140, 12 over
+  // 3,000 41 and 48, 16 59 and 48 (12 over 4,000 49 and 54: two come early).  So from (places / tiles)^2 times 1,000 keys of 128 on,
+  // in the mean of what the call turns out to have, and from a quarter of the places (the
+  // cut of 22 and 26 of 64 places suits neither: 312 and 330, 394 and 409 over 32,768).
+  // A single tile is cut evenly either way.  (Rows of 16 bits keep one round: unmeasured.)
+  const double long_values = 1000.0 * 128 * places * places / static_cast<double>(x.max_tiles);  // of the call's rows
+  const bool may_be_long = codes && !x.wide && x.max_tiles > 1 && 2 * x.max_tiles <= places &&
+                           4 * x.max_tiles > places &&
+                           static_cast<double>(max_keys * a->head_dim * x.max_tiles) >= long_values;
+  x.long_work = may_be_long ? long_values / static_cast<double>(kPageTile * a->head_dim) : INFINITY;
+  x.long_target = may_be_long ? 2 * places : x.target;
   x.splits = max_keys > x.min_chunk * kPageTile;
-  x.max_units = x.max_tiles + (x.splits ? x.target + 1 : 0);
-  x.max_partials = x.splits ? 2 * x.target + 2 : 0;
+  x.max_units = x.max_tiles + (x.splits ? x.long_target + 1 : 0);
+  x.max_partials = x.splits ? 2 * x.long_target + 2 : 0;
   x.plan_at = x.max_partials * a->num_kv_heads * x.columns * (a->head_dim + 2);
   x.ws_floats = x.plan_at + (requests > kPlanned ? plan_ints(requests) : 0);
   return x;
@@ -725,6 +739,8 @@ int fill_params(const ll_paged_attention_args *a, const Launch &x, PagedParams *
   p.starts64 = a->query_starts_dtype == LL_DTYPE_INT64 ? 1 : 0;
   p.min_chunk = x.splits ? x.min_chunk : kOneChunk;
   p.inv_target = 1.0 / x.target;
+  p.long_work = x.long_work;
+  p.inv_long_target = 1.0 / x.long_target;
   p.max_partials = x.max_partials;
   p.scale_log2 = static_cast<float>(a->softmax_scale * 1.4426950408889634);  // log2(e)
   return LL_OK;

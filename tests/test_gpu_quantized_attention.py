@@ -470,3 +470,38 @@ def test_two_streams_at_once(gpu_device):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(result, want[i]) for result in got[i])
+
+
+@pytest.mark.parametrize("count", [8, 9, 13, 16])
+@pytest.mark.parametrize("lengths", ["long", "just long", "just short", "short", "uneven"])
+def test_rounds_go_by_the_lengths_of_the_call(gpu_device, count, lengths):
+    """Calls in tables of long rows, from a quarter of the places to half of them:
+    whichever target the lengths on the device make, every key counts once."""
+
+    report(f"rounds, {count} requests, {lengths}")
+    turn = math.ceil(500 * 1024 / count ** 2 / 64) * 64  # 32 places; 500 keys of 256 are 1,000 of 128
+    of = {"long": lambda r: turn + 1200, "just long": lambda r: turn, "just short": lambda r: turn - 64,
+          "short": lambda r: 40 + 61 * r, "uneven": lambda r: 0 if r % 5 == 3 else 9000 if r % 3 == 0 else 70}[lengths]
+    case = _marked(_case(gpu_device, [of(r) for r in range(count)], heads=(16, 8), dim=256, spare_columns=300))
+    _check_marked(quantized_paged_attention(**case), case)
+
+
+def test_a_captured_call_turns_from_one_target_to_the_other(gpu_device):
+    """One graph over tables of long rows, replayed with long and short lengths."""
+
+    case = _marked(_case(gpu_device, [4200] * 14, heads=(16, 8), dim=256, spare_columns=100))
+    quantized_paged_attention(**case)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = quantized_paged_attention(**case)
+    for lengths in ([4200] * 14, [300] * 14, [4200] * 13 + [0], [1] * 14, [4200 - 13 * r for r in range(14)]):
+        case["kv_lengths"].copy_(torch.tensor(lengths))
+        captured.fill_(9)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = captured.clone()
+        again = quantized_paged_attention(**case)
+        torch.cuda.synchronize()
+        assert torch.equal(got, again)
+        _check_marked(got, case)

@@ -4,6 +4,7 @@ the Python entries and of the C entries, none of which reaches a device."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -401,3 +402,31 @@ def test_the_largest_rows_are_held_as_two_to_the_128():
     assert byte == 247
     below, at = np.float64([1.9375 * 2.0 ** 127 * (1 - 2.0 ** -50), 1.9375 * 2.0 ** 127]) * 2.0 ** -120
     assert qm.VALUES[qm.encoded(np.array([below]))][0] == 240 and qm.VALUES[qm.encoded(np.array([at]))][0] == 256
+
+
+def _attention_workspace(requests, kv_heads, dim, keys):
+    args = _attention_block()
+    paged = args.paged
+    paged.num_queries = paged.num_requests = requests
+    paged.num_q_heads = paged.num_kv_heads = kv_heads
+    paged.head_dim = dim
+    paged.page_table_stride = paged.page_table_columns = -(-keys // 16)
+    return _native.quantized_attention_workspace_bytes(args)
+
+
+@pytest.mark.parametrize("kv_heads,dim,places", [(8, 128, 64), (10, 128, 51), (12, 128, 42), (8, 256, 32), (16, 64, 64),
+                                                 (7, 128, 36)])
+def test_the_rounds_of_single_tokens_have_no_point_of_their_own(kv_heads, dim, places):
+    """Partial results: 2 (places - requests) + 4 for one round of units, 4 places + 2 for
+    two; tables of 1,000 (places / requests)^2 keys of 128 leave room for two."""
+
+    partial = kv_heads * 16 * (dim + 2) * 4
+    for requests in range(-(-32 // kv_heads), places // 2 + 1):  # (heads that share a workgroup)
+        one, two = (2 * (places - requests) + 4) * partial, (4 * places + 2) * partial
+        pages = 1000 * (places / requests) ** 2 * 128 / dim / 16
+        for keys in (1024 * 128 // dim, 16 * math.floor(pages - 1e-9)):
+            assert _attention_workspace(requests, kv_heads, dim, keys) == one, (requests, keys)
+        for keys in (16 * math.ceil(pages + 1e-9), 131072):
+            want = two if 4 * requests > places else one
+            assert _attention_workspace(requests, kv_heads, dim, keys) == want, (requests, keys)
+    assert _attention_workspace(places // 2 + 1, kv_heads, dim, 1024) == (4 * places + 2) * partial
