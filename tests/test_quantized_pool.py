@@ -31,6 +31,12 @@ def test_the_model_of_the_format_is_torchs():
     assert [qm.least_byte(x) for x in (0.0, 448.0, 448.5, 896.0, 2.0 ** -130)] == [0, 127, 128, 128, 0]
 
 
+def test_the_package_names_the_module():
+    import legolink_amd
+
+    assert "quantized_pool" in legolink_amd.__all__ and "legolink_amd.quantized_pool" in legolink_amd.__doc__
+
+
 def _pool(slots=64, heads=2, dim=64, block=16):
     return dict(key_buffer=torch.zeros(slots, heads, dim, dtype=torch.float8_e4m3fn),
                 value_buffer=torch.zeros(slots, heads, dim, dtype=torch.float8_e4m3fn),
