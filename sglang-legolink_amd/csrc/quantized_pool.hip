@@ -500,7 +500,7 @@ struct RowBits<0> {
 
 // Waves a SIMD that the registers leave room for: what reads most latency away for few
 // spilled registers (32,768 tokens linked in blocks of 16: 39 us with four, 44 with
-// three; 8,192 in blocks of 128 34 and 37, but 8,192 appended 135 and 111).
+// three; 8,192 in blocks of 128 29 and 36, but 8,192 appended with norms 75 and 63).
 template <typename Source>
 constexpr int least_waves(int parts) {
   return parts <= 2 || (parts == 8 && !Source::kNorms) ? 4 : parts <= 8 ? 3 : 1;
@@ -594,10 +594,10 @@ __device__ inline int pack_tokens(const PoolParams &p, long long t0, Token *toke
 // lane i's pair j as element 9 R row + R j + i, R = rotary lanes of a row, so that 16
 // lanes' 16-byte reads meet every bank once.
 //
-// 4 heads of 128 in blocks of 16: 32,768 tokens linked 38 us (100 MB with the table's
+// 4 heads of 128 in blocks of 16: 32,768 tokens linked 37 us (100 MB with the table's
 // rows, 2.7 TB/s: the vector units are busy for more than half of it, the rest is what
 // four waves a SIMD leave of the latencies), 1,024 6.8 us; 16,384 tokens' keys and
-// values appended 31 us, 64 single tokens 6.1 us.
+// values appended 33 us, 64 single tokens 6.2 us.
 template <typename Source, typename E, int kGroup, int kParts, bool kQueries>
 __global__ void __launch_bounds__(kParts > 4 ? kParts * kWave : kThreads, least_waves<Source>(kParts))
     quantized_write_kernel(const PoolParams p) {
