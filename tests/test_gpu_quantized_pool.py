@@ -611,3 +611,40 @@ def test_rows_added_to_used_blocks_need_cleared_scales(gpu_device, block):
         for name in ("key_scales", "value_scales"):
             scales = case[name].view(torch.uint8)[:2]
             assert bool((scales[0] < 130).all()) and bool((scales[1] < 130).all() if cleared else (scales[1] == 200).all())
+
+
+@pytest.mark.parametrize("runs", list(PADDED))
+def test_padding_in_slots_of_32_bits(gpu_device, runs):
+    slots = PADDED[runs]
+    case = _append_case(gpu_device, slots, dim=64, slots=512, kv_heads=1, q_heads=1, index=torch.int32)
+    _check_append(case)
+    sources = [1024 + (7 * i) % 512 for i in range(len(slots))]
+    case = _link_case(gpu_device, sources, [s if s < 512 else 1536 for s in slots], dim=64, slots=1536, index=torch.int32)
+    _check_link(case)
+
+
+def test_a_captured_append_replays_with_other_padding(gpu_device):
+    """One graph of a padded batch, replayed with its padding elsewhere, against eager calls."""
+
+    tokens = 600
+    case = _append_case(gpu_device, [-1] * tokens, slots=tokens * 16, q_heads=2)
+    twin = {name: value.clone() if name.endswith(("_buffer", "_scales")) else value for name, value in case.items()}
+    append_quantized_kv_inplace(**case)
+    append_quantized_kv_inplace(**twin)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = append_quantized_kv_inplace(**case)
+    for turn, gaps in enumerate(([], [3, 4, 300], range(100, 590), range(1, tokens, 2), range(0, 599))):
+        slots = torch.arange(tokens) + 37 * turn
+        slots[list(gaps)] = -1
+        case["destination_slots"].copy_(slots)
+        graph.replay()
+        torch.cuda.synchronize()
+        before = _state(twin)
+        want = append_quantized_kv_inplace(**twin)
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want)
+        _check_pool(twin, before, 16, slots.tolist(), _rows_of(twin, True, "key"), _rows_of(twin, True, "value"),
+                    (slots >= 0).tolist())
+        assert all(np.array_equal(a, b) for a, b in zip(_state(case), _state(twin)))
